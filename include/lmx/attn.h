@@ -1,7 +1,8 @@
 /*
  * lmx/attn.h -- C ABI of the MI355X (gfx950) attention hot path for llmoxide.
  *
- * One shared library, libllmoxide_amd.so, exports exactly the functions below.
+ * One shared library, libllmoxide_amd.so, exports exactly the functions below
+ * and those of lmx/paged.h (the paged KV cache).
  * They replace the wgpu dispatches that llmoxide's crates/gpu records for
  * attention, KV append and the gated delta rule; each declaration cites the
  * reference code it stands in for (paths relative to the llmoxide tree).

@@ -22,6 +22,8 @@ this module                reference dispatch it mirrors
                            ``l2norm_qk`` (deltanet.wgsl:54-173)
 ``delta_back``             ``rms_norm`` + ``mul_silu`` after the recurrence
                            (qwen35.rs:968-986)
+``paged_append`` and the   the paged KV cache (include/lmx/paged.h), in
+other ``paged_`` calls     :mod:`llmoxide_amd.paged`
 =========================  ==================================================
 
 Tensors are torch tensors on a ROCm device (torch provides device memory and
@@ -704,3 +706,6 @@ class KvManager:
                                                     ctypes.byref(mx)))
         return list(kp), list(vp), list(cl), mx.value
 
+
+from .paged import (PagedBatch, PagedCache, paged_append, paged_attention,  # noqa: E402
+                    paged_prologue, paged_read)

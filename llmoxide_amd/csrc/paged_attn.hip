@@ -1,0 +1,646 @@
+// Attention of few query rows (decode) over pages on gfx950, and the merge of
+// key splits.
+//
+// A work item is 16 query rows of one kv head (row r: token r / G, head r % G)
+// over one split of the visible keys; a workgroup's four waves take a quarter
+// of the split each and join in LDS.  Everything goes from memory to MFMA
+// operands without LDS: both products are computed transposed,
+//   S^T[key, row] = K Q^T      A = K  (lane: one key, 8 dims)
+//   O^T[dim, row] += V^T P^T   A = V^T (lane: one dim, 8 keys), B = P^T
+// and v_mfma_f32_16x16x32_f16 leaves S^T with a lane holding one row's scores
+// for keys 4g..4g+3 of each 16-key block (g = lane / 16).  Which keys a block
+// takes is free, so block j takes keys 8g + 4j + (0..3) of each group g: the
+// two blocks of a 32-key tile give a lane 8 consecutive keys, exactly what the
+// B operand of the second product and a 16-byte load of a V column want.  8-bit
+// tiles are 64 keys in four blocks, 16 consecutive keys a lane.
+//
+// Softmax: one running reference m per row (log2 units), taken from the first
+// tile and moved only when a score passes it by 2^4; weights are
+// exp2(s - m + 10) <= 2^14, so f16 holds them, with a residual in a second f16
+// (22 bits together); sums are fp32.  An 8-bit V's scale joins the weight,
+// brought near 1 by a power of two common to the wave.
+#include <algorithm>
+
+#include "paged_attn.hpp"
+
+namespace lmx {
+
+constexpr int kBM = 16;       // query rows an item
+// Weights are exp2(s - m + kLift), and a score may pass m by kSlack before m
+// moves: at most 2^14, with the smallest f16 step 2^-34 of a weight at m.
+constexpr float kLift = 10.f;
+constexpr float kSlack = 4.f;
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// Maximum over the four lanes (g) that share a row.
+__device__ __forceinline__ float max_groups(float x) {
+    x = fmaxf(x, shfl_xor(x, 16));
+    return fmaxf(x, shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+    x += shfl_xor(x, 16);
+    return x + shfl_xor(x, 32);
+}
+
+// The halves of two f16 that are infinite or NaN, and the word without them.
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
+    const uint32_t e = x & 0x7c007c00u;
+    return ((e & 0xffffu) == 0x7c00u ? 0xffffu : 0u) | ((e >> 16) == 0x7c00u ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t finite2(uint32_t x) { return x & ~nonfinite2(x); }
+
+// The page of every 16-key granule of a wave's key range, 64 table entries at
+// a time in the wave's lanes, so that the loop's lookups wait on no memory.
+struct PageWindow {
+    const int32_t* row;  // the sequence's table
+    int first;           // entry in lane 0
+    int ids;             // the lane's page, -1: none
+    __device__ __forceinline__ void fill(const PagedArgs& a, int entry) {
+        first = entry;
+        const int e = entry + (int)__lane_id();
+        ids = e < a.g.table_stride ? paged_page(a.g, row[e]) : -1;
+    }
+    // Page of key k (wave-uniform, >= 0).
+    __device__ __forceinline__ int at(const PagedArgs& a, int k) {
+        const int e = k >> a.g.ps_log2;
+        if (e - first >= 64) fill(a, e);
+        return __builtin_amdgcn_readlane(ids, e - first);
+    }
+};
+
+template <int HD, bool I8>
+struct Tile {
+    static constexpr int KEYS = I8 ? 64 : 32;
+    static constexpr int NB = KEYS / 16;          // 16-key blocks
+    static constexpr int KL = I8 ? HD / 64 : HD / 32;  // 16-byte K loads a block
+    static constexpr int VL = HD / 16;            // 16-byte V loads
+    uint4 k[NB][KL];
+    uint4 v[VL];
+    f32x4 ks[I8 ? NB : 1], vs[I8 ? NB : 1];       // scales of the lane's keys
+    int pages[KEYS / 16];                         // per 16-key granule; -1: none
+};
+
+template <int HD, bool I8>
+__device__ __forceinline__ void load_tile(const AttnPagedArgs& a, PageWindow& pw, int h, int t0, Tile<HD, I8>& t) {
+    using T = Tile<HD, I8>;
+    const int lane = __lane_id(), c = lane & 15, g = lane >> 4;
+    const int psm = (1 << a.p.g.ps_log2) - 1;
+#pragma unroll
+    for (int i = 0; i < T::KEYS / 16; ++i) t.pages[i] = pw.at(a.p, t0 + 16 * i);
+    // Granule i's (page, head) block; a missing page reads page 0, and is masked.
+    auto slab = [&](int i) { return (size_t)imax(t.pages[i], 0) * a.p.g.Hkv + h; };
+    constexpr int ES = I8 ? 1 : 2;
+    size_t base[T::KEYS / 16];
+#pragma unroll
+    for (int i = 0; i < T::KEYS / 16; ++i) base[i] = slab(i) << a.p.g.ps_log2;  // in positions
+    // K: the lane's key in block j is KEYS/4 * (c/4) + 4j + c%4; V: its keys
+    // are KEYS/4 consecutive ones.  Neither leaves its granule.
+    size_t kb, vb;
+    if constexpr (I8) {
+        const int i = c >> 2;
+        kb = i == 0 ? base[0] : i == 1 ? base[1] : i == 2 ? base[2] : base[3];
+        vb = g == 0 ? base[0] : g == 1 ? base[1] : g == 2 ? base[2] : base[3];
+    } else {
+        kb = c >> 3 ? base[1] : base[0];
+        vb = g >> 1 ? base[1] : base[0];
+    }
+    constexpr int QUART = T::KEYS / 4;  // consecutive keys of a lane
+    const char* kr = a.p.k + (kb + ((t0 + QUART * (c >> 2)) & psm) + (c & 3)) * (HD * ES) + 16 * g;
+#pragma unroll
+    for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+        for (int l = 0; l < T::KL; ++l) t.k[j][l] = *reinterpret_cast<const uint4*>(kr + 4 * j * HD * ES + 64 * l);
+    const int vslot = (t0 + QUART * g) & psm;
+    const char* vc = a.p.v + (vb * HD + (c << a.p.g.ps_log2) + vslot) * ES;
+    const uint32_t vstep = (16u * ES) << a.p.g.ps_log2;
+#pragma unroll
+    for (int l = 0; l < T::VL; ++l) t.v[l] = *reinterpret_cast<const uint4*>(vc + l * vstep);
+    if constexpr (I8) {
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+            t.ks[j] = *reinterpret_cast<const f32x4*>(a.p.k_scale + vb + vslot + 4 * j);
+            t.vs[j] = *reinterpret_cast<const f32x4*>(a.p.v_scale + vb + vslot + 4 * j);
+        }
+    }
+}
+
+// F32: q and out are f32 and q has a residual part.
+template <int HD, bool I8, bool F32>
+__global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnPagedArgs a) {
+    using T = Tile<HD, I8>;
+    using QT = std::conditional_t<F32, float, f16>;
+    constexpr int KS = HD / 32;   // k-steps of QK
+    constexpr int DT = HD / 16;   // 16-dim blocks of the output
+    constexpr bool QLDS = HD == 512;
+    constexpr int OP = HD + 4;  // floats a row of the exchange (16-byte rows, rows 4 banks apart)
+    constexpr size_t kEx = 512 + 4 * 16 * OP * 4, kQ = QLDS ? (F32 ? 2 : 1) * KS * 64 * 16 : 0;
+    __shared__ __align__(16) char smem[kEx > kQ ? kEx : kQ];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+
+    Item it;
+    if (!find_item(a, blockIdx.x, kBM, true, it)) return;
+    const PagedGeom& pg = a.p.g;
+    if (it.split == 0 && tid == 0 && it.tile < a.rt_max)
+        a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile] = make_int4(it.first, it.stride, it.splits, 0);
+
+    // This wave's keys: its quarter of the split, in whole tiles.
+    const int split_lo = it.w.lo + it.split * it.per * kUnit;
+    const int split_hi = it.splits > 1 ? imin(it.s.ctx, split_lo + it.per * kUnit) : it.s.ctx;
+    const int tiles = (split_hi - split_lo + T::KEYS - 1) / T::KEYS;
+    const int t_lo = tiles * w / 4, t_hi = tiles * (w + 1) / 4;
+
+    // The lane's query row.
+    const int row = it.tile * kBM + c;
+    const bool have = row < it.s.n * pg.G;
+    const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
+    const int pos = have ? it.s.ctx - it.s.n + tok : -1;
+    const int seen_lo = pg.window ? imax(pos - pg.window + 1, 0) : 0;
+    // Keys that every row of the tile sees need no mask.
+    const int r_last = imin(it.tile * kBM + kBM, it.s.n * pg.G) - 1;
+    const int all_hi = it.s.ctx - it.s.n + (it.tile * kBM) / pg.G;                       // first row's position
+    const int all_lo = pg.window ? imax(it.s.ctx - it.s.n + r_last / pg.G - pg.window + 1, 0) : 0;
+
+    // Q: k-step s holds dims 32s + 8g (f16 tiles); an 8-bit tile's 16-byte load
+    // spans two k-steps, so there k-step 2l + e holds dims 64l + 16g + 8e.
+    f16x8 qh[QLDS ? 1 : KS], ql[F32 && !QLDS ? KS : 1];
+    float qscale = a.c;
+    auto q_dim = [&](int s) { return I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+    f16x8* const q_lds = reinterpret_cast<f16x8*>(smem);  // QLDS: [part][KS][64]
+    {
+        const QT* qr = static_cast<const QT*>(a.q) + (size_t)(it.s.row0 + tok) * a.q_row_stride + head * a.q_head_stride;
+        if constexpr (F32) {
+            // The row times a power of two that brings its largest element to
+            // [2^14, 2^15): both f16 parts then keep their bits.
+            float m = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                float x[8];
+                load_f32<8>(qr + q_dim(s), x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+            }
+            m = max_groups(m);
+            int e = 0;
+            if (m > 0.f && m < INFINITY) e = 15 - (__builtin_amdgcn_frexp_expf(m));
+            e = imin(imax(e, -120), 120);
+            const float up = ldexpf(1.f, e);
+            qscale = ldexpf(a.c, -e);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                float x[8];
+                load_f32<8>(qr + q_dim(s), x);
+                f16x8 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = have ? x[j] * up : 0.f;
+                    hi[j] = (f16)y;
+                    lo[j] = (f16)(y - (float)hi[j]);
+                }
+                if constexpr (QLDS) {
+                    if (w == 0) {
+                        q_lds[s * 64 + lane] = hi;
+                        q_lds[(KS + s) * 64 + lane] = lo;
+                    }
+                } else {
+                    qh[s] = hi;
+                    ql[s] = lo;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                f16x8 hi = *reinterpret_cast<const f16x8*>(qr + q_dim(s));
+                if (!have) hi = f16x8{};
+                if constexpr (QLDS) {
+                    if (w == 0) q_lds[s * 64 + lane] = hi;
+                } else {
+                    qh[s] = hi;
+                }
+            }
+        }
+        if constexpr (QLDS) __syncthreads();
+    }
+
+    f32x4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;  // m: reference exponent less kLift; -inf: nothing seen yet
+    float vref = 0.f;              // I8: weights carry v_scale * vref (a power of two); 0: not set
+
+    PageWindow pw;
+    pw.row = a.p.table + (size_t)it.b * pg.table_stride;
+    pw.fill(a.p, (split_lo + t_lo * T::KEYS) >> pg.ps_log2);
+
+    bool poison = false;           // a masked tile's V held an infinity or a NaN
+
+    // Whether every row of the item sees all of the tile.
+    auto all_seen = [&](const int (&pages)[T::KEYS / 16], int t0) {
+        bool whole = t0 + T::KEYS - 1 <= all_hi && t0 >= all_lo;
+#pragma unroll
+        for (int i = 0; i < T::KEYS / 16; ++i) whole = whole && pages[i] >= 0;
+        return whole;
+    };
+
+    auto step = [&](Tile<HD, I8>& t, int t0) {
+        // ---- scores
+        f32x4 s[T::NB];
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+            s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                f16x8 kf;
+                if constexpr (I8) {
+                    const uint4 x = t.k[j][k >> 1];
+                    kf = k & 1 ? i8x8_to_f16(x.z, x.w) : i8x8_to_f16(x.x, x.y);
+                } else {
+                    kf = __builtin_bit_cast(f16x8, t.k[j][k]);
+                }
+                if constexpr (QLDS) {
+                    s[j] = mfma16(kf, q_lds[k * 64 + lane], s[j]);
+                    if constexpr (F32) s[j] = mfma16(kf, q_lds[(KS + k) * 64 + lane], s[j]);
+                } else {
+                    s[j] = mfma16(kf, qh[k], s[j]);
+                    if constexpr (F32) s[j] = mfma16(kf, ql[k], s[j]);
+                }
+            }
+            if constexpr (I8) s[j] *= t.ks[j];
+            s[j] *= qscale;
+        }
+        // ---- mask: keys behind the row, before its window, in no page
+        constexpr int QUART = T::KEYS / 4;
+        const bool whole = all_seen(t.pages, t0);
+        uint32_t seen = 0xffffffffu;  // bit 4j + i: the lane's key 4j + i
+        if (!whole) {
+            const int gran = I8 ? g : g >> 1;
+            int page = t.pages[0];
+#pragma unroll
+            for (int i = 1; i < T::KEYS / 16; ++i) page = gran == i ? t.pages[i] : page;
+            const int key = t0 + QUART * g;
+            seen = 0;
+#pragma unroll
+            for (int i = 0; i < QUART; ++i)
+                seen |= (uint32_t)(page >= 0 && key + i <= pos && key + i >= seen_lo) << i;
+#pragma unroll
+            for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(seen >> (4 * j + i) & 1)) s[j][i] = -INFINITY;
+        }
+        // ---- the reference
+        float top = s[0][0];
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
+        if (__ballot(top > m + (kSlack + kLift))) {  // m = -inf: any score
+            top = max_groups(top);
+            float mn = m;
+            if (top > m + (kSlack + kLift)) mn = top - kLift;
+            const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= f;
+        }
+        // ---- weights
+        const float ms = m == -INFINITY ? 0.f : m;
+        f16x8 ph[T::NB / 2], pl[T::NB / 2];
+        float vmul[I8 ? T::NB : 1][4];
+        if constexpr (I8) {
+            // bring the largest scale of the tile's keys near 1; a larger one
+            // than before rescales what is there
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool on = seen >> (4 * j + i) & 1;
+                    if (on && t.vs[j][i] < INFINITY) big = fmaxf(big, t.vs[j][i]);
+                }
+            if (__ballot(big * vref > 1.f || (vref == 0.f && big > 0.f))) {
+#pragma unroll
+                for (int x = 1; x < 64; x <<= 1) big = fmaxf(big, shfl_xor(big, x));
+                // big * nref in (1/4, 1/2]: room for a doubling before the next rescale
+                const float nref = ldexpf(1.f, imin(imax(-1 - __builtin_amdgcn_frexp_expf(big), -120), 120));
+                const float f = vref == 0.f ? 0.f : nref / vref;
+                vref = nref;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= f;
+            }
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float p = fast_exp2(s[j][i] - ms);
+                sum += p;
+                if constexpr (I8) {
+                    const bool on = seen >> (4 * j + i) & 1;
+                    p = on ? p * (t.vs[j][i] * vref) : 0.f;
+                }
+                const int at = 4 * (j & 1) + i;
+                ph[j >> 1][at] = (f16)p;
+                pl[j >> 1][at] = (f16)(p - (float)(f16)p);
+            }
+        l += sum;
+        // ---- O^T += V^T P^T
+        if constexpr (!I8) {
+            // An infinity or NaN in V would meet the zero weights of rows that
+            // do not see its key (0 * inf): in tiles that hold such a key,
+            // these elements stay out of the product, and the rows that do see
+            // them get them after the loop.
+            if (!whole) {
+                uint32_t bad = 0;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    bad |= nonfinite2(t.v[d].x) | nonfinite2(t.v[d].y) | nonfinite2(t.v[d].z) | nonfinite2(t.v[d].w);
+                    t.v[d] = uint4{finite2(t.v[d].x), finite2(t.v[d].y), finite2(t.v[d].z), finite2(t.v[d].w)};
+                }
+                poison = poison || __ballot(bad != 0) != 0;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if constexpr (I8) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const f16x8 vf = e ? i8x8_to_f16(t.v[d].z, t.v[d].w) : i8x8_to_f16(t.v[d].x, t.v[d].y);
+                    o[d] = mfma16(vf, ph[e], o[d]);
+                    o[d] = mfma16(vf, pl[e], o[d]);
+                }
+            } else {
+                const f16x8 vf = __builtin_bit_cast(f16x8, t.v[d]);
+                o[d] = mfma16(vf, ph[0], o[d]);
+                o[d] = mfma16(vf, pl[0], o[d]);
+            }
+        }
+    };
+
+    if (t_lo < t_hi) {
+        constexpr bool PIPE = HD <= 256;
+        Tile<HD, I8> t0, t1;
+        load_tile<HD, I8>(a, pw, it.h, split_lo + t_lo * T::KEYS, t0);
+        if constexpr (PIPE) {
+            int t = t_lo;
+            while (true) {
+                if (t + 1 < t_hi) load_tile<HD, I8>(a, pw, it.h, split_lo + (t + 1) * T::KEYS, t1);
+                step(t0, split_lo + t * T::KEYS);
+                if (++t >= t_hi) break;
+                if (t + 1 < t_hi) load_tile<HD, I8>(a, pw, it.h, split_lo + (t + 1) * T::KEYS, t0);
+                step(t1, split_lo + t * T::KEYS);
+                if (++t >= t_hi) break;
+            }
+        } else {
+            for (int t = t_lo; t < t_hi; ++t) {
+                if (t != t_lo) load_tile<HD, I8>(a, pw, it.h, split_lo + t * T::KEYS, t0);
+                step(t0, split_lo + t * T::KEYS);
+            }
+        }
+    }
+
+    if constexpr (!I8) {
+        float z = 0.f;  // NaN where an element of o is not finite
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) z = fmaf(o[d][x], 0.f, z);
+        if (poison || __ballot(z != 0.f)) {
+            // Rare: the infinities and NaN among V go to the rows that see
+            // them (a product with a weight's parts made NaN of an infinity).
+            f32x4 add[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) add[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+            pw.fill(a.p, (split_lo + t_lo * T::KEYS) >> pg.ps_log2);
+            const size_t step = (size_t)1 << pg.ps_log2;
+            for (int key = split_lo + t_lo * T::KEYS; key < split_lo + t_hi * T::KEYS; ++key) {
+                const int page = pw.at(a.p, key);
+                if (page < 0 || key > pos || key < seen_lo) continue;
+                const f16* e = reinterpret_cast<const f16*>(a.p.v) +
+                               v_offset(a.p, page, it.h, key & ((1 << pg.ps_log2) - 1)) + ((4 * g) << pg.ps_log2);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float y = (float)*e;
+                        if (!(fabsf(y) < INFINITY)) add[d][x] += y;
+                        e += x < 3 ? step : 13 * step;  // dims 16d + 4g + x
+                    }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (!(fabsf(add[d][x]) < INFINITY)) o[d][x] = add[d][x];
+        }
+    }
+
+    // ---- join the four waves
+    l = sum_groups(l);
+    if constexpr (I8) {
+        const float back = vref == 0.f ? 0.f : 1.f / vref;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= back;
+    }
+    float* const ex_m = reinterpret_cast<float*>(smem);  // [4][16]
+    float* const ex_l = ex_m + 64;                       // [4][16]
+    float* const ex_o = ex_m + 128;                      // [4][16][OP]
+    if constexpr (QLDS) __syncthreads();                 // Q's place is taken over
+    if (g == 0) {
+        ex_m[w * 16 + c] = m;
+        ex_l[w * 16 + c] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&ex_o[(w * 16 + c) * OP + 16 * d + 4 * g]) = o[d];
+    __syncthreads();
+    const int rows = imin(kBM, it.s.n * pg.G - it.tile * kBM);
+    const int item = it.first + it.split * it.stride;
+    for (int i = tid; i < rows * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
+        const float m0 = ex_m[r], m1 = ex_m[16 + r], m2 = ex_m[32 + r], m3 = ex_m[48 + r];
+        const float mm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = fast_exp2(ex_m[16 * k + r] - ref);
+            sum = fmaf(ex_l[16 * k + r], f, sum);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&ex_o[(k * 16 + r) * OP + d]);
+            y += x * f;
+        }
+        if (it.splits > 1) {
+            *reinterpret_cast<f32x4*>(a.part_o + ((size_t)item * kBM + r) * HD + d) = y;
+            if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + ((size_t)item * kBM + r) * 2) = f32x2{mm, sum};
+        } else {
+            const int q = it.tile * kBM + r;
+            y *= sum == 0.f ? 0.f : 1.f / sum;
+            QT* dst = static_cast<QT*>(a.out) +
+                      ((size_t)(it.s.row0 + q / pg.G) * pg.Hkv * pg.G + it.h * pg.G + q % pg.G) * HD + d;
+            if constexpr (F32)
+                *reinterpret_cast<f32x4*>(dst) = y;
+            else
+                *reinterpret_cast<f16x4*>(dst) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+        }
+    }
+}
+
+// Joins the splits of one query row: a workgroup for each (sequence, kv head,
+// row of that sequence), HD/4 columns x 1024/HD groups of splits.
+template <int HD, bool F32>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int bm) {
+    using QT = std::conditional_t<F32, float, f16>;
+    constexpr int C4 = HD / 4, NG = 256 / C4;
+    __shared__ f32x4 ex[NG][C4];
+    __shared__ float ex_m[NG], ex_l[NG];
+    const PagedGeom& pg = a.p.g;
+    const int n_rows = pg.max_new * pg.G;
+    const int row = blockIdx.x % n_rows, bh = blockIdx.x / n_rows, b = bh / pg.Hkv, h = bh % pg.Hkv, tile = row / bm;
+    const int4 info = a.rows[((size_t)b * pg.Hkv + h) * a.rt_max + tile];
+    PagedSeq s;
+    SeqWork w;
+    load_work(a, b, bm, s, w);
+    if (tile >= w.rt || row >= s.n * pg.G) return;
+    const int splits = imin(info.z, a.n_items);
+    if (splits <= 1) return;
+    const int col = threadIdx.x % C4, grp = threadIdx.x / C4;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;
+    for (int s0 = grp; s0 < splits; s0 += NG * U) {
+        f32x2 ml[U];
+        f32x4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int sp = s0 + u * NG < splits ? s0 + u * NG : s0;
+            // in range whatever the table of rows holds
+            const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm + row % bm;
+            ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+            x[u] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + 4 * col);
+            if (s0 + u * NG >= splits) ml[u] = f32x2{-INFINITY, 0.f};
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u][0]);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float f = fast_exp2(m - ref);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float fu = fast_exp2(ml[u][0] - ref);
+            l = fmaf(ml[u][1], fu, l);
+            if (s0 + u * NG < splits) o += x[u] * fu;
+        }
+        m = mn;
+    }
+    ex[grp][col] = o;
+    if (col == 0) {
+        ex_m[grp] = m;
+        ex_l[grp] = l;
+    }
+    __syncthreads();
+    if (grp) return;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) mm = fmaxf(mm, ex_m[k]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+        const float f = fast_exp2(ex_m[k] - ref);
+        sum = fmaf(ex_l[k], f, sum);
+        y += ex[k][col] * f;
+    }
+    y *= sum == 0.f ? 0.f : 1.f / sum;
+    QT* dst = static_cast<QT*>(a.out) + ((size_t)(s.row0 + row / pg.G) * pg.Hkv * pg.G + h * pg.G + row % pg.G) * HD + 4 * col;
+    if constexpr (F32)
+        *reinterpret_cast<f32x4*>(dst) = y;
+    else
+        *reinterpret_cast<f16x4*>(dst) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+}
+
+// ------------------------------------------------------------------- host --
+constexpr int kRowsTarget = 512;  // items aimed at: two workgroups a CU
+constexpr int kRowsLeast = 2;     // units a split has at least (128 keys)
+
+struct RowsPlan {
+    int64_t items;   // workgroups, an upper bound of the batch's items
+    int rt_max;
+    size_t o_bytes, ml_bytes, rows_bytes;
+    bool splits;
+};
+static RowsPlan rows_plan(const PagedGeom& g, int hd) {
+    RowsPlan r;
+    const int64_t tiles = row_tiles_bound(g, kBM) * g.Hkv;
+    // A single split reaches every key of a short call: no partials then.
+    r.splits = g.max_ctx > kRowsLeast * kUnit;
+    r.items = tiles + (r.splits ? kRowsTarget : 0);
+    r.rt_max = (int)(((int64_t)g.max_new * g.G + kBM - 1) / kBM);
+    r.o_bytes = r.splits ? (size_t)r.items * kBM * hd * 4 : 0;
+    r.ml_bytes = r.splits ? (size_t)r.items * kBM * 8 : 0;
+    r.rows_bytes = (size_t)g.n_seq * g.Hkv * r.rt_max * 16;
+    return r;
+}
+
+size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
+    PagedGeom g = paged_args(p, b).g;
+    g.G = (int)(d->n_heads / p->n_kv_heads);
+    const RowsPlan r = rows_plan(g, (int)p->head_dim);
+    return r.o_bytes + r.ml_bytes + r.rows_bytes;
+}
+
+template <int HD, bool I8, bool F32>
+static lmx_status launch_rows(const AttnPagedArgs& a, const RowsPlan& r, hipStream_t st) {
+    hipLaunchKernelGGL((paged_rows_kernel<HD, I8, F32>), dim3((unsigned)r.items), dim3(256), 0, st, a);
+    LMX_CHECK_LAUNCH();
+    if (r.splits) {
+        const unsigned rows = (unsigned)(a.p.g.max_new * a.p.g.G) * (unsigned)(a.p.g.n_seq * a.p.g.Hkv);
+        hipLaunchKernelGGL((paged_merge_kernel<HD, F32>), dim3(rows), dim3(256), 0, st, a, kBM);
+        LMX_CHECK_LAUNCH();
+    }
+    return LMX_OK;
+}
+
+lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const void* q, lmx_dtype dt,
+                      void* out, void* ws, hipStream_t st) {
+    AttnPagedArgs a{};
+    a.p = paged_args(p, b);
+    a.p.g.G = (int)(d->n_heads / p->n_kv_heads);
+    a.p.g.window = (int)d->window;
+    a.q = q;
+    a.out = out;
+    a.q_head_stride = d->q_head_stride ? d->q_head_stride : p->head_dim;
+    a.q_row_stride = d->q_row_stride ? d->q_row_stride : a.q_head_stride * d->n_heads;
+    a.c = d->scale * kLog2e;
+    const RowsPlan r = rows_plan(a.p.g, (int)p->head_dim);
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + r.o_bytes);
+    a.rows = reinterpret_cast<int4*>(static_cast<char*>(ws) + r.o_bytes + r.ml_bytes);
+    a.n_items = (int)r.items;
+    a.target = kRowsTarget;
+    a.least = r.splits ? kRowsLeast : 1000000000;
+    a.rt_max = r.rt_max;
+    a.lo_rows = 0;
+    a.hi_rows = 0x7fffffff;
+    (void)hipGetLastError();
+    const bool i8 = p->store == LMXP_I8, f32 = dt == LMX_F32;
+    auto go = [&](auto tag) {
+        constexpr int HD = decltype(tag)::value;
+        if (i8) return f32 ? launch_rows<HD, true, true>(a, r, st) : launch_rows<HD, true, false>(a, r, st);
+        return f32 ? launch_rows<HD, false, true>(a, r, st) : launch_rows<HD, false, false>(a, r, st);
+    };
+    switch (p->head_dim) {
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 128: return go(std::integral_constant<int, 128>{});
+        case 256: return go(std::integral_constant<int, 256>{});
+        default: return go(std::integral_constant<int, 512>{});
+    }
+}
+
+}  // namespace lmx

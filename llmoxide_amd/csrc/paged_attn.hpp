@@ -1,0 +1,128 @@
+// Attention over pages: what its kernels share.
+#pragma once
+
+#include "paged.hpp"
+
+namespace lmx {
+
+struct AttnPagedArgs {
+    PagedArgs p;
+    const void* q;
+    void* out;
+    size_t q_row_stride, q_head_stride;
+    float c;              // scale * log2(e)
+    float* part_o;        // [items][bm][hd]   partial outputs, unnormalised
+    float* part_ml;       // [items][bm][2]    (reference exponent, sum)
+    int4* rows;           // [n_seq][Hkv][rt_max]  (first item, item stride, splits, 0)
+    int n_items;          // workgroups, and slots in part_o
+    int target;           // items aimed at where splits help
+    int least;            // units a split has at least
+    int rt_max;           // entries of `rows` a (sequence, head)
+    int lo_rows, hi_rows; // this kernel takes sequences with lo_rows < rows * G <= hi_rows
+};
+
+// One work item: a row tile of one sequence and kv head, over one split.
+struct Item {
+    int b, tile, h, split, splits;
+    int first, stride;  // item index of split 0, and from one split to the next
+    PagedSeq s;
+    SeqWork w;
+    int per;
+};
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = __lane_id();
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d, 64);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+
+// Sequence b's rows and work; no work where it has none or another kernel's
+// share of them.
+__device__ __forceinline__ void load_work(const AttnPagedArgs& a, int b, int bm, PagedSeq& s, SeqWork& w) {
+    s = PagedSeq{0, 0, 0};
+    w = SeqWork{0, 0, 0};
+    if (b < a.p.g.n_seq) {
+        s = paged_seq(a.p.g, a.p.cu[b], a.p.cu[b + 1], a.p.ctx[b]);
+        w = seq_work(a.p.g, s, bm);
+        const int64_t rows = (int64_t)s.n * a.p.g.G;
+        if (rows <= a.lo_rows || rows > a.hi_rows) w.rt = 0;
+    }
+}
+
+// Item `id` of the batch, by every wave for itself: the lengths are read from
+// the device in the call, so a replayed graph splits by the lengths of that
+// replay.  Each lane takes a sequence (64 at a time); the total of units x
+// row tiles decides how long a split is, a scan over the sequences' item
+// counts finds the one that holds `id`.  False: no such item.
+__device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm, bool splits_on, Item& o) {
+    const int lane = __lane_id(), Hkv = a.p.g.Hkv;
+    PagedSeq s;
+    SeqWork w;
+    load_work(a, lane, bm, s, w);
+    o.per = 1000000000;
+    if (splits_on) {
+        float work = (float)w.rt * (float)w.units;
+        for (int c0 = 64; c0 < a.p.g.n_seq; c0 += 64) {
+            PagedSeq s2;
+            SeqWork w2;
+            load_work(a, c0 + lane, bm, s2, w2);
+            work += (float)w2.rt * (float)w2.units;
+        }
+        o.per = units_per_split(wave_sum64(work) * (float)Hkv, a.target, a.least);
+    }
+    int base = 0;
+    for (int c0 = 0;; ) {
+        const int n = w.rt * Hkv * seq_splits(w, o.per);
+        const int upto = a.p.g.n_seq == 1 ? n : wave_scan(n);
+        const uint64_t has = __ballot(base + upto > id);
+        if (has) {
+            const int l = __builtin_ctzll(has);
+            auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            o.b = c0 + l;
+            o.s = PagedSeq{get(s.row0), get(s.n), get(s.ctx)};
+            o.w = SeqWork{get(w.rt), get(w.lo), get(w.units)};
+            o.splits = seq_splits(o.w, o.per);
+            const int first = base + get(upto) - get(n);
+            // item order within a sequence: split, then row tile, then kv head
+            // (with 8 heads every XCD keeps to one, and the row tiles that
+            // share its keys meet in that XCD's L2)
+            const int i = id - first;
+            o.h = i % Hkv;
+            o.tile = (i / Hkv) % o.w.rt;
+            o.split = i / Hkv / o.w.rt;
+            o.first = first + o.tile * Hkv + o.h;
+            o.stride = Hkv * o.w.rt;
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+        c0 += 64;
+        if (c0 >= a.p.g.n_seq) return false;
+        load_work(a, c0 + lane, bm, s, w);
+    }
+}
+
+// Two int8 words -> f16: x's bytes 0, 1 (lo) and 2, 3 (hi) as f16 pairs.  A
+// byte b + 128 set under 0x6400 is the f16 1024 + b + 128: exact, so is the
+// difference.
+__device__ __forceinline__ void i8x4_to_f16(uint32_t x, f16x2& lo, f16x2& hi) {
+    x ^= 0x80808080u;
+    const uint32_t a = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+    const f16x2 k = {(f16)1152.f, (f16)1152.f};
+    lo = __builtin_bit_cast(f16x2, a) - k;
+    hi = __builtin_bit_cast(f16x2, b) - k;
+}
+// Eight int8 in two words as eight f16.
+__device__ __forceinline__ f16x8 i8x8_to_f16(uint32_t x, uint32_t y) {
+    f16x2 a, b, c, d;
+    i8x4_to_f16(x, a, b);
+    i8x4_to_f16(y, c, d);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+}  // namespace lmx

@@ -13,6 +13,8 @@
 use std::ffi::{c_char, c_void, CStr};
 use std::fmt;
 
+pub mod paged;
+
 /// `lmx_stream`: binary-compatible with `hipStream_t`.
 pub type HipStream = *mut c_void;
 
