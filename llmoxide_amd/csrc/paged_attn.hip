@@ -17,8 +17,9 @@
 // Softmax: one running reference m per row (log2 units), taken from the first
 // tile and moved only when a score passes it by 2^4; weights are
 // exp2(s - m + 10) <= 2^14, so f16 holds them, with a residual in a second f16
-// (22 bits together); sums are fp32.  An 8-bit V's scale joins the weight,
-// brought near 1 by a power of two common to the wave.
+// (22 bits together); sums are fp32.  An 8-bit V's scale joins the exponent as
+// its logarithm, and the sum divides it out again, so that what f16 holds are
+// the weights that V's integers meet, row by row.
 #include <algorithm>
 
 #include "paged_attn.hpp"
@@ -43,32 +44,6 @@ __device__ __forceinline__ float sum_groups(float x) {
     x += shfl_xor(x, 16);
     return x + shfl_xor(x, 32);
 }
-
-// The halves of two f16 that are infinite or NaN, and the word without them.
-__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
-    const uint32_t e = x & 0x7c007c00u;
-    return ((e & 0xffffu) == 0x7c00u ? 0xffffu : 0u) | ((e >> 16) == 0x7c00u ? 0xffff0000u : 0u);
-}
-__device__ __forceinline__ uint32_t finite2(uint32_t x) { return x & ~nonfinite2(x); }
-
-// The page of every 16-key granule of a wave's key range, 64 table entries at
-// a time in the wave's lanes, so that the loop's lookups wait on no memory.
-struct PageWindow {
-    const int32_t* row;  // the sequence's table
-    int first;           // entry in lane 0
-    int ids;             // the lane's page, -1: none
-    __device__ __forceinline__ void fill(const PagedArgs& a, int entry) {
-        first = entry;
-        const int e = entry + (int)__lane_id();
-        ids = e < a.g.table_stride ? paged_page(a.g, row[e]) : -1;
-    }
-    // Page of key k (wave-uniform, >= 0).
-    __device__ __forceinline__ int at(const PagedArgs& a, int k) {
-        const int e = k >> a.g.ps_log2;
-        if (e - first >= 64) fill(a, e);
-        return __builtin_amdgcn_readlane(ids, e - first);
-    }
-};
 
 template <int HD, bool I8>
 struct Tile {
@@ -228,7 +203,6 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // m: reference exponent less kLift; -inf: nothing seen yet
-    float vref = 0.f;              // I8: weights carry v_scale * vref (a power of two); 0: not set
 
     PageWindow pw;
     pw.row = a.p.table + (size_t)it.b * pg.table_stride;
@@ -267,8 +241,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
                     if constexpr (F32) s[j] = mfma16(kf, ql[k], s[j]);
                 }
             }
-            if constexpr (I8) s[j] *= t.ks[j];
-            s[j] *= qscale;
+            if constexpr (I8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[j][i] = fmaf(s[j][i] * t.ks[j][i], qscale, __builtin_amdgcn_logf(v_scale_of(t.vs[j][i])));
+            } else {
+                s[j] *= qscale;
+            }
         }
         // ---- mask: keys behind the row, before its window, in no page
         constexpr int QUART = T::KEYS / 4;
@@ -309,40 +288,16 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
         // ---- weights
         const float ms = m == -INFINITY ? 0.f : m;
         f16x8 ph[T::NB / 2], pl[T::NB / 2];
-        float vmul[I8 ? T::NB : 1][4];
-        if constexpr (I8) {
-            // bring the largest scale of the tile's keys near 1; a larger one
-            // than before rescales what is there
-            float big = 0.f;
-#pragma unroll
-            for (int j = 0; j < T::NB; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool on = seen >> (4 * j + i) & 1;
-                    if (on && t.vs[j][i] < INFINITY) big = fmaxf(big, t.vs[j][i]);
-                }
-            if (__ballot(big * vref > 1.f || (vref == 0.f && big > 0.f))) {
-#pragma unroll
-                for (int x = 1; x < 64; x <<= 1) big = fmaxf(big, shfl_xor(big, x));
-                // big * nref in (1/4, 1/2]: room for a doubling before the next rescale
-                const float nref = ldexpf(1.f, imin(imax(-1 - __builtin_amdgcn_frexp_expf(big), -120), 120));
-                const float f = vref == 0.f ? 0.f : nref / vref;
-                vref = nref;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= f;
-            }
-        }
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < T::NB; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float p = fast_exp2(s[j][i] - ms);
-                sum += p;
-                if constexpr (I8) {
-                    const bool on = seen >> (4 * j + i) & 1;
-                    p = on ? p * (t.vs[j][i] * vref) : 0.f;
-                }
+                const float p = fast_exp2(s[j][i] - ms);
+                if constexpr (I8)
+                    sum += seen >> (4 * j + i) & 1 ? p * __builtin_amdgcn_rcpf(v_scale_of(t.vs[j][i])) : 0.f;
+                else
+                    sum += p;
                 const int at = 4 * (j & 1) + i;
                 ph[j >> 1][at] = (f16)p;
                 pl[j >> 1][at] = (f16)(p - (float)(f16)p);
@@ -441,11 +396,6 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
 
     // ---- join the four waves
     l = sum_groups(l);
-    if constexpr (I8) {
-        const float back = vref == 0.f ? 0.f : 1.f / vref;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= back;
-    }
     float* const ex_m = reinterpret_cast<float*>(smem);  // [4][16]
     float* const ex_l = ex_m + 64;                       // [4][16]
     float* const ex_o = ex_m + 128;                      // [4][16][OP]
@@ -489,22 +439,23 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
     }
 }
 
-// Joins the splits of one query row: a workgroup for each (sequence, kv head,
-// row of that sequence), HD/4 columns x 1024/HD groups of splits.
+// Joins the splits of one query row: HD/4 columns x 1024/HD groups of splits.
+// A workgroup for each row that a row tile can have (`rows` of them; tiles in
+// find_item's order with one split each).
 template <int HD, bool F32>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int bm) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int bm, int rows) {
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int C4 = HD / 4, NG = 256 / C4;
     __shared__ f32x4 ex[NG][C4];
     __shared__ float ex_m[NG], ex_l[NG];
     const PagedGeom& pg = a.p.g;
-    const int n_rows = pg.max_new * pg.G;
-    const int row = blockIdx.x % n_rows, bh = blockIdx.x / n_rows, b = bh / pg.Hkv, h = bh % pg.Hkv, tile = row / bm;
-    const int4 info = a.rows[((size_t)b * pg.Hkv + h) * a.rt_max + tile];
-    PagedSeq s;
-    SeqWork w;
-    load_work(a, b, bm, s, w);
-    if (tile >= w.rt || row >= s.n * pg.G) return;
+    Item it;
+    if (!find_item(a, blockIdx.x / rows, bm, false, it)) return;
+    const PagedSeq& s = it.s;
+    const int h = it.h, row = it.tile * bm + blockIdx.x % rows;
+    if (row >= s.n * pg.G || it.tile >= a.rt_max) return;
+    const int4 info = a.rows[((size_t)it.b * pg.Hkv + h) * a.rt_max + it.tile];
+    // written by this call's split 0; in range whatever it holds
     const int splits = imin(info.z, a.n_items);
     if (splits <= 1) return;
     const int col = threadIdx.x % C4, grp = threadIdx.x / C4;
@@ -566,42 +517,98 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
 }
 
 // ------------------------------------------------------------------- host --
-constexpr int kRowsTarget = 512;  // items aimed at: two workgroups a CU
-constexpr int kRowsLeast = 2;     // units a split has at least (128 keys)
+constexpr int kRowsTarget = 512;   // items aimed at: two workgroups a CU
+constexpr int kRowsLeast = 2;      // units a split has at least (128 keys)
+constexpr int kChunkTarget = 512;
+constexpr int kChunkLeast = 8;
+// Query rows a sequence may have per kv head for the rows kernel.
+constexpr int kRowsMost = 32;
 
-struct RowsPlan {
-    int64_t items;   // workgroups, an upper bound of the batch's items
-    int rt_max;
+// One kernel's share of a call.
+struct Part {
+    bool on, splits;
+    int bm, lo_rows, hi_rows, target, least, rt_max;
+    int64_t items;  // workgroups: an upper bound of its items
     size_t o_bytes, ml_bytes, rows_bytes;
-    bool splits;
+    size_t bytes() const { return o_bytes + ml_bytes + rows_bytes; }
 };
-static RowsPlan rows_plan(const PagedGeom& g, int hd) {
-    RowsPlan r;
-    const int64_t tiles = row_tiles_bound(g, kBM) * g.Hkv;
-    // A single split reaches every key of a short call: no partials then.
-    r.splits = g.max_ctx > kRowsLeast * kUnit;
-    r.items = tiles + (r.splits ? kRowsTarget : 0);
-    r.rt_max = (int)(((int64_t)g.max_new * g.G + kBM - 1) / kBM);
-    r.o_bytes = r.splits ? (size_t)r.items * kBM * hd * 4 : 0;
-    r.ml_bytes = r.splits ? (size_t)r.items * kBM * 8 : 0;
-    r.rows_bytes = (size_t)g.n_seq * g.Hkv * r.rt_max * 16;
+static Part make_part(const PagedGeom& g, int hd, int bm, int64_t tiles, int64_t seq_rows, bool splits, int target, int least) {
+    Part r{};
+    r.on = true;
+    r.bm = bm;
+    r.splits = splits && g.max_ctx > least * kUnit;  // else a single split reaches every key
+    r.target = target;
+    r.least = r.splits ? least : 1000000000;
+    r.items = tiles * g.Hkv + (r.splits ? target : 0);
+    r.rt_max = (int)((seq_rows + bm - 1) / bm);
+    r.o_bytes = r.splits ? (size_t)r.items * bm * hd * 4 : 0;
+    r.ml_bytes = r.splits ? (size_t)r.items * bm * 8 : 0;
+    r.rows_bytes = r.splits ? ((size_t)g.n_seq * g.Hkv * r.rt_max * 16) : 0;
+    r.hi_rows = 0x7fffffff;
     return r;
+}
+struct Plan {
+    Part rows, chunk;
+};
+static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
+    Plan p{};
+    const int64_t most = (int64_t)g.max_new * g.G;  // rows of a sequence
+    const int cm = chunk_rows(hd, i8, f32);
+    const bool chunks = cm && most > kRowsMost;
+    if (!chunks || g.n_seq > 1) {
+        const int64_t seq_rows = chunks ? kRowsMost : most;
+        int64_t tiles = row_tiles_bound(g, kBM);
+        if (chunks) tiles = std::min<int64_t>(tiles, (int64_t)g.n_seq * ((kRowsMost + kBM - 1) / kBM));
+        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, kRowsTarget, kRowsLeast);
+        if (chunks) p.rows.hi_rows = kRowsMost;
+    }
+    if (chunks) {
+        const int64_t tiles = row_tiles_bound(g, cm);
+        p.chunk = make_part(g, hd, cm, tiles, most, tiles * g.Hkv < kChunkTarget, kChunkTarget, kChunkLeast);
+        if (p.rows.on) p.chunk.lo_rows = kRowsMost;
+    }
+    return p;
 }
 
 size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
     PagedGeom g = paged_args(p, b).g;
     g.G = (int)(d->n_heads / p->n_kv_heads);
-    const RowsPlan r = rows_plan(g, (int)p->head_dim);
-    return r.o_bytes + r.ml_bytes + r.rows_bytes;
+    size_t most = 0;
+    for (bool f32 : {false, true}) {
+        const Plan pl = make_plan(g, (int)p->head_dim, p->store == LMXP_I8, f32);
+        most = std::max(most, pl.rows.bytes() + pl.chunk.bytes());
+    }
+    return most;
 }
 
-template <int HD, bool I8, bool F32>
-static lmx_status launch_rows(const AttnPagedArgs& a, const RowsPlan& r, hipStream_t st) {
-    hipLaunchKernelGGL((paged_rows_kernel<HD, I8, F32>), dim3((unsigned)r.items), dim3(256), 0, st, a);
+template <int HD>
+static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i8, bool f32, char* ws, hipStream_t st) {
+    if (!r.on) return LMX_OK;
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + r.o_bytes);
+    a.rows = reinterpret_cast<int4*>(ws + r.o_bytes + r.ml_bytes);
+    a.n_items = (int)r.items;
+    a.target = r.target;
+    a.least = r.least;
+    a.rt_max = r.splits ? r.rt_max : 0;
+    a.lo_rows = r.lo_rows;
+    a.hi_rows = r.hi_rows;
+    const dim3 grid((unsigned)r.items);
+    if (chunk) {
+        launch_chunk(a, HD, i8, f32, grid.x, st);
+    } else if (i8) {
+        if (f32) hipLaunchKernelGGL((paged_rows_kernel<HD, true, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((paged_rows_kernel<HD, true, false>), grid, dim3(256), 0, st, a);
+    } else {
+        if (f32) hipLaunchKernelGGL((paged_rows_kernel<HD, false, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((paged_rows_kernel<HD, false, false>), grid, dim3(256), 0, st, a);
+    }
     LMX_CHECK_LAUNCH();
     if (r.splits) {
-        const unsigned rows = (unsigned)(a.p.g.max_new * a.p.g.G) * (unsigned)(a.p.g.n_seq * a.p.g.Hkv);
-        hipLaunchKernelGGL((paged_merge_kernel<HD, F32>), dim3(rows), dim3(256), 0, st, a, kBM);
+        const int rows = (int)std::min<int64_t>(r.bm, (int64_t)a.p.g.max_new * a.p.g.G);
+        const dim3 mgrid((unsigned)(r.items - r.target) * (unsigned)rows);
+        if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+        else hipLaunchKernelGGL((paged_merge_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm, rows);
         LMX_CHECK_LAUNCH();
     }
     return LMX_OK;
@@ -618,22 +625,13 @@ lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_d
     a.q_head_stride = d->q_head_stride ? d->q_head_stride : p->head_dim;
     a.q_row_stride = d->q_row_stride ? d->q_row_stride : a.q_head_stride * d->n_heads;
     a.c = d->scale * kLog2e;
-    const RowsPlan r = rows_plan(a.p.g, (int)p->head_dim);
-    a.part_o = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + r.o_bytes);
-    a.rows = reinterpret_cast<int4*>(static_cast<char*>(ws) + r.o_bytes + r.ml_bytes);
-    a.n_items = (int)r.items;
-    a.target = kRowsTarget;
-    a.least = r.splits ? kRowsLeast : 1000000000;
-    a.rt_max = r.rt_max;
-    a.lo_rows = 0;
-    a.hi_rows = 0x7fffffff;
-    (void)hipGetLastError();
     const bool i8 = p->store == LMXP_I8, f32 = dt == LMX_F32;
+    const Plan pl = make_plan(a.p.g, (int)p->head_dim, i8, f32);
+    (void)hipGetLastError();
     auto go = [&](auto tag) {
         constexpr int HD = decltype(tag)::value;
-        if (i8) return f32 ? launch_rows<HD, true, true>(a, r, st) : launch_rows<HD, true, false>(a, r, st);
-        return f32 ? launch_rows<HD, false, true>(a, r, st) : launch_rows<HD, false, false>(a, r, st);
+        const lmx_status s = launch_part<HD>(a, pl.chunk, true, i8, f32, static_cast<char*>(ws) + pl.rows.bytes(), st);
+        return s != LMX_OK ? s : launch_part<HD>(a, pl.rows, false, i8, f32, static_cast<char*>(ws), st);
     };
     switch (p->head_dim) {
         case 64: return go(std::integral_constant<int, 64>{});

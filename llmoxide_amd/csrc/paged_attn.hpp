@@ -21,6 +21,10 @@ struct AttnPagedArgs {
     int lo_rows, hi_rows; // this kernel takes sequences with lo_rows < rows * G <= hi_rows
 };
 
+// paged_chunk.hip: rows of its workgroups (0: no kernel for this head_dim), and the launch.
+int chunk_rows(int hd, bool i8, bool f32);
+void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);
+
 // One work item: a row tile of one sequence and kv head, over one split.
 struct Item {
     int b, tile, h, split, splits;
@@ -93,9 +97,10 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
             // share its keys meet in that XCD's L2)
             const int i = id - first;
             o.h = i % Hkv;
-            o.tile = (i / Hkv) % o.w.rt;
+            const int at = (i / Hkv) % o.w.rt;
+            o.tile = o.w.rt - 1 - at;  // the last rows, which see the most keys, first
             o.split = i / Hkv / o.w.rt;
-            o.first = first + o.tile * Hkv + o.h;
+            o.first = first + at * Hkv + o.h;
             o.stride = Hkv * o.w.rt;
             return true;
         }
@@ -105,6 +110,17 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
         load_work(a, c0 + lane, bm, s, w);
     }
 }
+
+// The halves of two f16 that are infinite or NaN, and the word without them.
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
+    const uint32_t e = x & 0x7c007c00u;
+    return ((e & 0xffffu) == 0x7c00u ? 0xffffu : 0u) | ((e >> 16) == 0x7c00u ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t finite2(uint32_t x) { return x & ~nonfinite2(x); }
+
+// A V scale as the attention kernels use it: at least 2^-90 (which only values
+// below 1e-24 notice), so that its logarithm and reciprocal are finite.
+__device__ __forceinline__ float v_scale_of(float s) { return s < 0x1p-90f ? 0x1p-90f : s; }
 
 // Two int8 words -> f16: x's bytes 0, 1 (lo) and 2, 3 (hi) as f16 pairs.  A
 // byte b + 128 set under 0x6400 is the f16 1024 + b + 128: exact, so is the
@@ -124,5 +140,24 @@ __device__ __forceinline__ f16x8 i8x8_to_f16(uint32_t x, uint32_t y) {
     i8x4_to_f16(y, c, d);
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+
+// The page of every 16-key granule of a wave's key range, 64 table entries at
+// a time in the wave's lanes, so that the loop's lookups wait on no memory.
+struct PageWindow {
+    const int32_t* row;  // the sequence's table
+    int first;           // entry in lane 0
+    int ids;             // the lane's page, -1: none
+    __device__ __forceinline__ void fill(const PagedArgs& a, int entry) {
+        first = entry;
+        const int e = entry + (int)__lane_id();
+        ids = e < a.g.table_stride ? paged_page(a.g, row[e]) : -1;
+    }
+    // Page of key k (wave-uniform, >= 0).
+    __device__ __forceinline__ int at(const PagedArgs& a, int k) {
+        const int e = k >> a.g.ps_log2;
+        if (e - first >= 64) fill(a, e);
+        return __builtin_amdgcn_readlane(ids, e - first);
+    }
+};
 
 }  // namespace lmx

@@ -1,0 +1,460 @@
+// Attention of prompt chunks over pages on gfx950 (MFMA-bound).
+//
+// A workgroup takes a tile of 128 * RB query rows of one kv head (row r: token
+// r / G, head r % G, so that all heads of a group share the tile's keys) and
+// walks its 64-key tiles; four waves of 32 * RB rows share each K/V tile in
+// LDS.  As in the rows kernel the products are computed transposed,
+//   S^T = K Q^T, O^T += V^T P^T   on v_mfma_f32_32x32x16_f16,
+// Q^T in registers for the whole walk.  The keys that MFMA row r of a 32-key
+// block stands for are chosen so that a lane's scores are 8 consecutive keys
+// of each 16, the B operand of the second product; and V lies transposed in
+// the pages, so both A operands are 16-byte LDS reads and nothing is shuffled
+// or turned.  K rows and V columns sit in LDS in 16-byte chunks, chunk c of
+// row r at place c ^ (r & 7): eight neighbouring rows' chunks fall into
+// different banks.
+//
+// f16 pages go from memory straight to LDS (the chunk permutation is made on
+// the addresses that the lanes read); 8-bit pages go through registers, where
+// they become f16 (exact), and their scales stay apart: K's multiplies the
+// score, V's joins the exponent as its logarithm, and the sum divides it out
+// again: weights are then weighed against each other with it, row by row.
+#include <algorithm>
+
+#include "lds_dma.hpp"
+#include "paged_attn.hpp"
+
+namespace lmx {
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kBN = 64;  // keys a tile
+
+// Weights are exp2(arg), arg = score - m, with m kLift below the largest score
+// that set it; a tile with an arg above kLift + kSlack moves m.
+template <bool F32>
+struct Lift {
+    static constexpr float lift = F32 ? 10.f : 6.f, most = 14.f;
+};
+
+template <int HD, bool I8, bool F32, int RB>
+struct ChunkTile {
+    static constexpr int KS = HD / 16;   // k-steps of QK
+    static constexpr int NB = HD / 32;   // 32-dim blocks of the output
+    static constexpr int BM = 128 * RB;  // rows a workgroup
+    static constexpr int CH = HD / 8;    // 16-byte chunks of a K row
+    static constexpr int LOADS = HD / 32;  // 1 KB transfers a wave makes of a tile's K, and of its V
+    static constexpr int STAGE = 2 * kBN * HD;  // halfs: K then V
+};
+
+template <int HD, bool I8, bool F32, int RB, int OCC>
+__global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) {
+    using T = ChunkTile<HD, I8, F32, RB>;
+    using QT = std::conditional_t<F32, float, f16>;
+    constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH;
+    constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
+    __shared__ __align__(1024) f16 tiles[2][T::STAGE];
+    __shared__ __align__(16) float scales[I8 ? 2 : 1][3][kBN];  // K's, log2 of V's, 1 / V's
+
+    Item it;
+    if (!find_item(a, blockIdx.x, BM, true, it)) return;
+    const PagedGeom& pg = a.p.g;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hh = lane >> 5;
+    if (it.split == 0 && tid == 0 && it.tile < a.rt_max)
+        a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile] = make_int4(it.first, it.stride, it.splits, 0);
+
+    // ---- rows, and the keys they see
+    const int n_rows = it.s.n * pg.G, first_pos = it.s.ctx - it.s.n;
+    const int r0 = it.tile * BM, r1 = imin(r0 + BM, n_rows) - 1;
+    auto pos_of = [&](int r) { return first_pos + r / pg.G; };
+    auto low_of = [&](int pos) { return pg.window ? imax(pos - pg.window + 1, 0) : 0; };
+    const int split_lo = it.splits > 1 ? it.w.lo + it.split * it.per * kUnit : it.w.lo;
+    const int split_hi = it.splits > 1 ? split_lo + it.per * kUnit : 0x7fffffff;
+    const int k_lo = imax(low_of(pos_of(r0)) & ~(kBN - 1), split_lo);
+    const int k_hi = imin(pos_of(r1) + 1, split_hi);  // one behind the last key
+    const int n_t = k_hi > k_lo ? (k_hi - k_lo + kBN - 1) / kBN : 0;
+    // the wave's: keys some row sees, keys all rows see
+    const int w0 = r0 + w * 32 * RB, w1 = imin(w0 + 32 * RB, n_rows) - 1;
+    const bool live = w0 <= r1;
+    const int any_hi = live ? pos_of(w1) : -1, all_hi = live ? pos_of(w0) : -1;
+    const int any_lo = live ? low_of(pos_of(w0)) : 0, all_lo = live ? low_of(pos_of(w1)) : 0;
+
+    int pos[RB], seen_lo[RB];
+    float qs[RB];  // what a score is multiplied by
+    f16x8 qh[RB][KS], ql[F32 ? RB : 1][F32 ? KS : 1];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = w0 + 32 * rb + l32;
+        const bool have = row < n_rows;
+        const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
+        pos[rb] = have ? first_pos + tok : -1;
+        seen_lo[rb] = low_of(pos[rb]);
+        qs[rb] = a.c;
+        const QT* qr = static_cast<const QT*>(a.q) + (size_t)(it.s.row0 + tok) * a.q_row_stride + head * a.q_head_stride + 8 * hh;
+        if constexpr (F32) {
+            float m = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                float x[8];
+                load_f32<8>(qr + 16 * k, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+            }
+            m = fmaxf(m, shfl_xor(m, 32));
+            int e = 0;  // the row's largest element to [2^14, 2^15), as in the rows kernel
+            if (m > 0.f && m < INFINITY) e = 15 - __builtin_amdgcn_frexp_expf(m);
+            e = imin(imax(e, -120), 120);
+            const float up = ldexpf(1.f, e);
+            qs[rb] = ldexpf(a.c, -e);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                float x[8];
+                load_f32<8>(qr + 16 * k, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = have ? x[j] * up : 0.f;
+                    qh[rb][k][j] = (f16)y;
+                    ql[rb][k][j] = (f16)(y - (float)(f16)y);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                qh[rb][k] = *reinterpret_cast<const f16x8*>(qr + 16 * k);
+                if (!have) qh[rb][k] = f16x8{};
+            }
+        }
+    }
+
+    // ---- copies.  Granule j of a tile: its keys 16j .. 16j+15, in one page.
+    const int psm = (1 << pg.ps_log2) - 1;
+    PageWindow pw;
+    pw.row = a.p.table + (size_t)it.b * pg.table_stride;
+    pw.fill(a.p, k_lo >> pg.ps_log2);
+    int pages[4], next_pages[4];
+    auto look_up = [&](int t0, int (&p)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = pw.at(a.p, t0 + 16 * j);
+    };
+    auto slab = [&](int page) {  // positions of the pool before the page's
+        return ((size_t)imax(page, 0) * pg.Hkv + it.h) << pg.ps_log2;
+    };
+    uint4 rk[I8 ? HD / 64 : 1], rv[I8 ? HD / 64 : 1];
+    float rs = 0.f;
+    // f16: K, lane l of transfer i: chunk place (64 i + l) % CH of row (64 i + l) / CH of the
+    // wave's 16 rows; V: dims 8 a transfer, place l % 8 of dim l / 8.
+    auto fetch = [&](int t0, const int (&p)[4], int stage) {
+        if constexpr (!I8) {
+            const uint32_t lds = lds_addr(&tiles[stage][0]);
+            const int pk = w == 0 ? p[0] : w == 1 ? p[1] : w == 2 ? p[2] : p[3];
+            const char* kb = a.p.k + (slab(pk) + ((t0 + 16 * w) & psm)) * (HD * 2);
+            constexpr int RPT = 64 / CH;  // rows a transfer
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) {
+                const int r = i * RPT + lane / CH;  // of the wave's 16
+                const uint32_t off = r * (HD * 2) + (((lane % CH) ^ (r & 7)) * 16);
+                dma16(kb, off, lds + (w * 16 * HD * 2) + i * 1024);
+            }
+            const int d8 = lane >> 3, c = (lane & 7) ^ d8;  // dim within the transfer's 8, chunk
+            const int j = c >> 1;
+            const int pv = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+            const char* vb = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm)) * 2;
+            const int dw = w * (HD / 4) + d8;
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i)
+                dma16_lane(vb + ((size_t)(dw + 8 * i) << (pg.ps_log2 + 1)),
+                           lds + kBN * HD * 2 + (w * (HD / 4) + 8 * i) * 128);
+        } else {
+            // K: 16 dims of a key a load; V: the 16 keys of a granule of one dim
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) {
+                const int x = tid + 256 * i, key = x / (HD / 16), c = x % (HD / 16), j = key >> 4;
+                const int pk = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+                rk[i] = *reinterpret_cast<const uint4*>(a.p.k + (slab(pk) + ((t0 + key) & psm)) * HD + 16 * c);
+                const int dim = x >> 2, g = x & 3;
+                const int pv = g == 0 ? p[0] : g == 1 ? p[1] : g == 2 ? p[2] : p[3];
+                rv[i] = *reinterpret_cast<const uint4*>(a.p.v + slab(pv) * HD + ((size_t)dim << pg.ps_log2) + ((t0 + 16 * g) & psm));
+            }
+            const int key = lane, j = lane >> 4;
+            const int pk = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+            if (w < 2) rs = (w ? a.p.v_scale : a.p.k_scale)[slab(pk) + ((t0 + key) & psm)];
+        }
+    };
+    auto stash = [&](int stage) {  // 8-bit tiles: registers to LDS as f16
+        if constexpr (I8) {
+            f16* Ks = tiles[stage];
+            f16* Vs = tiles[stage] + kBN * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) {
+                const int x = tid + 256 * i, key = x / (HD / 16), c = 2 * (x % (HD / 16));
+                *reinterpret_cast<f16x8*>(&Ks[key * HD + ((c ^ (key & 7)) * 8)]) = i8x8_to_f16(rk[i].x, rk[i].y);
+                *reinterpret_cast<f16x8*>(&Ks[key * HD + (((c + 1) ^ (key & 7)) * 8)]) = i8x8_to_f16(rk[i].z, rk[i].w);
+                const int dim = x >> 2, g = 2 * (x & 3);
+                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + ((g ^ (dim & 7)) * 8)]) = i8x8_to_f16(rv[i].x, rv[i].y);
+                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + (((g + 1) ^ (dim & 7)) * 8)]) = i8x8_to_f16(rv[i].z, rv[i].w);
+            }
+            if (w == 0) scales[stage][0][lane] = rs;
+            if (w == 1) {
+                const float v = v_scale_of(rs);
+                scales[stage][1][lane] = __builtin_amdgcn_logf(v);
+                scales[stage][2][lane] = 1.f / v;
+            }
+        }
+    };
+
+    f32x16 o[RB][NB];
+    float m[RB], l[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        m[rb] = pos[rb] < 0 ? 0.f : -INFINITY;
+        l[rb] = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[rb][nb][i] = 0.f;
+    }
+    bool poison = false;
+
+    // MFMA row l32 of a 32-key block stands for this key of it
+    const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
+
+    auto compute = [&](int t0, const int (&p)[4], int stage) {
+        const f16* Ks = tiles[stage];
+        const f16* Vs = tiles[stage] + kBN * HD;
+        f32x16 s[RB][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[rb][kb][i] = 0.f;
+            const f16* kr = &Ks[(32 * kb + krow) * HD];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(&kr[((2 * k + hh) ^ (krow & 7)) * 8]);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    s[rb][kb] = mfma32(kf, qh[rb][k], s[rb][kb]);
+                    if constexpr (F32) s[rb][kb] = mfma32(kf, ql[rb][k], s[rb][kb]);
+                }
+            }
+        }
+        bool whole = t0 + kBN - 1 <= all_hi && t0 >= all_lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) whole = whole && p[j] >= 0;
+        // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
+        f16x8 ph[RB][4], pl[F32 ? RB : 1][F32 ? 4 : 1];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float mb = m[rb] == -INFINITY ? 0.f : m[rb];
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {  // four registers: keys 32 kb + 16 (q/2) + 8 hh + 4 (q%2) ..
+                    f32x4 ks, lv;
+                    if constexpr (I8) {
+                        const int at = 32 * kb + 16 * (q >> 1) + 8 * hh + 4 * (q & 1);
+                        ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][at]);
+                        lv = *reinterpret_cast<const f32x4*>(&scales[stage][1][at]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = s[rb][kb][4 * q + e];
+                        if constexpr (I8)
+                            s[rb][kb][4 * q + e] = fmaf(x * ks[e], qs[rb], lv[e] - mb);
+                        else
+                            s[rb][kb][4 * q + e] = fmaf(x, qs[rb], -mb);
+                    }
+                }
+            if (!whole) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = t0 + 32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7);
+                        const bool on = p[2 * kb + (i >> 3)] >= 0 && key <= pos[rb] && key >= seen_lo[rb];
+                        if (!on) s[rb][kb][i] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rb][kb][i]);
+            if (__ballot(top > kMost || m[rb] == -INFINITY)) {
+                top = fmaxf(top, shfl_xor(top, 32));
+                float mn = m[rb];
+                if (mn == -INFINITY)
+                    mn = top > -INFINITY ? top - kLift : -INFINITY;  // mb = 0
+                else if (top > kMost)
+                    mn = mb + top - kLift;
+                const float f = m[rb] == -INFINITY ? 0.f : fast_exp2(m[rb] - mn);
+                const float delta = mn == -INFINITY ? 0.f : mn - mb;
+                m[rb] = mn;
+                l[rb] *= f;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) o[rb][nb] *= f;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) s[rb][kb] -= delta;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = fast_exp2(s[rb][kb][i]), p1 = fast_exp2(s[rb][kb][i + 1]);
+                    const f16x2 hi = {(f16)p0, (f16)p1};
+                    ph[rb][2 * kb + (i >> 3)][i & 7] = hi[0];
+                    ph[rb][2 * kb + (i >> 3)][(i & 7) + 1] = hi[1];
+                    if constexpr (F32) {
+                        pl[rb][2 * kb + (i >> 3)][i & 7] = (f16)(p0 - (float)hi[0]);
+                        pl[rb][2 * kb + (i >> 3)][(i & 7) + 1] = (f16)(p1 - (float)hi[1]);
+                    }
+                    if constexpr (I8) {
+                        const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
+                        sum += p0 > 0.f || !(p0 == 0.f) ? p0 * iv[0] : 0.f;
+                        sum += p1 > 0.f || !(p1 == 0.f) ? p1 * iv[1] : 0.f;
+                    } else if constexpr (F32) {
+                        sum += p0 + p1;
+                    } else {
+                        sum = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, sum, false);
+                    }
+                }
+            l[rb] += sum;
+        }
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const int dim = 32 * nb + l32;
+                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * 64 + (((2 * st + hh) ^ (dim & 7)) * 8)]);
+                if constexpr (!I8) {
+                    if (!whole) {  // see the rows kernel: infinities and NaN that not all rows see
+                        uint4 u = __builtin_bit_cast(uint4, vf);
+                        const uint32_t bad = nonfinite2(u.x) | nonfinite2(u.y) | nonfinite2(u.z) | nonfinite2(u.w);
+                        if (__ballot(bad != 0)) poison = true;
+                        u = uint4{finite2(u.x), finite2(u.y), finite2(u.z), finite2(u.w)};
+                        vf = __builtin_bit_cast(f16x8, u);
+                    }
+                }
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    o[rb][nb] = mfma32(vf, ph[rb][st], o[rb][nb]);
+                    if constexpr (F32) o[rb][nb] = mfma32(vf, pl[rb][st], o[rb][nb]);
+                }
+            }
+    };
+
+    if (n_t > 0) {
+        look_up(k_lo, pages);
+        fetch(k_lo, pages, 0);
+        stash(0);
+        for (int t = 0; t < n_t; ++t) {
+            const int t0 = k_lo + t * kBN;
+            if constexpr (!I8) wait_dma<0>();
+            __syncthreads();
+            if (t + 1 < n_t) {
+                look_up(t0 + kBN, next_pages);
+                fetch(t0 + kBN, next_pages, (t + 1) & 1);
+            }
+            if (t0 <= any_hi && t0 + kBN - 1 >= any_lo) compute(t0, pages, t & 1);
+            if (t + 1 < n_t) stash((t + 1) & 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pages[j] = next_pages[j];
+        }
+    }
+
+    // ---- results
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = w0 + 32 * rb + l32;
+        if constexpr (!I8) {
+            float z = 0.f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z = fmaf(o[rb][nb][i], 0.f, z);
+            if (poison || __ballot(z != 0.f)) {
+                // rare, as in the rows kernel: V's infinities and NaN go to the rows that see them
+                const size_t step = (size_t)1 << pg.ps_log2;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    f32x16 add;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) add[i] = 0.f;
+                    pw.fill(a.p, k_lo >> pg.ps_log2);
+                    for (int key = k_lo; key < k_hi; ++key) {
+                        const int page = pw.at(a.p, key);
+                        if (page < 0 || key > pos[rb] || key < seen_lo[rb]) continue;
+                        const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
+                                       ((32 * nb + 4 * hh) << pg.ps_log2);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float y = (float)*e;
+                            if (!(fabsf(y) < INFINITY)) add[i] += y;
+                            e += (i & 3) < 3 ? step : 5 * step;  // dims 32 nb + 8 (i/4) + 4 hh + i%4
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!(fabsf(add[i]) < INFINITY)) o[rb][nb][i] = add[i];
+                }
+            }
+        }
+        float sum = l[rb] + shfl_xor(l[rb], 32);
+        if (row >= n_rows) continue;
+        if (it.splits > 1) {
+            const size_t at = (size_t)(it.first + it.split * it.stride) * BM + (row - r0);
+            float* dst = a.part_o + at * HD;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
+                        f32x4{o[rb][nb][4 * q], o[rb][nb][4 * q + 1], o[rb][nb][4 * q + 2], o[rb][nb][4 * q + 3]};
+            if (hh == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m[rb], sum};
+        } else {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            QT* dst = static_cast<QT*>(a.out) +
+                      ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 y = f32x4{o[rb][nb][4 * q], o[rb][nb][4 * q + 1], o[rb][nb][4 * q + 2], o[rb][nb][4 * q + 3]} * inv;
+                    if constexpr (F32)
+                        *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) = y;
+                    else
+                        *reinterpret_cast<f16x4*>(dst + 32 * nb + 8 * q + 4 * hh) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+                }
+        }
+    }
+}
+
+// What the launch in paged_attn.hip picks from: rows a workgroup, 0 where
+// head_dim has no chunk kernel.
+template <int HD, bool I8, bool F32>
+constexpr int chunk_rb() { return HD == 64 ? 2 : HD == 128 ? 2 : 1; }
+template <int HD, bool I8, bool F32>
+constexpr int chunk_occ() { return HD <= 128 && chunk_rb<HD, I8, F32>() == 1 && !F32 ? 2 : 1; }
+
+int chunk_rows(int hd, bool, bool) { return hd == 64 ? 256 : hd == 128 ? 128 * 2 : hd == 256 ? 128 : 0; }
+
+template <int HD, bool I8, bool F32>
+static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb<HD, I8, F32>(), chunk_occ<HD, I8, F32>()>), dim3(items), dim3(256), 0, st, a);
+}
+void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
+    auto by = [&](auto tag) {
+        constexpr int HD = decltype(tag)::value;
+        if (i8) f32 ? go_chunk<HD, true, true>(a, items, st) : go_chunk<HD, true, false>(a, items, st);
+        else f32 ? go_chunk<HD, false, true>(a, items, st) : go_chunk<HD, false, false>(a, items, st);
+    };
+    if (hd == 64) by(std::integral_constant<int, 64>{});
+    else if (hd == 128) by(std::integral_constant<int, 128>{});
+    else by(std::integral_constant<int, 256>{});
+}
+
+}  // namespace lmx
