@@ -111,12 +111,13 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
     }
 }
 
-// The halves of two f16 that are infinite or NaN, and the word without them.
-__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
-    const uint32_t e = x & 0x7c007c00u;
-    return ((e & 0xffffu) == 0x7c00u ? 0xffffu : 0u) | ((e >> 16) == 0x7c00u ? 0xffff0000u : 0u);
+// Two f16 in a word: the sign bit of each half that is infinite or NaN (an
+// exponent of all ones carries into it), and the word without those halves.
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) { return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+    const uint32_t m = nonfinite2(x);
+    return x & ~(m | (m - (m >> 15)));
 }
-__device__ __forceinline__ uint32_t finite2(uint32_t x) { return x & ~nonfinite2(x); }
 
 // A V scale as the attention kernels use it: at least 2^-90 (which only values
 // below 1e-24 notice), so that its logarithm and reciprocal are finite.

@@ -9,9 +9,9 @@
 // block stands for are chosen so that a lane's scores are 8 consecutive keys
 // of each 16, the B operand of the second product; and V lies transposed in
 // the pages, so both A operands are 16-byte LDS reads and nothing is shuffled
-// or turned.  K rows and V columns sit in LDS in 16-byte chunks, chunk c of
-// row r at place c ^ (r & 7): eight neighbouring rows' chunks fall into
-// different banks.
+// or turned.  K rows and V columns sit in LDS in 16-byte chunks, those of row
+// r permuted by an XOR with swizzle(r): what 16 neighbouring rows have at one
+// chunk then covers the 64 banks once.
 //
 // f16 pages go from memory straight to LDS (the chunk permutation is made on
 // the addresses that the lanes read); 8-bit pages go through registers, where
@@ -37,6 +37,11 @@ template <bool F32>
 struct Lift {
     static constexpr float lift = F32 ? 10.f : 6.f, most = 14.f;
 };
+
+// Place of row r's chunk c is c ^ swizzle(r): rows of 256 bytes and more start
+// at the same bank, of rows of 128 bytes every other one does.
+template <int ROW_BYTES>
+__device__ __forceinline__ int swizzle(int r) { return ROW_BYTES >= 256 ? r & 15 : (r >> 1) & 7; }
 
 template <int HD, bool I8, bool F32, int RB>
 struct ChunkTile {
@@ -144,7 +149,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     uint4 rk[I8 ? HD / 64 : 1], rv[I8 ? HD / 64 : 1];
     float rs = 0.f;
     // f16: K, lane l of transfer i: chunk place (64 i + l) % CH of row (64 i + l) / CH of the
-    // wave's 16 rows; V: dims 8 a transfer, place l % 8 of dim l / 8.
+    // wave's 16 rows; V: 8 dims a transfer, place l % 8 of dim l / 8.
     auto fetch = [&](int t0, const int (&p)[4], int stage) {
         if constexpr (!I8) {
             const uint32_t lds = lds_addr(&tiles[stage][0]);
@@ -154,18 +159,21 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) {
                 const int r = i * RPT + lane / CH;  // of the wave's 16
-                const uint32_t off = r * (HD * 2) + (((lane % CH) ^ (r & 7)) * 16);
+                const uint32_t off = r * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
                 dma16(kb, off, lds + (w * 16 * HD * 2) + i * 1024);
             }
-            const int d8 = lane >> 3, c = (lane & 7) ^ d8;  // dim within the transfer's 8, chunk
-            const int j = c >> 1;
-            const int pv = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
-            const char* vb = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm)) * 2;
-            const int dw = w * (HD / 4) + d8;
+            // every other transfer's dims swap the halves of the tile's keys
+            const int d8 = lane >> 3, dw = w * (HD / 4) + d8;
+            const char* vb[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int c = (lane & 7) ^ swizzle<128>(8 * x + d8), j = c >> 1;
+                const int pv = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+                vb[x] = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm) + ((size_t)dw << pg.ps_log2)) * 2;
+            }
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i)
-                dma16_lane(vb + ((size_t)(dw + 8 * i) << (pg.ps_log2 + 1)),
-                           lds + kBN * HD * 2 + (w * (HD / 4) + 8 * i) * 128);
+                dma16_lane(vb[i & 1] + ((size_t)i << (pg.ps_log2 + 4)), lds + kBN * HD * 2 + (w * (HD / 4) + 8 * i) * 128);
         } else {
             // K: 16 dims of a key a load; V: the 16 keys of a granule of one dim
 #pragma unroll
@@ -189,11 +197,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 #pragma unroll
             for (int i = 0; i < HD / 64; ++i) {
                 const int x = tid + 256 * i, key = x / (HD / 16), c = 2 * (x % (HD / 16));
-                *reinterpret_cast<f16x8*>(&Ks[key * HD + ((c ^ (key & 7)) * 8)]) = i8x8_to_f16(rk[i].x, rk[i].y);
-                *reinterpret_cast<f16x8*>(&Ks[key * HD + (((c + 1) ^ (key & 7)) * 8)]) = i8x8_to_f16(rk[i].z, rk[i].w);
+                *reinterpret_cast<f16x8*>(&Ks[key * HD + ((c ^ swizzle<HD * 2>(key)) * 8)]) = i8x8_to_f16(rk[i].x, rk[i].y);
+                *reinterpret_cast<f16x8*>(&Ks[key * HD + (((c + 1) ^ swizzle<HD * 2>(key)) * 8)]) = i8x8_to_f16(rk[i].z, rk[i].w);
                 const int dim = x >> 2, g = 2 * (x & 3);
-                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + ((g ^ (dim & 7)) * 8)]) = i8x8_to_f16(rv[i].x, rv[i].y);
-                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + (((g + 1) ^ (dim & 7)) * 8)]) = i8x8_to_f16(rv[i].z, rv[i].w);
+                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + ((g ^ swizzle<128>(dim)) * 8)]) = i8x8_to_f16(rv[i].x, rv[i].y);
+                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + (((g + 1) ^ swizzle<128>(dim)) * 8)]) = i8x8_to_f16(rv[i].z, rv[i].w);
             }
             if (w == 0) scales[stage][0][lane] = rs;
             if (w == 1) {
@@ -220,30 +228,25 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     // MFMA row l32 of a 32-key block stands for this key of it
     const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
 
-    auto compute = [&](int t0, const int (&p)[4], int stage) {
+    // WHOLE: every row of the wave sees every key of the tile.
+    auto compute = [&](auto whole_tag, int t0, const int (&p)[4], int stage) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;
         const f16* Ks = tiles[stage];
         const f16* Vs = tiles[stage] + kBN * HD;
         f32x16 s[RB][2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[rb][kb][i] = 0.f;
             const f16* kr = &Ks[(32 * kb + krow) * HD];
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(&kr[((2 * k + hh) ^ (krow & 7)) * 8]);
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(&kr[((2 * k + hh) ^ swizzle<HD * 2>(krow)) * 8]);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    s[rb][kb] = mfma32(kf, qh[rb][k], s[rb][kb]);
+                    s[rb][kb] = mfma32(kf, qh[rb][k], k ? s[rb][kb] : f32x16{});
                     if constexpr (F32) s[rb][kb] = mfma32(kf, ql[rb][k], s[rb][kb]);
                 }
             }
         }
-        bool whole = t0 + kBN - 1 <= all_hi && t0 >= all_lo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) whole = whole && p[j] >= 0;
         // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
         f16x8 ph[RB][4], pl[F32 ? RB : 1][F32 ? 4 : 1];
 #pragma unroll
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                             s[rb][kb][4 * q + e] = fmaf(x, qs[rb], -mb);
                     }
                 }
-            if (!whole) {
+            if constexpr (!WHOLE) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -305,12 +308,13 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float p0 = fast_exp2(s[rb][kb][i]), p1 = fast_exp2(s[rb][kb][i + 1]);
-                    const f16x2 hi = {(f16)p0, (f16)p1};
+                    const f16x2 hi = __builtin_convertvector(f32x2{p0, p1}, f16x2);
                     ph[rb][2 * kb + (i >> 3)][i & 7] = hi[0];
                     ph[rb][2 * kb + (i >> 3)][(i & 7) + 1] = hi[1];
                     if constexpr (F32) {
-                        pl[rb][2 * kb + (i >> 3)][i & 7] = (f16)(p0 - (float)hi[0]);
-                        pl[rb][2 * kb + (i >> 3)][(i & 7) + 1] = (f16)(p1 - (float)hi[1]);
+                        const f16x2 lo = __builtin_convertvector(f32x2{p0 - (float)hi[0], p1 - (float)hi[1]}, f16x2);
+                        pl[rb][2 * kb + (i >> 3)][i & 7] = lo[0];
+                        pl[rb][2 * kb + (i >> 3)][(i & 7) + 1] = lo[1];
                     }
                     if constexpr (I8) {
                         const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
@@ -324,45 +328,68 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 }
             l[rb] += sum;
         }
+        uint32_t bad = 0;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const int dim = 32 * nb + l32;
-                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * 64 + (((2 * st + hh) ^ (dim & 7)) * 8)]);
-                if constexpr (!I8) {
-                    if (!whole) {  // see the rows kernel: infinities and NaN that not all rows see
-                        uint4 u = __builtin_bit_cast(uint4, vf);
-                        const uint32_t bad = nonfinite2(u.x) | nonfinite2(u.y) | nonfinite2(u.z) | nonfinite2(u.w);
-                        if (__ballot(bad != 0)) poison = true;
-                        u = uint4{finite2(u.x), finite2(u.y), finite2(u.z), finite2(u.w)};
-                        vf = __builtin_bit_cast(f16x8, u);
-                    }
+                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * 64 + (((2 * st + hh) ^ swizzle<128>(dim)) * 8)]);
+                if constexpr (!I8 && !WHOLE) {  // as in the rows kernel: infinities and NaN that not all rows see
+                    uint4 u = __builtin_bit_cast(uint4, vf);
+                    bad |= nonfinite2(u.x) | nonfinite2(u.y) | nonfinite2(u.z) | nonfinite2(u.w);
+                    u = uint4{finite2(u.x), finite2(u.y), finite2(u.z), finite2(u.w)};
+                    vf = __builtin_bit_cast(f16x8, u);
                 }
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     o[rb][nb] = mfma32(vf, ph[rb][st], o[rb][nb]);
                     if constexpr (F32) o[rb][nb] = mfma32(vf, pl[rb][st], o[rb][nb]);
                 }
+                if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // few operands in flight: registers
             }
+        if constexpr (!I8 && !WHOLE) poison = poison || __ballot(bad != 0) != 0;
     };
 
     if (n_t > 0) {
         look_up(k_lo, pages);
         fetch(k_lo, pages, 0);
         stash(0);
-        for (int t = 0; t < n_t; ++t) {
-            const int t0 = k_lo + t * kBN;
+        // Tiles of one kind run in a loop of their own: with a branch inside one
+        // loop the output's registers are copied at every join.
+        int t = 0;
+        auto begin = [&]() {  // the tile is in LDS, the next one on its way
             if constexpr (!I8) wait_dma<0>();
             __syncthreads();
             if (t + 1 < n_t) {
-                look_up(t0 + kBN, next_pages);
-                fetch(t0 + kBN, next_pages, (t + 1) & 1);
+                look_up(k_lo + (t + 1) * kBN, next_pages);
+                fetch(k_lo + (t + 1) * kBN, next_pages, (t + 1) & 1);
             }
-            if (t0 <= any_hi && t0 + kBN - 1 >= any_lo) compute(t0, pages, t & 1);
+        };
+        auto end = [&]() {
             if (t + 1 < n_t) stash((t + 1) & 1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) pages[j] = next_pages[j];
+            ++t;
+        };
+        auto whole = [&]() {
+            const int t0 = k_lo + t * kBN;
+            bool all = t < n_t && t0 + kBN - 1 <= all_hi && t0 >= all_lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) all = all && pages[j] >= 0;
+            return all;
+        };
+        while (t < n_t) {
+            while (whole()) {
+                begin();
+                compute(std::true_type{}, k_lo + t * kBN, pages, t & 1);
+                end();
+            }
+            if (t >= n_t) break;
+            begin();
+            const int t0 = k_lo + t * kBN;
+            if (t0 <= any_hi && t0 + kBN - 1 >= any_lo) compute(std::false_type{}, t0, pages, t & 1);
+            end();
         }
     }
 
@@ -436,11 +463,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 // What the launch in paged_attn.hip picks from: rows a workgroup, 0 where
 // head_dim has no chunk kernel.
 template <int HD, bool I8, bool F32>
-constexpr int chunk_rb() { return HD == 64 ? 2 : HD == 128 ? 2 : 1; }
+constexpr int chunk_rb() { return HD == 64 ? 2 : HD == 128 ? 1 : 1; }
 template <int HD, bool I8, bool F32>
 constexpr int chunk_occ() { return HD <= 128 && chunk_rb<HD, I8, F32>() == 1 && !F32 ? 2 : 1; }
 
-int chunk_rows(int hd, bool, bool) { return hd == 64 ? 256 : hd == 128 ? 128 * 2 : hd == 256 ? 128 : 0; }
+int chunk_rows(int hd, bool, bool) { return hd == 64 ? 256 : hd == 128 ? 128 * 1 : hd == 256 ? 128 : 0; }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
