@@ -516,11 +516,78 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         *reinterpret_cast<f16x4*>(dst) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
 }
 
+// The same for row tiles with few splits and many rows (chunks): eight rows
+// at a time, HD/4 lanes (a wave at most) a row, 32 rows a workgroup.
+constexpr int kMergeRows = 32;
+template <int HD, bool F32>
+__global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a, int bm) {
+    using QT = std::conditional_t<F32, float, f16>;
+    constexpr int C = HD / 4 < 64 ? HD / 4 : 64, V = HD / 4 / C;  // lanes a row, float4s a lane
+    const PagedGeom& pg = a.p.g;
+    const int per = bm / kMergeRows;
+    Item it;
+    if (!find_item(a, blockIdx.x / per, bm, false, it) || it.tile >= a.rt_max) return;
+    const int4 info = a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile];
+    const int splits = imin(info.z, a.n_items);  // written by this call's split 0; in range whatever it holds
+    if (splits <= 1) return;
+    const int col = threadIdx.x % C;
+    const int r_lo = blockIdx.x % per * kMergeRows;
+    for (int r = r_lo + threadIdx.x / C; r < r_lo + kMergeRows; r += 256 / C) {
+        const int row = it.tile * bm + r;
+        if (row >= it.s.n * pg.G) return;
+        float m = -INFINITY, l = 0.f;
+        f32x4 o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int U = 4;
+        for (int s0 = 0; s0 < splits; s0 += U) {
+            f32x2 ml[U];
+            f32x4 x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int sp = imin(s0 + u, splits - 1);
+                const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm + r;
+                ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[u][v] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + 4 * (col + C * v));
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s0 + u < splits) mn = fmaxf(mn, ml[u][0]);
+            const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
+            l *= f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] *= f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s0 + u < splits) {
+                    const float fu = fast_exp2(ml[u][0] - ref);
+                    l = fmaf(ml[u][1], fu, l);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;
+                }
+            m = mn;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        QT* dst = static_cast<QT*>(a.out) +
+                  ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 4 * col;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const f32x4 y = o[v] * inv;
+            if constexpr (F32)
+                *reinterpret_cast<f32x4*>(dst + 4 * C * v) = y;
+            else
+                *reinterpret_cast<f16x4*>(dst + 4 * C * v) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+        }
+    }
+}
+
 // ------------------------------------------------------------------- host --
 constexpr int kRowsTarget = 512;   // items aimed at: two workgroups a CU
 constexpr int kRowsLeast = 2;      // units a split has at least (128 keys)
-constexpr int kChunkTarget = 512;
-constexpr int kChunkLeast = 8;
+constexpr int kCus = 256;          // compute units of the target (MI355X)
+constexpr int kChunkLeast = 8;     // 64-key units a chunk's split has at least
 // Query rows a sequence may have per kv head for the rows kernel.
 constexpr int kRowsMost = 32;
 
@@ -564,7 +631,9 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     }
     if (chunks) {
         const int64_t tiles = row_tiles_bound(g, cm);
-        p.chunk = make_part(g, hd, cm, tiles, most, tiles * g.Hkv < kChunkTarget, kChunkTarget, kChunkLeast);
+        // Splits where two or more of them a tile still start at once.
+        const int slots = kCus * chunk_occ_of(hd, i8, f32);
+        p.chunk = make_part(g, hd, cm, tiles, most, 2 * tiles * g.Hkv <= slots, slots, kChunkLeast);
         if (p.rows.on) p.chunk.lo_rows = kRowsMost;
     }
     return p;
@@ -605,6 +674,13 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     }
     LMX_CHECK_LAUNCH();
     if (r.splits) {
+        if (chunk) {
+            const dim3 mgrid((unsigned)(r.items - r.target) * (unsigned)(r.bm / kMergeRows));
+            if (f32) hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm);
+            else hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm);
+            LMX_CHECK_LAUNCH();
+            return LMX_OK;
+        }
         const int rows = (int)std::min<int64_t>(r.bm, (int64_t)a.p.g.max_new * a.p.g.G);
         const dim3 mgrid((unsigned)(r.items - r.target) * (unsigned)rows);
         if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);

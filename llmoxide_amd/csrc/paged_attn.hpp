@@ -23,6 +23,7 @@ struct AttnPagedArgs {
 
 // paged_chunk.hip: rows of its workgroups (0: no kernel for this head_dim), and the launch.
 int chunk_rows(int hd, bool i8, bool f32);
+int chunk_occ_of(int hd, bool i8, bool f32);  // workgroups a CU holds
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);
 
 // One work item: a row tile of one sequence and kv head, over one split.
@@ -158,6 +159,10 @@ struct PageWindow {
         const int e = k >> a.g.ps_log2;
         if (e - first >= 64) fill(a, e);
         return __builtin_amdgcn_readlane(ids, e - first);
+    }
+    // Page of the lane's own key, one of those that at() was last asked for.
+    __device__ __forceinline__ int lane_at(const PagedArgs& a, int k) const {
+        return __shfl(ids, (k >> a.g.ps_log2) - first, 64);
     }
 };
 

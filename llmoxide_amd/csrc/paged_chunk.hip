@@ -30,6 +30,7 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 }
 
 constexpr int kBN = 64;  // keys a tile
+constexpr int kAhead = 6;
 
 // Weights are exp2(arg), arg = score - m, with m kLift below the largest score
 // that set it; a tile with an arg above kLift + kSlack moves m.
@@ -148,6 +149,20 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     };
     uint4 rk[I8 ? HD / 64 : 1], rv[I8 ? HD / 64 : 1];
     float rs = 0.f;
+    // Offsets of the lane's chunks from a wave's base: K's transfers, and V's
+    // even and odd ones where a tile lies in one page.
+    uint32_t k_off[I8 ? 1 : T::LOADS], v_off[2];
+    if constexpr (!I8) {
+        constexpr int RPT = 64 / CH;  // rows a transfer
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) {
+            const int r = i * RPT + lane / CH;  // of the wave's 16
+            k_off[i] = r * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            v_off[x] = ((lane >> 3) << (pg.ps_log2 + 1)) + (((lane & 7) ^ swizzle<128>(8 * x + (lane >> 3))) * 16);
+    }
     // f16: K, lane l of transfer i: chunk place (64 i + l) % CH of row (64 i + l) / CH of the
     // wave's 16 rows; V: 8 dims a transfer, place l % 8 of dim l / 8.
     auto fetch = [&](int t0, const int (&p)[4], int stage) {
@@ -155,25 +170,28 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             const uint32_t lds = lds_addr(&tiles[stage][0]);
             const int pk = w == 0 ? p[0] : w == 1 ? p[1] : w == 2 ? p[2] : p[3];
             const char* kb = a.p.k + (slab(pk) + ((t0 + 16 * w) & psm)) * (HD * 2);
-            constexpr int RPT = 64 / CH;  // rows a transfer
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) {
-                const int r = i * RPT + lane / CH;  // of the wave's 16
-                const uint32_t off = r * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
-                dma16(kb, off, lds + (w * 16 * HD * 2) + i * 1024);
+            for (int i = 0; i < T::LOADS; ++i) dma16(kb, k_off[i], lds + (w * 16 * HD * 2) + i * 1024);
+            const uint32_t v_lds = lds + kBN * HD * 2 + w * (HD / 4) * 128;
+            if (pg.ps_log2 >= 6) {  // the tile lies in one page: a base for the wave, offsets that stay
+                const char* vb = a.p.v + (slab(p[0]) * HD + ((size_t)(w * (HD / 4)) << pg.ps_log2) + (t0 & psm)) * 2;
+#pragma unroll
+                for (int i = 0; i < T::LOADS; ++i)
+                    dma16(vb + ((size_t)i << (pg.ps_log2 + 4)), v_off[i & 1], v_lds + 8 * i * 128);
+            } else {
+                // every other transfer's dims swap the halves of the tile's keys
+                const int d8 = lane >> 3;
+                const char* vb[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int c = (lane & 7) ^ swizzle<128>(8 * x + d8);
+                    const int pv = pw.lane_at(a.p, t0 + 8 * c);
+                    vb[x] = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm) + ((size_t)(w * (HD / 4) + d8) << pg.ps_log2)) * 2;
+                }
+#pragma unroll
+                for (int i = 0; i < T::LOADS; ++i)
+                    dma16_lane(vb[i & 1] + ((size_t)i << (pg.ps_log2 + 4)), v_lds + 8 * i * 128);
             }
-            // every other transfer's dims swap the halves of the tile's keys
-            const int d8 = lane >> 3, dw = w * (HD / 4) + d8;
-            const char* vb[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int c = (lane & 7) ^ swizzle<128>(8 * x + d8), j = c >> 1;
-                const int pv = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
-                vb[x] = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm) + ((size_t)dw << pg.ps_log2)) * 2;
-            }
-#pragma unroll
-            for (int i = 0; i < T::LOADS; ++i)
-                dma16_lane(vb[i & 1] + ((size_t)i << (pg.ps_log2 + 4)), lds + kBN * HD * 2 + (w * (HD / 4) + 8 * i) * 128);
         } else {
             // K: 16 dims of a key a load; V: the 16 keys of a granule of one dim
 #pragma unroll
@@ -245,6 +263,15 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     s[rb][kb] = mfma32(kf, qh[rb][k], k ? s[rb][kb] : f32x16{});
                     if constexpr (F32) s[rb][kb] = mfma32(kf, ql[rb][k], s[rb][kb]);
                 }
+            }
+        }
+        {   // operand reads kAhead ahead of their products
+            constexpr int N = 2 * KS, PER = RB * (F32 ? 2 : 1), AHEAD = N < kAhead ? N : kAhead;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
+                if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
         // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
@@ -348,6 +375,20 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 }
                 if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // few operands in flight: registers
             }
+        if constexpr (WHOLE && !I8 && RB == 1) {
+            // the first operands are on their way during the first weights'
+            // exponentials; the others' run beside the products
+            constexpr int N = 4 * NB, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
+            constexpr int FIRST = F32 ? 24 : 14, EACH = (F32 ? 96 : 52) / N;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, FIRST, 0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
+                if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, EACH, 0);
+            }
+        }
         if constexpr (!I8 && !WHOLE) poison = poison || __ballot(bad != 0) != 0;
     };
 
@@ -460,18 +501,15 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     }
 }
 
-// What the launch in paged_attn.hip picks from: rows a workgroup, 0 where
-// head_dim has no chunk kernel.
-template <int HD, bool I8, bool F32>
-constexpr int chunk_rb() { return HD == 64 ? 2 : HD == 128 ? 1 : 1; }
-template <int HD, bool I8, bool F32>
-constexpr int chunk_occ() { return HD <= 128 && chunk_rb<HD, I8, F32>() == 1 && !F32 ? 2 : 1; }
-
-int chunk_rows(int hd, bool, bool) { return hd == 64 ? 256 : hd == 128 ? 128 * 1 : hd == 256 ? 128 : 0; }
+// Row blocks a wave and workgroups a CU, by what fits the registers.
+constexpr int chunk_rb(int hd, bool, bool) { return hd == 64 ? 2 : 1; }
+constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd == 128 && !f32 ? 2 : 1; }
+int chunk_rows(int hd, bool i8, bool f32) { return hd <= 256 ? 128 * chunk_rb(hd, i8, f32) : 0; }
+int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb<HD, I8, F32>(), chunk_occ<HD, I8, F32>()>), dim3(items), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
 }
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
     auto by = [&](auto tag) {
