@@ -29,8 +29,7 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-constexpr int kBN = 64;  // keys a tile
-constexpr int kAhead = 6;
+constexpr int kAhead = 6;  // operand reads in flight ahead of their product
 
 // Weights are exp2(arg), arg = score - m, with m kLift below the largest score
 // that set it; a tile with an arg above kLift + kSlack moves m.
@@ -40,28 +39,35 @@ struct Lift {
 };
 
 // Place of row r's chunk c is c ^ swizzle(r): rows of 256 bytes and more start
-// at the same bank, of rows of 128 bytes every other one does.
+// at the same bank, of rows of 128 (64) bytes every second (fourth) one does.
 template <int ROW_BYTES>
-__device__ __forceinline__ int swizzle(int r) { return ROW_BYTES >= 256 ? r & 15 : (r >> 1) & 7; }
+__device__ __forceinline__ int swizzle(int r) {
+    return ROW_BYTES >= 256 ? r & 15 : ROW_BYTES == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
 
-template <int HD, bool I8, bool F32, int RB>
+template <int HD, int RB, int BN>
 struct ChunkTile {
     static constexpr int KS = HD / 16;   // k-steps of QK
     static constexpr int NB = HD / 32;   // 32-dim blocks of the output
     static constexpr int BM = 128 * RB;  // rows a workgroup
+    static constexpr int KB = BN / 32;   // 32-key blocks a tile
+    static constexpr int ST = BN / 16;   // k-steps of PV
+    static constexpr int GR = BN / 16;   // 16-key granules a tile, each in one page
     static constexpr int CH = HD / 8;    // 16-byte chunks of a K row
-    static constexpr int LOADS = HD / 32;  // 1 KB transfers a wave makes of a tile's K, and of its V
-    static constexpr int STAGE = 2 * kBN * HD;  // halfs: K then V
+    static constexpr int CV = BN / 8;    // 16-byte chunks of a V column
+    static constexpr int LOADS = BN * HD / 2048;  // 1 KB transfers a wave makes of a tile's K, and of its V
+    static constexpr int STAGE = 2 * BN * HD;     // halfs: K then V
 };
 
-template <int HD, bool I8, bool F32, int RB, int OCC>
+// BN: keys a tile.  RB: 32-row blocks a wave.  OCC: workgroups a CU.
+template <int HD, bool I8, bool F32, int RB, int BN, int OCC>
 __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) {
-    using T = ChunkTile<HD, I8, F32, RB>;
+    using T = ChunkTile<HD, RB, BN>;
     using QT = std::conditional_t<F32, float, f16>;
-    constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH;
+    constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH, KB = T::KB, ST = T::ST, GR = T::GR, CV = T::CV;
     constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
     __shared__ __align__(1024) f16 tiles[2][T::STAGE];
-    __shared__ __align__(16) float scales[I8 ? 2 : 1][3][kBN];  // K's, log2 of V's, 1 / V's
+    __shared__ __align__(16) float scales[I8 ? 2 : 1][3][BN];  // K's, log2 of V's, 1 / V's
 
     Item it;
     if (!find_item(a, blockIdx.x, BM, true, it)) return;
@@ -78,9 +84,9 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     auto low_of = [&](int pos) { return pg.window ? imax(pos - pg.window + 1, 0) : 0; };
     const int split_lo = it.splits > 1 ? it.w.lo + it.split * it.per * kUnit : it.w.lo;
     const int split_hi = it.splits > 1 ? split_lo + it.per * kUnit : 0x7fffffff;
-    const int k_lo = imax(low_of(pos_of(r0)) & ~(kBN - 1), split_lo);
+    const int k_lo = imax(low_of(pos_of(r0)) & ~(BN - 1), split_lo);
     const int k_hi = imin(pos_of(r1) + 1, split_hi);  // one behind the last key
-    const int n_t = k_hi > k_lo ? (k_hi - k_lo + kBN - 1) / kBN : 0;
+    const int n_t = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
     // the wave's: keys some row sees, keys all rows see
     const int w0 = r0 + w * 32 * RB, w1 = imin(w0 + 32 * RB, n_rows) - 1;
     const bool live = w0 <= r1;
@@ -139,93 +145,100 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     PageWindow pw;
     pw.row = a.p.table + (size_t)it.b * pg.table_stride;
     pw.fill(a.p, k_lo >> pg.ps_log2);
-    int pages[4], next_pages[4];
-    auto look_up = [&](int t0, int (&p)[4]) {
+    int pages[GR], next_pages[GR];
+    auto look_up = [&](int t0, int (&p)[GR]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = pw.at(a.p, t0 + 16 * j);
+        for (int j = 0; j < GR; ++j) p[j] = pw.at(a.p, t0 + 16 * j);
     };
     auto slab = [&](int page) {  // positions of the pool before the page's
         return ((size_t)imax(page, 0) * pg.Hkv + it.h) << pg.ps_log2;
     };
-    uint4 rk[I8 ? HD / 64 : 1], rv[I8 ? HD / 64 : 1];
+    constexpr int RL = BN * HD / 4096;  // 16-byte loads a thread makes of an 8-bit tile's K, and of its V
+    static_assert(!I8 || RL >= 1, "8-bit tile split");
+    uint4 rk[I8 ? RL : 1], rv[I8 ? RL : 1];
     float rs = 0.f;
+    // Of four values, or two, the one at j.
+    auto pick = [&](const int (&p)[GR], int j) {
+        if constexpr (GR == 2) return j ? p[1] : p[0];
+        else return j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+    };
     // Offsets of the lane's chunks from a wave's base: K's transfers, and V's
     // even and odd ones where a tile lies in one page.
+    constexpr int DPT = 64 / CV;  // dims a transfer of V
     uint32_t k_off[I8 ? 1 : T::LOADS], v_off[2];
     if constexpr (!I8) {
         constexpr int RPT = 64 / CH;  // rows a transfer
 #pragma unroll
         for (int i = 0; i < T::LOADS; ++i) {
-            const int r = i * RPT + lane / CH;  // of the wave's 16
-            k_off[i] = r * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
+            const int r = i * RPT + lane / CH + w * (BN / 4);
+            k_off[i] = (r - w * (BN / 4)) * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-            v_off[x] = ((lane >> 3) << (pg.ps_log2 + 1)) + (((lane & 7) ^ swizzle<128>(8 * x + (lane >> 3))) * 16);
+            v_off[x] = ((lane / CV) << (pg.ps_log2 + 1)) + (((lane % CV) ^ swizzle<BN * 2>(DPT * x + lane / CV)) * 16);
     }
-    // f16: K, lane l of transfer i: chunk place (64 i + l) % CH of row (64 i + l) / CH of the
-    // wave's 16 rows; V: 8 dims a transfer, place l % 8 of dim l / 8.
-    auto fetch = [&](int t0, const int (&p)[4], int stage) {
+    // f16: a wave copies BN / 4 rows of K and HD / 4 columns of V; lane l of a
+    // transfer fills place l % CH (CV) of its row (column) l / CH (CV).
+    auto fetch = [&](int t0, const int (&p)[GR], int stage) {
         if constexpr (!I8) {
             const uint32_t lds = lds_addr(&tiles[stage][0]);
-            const int pk = w == 0 ? p[0] : w == 1 ? p[1] : w == 2 ? p[2] : p[3];
-            const char* kb = a.p.k + (slab(pk) + ((t0 + 16 * w) & psm)) * (HD * 2);
+            const char* kb = a.p.k + (slab(pick(p, w * GR / 4)) + ((t0 + w * (BN / 4)) & psm)) * (HD * 2);
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) dma16(kb, k_off[i], lds + (w * 16 * HD * 2) + i * 1024);
-            const uint32_t v_lds = lds + kBN * HD * 2 + w * (HD / 4) * 128;
-            if (pg.ps_log2 >= 6) {  // the tile lies in one page: a base for the wave, offsets that stay
+            for (int i = 0; i < T::LOADS; ++i) dma16(kb, k_off[i], lds + w * (BN / 4) * (HD * 2) + i * 1024);
+            const uint32_t v_lds = lds + BN * HD * 2 + w * (HD / 4) * (BN * 2);
+            if ((16 << pg.ps_log2) >= 16 * BN) {  // the tile lies in one page: a base for the wave, offsets that stay
                 const char* vb = a.p.v + (slab(p[0]) * HD + ((size_t)(w * (HD / 4)) << pg.ps_log2) + (t0 & psm)) * 2;
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i)
-                    dma16(vb + ((size_t)i << (pg.ps_log2 + 4)), v_off[i & 1], v_lds + 8 * i * 128);
+                    dma16(vb + ((size_t)(DPT * i) << (pg.ps_log2 + 1)), v_off[i & 1], v_lds + i * 1024);
             } else {
-                // every other transfer's dims swap the halves of the tile's keys
-                const int d8 = lane >> 3;
+                // (of 64-key tiles, every other transfer's dims swap the halves of the keys)
                 const char* vb[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int c = (lane & 7) ^ swizzle<128>(8 * x + d8);
+                    const int c = (lane % CV) ^ swizzle<BN * 2>(DPT * x + lane / CV);
                     const int pv = pw.lane_at(a.p, t0 + 8 * c);
-                    vb[x] = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm) + ((size_t)(w * (HD / 4) + d8) << pg.ps_log2)) * 2;
+                    vb[x] = a.p.v + (slab(pv) * HD + ((t0 + 8 * c) & psm) + ((size_t)(w * (HD / 4) + lane / CV) << pg.ps_log2)) * 2;
                 }
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i)
-                    dma16_lane(vb[i & 1] + ((size_t)i << (pg.ps_log2 + 4)), v_lds + 8 * i * 128);
+                    dma16_lane(vb[i & 1] + ((size_t)(DPT * i) << (pg.ps_log2 + 1)), v_lds + i * 1024);
             }
         } else {
             // K: 16 dims of a key a load; V: the 16 keys of a granule of one dim
 #pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                const int x = tid + 256 * i, key = x / (HD / 16), c = x % (HD / 16), j = key >> 4;
-                const int pk = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
-                rk[i] = *reinterpret_cast<const uint4*>(a.p.k + (slab(pk) + ((t0 + key) & psm)) * HD + 16 * c);
-                const int dim = x >> 2, g = x & 3;
-                const int pv = g == 0 ? p[0] : g == 1 ? p[1] : g == 2 ? p[2] : p[3];
-                rv[i] = *reinterpret_cast<const uint4*>(a.p.v + slab(pv) * HD + ((size_t)dim << pg.ps_log2) + ((t0 + 16 * g) & psm));
+            for (int i = 0; i < RL; ++i) {
+                const int x = tid + 256 * i, key = x / (HD / 16), c = x % (HD / 16);
+                rk[i] = *reinterpret_cast<const uint4*>(a.p.k + (slab(pick(p, key >> 4)) + ((t0 + key) & psm)) * HD + 16 * c);
+                const int dim = x / GR, g = x % GR;
+                rv[i] = *reinterpret_cast<const uint4*>(a.p.v + slab(pick(p, g)) * HD + ((size_t)dim << pg.ps_log2) + ((t0 + 16 * g) & psm));
             }
-            const int key = lane, j = lane >> 4;
-            const int pk = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
-            if (w < 2) rs = (w ? a.p.v_scale : a.p.k_scale)[slab(pk) + ((t0 + key) & psm)];
+            if (w < 2 && lane < BN)
+                rs = (w ? a.p.v_scale : a.p.k_scale)[slab(pick(p, lane >> 4)) + ((t0 + lane) & psm)];
         }
     };
     auto stash = [&](int stage) {  // 8-bit tiles: registers to LDS as f16
         if constexpr (I8) {
             f16* Ks = tiles[stage];
-            f16* Vs = tiles[stage] + kBN * HD;
+            f16* Vs = tiles[stage] + BN * HD;
+            auto put = [&](f16* row, int c, int sw, const uint4& x) {  // chunks c and c + 1 of a row
+                *reinterpret_cast<f16x8*>(&row[(c ^ sw) * 8]) = i8x8_to_f16(x.x, x.y);
+                *reinterpret_cast<f16x8*>(&row[((c + 1) ^ sw) * 8]) = i8x8_to_f16(x.z, x.w);
+            };
 #pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                const int x = tid + 256 * i, key = x / (HD / 16), c = 2 * (x % (HD / 16));
-                *reinterpret_cast<f16x8*>(&Ks[key * HD + ((c ^ swizzle<HD * 2>(key)) * 8)]) = i8x8_to_f16(rk[i].x, rk[i].y);
-                *reinterpret_cast<f16x8*>(&Ks[key * HD + (((c + 1) ^ swizzle<HD * 2>(key)) * 8)]) = i8x8_to_f16(rk[i].z, rk[i].w);
-                const int dim = x >> 2, g = 2 * (x & 3);
-                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + ((g ^ swizzle<128>(dim)) * 8)]) = i8x8_to_f16(rv[i].x, rv[i].y);
-                *reinterpret_cast<f16x8*>(&Vs[dim * 64 + (((g + 1) ^ swizzle<128>(dim)) * 8)]) = i8x8_to_f16(rv[i].z, rv[i].w);
+            for (int i = 0; i < RL; ++i) {
+                const int x = tid + 256 * i, key = x / (HD / 16);
+                put(&Ks[key * HD], 2 * (x % (HD / 16)), swizzle<HD * 2>(key), rk[i]);
+                const int dim = x / GR;
+                put(&Vs[dim * BN], 2 * (x % GR), swizzle<BN * 2>(dim), rv[i]);
             }
-            if (w == 0) scales[stage][0][lane] = rs;
-            if (w == 1) {
-                const float v = v_scale_of(rs);
-                scales[stage][1][lane] = __builtin_amdgcn_logf(v);
-                scales[stage][2][lane] = 1.f / v;
+            if (lane < BN) {
+                if (w == 0) scales[stage][0][lane] = rs;
+                if (w == 1) {
+                    const float v = v_scale_of(rs);
+                    scales[stage][1][lane] = __builtin_amdgcn_logf(v);
+                    scales[stage][2][lane] = 1.f / v;
+                }
             }
         }
     };
@@ -247,13 +260,13 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
 
     // WHOLE: every row of the wave sees every key of the tile.
-    auto compute = [&](auto whole_tag, int t0, const int (&p)[4], int stage) {
+    auto compute = [&](auto whole_tag, int t0, const int (&p)[GR], int stage) {
         constexpr bool WHOLE = decltype(whole_tag)::value;
         const f16* Ks = tiles[stage];
-        const f16* Vs = tiles[stage] + kBN * HD;
-        f32x16 s[RB][2];
+        const f16* Vs = tiles[stage] + BN * HD;
+        f32x16 s[RB][KB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             const f16* kr = &Ks[(32 * kb + krow) * HD];
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -265,8 +278,8 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 }
             }
         }
-        {   // operand reads kAhead ahead of their products
-            constexpr int N = 2 * KS, PER = RB * (F32 ? 2 : 1), AHEAD = N < kAhead ? N : kAhead;
+        {
+            constexpr int N = KB * KS, PER = RB * (F32 ? 2 : 1), AHEAD = N < kAhead ? N : kAhead;
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -275,13 +288,13 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             }
         }
         // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
-        f16x8 ph[RB][4], pl[F32 ? RB : 1][F32 ? 4 : 1];
+        f16x8 ph[RB][ST], pl[F32 ? RB : 1][F32 ? ST : 1];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             float mb = m[rb] == -INFINITY ? 0.f : m[rb];
             float top = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {  // four registers: keys 32 kb + 16 (q/2) + 8 hh + 4 (q%2) ..
                     f32x4 ks, lv;
@@ -301,7 +314,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 }
             if constexpr (!WHOLE) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int key = t0 + 32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7);
@@ -310,7 +323,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     }
             }
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rb][kb][i]);
             if (__ballot(top > kMost || m[rb] == -INFINITY)) {
@@ -327,11 +340,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) o[rb][nb] *= f;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) s[rb][kb] -= delta;
+                for (int kb = 0; kb < KB; ++kb) s[rb][kb] -= delta;
             }
             float sum = 0.f;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float p0 = fast_exp2(s[rb][kb][i]), p1 = fast_exp2(s[rb][kb][i + 1]);
@@ -357,11 +370,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         }
         uint32_t bad = 0;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+        for (int st = 0; st < ST; ++st)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const int dim = 32 * nb + l32;
-                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * 64 + (((2 * st + hh) ^ swizzle<128>(dim)) * 8)]);
+                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * BN + (((2 * st + hh) ^ swizzle<BN * 2>(dim)) * 8)]);
                 if constexpr (!I8 && !WHOLE) {  // as in the rows kernel: infinities and NaN that not all rows see
                     uint4 u = __builtin_bit_cast(uint4, vf);
                     bad |= nonfinite2(u.x) | nonfinite2(u.y) | nonfinite2(u.z) | nonfinite2(u.w);
@@ -378,8 +391,8 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         if constexpr (WHOLE && !I8 && RB == 1) {
             // the first operands are on their way during the first weights'
             // exponentials; the others' run beside the products
-            constexpr int N = 4 * NB, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
-            constexpr int FIRST = F32 ? 24 : 14, EACH = (F32 ? 96 : 52) / N;
+            constexpr int N = ST * NB, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
+            constexpr int FIRST = F32 ? 24 : 14, EACH = (F32 ? 24 : 13) * ST / N;
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
             __builtin_amdgcn_sched_group_barrier(0x2, FIRST, 0);
 #pragma unroll
@@ -403,33 +416,33 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             if constexpr (!I8) wait_dma<0>();
             __syncthreads();
             if (t + 1 < n_t) {
-                look_up(k_lo + (t + 1) * kBN, next_pages);
-                fetch(k_lo + (t + 1) * kBN, next_pages, (t + 1) & 1);
+                look_up(k_lo + (t + 1) * BN, next_pages);
+                fetch(k_lo + (t + 1) * BN, next_pages, (t + 1) & 1);
             }
         };
         auto end = [&]() {
             if (t + 1 < n_t) stash((t + 1) & 1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) pages[j] = next_pages[j];
+            for (int j = 0; j < GR; ++j) pages[j] = next_pages[j];
             ++t;
         };
         auto whole = [&]() {
-            const int t0 = k_lo + t * kBN;
-            bool all = t < n_t && t0 + kBN - 1 <= all_hi && t0 >= all_lo;
+            const int t0 = k_lo + t * BN;
+            bool all = t < n_t && t0 + BN - 1 <= all_hi && t0 >= all_lo;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) all = all && pages[j] >= 0;
+            for (int j = 0; j < GR; ++j) all = all && pages[j] >= 0;
             return all;
         };
         while (t < n_t) {
             while (whole()) {
                 begin();
-                compute(std::true_type{}, k_lo + t * kBN, pages, t & 1);
+                compute(std::true_type{}, k_lo + t * BN, pages, t & 1);
                 end();
             }
             if (t >= n_t) break;
             begin();
-            const int t0 = k_lo + t * kBN;
-            if (t0 <= any_hi && t0 + kBN - 1 >= any_lo) compute(std::false_type{}, t0, pages, t & 1);
+            const int t0 = k_lo + t * BN;
+            if (t0 <= any_hi && t0 + BN - 1 >= any_lo) compute(std::false_type{}, t0, pages, t & 1);
             end();
         }
     }
@@ -503,13 +516,14 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 
 // Row blocks a wave and workgroups a CU, by what fits the registers.
 constexpr int chunk_rb(int hd, bool, bool) { return hd == 64 ? 2 : 1; }
-constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd == 128 && !f32 ? 2 : 1; }
+constexpr int chunk_bn(int hd, bool, bool f32) { return hd == 256 || (hd == 128 && f32) ? 32 : 64; }
+constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd == 128 || (hd == 256 && !f32) ? 2 : 1; }
 int chunk_rows(int hd, bool i8, bool f32) { return hd <= 256 ? 128 * chunk_rb(hd, i8, f32) : 0; }
 int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb(HD, I8, F32), chunk_bn(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
 }
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
     auto by = [&](auto tag) {
