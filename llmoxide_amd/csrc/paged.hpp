@@ -27,7 +27,7 @@ struct RowPlace {
     int page;  // -1: in no page, or the row belongs to no sequence
     int slot;
     int pos;
-    bool owned;  // belongs to a sequence
+    int seq;   // -1: none
 };
 
 // The place of row `row` (a value of the lane's own; rows first .. last are
@@ -54,18 +54,66 @@ __device__ __forceinline__ RowPlace locate_row(const PagedArgs& a, int row, int 
         }
         if (upto != ~0ull) break;
     }
-    RowPlace p{-1, 0, 0, false};
+    RowPlace p{-1, 0, 0, -1};
     if (seq >= a.g.n_seq || row >= a.g.n_tokens) return p;
     const int cu0 = a.cu[seq], cu1 = a.cu[seq + 1];
     const PagedSeq s = paged_seq(a.g, cu0, cu1, a.ctx[seq]);
     if (row < s.row0 || row >= s.row0 + s.n) return p;
-    p.owned = true;
+    p.seq = seq;
     p.pos = s.ctx - s.n + (row - s.row0);
     const int e = p.pos < s.ctx ? paged_entry(a.g, p.pos) : -1;
     if (e < 0) return p;
     p.page = paged_page(a.g, a.table[(size_t)seq * a.g.table_stride + e]);
     p.slot = p.pos & ((1 << a.g.ps_log2) - 1);
     return p;
+}
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = __lane_id();
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d, 64);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+
+// Row block `id` of the batch (every wave for itself): its first row r0 and row
+// count, and in lane l the place of row r0 + l % R.  False: no such block.
+template <int LOG2_R>
+__device__ __forceinline__ bool find_block(const PagedArgs& a, int id, int& r0, int& n_rows, RowPlace& at) {
+    const int lane = __lane_id();
+    int base = 0;
+    for (int c0 = 0; c0 < a.g.n_seq; c0 += 64) {
+        const int b = c0 + lane;
+        PagedSeq s{0, 0, 0};
+        if (b < a.g.n_seq) s = paged_seq(a.g, a.cu[b], a.cu[b + 1], a.ctx[b]);
+        const int n = row_blocks(s, LOG2_R), upto = a.g.n_seq == 1 ? n : wave_scan(n);
+        const uint64_t has = __ballot(base + upto > id);
+        if (has) {
+            const int l = __builtin_ctzll(has);
+            auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            const PagedSeq q{get(s.row0), get(s.n), get(s.ctx)};
+            const RowBlock blk = row_block(q, id - base - (get(upto) - get(n)), LOG2_R);
+            r0 = q.row0 + blk.first;
+            n_rows = blk.count;
+            at = RowPlace{-1, 0, 0, -1};
+            const int row = lane & ((1 << LOG2_R) - 1);
+            if (row < n_rows) {
+                at.seq = c0 + l;
+                at.pos = q.ctx - q.n + blk.first + row;
+                const int e = paged_entry(a.g, at.pos);
+                if (e >= 0) {
+                    at.page = paged_page(a.g, a.table[(size_t)at.seq * a.g.table_stride + e]);
+                    at.slot = at.pos & ((1 << a.g.ps_log2) - 1);
+                }
+            }
+            return n_rows > 0;
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
 }
 
 // Offset in elements of (page, head, slot)'s K row, of its V column's first

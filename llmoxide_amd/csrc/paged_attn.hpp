@@ -35,17 +35,6 @@ struct Item {
     int per;
 };
 
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-    const int lane = __lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d, 64);
-        x += lane >= d ? y : 0;
-    }
-    return x;
-}
-
 // Sequence b's rows and work; no work where it has none or another kernel's
 // share of them.
 __device__ __forceinline__ void load_work(const AttnPagedArgs& a, int b, int bm, PagedSeq& s, SeqWork& w) {

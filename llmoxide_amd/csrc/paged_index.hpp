@@ -51,6 +51,31 @@ LMX_FN int paged_page(const PagedGeom& g, int entry) {
     return (uint32_t)entry < (uint32_t)g.n_pages ? entry : -1;
 }
 
+// ---- row blocks: a sequence's new rows, cut where its positions are multiples
+// of R (a power of two), so that a block's rows meet whole granules of a page
+// except at the sequence's own ends.  A first position below 0 (a length
+// shorter than its new rows) is cut the same way.
+LMX_FN int row_blocks(const PagedSeq& s, int log2_r) {
+    return s.n ? ((s.ctx - 1) >> log2_r) - ((s.ctx - s.n) >> log2_r) + 1 : 0;
+}
+// Block i's rows: [first, first + count) of the sequence's.
+struct RowBlock {
+    int first, count;
+};
+LMX_FN RowBlock row_block(const PagedSeq& s, int i, int log2_r) {
+    const int p0 = s.ctx - s.n, lo = ((p0 >> log2_r) + i) * (1 << log2_r);
+    RowBlock b;
+    b.first = imax(lo - p0, 0);
+    b.count = imin(lo + (1 << log2_r) - p0, s.n) - b.first;
+    return b;
+}
+// Blocks of all sequences together: a sequence of n rows has at most n / R + 2,
+// and no more than n.
+LMX_FN int64_t row_blocks_bound(const PagedGeom& g, int log2_r) {
+    const int64_t a = ((int64_t)g.n_tokens >> log2_r) + 2 * (int64_t)g.n_seq;
+    return a < g.n_tokens ? a : g.n_tokens;
+}
+
 // ---- attention's work items.
 //
 // A sequence's rows meet a kv head as n * G query rows (row r: token r / G,
