@@ -45,65 +45,76 @@ __device__ __forceinline__ float sum_groups(float x) {
     return x + shfl_xor(x, 32);
 }
 
+// LDS traffic among the lanes of one wave, in program order.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int HD, bool I8>
 struct Tile {
     static constexpr int KEYS = I8 ? 64 : 32;
     static constexpr int NB = KEYS / 16;          // 16-key blocks
+    static constexpr int GR = KEYS / 16;          // 16-key granules, each in one page
     static constexpr int KL = I8 ? HD / 64 : HD / 32;  // 16-byte K loads a block
     static constexpr int VL = HD / 16;            // 16-byte V loads
     uint4 k[NB][KL];
     uint4 v[VL];
-    f32x4 ks[I8 ? NB : 1], vs[I8 ? NB : 1];       // scales of the lane's keys
-    int pages[KEYS / 16];                         // per 16-key granule; -1: none
+    float ks, vs;                                 // 8-bit: the scales of key t0 + lane
 };
 
+// Positions of the pool before the (page, head) block of granule i of a tile;
+// a missing page reads page 0, and is masked.
 template <int HD, bool I8>
-__device__ __forceinline__ void load_tile(const AttnPagedArgs& a, PageWindow& pw, int h, int t0, Tile<HD, I8>& t) {
-    using T = Tile<HD, I8>;
-    const int lane = __lane_id(), c = lane & 15, g = lane >> 4;
-    const int psm = (1 << a.p.g.ps_log2) - 1;
-#pragma unroll
-    for (int i = 0; i < T::KEYS / 16; ++i) t.pages[i] = pw.at(a.p, t0 + 16 * i);
-    // Granule i's (page, head) block; a missing page reads page 0, and is masked.
-    auto slab = [&](int i) { return (size_t)imax(t.pages[i], 0) * a.p.g.Hkv + h; };
-    constexpr int ES = I8 ? 1 : 2;
-    size_t base[T::KEYS / 16];
-#pragma unroll
-    for (int i = 0; i < T::KEYS / 16; ++i) base[i] = slab(i) << a.p.g.ps_log2;  // in positions
-    // K: the lane's key in block j is KEYS/4 * (c/4) + 4j + c%4; V: its keys
-    // are KEYS/4 consecutive ones.  Neither leaves its granule.
-    size_t kb, vb;
-    if constexpr (I8) {
-        const int i = c >> 2;
-        kb = i == 0 ? base[0] : i == 1 ? base[1] : i == 2 ? base[2] : base[3];
-        vb = g == 0 ? base[0] : g == 1 ? base[1] : g == 2 ? base[2] : base[3];
-    } else {
-        kb = c >> 3 ? base[1] : base[0];
-        vb = g >> 1 ? base[1] : base[0];
+__device__ __forceinline__ size_t granule_base(const AttnPagedArgs& a, const int (&pages)[Tile<HD, I8>::GR], int h, int i) {
+    constexpr int GR = Tile<HD, I8>::GR;
+    // (Values first, then the choice: a choice among elements makes the array
+    // one in memory, which the compiler then keeps in LDS.)
+    const int p0 = pages[0], p1 = pages[1];
+    int p = i & 1 ? p1 : p0;
+    if constexpr (GR == 4) {
+        const int p2 = pages[2], p3 = pages[3], q = i & 1 ? p3 : p2;
+        p = i & 2 ? q : p;
     }
-    constexpr int QUART = T::KEYS / 4;  // consecutive keys of a lane
+    return ((size_t)imax(p, 0) * a.p.g.Hkv + h) << a.p.g.ps_log2;
+}
+
+// The tile's K operands (and 8-bit scales): the lane's key in block j is
+// KEYS/4 * (c/4) + 4j + c%4; those of a lane do not leave a granule.
+template <int HD, bool I8>
+__device__ __forceinline__ void load_k(const AttnPagedArgs& a, const int (&pages)[Tile<HD, I8>::GR], int h, int t0, Tile<HD, I8>& t) {
+    using T = Tile<HD, I8>;
+    constexpr int ES = I8 ? 1 : 2, QUART = T::KEYS / 4;
+    const int lane = __lane_id(), c = lane & 15, g = lane >> 4, psm = (1 << a.p.g.ps_log2) - 1;
+    const size_t kb = granule_base<HD, I8>(a, pages, h, QUART * (c >> 2) / 16);
     const char* kr = a.p.k + (kb + ((t0 + QUART * (c >> 2)) & psm) + (c & 3)) * (HD * ES) + 16 * g;
 #pragma unroll
     for (int j = 0; j < T::NB; ++j)
 #pragma unroll
         for (int l = 0; l < T::KL; ++l) t.k[j][l] = *reinterpret_cast<const uint4*>(kr + 4 * j * HD * ES + 64 * l);
-    const int vslot = (t0 + QUART * g) & psm;
-    const char* vc = a.p.v + (vb * HD + (c << a.p.g.ps_log2) + vslot) * ES;
+    if constexpr (I8) {
+        const size_t at = granule_base<HD, I8>(a, pages, h, g) + ((t0 + lane) & psm);
+        t.ks = a.p.k_scale[at];
+        t.vs = a.p.v_scale[at];
+    }
+}
+// Its V operands: the lane's KEYS/4 consecutive keys of dims c, c + 16, ...
+template <int HD, bool I8>
+__device__ __forceinline__ void load_v(const AttnPagedArgs& a, const int (&pages)[Tile<HD, I8>::GR], int h, int t0, Tile<HD, I8>& t) {
+    using T = Tile<HD, I8>;
+    constexpr int ES = I8 ? 1 : 2, QUART = T::KEYS / 4;
+    const int lane = __lane_id(), c = lane & 15, g = lane >> 4, psm = (1 << a.p.g.ps_log2) - 1;
+    const size_t vb = granule_base<HD, I8>(a, pages, h, QUART * g / 16);
+    const char* vc = a.p.v + (vb * HD + ((size_t)c << a.p.g.ps_log2) + ((t0 + QUART * g) & psm)) * ES;
     const uint32_t vstep = (16u * ES) << a.p.g.ps_log2;
 #pragma unroll
     for (int l = 0; l < T::VL; ++l) t.v[l] = *reinterpret_cast<const uint4*>(vc + l * vstep);
-    if constexpr (I8) {
-#pragma unroll
-        for (int j = 0; j < T::NB; ++j) {
-            t.ks[j] = *reinterpret_cast<const f32x4*>(a.p.k_scale + vb + vslot + 4 * j);
-            t.vs[j] = *reinterpret_cast<const f32x4*>(a.p.v_scale + vb + vslot + 4 * j);
-        }
-    }
 }
 
 // F32: q and out are f32 and q has a residual part.
 template <int HD, bool I8, bool F32>
-__global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnPagedArgs a) {
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(AttnPagedArgs a) {
     using T = Tile<HD, I8>;
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int KS = HD / 32;   // k-steps of QK
@@ -112,6 +123,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
     constexpr int OP = HD + 4;  // floats a row of the exchange (16-byte rows, rows 4 banks apart)
     constexpr size_t kEx = 512 + 4 * 16 * OP * 4, kQ = QLDS ? (F32 ? 2 : 1) * KS * 64 * 16 : 0;
     __shared__ __align__(16) char smem[kEx > kQ ? kEx : kQ];
+    __shared__ __align__(16) float scales[I8 ? 4 : 1][3][64];  // a wave's: K's, log2 of V's, 1 / V's
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
 
@@ -121,11 +133,13 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
     if (it.split == 0 && tid == 0 && it.tile < a.rt_max)
         a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile] = make_int4(it.first, it.stride, it.splits, 0);
 
-    // This wave's keys: its quarter of the split, in whole tiles.
+    // The split's tiles go round the four waves: what shares a 128-byte line of V
+    // (a column's neighbouring tiles) is asked for at one time, not once and
+    // again when the caches have lost it.
     const int split_lo = it.w.lo + it.split * it.per * kUnit;
     const int split_hi = it.splits > 1 ? imin(it.s.ctx, split_lo + it.per * kUnit) : it.s.ctx;
-    const int tiles = (split_hi - split_lo + T::KEYS - 1) / T::KEYS;
-    const int t_lo = tiles * w / 4, t_hi = tiles * (w + 1) / 4;
+    constexpr int STEP = 4 * T::KEYS;
+    const int key_lo = split_lo + w * T::KEYS, key_hi = split_hi;
 
     // The lane's query row.
     const int row = it.tile * kBM + c;
@@ -206,19 +220,37 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
 
     PageWindow pw;
     pw.row = a.p.table + (size_t)it.b * pg.table_stride;
-    pw.fill(a.p, (split_lo + t_lo * T::KEYS) >> pg.ps_log2);
 
     bool poison = false;           // a masked tile's V held an infinity or a NaN
 
     // Whether every row of the item sees all of the tile.
-    auto all_seen = [&](const int (&pages)[T::KEYS / 16], int t0) {
+    auto all_seen = [&](const int (&pages)[T::GR], int t0) {
         bool whole = t0 + T::KEYS - 1 <= all_hi && t0 >= all_lo;
 #pragma unroll
-        for (int i = 0; i < T::KEYS / 16; ++i) whole = whole && pages[i] >= 0;
+        for (int i = 0; i < T::GR; ++i) whole = whole && pages[i] >= 0;
         return whole;
     };
 
-    auto step = [&](Tile<HD, I8>& t, int t0) {
+    Tile<HD, I8> t;
+    int pages[T::GR], next[T::GR];
+    // The tile at t0; the loads of the one at t1 take the registers as they fall
+    // free.  One copy of this code, and no branch around the loads: a wave runs
+    // it a few times per launch, so code that is fetched for one more copy costs
+    // microseconds, and with a branch the compiler loses count of the loads and
+    // waits for V where K would do.  (After its last tile a wave reads that tile
+    // once more, from the caches.)
+    auto step = [&](int t0, int t1) {
+        // ---- 8-bit scales: a lane prepares one key's, all read theirs back (wave's own LDS)
+        if constexpr (I8) {
+            const float v = v_scale_of(t.vs);
+            scales[w][0][lane] = t.ks;
+            scales[w][1][lane] = __builtin_amdgcn_logf(v);
+            scales[w][2][lane] = 1.f / v;
+            wave_lds_order();
+        }
+        auto scale4 = [&](int what, int j) {  // of the lane's keys in block j
+            return *reinterpret_cast<const f32x4*>(&scales[w][what][16 * g + 4 * j]);
+        };
         // ---- scores
         f32x4 s[T::NB];
 #pragma unroll
@@ -242,22 +274,28 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
                 }
             }
             if constexpr (I8) {
+                const f32x4 ks = scale4(0, j), lv = scale4(1, j);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[j][i] = fmaf(s[j][i] * t.ks[j][i], qscale, __builtin_amdgcn_logf(v_scale_of(t.vs[j][i])));
+                for (int i = 0; i < 4; ++i) s[j][i] = fmaf(s[j][i] * ks[i], qscale, lv[i]);
             } else {
                 s[j] *= qscale;
             }
         }
         // ---- mask: keys behind the row, before its window, in no page
         constexpr int QUART = T::KEYS / 4;
-        const bool whole = all_seen(t.pages, t0);
+#pragma unroll
+        for (int i = 0; i < T::GR; ++i) next[i] = pw.at(a.p, t1 + 16 * i);
+        load_k<HD, I8>(a, next, it.h, t1, t);
+        const bool whole = all_seen(pages, t0);
         uint32_t seen = 0xffffffffu;  // bit 4j + i: the lane's key 4j + i
         if (!whole) {
             const int gran = I8 ? g : g >> 1;
-            int page = t.pages[0];
-#pragma unroll
-            for (int i = 1; i < T::KEYS / 16; ++i) page = gran == i ? t.pages[i] : page;
+            const int p0 = pages[0], p1 = pages[1];
+            int page = gran & 1 ? p1 : p0;
+            if constexpr (T::GR == 4) {
+                const int p2 = pages[2], p3 = pages[3], q = gran & 1 ? p3 : p2;
+                page = gran & 2 ? q : page;
+            }
             const int key = t0 + QUART * g;
             seen = 0;
 #pragma unroll
@@ -290,18 +328,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
         f16x8 ph[T::NB / 2], pl[T::NB / 2];
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < T::NB; ++j)
+        for (int j = 0; j < T::NB; ++j) {
+            f32x4 iv;
+            if constexpr (I8) iv = scale4(2, j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = fast_exp2(s[j][i] - ms);
                 if constexpr (I8)
-                    sum += seen >> (4 * j + i) & 1 ? p * __builtin_amdgcn_rcpf(v_scale_of(t.vs[j][i])) : 0.f;
+                    sum += seen >> (4 * j + i) & 1 ? p * iv[i] : 0.f;
                 else
                     sum += p;
                 const int at = 4 * (j & 1) + i;
                 ph[j >> 1][at] = (f16)p;
                 pl[j >> 1][at] = (f16)(p - (float)(f16)p);
             }
+        }
+        if constexpr (I8) wave_lds_order();  // the next tile's scales go where these were
         l += sum;
         // ---- O^T += V^T P^T
         if constexpr (!I8) {
@@ -334,28 +376,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
                 o[d] = mfma16(vf, pl[0], o[d]);
             }
         }
+        load_v<HD, I8>(a, next, it.h, t1, t);
+#pragma unroll
+        for (int i = 0; i < T::GR; ++i) pages[i] = next[i];
     };
 
-    if (t_lo < t_hi) {
-        constexpr bool PIPE = HD <= 256;
-        Tile<HD, I8> t0, t1;
-        load_tile<HD, I8>(a, pw, it.h, split_lo + t_lo * T::KEYS, t0);
-        if constexpr (PIPE) {
-            int t = t_lo;
-            while (true) {
-                if (t + 1 < t_hi) load_tile<HD, I8>(a, pw, it.h, split_lo + (t + 1) * T::KEYS, t1);
-                step(t0, split_lo + t * T::KEYS);
-                if (++t >= t_hi) break;
-                if (t + 1 < t_hi) load_tile<HD, I8>(a, pw, it.h, split_lo + (t + 1) * T::KEYS, t0);
-                step(t1, split_lo + t * T::KEYS);
-                if (++t >= t_hi) break;
-            }
-        } else {
-            for (int t = t_lo; t < t_hi; ++t) {
-                if (t != t_lo) load_tile<HD, I8>(a, pw, it.h, split_lo + t * T::KEYS, t0);
-                step(t0, split_lo + t * T::KEYS);
-            }
-        }
+    // A window of pages at a time (1024 keys and more): within it no lookup
+    // waits, and the loads of two tiles stay counted apart.
+    for (int k0 = key_lo; k0 < key_hi;) {
+        pw.fill(a.p, k0);
+        const int k1 = imin(key_hi, pw.end(a.p));
+#pragma unroll
+        for (int i = 0; i < T::GR; ++i) pages[i] = pw.at(a.p, k0 + 16 * i);
+        load_k<HD, I8>(a, pages, it.h, k0, t);
+        __builtin_amdgcn_sched_barrier(0);  // K's loads before V's, as in the loop
+        load_v<HD, I8>(a, pages, it.h, k0, t);
+        for (; k0 < k1; k0 += STEP) step(k0, k0 + STEP < k1 ? k0 + STEP : k0);
     }
 
     if constexpr (!I8) {
@@ -370,9 +406,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 2 : 1) void paged_rows_kernel(AttnP
             f32x4 add[DT];
 #pragma unroll
             for (int d = 0; d < DT; ++d) add[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-            pw.fill(a.p, (split_lo + t_lo * T::KEYS) >> pg.ps_log2);
+            pw.fill(a.p, key_lo);
             const size_t step = (size_t)1 << pg.ps_log2;
-            for (int key = split_lo + t_lo * T::KEYS; key < split_lo + t_hi * T::KEYS; ++key) {
+            for (int key = key_lo; key < key_hi; ++key) {
+                if ((key - key_lo) % STEP == T::KEYS) key += STEP - T::KEYS;  // the other waves' tiles
+                if (key >= key_hi) break;
+                if (key >= pw.end(a.p)) pw.fill(a.p, key);
                 const int page = pw.at(a.p, key);
                 if (page < 0 || key > pos || key < seen_lo) continue;
                 const f16* e = reinterpret_cast<const f16*>(a.p.v) +
@@ -584,8 +623,10 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
 }
 
 // ------------------------------------------------------------------- host --
-constexpr int kRowsTarget = 512;   // items aimed at: two workgroups a CU
-constexpr int kRowsLeast = 2;      // units a split has at least (128 keys)
+// Items the rows kernel aims at: two rounds of the workgroups that the CUs hold
+// (two a CU up to head_dim 128, else one), so that uneven sequences level out.
+constexpr int rows_target(int hd) { return hd <= 128 ? 1024 : 512; }
+constexpr int kRowsLeast = 8;      // units a split has at least (512 keys)
 constexpr int kCus = 256;          // compute units of the target (MI355X)
 constexpr int kChunkLeast = 8;     // 64-key units a chunk's split has at least
 // Query rows a sequence may have per kv head for the rows kernel.
@@ -626,7 +667,7 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
         const int64_t seq_rows = chunks ? kRowsMost : most;
         int64_t tiles = row_tiles_bound(g, kBM);
         if (chunks) tiles = std::min<int64_t>(tiles, (int64_t)g.n_seq * ((kRowsMost + kBM - 1) / kBM));
-        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, kRowsTarget, kRowsLeast);
+        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, rows_target(hd), kRowsLeast);
         if (chunks) p.rows.hi_rows = kRowsMost;
     }
     if (chunks) {

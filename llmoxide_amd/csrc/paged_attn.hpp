@@ -132,24 +132,26 @@ __device__ __forceinline__ f16x8 i8x8_to_f16(uint32_t x, uint32_t y) {
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// The page of every 16-key granule of a wave's key range, 64 table entries at
-// a time in the wave's lanes, so that the loop's lookups wait on no memory.
+// The pages of a run of keys, 64 table entries in the wave's lanes, so that
+// lookups in a loop wait on no memory.  at() and lane_at() take keys of the
+// entries that fill() was given; keys of a tile whose first key is a multiple
+// of 64 never straddle two fills that begin at such a key.
 struct PageWindow {
     const int32_t* row;  // the sequence's table
     int first;           // entry in lane 0
     int ids;             // the lane's page, -1: none
-    __device__ __forceinline__ void fill(const PagedArgs& a, int entry) {
-        first = entry;
-        const int e = entry + (int)__lane_id();
+    __device__ __forceinline__ void fill(const PagedArgs& a, int key) {
+        first = key >> a.g.ps_log2;
+        const int e = first + (int)__lane_id();
         ids = e < a.g.table_stride ? paged_page(a.g, row[e]) : -1;
     }
-    // Page of key k (wave-uniform, >= 0).
-    __device__ __forceinline__ int at(const PagedArgs& a, int k) {
-        const int e = k >> a.g.ps_log2;
-        if (e - first >= 64) fill(a, e);
-        return __builtin_amdgcn_readlane(ids, e - first);
+    // One behind the last key of the window (a multiple of 64 where fill's was).
+    __device__ __forceinline__ int end(const PagedArgs& a) const { return (first + 64) << a.g.ps_log2; }
+    // Page of key k (wave-uniform).
+    __device__ __forceinline__ int at(const PagedArgs& a, int k) const {
+        return __builtin_amdgcn_readlane(ids, (k >> a.g.ps_log2) - first);
     }
-    // Page of the lane's own key, one of those that at() was last asked for.
+    // Page of the lane's own key.
     __device__ __forceinline__ int lane_at(const PagedArgs& a, int k) const {
         return __shfl(ids, (k >> a.g.ps_log2) - first, 64);
     }

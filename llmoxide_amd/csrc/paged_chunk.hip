@@ -144,9 +144,10 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int psm = (1 << pg.ps_log2) - 1;
     PageWindow pw;
     pw.row = a.p.table + (size_t)it.b * pg.table_stride;
-    pw.fill(a.p, k_lo >> pg.ps_log2);
+    pw.fill(a.p, k_lo);
     int pages[GR], next_pages[GR];
     auto look_up = [&](int t0, int (&p)[GR]) {
+        if (t0 >= pw.end(a.p)) pw.fill(a.p, t0);
 #pragma unroll
         for (int j = 0; j < GR; ++j) p[j] = pw.at(a.p, t0 + 16 * j);
     };
@@ -159,8 +160,13 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     float rs = 0.f;
     // Of four values, or two, the one at j.
     auto pick = [&](const int (&p)[GR], int j) {
-        if constexpr (GR == 2) return j ? p[1] : p[0];
-        else return j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+        const int p0 = p[0], p1 = p[1];
+        int x = j & 1 ? p1 : p0;
+        if constexpr (GR == 4) {
+            const int p2 = p[2], p3 = p[3], y = j & 1 ? p3 : p2;
+            x = j & 2 ? y : x;
+        }
+        return x;
     };
     // Offsets of the lane's chunks from a wave's base: K's transfers, and V's
     // even and odd ones where a tile lies in one page.
@@ -465,8 +471,9 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     f32x16 add;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) add[i] = 0.f;
-                    pw.fill(a.p, k_lo >> pg.ps_log2);
+                    pw.fill(a.p, k_lo);
                     for (int key = k_lo; key < k_hi; ++key) {
+                        if (key >= pw.end(a.p)) pw.fill(a.p, key);
                         const int page = pw.at(a.p, key);
                         if (page < 0 || key > pos[rb] || key < seen_lo[rb]) continue;
                         const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
