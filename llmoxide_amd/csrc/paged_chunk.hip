@@ -45,6 +45,11 @@ __device__ __forceinline__ int swizzle(int r) {
     return ROW_BYTES >= 256 ? r & 15 : ROW_BYTES == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 
+// 16 bytes of LDS at a byte address.
+__device__ __forceinline__ f16x8 lds16(uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(at);
+}
+
 template <int HD, int RB, int BN>
 struct ChunkTile {
     static constexpr int KS = HD / 16;   // k-steps of QK
@@ -168,21 +173,14 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         }
         return x;
     };
-    // Offsets of the lane's chunks from a wave's base: K's transfers, and V's
-    // even and odd ones where a tile lies in one page.
-    constexpr int DPT = 64 / CV;  // dims a transfer of V
-    uint32_t k_off[I8 ? 1 : T::LOADS], v_off[2];
-    if constexpr (!I8) {
-        constexpr int RPT = 64 / CH;  // rows a transfer
-#pragma unroll
-        for (int i = 0; i < T::LOADS; ++i) {
-            const int r = i * RPT + lane / CH + w * (BN / 4);
-            k_off[i] = (r - w * (BN / 4)) * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(r)) * 16);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-            v_off[x] = ((lane / CV) << (pg.ps_log2 + 1)) + (((lane % CV) ^ swizzle<BN * 2>(DPT * x + lane / CV)) * 16);
-    }
+    // Offsets of the lane's chunks in transfer 0 from a wave's base; transfer i's
+    // differ by the swizzle's bits that i moves (an XOR, as the bits of rows
+    // within a transfer and of transfers are apart).  V's: where a tile lies in
+    // one page.
+    constexpr int RPT = 64 / CH, DPT = 64 / CV;  // rows of K, dims of V a transfer
+    const int k_row0 = w * (BN / 4) + lane / CH;
+    const uint32_t k_off = (lane / CH) * (HD * 2) + (((lane % CH) ^ swizzle<HD * 2>(k_row0)) * 16);
+    const uint32_t v_off = ((lane / CV) << (pg.ps_log2 + 1)) + (((lane % CV) ^ swizzle<BN * 2>(lane / CV)) * 16);
     // f16: a wave copies BN / 4 rows of K and HD / 4 columns of V; lane l of a
     // transfer fills place l % CH (CV) of its row (column) l / CH (CV).
     auto fetch = [&](int t0, const int (&p)[GR], int stage) {
@@ -190,13 +188,14 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             const uint32_t lds = lds_addr(&tiles[stage][0]);
             const char* kb = a.p.k + (slab(pick(p, w * GR / 4)) + ((t0 + w * (BN / 4)) & psm)) * (HD * 2);
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) dma16(kb, k_off[i], lds + w * (BN / 4) * (HD * 2) + i * 1024);
+            for (int i = 0; i < T::LOADS; ++i)
+                dma16(kb + i * 1024, k_off ^ (swizzle<HD * 2>(RPT * i) * 16), lds + w * (BN / 4) * (HD * 2) + i * 1024);
             const uint32_t v_lds = lds + BN * HD * 2 + w * (HD / 4) * (BN * 2);
             if ((16 << pg.ps_log2) >= 16 * BN) {  // the tile lies in one page: a base for the wave, offsets that stay
                 const char* vb = a.p.v + (slab(p[0]) * HD + ((size_t)(w * (HD / 4)) << pg.ps_log2) + (t0 & psm)) * 2;
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i)
-                    dma16(vb + ((size_t)(DPT * i) << (pg.ps_log2 + 1)), v_off[i & 1], v_lds + i * 1024);
+                    dma16(vb + ((size_t)(DPT * i) << (pg.ps_log2 + 1)), v_off ^ (swizzle<BN * 2>(DPT * i) * 16), v_lds + i * 1024);
             } else {
                 // (of 64-key tiles, every other transfer's dims swap the halves of the keys)
                 const char* vb[2];
@@ -265,18 +264,25 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     // MFMA row l32 of a 32-key block stands for this key of it
     const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
 
+    const uint32_t k_lane = krow * (HD * 2) + ((hh ^ swizzle<HD * 2>(krow)) * 16);
+    const uint32_t v_lane = BN * HD * 2 + l32 * (BN * 2) + ((hh ^ swizzle<BN * 2>(l32)) * 16);
+
     // WHOLE: every row of the wave sees every key of the tile.
     auto compute = [&](auto whole_tag, int t0, const int (&p)[GR], int stage) {
         constexpr bool WHOLE = decltype(whole_tag)::value;
-        const f16* Ks = tiles[stage];
-        const f16* Vs = tiles[stage] + BN * HD;
+        // Operand addresses: of k-step 0; a k-step's chunk moves bits that an XOR
+        // reaches, blocks of rows lie constants apart.  (Opaque, so that they
+        // are made from one register here, not held in many across the loop.)
+        uint32_t k_at = lds_addr(&tiles[0][0]) + stage * (T::STAGE * 2) + k_lane;
+        uint32_t v_at = lds_addr(&tiles[0][0]) + stage * (T::STAGE * 2) + v_lane;
+        opaque(k_at);
+        opaque(v_at);
         f32x16 s[RB][KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            const f16* kr = &Ks[(32 * kb + krow) * HD];
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(&kr[((2 * k + hh) ^ swizzle<HD * 2>(krow)) * 8]);
+                const f16x8 kf = lds16((k_at ^ (32 * (k & 7))) + 256 * (k >> 3) + kb * (32 * HD * 2));
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     s[rb][kb] = mfma32(kf, qh[rb][k], k ? s[rb][kb] : f32x16{});
@@ -364,8 +370,9 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     }
                     if constexpr (I8) {
                         const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
-                        sum += p0 > 0.f || !(p0 == 0.f) ? p0 * iv[0] : 0.f;
-                        sum += p1 > 0.f || !(p1 == 0.f) ? p1 * iv[1] : 0.f;
+                        // (an unseen key's scale may be anything)
+                        sum = WHOLE || !(p0 == 0.f) ? fmaf(p0, iv[0], sum) : sum;
+                        sum = WHOLE || !(p1 == 0.f) ? fmaf(p1, iv[1], sum) : sum;
                     } else if constexpr (F32) {
                         sum += p0 + p1;
                     } else {
@@ -379,8 +386,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         for (int st = 0; st < ST; ++st)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const int dim = 32 * nb + l32;
-                f16x8 vf = *reinterpret_cast<const f16x8*>(&Vs[dim * BN + (((2 * st + hh) ^ swizzle<BN * 2>(dim)) * 8)]);
+                f16x8 vf = lds16((v_at ^ (32 * st)) + nb * (32 * BN * 2));
                 if constexpr (!I8 && !WHOLE) {  // as in the rows kernel: infinities and NaN that not all rows see
                     uint4 u = __builtin_bit_cast(uint4, vf);
                     bad |= nonfinite2(u.x) | nonfinite2(u.y) | nonfinite2(u.z) | nonfinite2(u.w);
@@ -522,9 +528,9 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 }
 
 // Row blocks a wave and workgroups a CU, by what fits the registers.
-constexpr int chunk_rb(int hd, bool, bool) { return hd == 64 ? 2 : 1; }
-constexpr int chunk_bn(int hd, bool, bool f32) { return hd == 256 || (hd == 128 && f32) ? 32 : 64; }
-constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd == 128 || (hd == 256 && !f32) ? 2 : 1; }
+constexpr int chunk_rb(int, bool, bool) { return 1; }
+constexpr int chunk_bn(int hd, bool i8, bool f32) { return (hd == 256 && (f32 || !i8)) || (hd == 128 && f32) ? 32 : 64; }
+constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd <= 128 || (!f32 && !i8) ? 2 : 1; }
 int chunk_rows(int hd, bool i8, bool f32) { return hd <= 256 ? 128 * chunk_rb(hd, i8, f32) : 0; }
 int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 

@@ -21,6 +21,7 @@ replays with what these tensors hold then.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -162,25 +163,39 @@ class PagedBatch:
         self.ref = ctypes.byref(self.desc)
 
 
+_current_device = None
+
+
 def _place(cache: PagedCache, batch: PagedBatch, *ts) -> None:
     """All on the current device: the stream a call takes is that device's."""
-    dev = cache.device
-    if batch.device != dev or dev.index != _torch().cuda.current_device():
+    global _current_device
+    if _current_device is None:
+        torch = _torch()
+        _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    at = cache.device.index
+    if batch.device.index != at or at != _current_device():
         raise ValueError("cache and batch must be on the current device")
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and (not t.is_cuda or t.get_device() != at):
             raise ValueError("tensors must be on the cache's device")
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_desc(n_heads: int, window: int, head: int, row: int, scale: float):
+    """(structure, reference) of an attention call's scalars."""
+    d = PagedAttnDesc(n_heads, window, head, row, scale)
+    return d, ctypes.byref(d)
 
 
 def _rows(t, n_tokens: int, width: int, what: str) -> int:
     """Row stride of a [n_tokens, width] tensor whose rows may be columns of a
     wider one (0: dense)."""
-    if t.dim() != 2 or t.shape[0] != n_tokens or t.shape[1] != width:
+    if t.shape != (n_tokens, width):
         raise ValueError(f"{what} is [{n_tokens}, {width}], not {list(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
+    row, col = t.stride()
+    if col != 1:
         raise ValueError(f"{what}'s rows must be contiguous")
-    s = t.stride(0)
-    return 0 if n_tokens == 1 or s == width else s
+    return 0 if n_tokens == 1 or row == width else row
 
 
 def _kv_rows(k, v, cache: PagedCache, batch: PagedBatch, names=("k", "v")):
@@ -189,10 +204,10 @@ def _kv_rows(k, v, cache: PagedCache, batch: PagedBatch, names=("k", "v")):
     some = k if k is not None else v
     if some is None:
         raise ValueError(f"{names[0]} or {names[1]} must be given")
-    stride = {_rows(t, batch.n_tokens, width, n) for t, n in ((k, names[0]), (v, names[1])) if t is not None}
-    if len(stride) > 1 or (k is not None and v is not None and k.dtype != v.dtype):
+    stride = _rows(some, batch.n_tokens, width, names[0] if k is not None else names[1])
+    if k is not None and v is not None and (_rows(v, batch.n_tokens, width, names[1]) != stride or v.dtype != k.dtype):
         raise ValueError(f"{names[0]} and {names[1]} have one dtype and one row stride")
-    return _dt_of(some.dtype), stride.pop()
+    return _dt_of(some.dtype), stride
 
 
 def paged_append(k, v, cache: PagedCache, batch: PagedBatch, *, stream=None) -> None:
@@ -283,21 +298,22 @@ def paged_attention(q, cache: PagedCache, batch: PagedBatch, *, n_heads: int, wi
     if not (n_heads - 1) * head + hd <= width <= n_heads * head:
         raise ValueError(f"q is [{batch.n_tokens}, {n_heads * head}], not {list(q.shape)}")
     _rows(q, batch.n_tokens, width, "q")
+    dt = _dt_of(q.dtype)
     if out is None:
         out = _new_out((batch.n_tokens, n_heads * hd), q.dtype, cache.device, stream)
     elif out.dtype != q.dtype or _rows(out, batch.n_tokens, n_heads * hd, "out"):
         raise ValueError("out is contiguous and of q's dtype")
     _place(cache, batch, q, out)
-    d = PagedAttnDesc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
-                      1.0 / math.sqrt(hd) if scale is None else scale)
+    dref = _attn_desc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
+                      1.0 / math.sqrt(hd) if scale is None else float(scale))[1]
     L = paged_lib()
-    dref = ctypes.byref(d)
     need = L.lmxp_attn_workspace_bytes(cache.ref, batch.ref, dref)
     ws_ptr, ws_bytes = None, 0
     if need:
         workspace = workspace or Workspace(device=cache.device)
-        workspace.ensure(need, stream)
+        if need > workspace.nbytes:
+            workspace.ensure(need, stream)
         ws_ptr, ws_bytes = workspace.base, workspace.nbytes
-    _check("lmxp_attn", L.lmxp_attn(cache.ref, batch.ref, dref, _ptr(q), _dt_of(q.dtype), _ptr(out), ws_ptr,
-                                    ws_bytes, _stream(stream)))
+    _check("lmxp_attn", L.lmxp_attn(cache.ref, batch.ref, dref, q.data_ptr(), dt, out.data_ptr(), ws_ptr, ws_bytes,
+                                    _stream(stream)))
     return out

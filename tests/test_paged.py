@@ -179,10 +179,17 @@ def test_bad_prologues_are_refused(kw, code):
     (dict(q_head_stride=132), S.E_SHAPE), (dict(q_head_stride=120), S.E_SHAPE), (dict(q_row_stride=504), S.E_SHAPE),
     (dict(window=1 << 30), S.E_SHAPE), (dict(q=FAKE + 8), S.E_ALIGN), (dict(out=FAR + 8), S.E_ALIGN),
     (dict(out=FAKE), S.E_SHAPE), (dict(out=FAKE + 4 * 512 * 4 - 16), S.E_SHAPE),
-    (dict(), S.E_WORKSPACE), (dict(ws=FAKE, ws_bytes=16), S.E_WORKSPACE), (dict(ws=FAKE + 8, ws_bytes=1 << 30), S.E_ALIGN),
 ])
 def test_bad_attention_calls_are_refused(kw, code):
     assert attn(**kw) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(), S.E_WORKSPACE), (dict(ws=FAKE, ws_bytes=16), S.E_WORKSPACE), (dict(ws=FAKE + 8, ws_bytes=1 << 30), S.E_ALIGN),
+])
+def test_a_split_attention_needs_its_workspace(kw, code):
+    """Contexts long enough to be cut between workgroups."""
+    assert attn(b=batch(max_ctx=4096, table_stride=256), **kw) == code
 
 
 def test_null_descriptions_are_refused():
