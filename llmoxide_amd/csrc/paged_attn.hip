@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     const int c = lane & 15, g = lane >> 4;
 
     Item it;
-    if (!find_item(a, blockIdx.x, kBM, true, it)) return;
+    if (!find_item(a, blockIdx.x, kBM, true, false, it)) return;
     const PagedGeom& pg = a.p.g;
     if (it.split == 0 && tid == 0 && it.tile < a.rt_max)
         a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile] = make_int4(it.first, it.stride, it.splits, 0);
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
     __shared__ float ex_m[NG], ex_l[NG];
     const PagedGeom& pg = a.p.g;
     Item it;
-    if (!find_item(a, blockIdx.x / rows, bm, false, it)) return;
+    if (!find_item(a, blockIdx.x / rows, bm, false, false, it)) return;
     const PagedSeq& s = it.s;
     const int h = it.h, row = it.tile * bm + blockIdx.x % rows;
     if (row >= s.n * pg.G || it.tile >= a.rt_max) return;
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
     const PagedGeom& pg = a.p.g;
     const int per = bm / kMergeRows;
     Item it;
-    if (!find_item(a, blockIdx.x / per, bm, false, it) || it.tile >= a.rt_max) return;
+    if (!find_item(a, blockIdx.x / per, bm, false, false, it) || it.tile >= a.rt_max) return;
     const int4 info = a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile];
     const int splits = imin(info.z, a.n_items);  // written by this call's split 0; in range whatever it holds
     if (splits <= 1) return;

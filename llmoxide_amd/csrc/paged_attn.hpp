@@ -53,11 +53,29 @@ __device__ __forceinline__ void load_work(const AttnPagedArgs& a, int b, int bm,
 // replay.  Each lane takes a sequence (64 at a time); the total of units x
 // row tiles decides how long a split is, a scan over the sequences' item
 // counts finds the one that holds `id`.  False: no such item.
-__device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm, bool splits_on, Item& o) {
+// `longest_first`: of 64 sequences, those with the longest reach come first.
+__device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm, bool splits_on, bool longest_first,
+                                          Item& o) {
     const int lane = __lane_id(), Hkv = a.p.g.Hkv;
     PagedSeq s;
     SeqWork w;
-    load_work(a, lane, bm, s, w);
+    int b;
+    auto load = [&](int c0) {
+        b = c0 + lane;
+        load_work(a, b, bm, s, w);
+        const int n = min(64, a.p.g.n_seq - c0);
+        if (!longest_first || n == 1) return;
+        int rank = 0;
+        for (int j = 0; j < n; ++j) {
+            const int u = __builtin_amdgcn_readlane(w.units, j);
+            rank += u > w.units || (u == w.units && j < lane);
+        }
+        // lanes behind the last sequence, of no work, stay where they are
+        const int to = 4 * (lane < n ? rank : lane);
+        auto put = [&](int& x) { x = __builtin_amdgcn_ds_permute(to, x); };
+        put(b), put(s.row0), put(s.n), put(s.ctx), put(w.rt), put(w.lo), put(w.units);
+    };
+    load(0);
     o.per = 1000000000;
     if (splits_on) {
         float work = (float)w.rt * (float)w.units;
@@ -77,7 +95,7 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
         if (has) {
             const int l = __builtin_ctzll(has);
             auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            o.b = c0 + l;
+            o.b = get(b);
             o.s = PagedSeq{get(s.row0), get(s.n), get(s.ctx)};
             o.w = SeqWork{get(w.rt), get(w.lo), get(w.units)};
             o.splits = seq_splits(o.w, o.per);
@@ -97,7 +115,7 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
         base += __builtin_amdgcn_readlane(upto, 63);
         c0 += 64;
         if (c0 >= a.p.g.n_seq) return false;
-        load_work(a, c0 + lane, bm, s, w);
+        load(c0);
     }
 }
 

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     __shared__ __align__(16) float scales[I8 ? 2 : 1][3][BN];  // K's, log2 of V's, 1 / V's
 
     Item it;
-    if (!find_item(a, blockIdx.x, BM, true, it)) return;
+    if (!find_item(a, blockIdx.x, BM, true, true, it)) return;
     const PagedGeom& pg = a.p.g;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hh = lane >> 5;
