@@ -26,6 +26,8 @@
  *   ctx_lens    int32 [n_seq], each at most max_ctx and at least its new rows
  *   max_new     at least the largest number of new rows of a sequence
  *   max_ctx     at most table_stride * page_size
+ * A call whose work would take 2^24 workgroups or more (some 10^8 row heads) is
+ * refused with LMX_E_SHAPE.
  * cu, ctx_lens and page_table are read on the device, so a captured graph
  * replays with the lengths that they hold then.  A position whose table entry
  * is not in [0, n_pages) is in no page: it is not stored, reads back as 0 and
@@ -135,7 +137,8 @@ lmx_status lmxp_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  * that are in a page, pos being the row's position.  The batch's own rows are
  * read from the pages: append them first.  A row that sees no position, or
  * whose every score is -infinity, gets zeros.  What a row does not see has no
- * part in its result, infinities and NaN included.
+ * part in its result, infinities and NaN included.  An 8-bit V scale below
+ * 2^-90 (values below 1e-25) is taken as 2^-90.
  *   dt   LMX_F16: q and out are f16; the weights p are rounded to f16 before
  *        they meet V where chunks are long, the sums are fp32.
  *        LMX_F32: q and out are f32; q and p are carried as two f16 parts each

@@ -637,8 +637,11 @@ struct Part {
     bool on, splits;
     int bm, lo_rows, hi_rows, target, least, rt_max;
     int64_t items;  // workgroups: an upper bound of its items
+    int64_t merge;  // workgroups of its merge
     size_t o_bytes, ml_bytes, rows_bytes;
     size_t bytes() const { return o_bytes + ml_bytes + rows_bytes; }
+    // 256 threads a workgroup are counted in 32 bits
+    bool fits() const { return items < (1 << 24) && merge < (1 << 24); }
 };
 static Part make_part(const PagedGeom& g, int hd, int bm, int64_t tiles, int64_t seq_rows, bool splits, int target, int least) {
     Part r{};
@@ -653,6 +656,8 @@ static Part make_part(const PagedGeom& g, int hd, int bm, int64_t tiles, int64_t
     r.ml_bytes = r.splits ? (size_t)r.items * bm * 8 : 0;
     r.rows_bytes = r.splits ? ((size_t)g.n_seq * g.Hkv * r.rt_max * 16) : 0;
     r.hi_rows = 0x7fffffff;
+    // a workgroup of the merge takes a row, of a chunk's tiles kMergeRows
+    r.merge = r.splits ? tiles * g.Hkv * (bm == kBM ? std::min<int64_t>(bm, (int64_t)g.max_new * g.G) : bm / kMergeRows) : 0;
     return r;
 }
 struct Plan {
@@ -661,7 +666,7 @@ struct Plan {
 static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     Plan p{};
     const int64_t most = (int64_t)g.max_new * g.G;  // rows of a sequence
-    const int cm = chunk_rows(hd, i8, f32);
+    const int cm = chunk_rows(hd);
     const bool chunks = cm && most > kRowsMost;
     if (!chunks || g.n_seq > 1) {
         const int64_t seq_rows = chunks ? kRowsMost : most;
@@ -680,15 +685,17 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     return p;
 }
 
-size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
+// The workspace that a call of either type needs; false where its launches could not name their work.
+bool paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, size_t* bytes) {
     PagedGeom g = paged_args(p, b).g;
     g.G = (int)(d->n_heads / p->n_kv_heads);
-    size_t most = 0;
+    *bytes = 0;
     for (bool f32 : {false, true}) {
         const Plan pl = make_plan(g, (int)p->head_dim, p->store == LMXP_I8, f32);
-        most = std::max(most, pl.rows.bytes() + pl.chunk.bytes());
+        if (!pl.rows.fits() || !pl.chunk.fits()) return false;
+        *bytes = std::max(*bytes, pl.rows.bytes() + pl.chunk.bytes());
     }
-    return most;
+    return true;
 }
 
 template <int HD>
@@ -716,14 +723,14 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     LMX_CHECK_LAUNCH();
     if (r.splits) {
         if (chunk) {
-            const dim3 mgrid((unsigned)(r.items - r.target) * (unsigned)(r.bm / kMergeRows));
+            const dim3 mgrid((unsigned)r.merge);
             if (f32) hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm);
             else hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm);
             LMX_CHECK_LAUNCH();
             return LMX_OK;
         }
         const int rows = (int)std::min<int64_t>(r.bm, (int64_t)a.p.g.max_new * a.p.g.G);
-        const dim3 mgrid((unsigned)(r.items - r.target) * (unsigned)rows);
+        const dim3 mgrid((unsigned)r.merge);
         if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
         else hipLaunchKernelGGL((paged_merge_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm, rows);
         LMX_CHECK_LAUNCH();

@@ -1,8 +1,8 @@
 // Attention of prompt chunks over pages on gfx950 (MFMA-bound).
 //
-// A workgroup takes a tile of 128 * RB query rows of one kv head (row r: token
+// A workgroup takes a tile of 128 query rows of one kv head (row r: token
 // r / G, head r % G, so that all heads of a group share the tile's keys) and
-// walks its 64-key tiles; four waves of 32 * RB rows share each K/V tile in
+// walks its 64-key tiles; four waves of 32 rows share each K/V tile in
 // LDS.  As in the rows kernel the products are computed transposed,
 //   S^T = K Q^T, O^T += V^T P^T   on v_mfma_f32_32x32x16_f16,
 // Q^T in registers for the whole walk.  The keys that MFMA row r of a 32-key
@@ -50,11 +50,11 @@ __device__ __forceinline__ f16x8 lds16(uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(at);
 }
 
-template <int HD, int RB, int BN>
+template <int HD, int BN>
 struct ChunkTile {
     static constexpr int KS = HD / 16;   // k-steps of QK
     static constexpr int NB = HD / 32;   // 32-dim blocks of the output
-    static constexpr int BM = 128 * RB;  // rows a workgroup
+    static constexpr int BM = 128;  // rows a workgroup
     static constexpr int KB = BN / 32;   // 32-key blocks a tile
     static constexpr int ST = BN / 16;   // k-steps of PV
     static constexpr int GR = BN / 16;   // 16-key granules a tile, each in one page
@@ -64,10 +64,10 @@ struct ChunkTile {
     static constexpr int STAGE = 2 * BN * HD;     // halfs: K then V
 };
 
-// BN: keys a tile.  RB: 32-row blocks a wave.  OCC: workgroups a CU.
-template <int HD, bool I8, bool F32, int RB, int BN, int OCC>
+// BN: keys a tile.  OCC: workgroups a CU.
+template <int HD, bool I8, bool F32, int BN, int OCC>
 __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) {
-    using T = ChunkTile<HD, RB, BN>;
+    using T = ChunkTile<HD, BN>;
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH, KB = T::KB, ST = T::ST, GR = T::GR, CV = T::CV;
     constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
@@ -93,55 +93,49 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int k_hi = imin(pos_of(r1) + 1, split_hi);  // one behind the last key
     const int n_t = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
     // the wave's: keys some row sees, keys all rows see
-    const int w0 = r0 + w * 32 * RB, w1 = imin(w0 + 32 * RB, n_rows) - 1;
+    const int w0 = r0 + w * 32, w1 = imin(w0 + 32, n_rows) - 1;
     const bool live = w0 <= r1;
     const int any_hi = live ? pos_of(w1) : -1, all_hi = live ? pos_of(w0) : -1;
     const int any_lo = live ? low_of(pos_of(w0)) : 0, all_lo = live ? low_of(pos_of(w1)) : 0;
 
-    int pos[RB], seen_lo[RB];
-    float qs[RB];  // what a score is multiplied by
-    f16x8 qh[RB][KS], ql[F32 ? RB : 1][F32 ? KS : 1];
+    f16x8 qh[KS], ql[F32 ? KS : 1];
+    const int row = w0 + l32;
+    const bool have = row < n_rows;
+    const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
+    const int pos = have ? first_pos + tok : -1, seen_lo = low_of(pos);
+    float qs = a.c;  // what a score is multiplied by
+    const QT* qr = static_cast<const QT*>(a.q) + (size_t)(it.s.row0 + tok) * a.q_row_stride + head * a.q_head_stride + 8 * hh;
+    if constexpr (F32) {
+        float m = 0.f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int row = w0 + 32 * rb + l32;
-        const bool have = row < n_rows;
-        const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
-        pos[rb] = have ? first_pos + tok : -1;
-        seen_lo[rb] = low_of(pos[rb]);
-        qs[rb] = a.c;
-        const QT* qr = static_cast<const QT*>(a.q) + (size_t)(it.s.row0 + tok) * a.q_row_stride + head * a.q_head_stride + 8 * hh;
-        if constexpr (F32) {
-            float m = 0.f;
+        for (int k = 0; k < KS; ++k) {
+            float x[8];
+            load_f32<8>(qr + 16 * k, x);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                float x[8];
-                load_f32<8>(qr + 16 * k, x);
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+        }
+        m = fmaxf(m, shfl_xor(m, 32));
+        int e = 0;  // the row's largest element to [2^14, 2^15), as in the rows kernel
+        if (m > 0.f && m < INFINITY) e = 15 - __builtin_amdgcn_frexp_expf(m);
+        e = imin(imax(e, -120), 120);
+        const float up = ldexpf(1.f, e);
+        qs = ldexpf(a.c, -e);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+        for (int k = 0; k < KS; ++k) {
+            float x[8];
+            load_f32<8>(qr + 16 * k, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = have ? x[j] * up : 0.f;
+                qh[k][j] = (f16)y;
+                ql[k][j] = (f16)(y - (float)(f16)y);
             }
-            m = fmaxf(m, shfl_xor(m, 32));
-            int e = 0;  // the row's largest element to [2^14, 2^15), as in the rows kernel
-            if (m > 0.f && m < INFINITY) e = 15 - __builtin_amdgcn_frexp_expf(m);
-            e = imin(imax(e, -120), 120);
-            const float up = ldexpf(1.f, e);
-            qs[rb] = ldexpf(a.c, -e);
+        }
+    } else {
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                float x[8];
-                load_f32<8>(qr + 16 * k, x);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = have ? x[j] * up : 0.f;
-                    qh[rb][k][j] = (f16)y;
-                    ql[rb][k][j] = (f16)(y - (float)(f16)y);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                qh[rb][k] = *reinterpret_cast<const f16x8*>(qr + 16 * k);
-                if (!have) qh[rb][k] = f16x8{};
-            }
+        for (int k = 0; k < KS; ++k) {
+            qh[k] = *reinterpret_cast<const f16x8*>(qr + 16 * k);
+            if (!have) qh[k] = f16x8{};
         }
     }
 
@@ -248,17 +242,12 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         }
     };
 
-    f32x16 o[RB][NB];
-    float m[RB], l[RB];
+    f32x16 o[NB];
+    float m = pos < 0 ? 0.f : -INFINITY, l = 0.f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        m[rb] = pos[rb] < 0 ? 0.f : -INFINITY;
-        l[rb] = 0.f;
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[rb][nb][i] = 0.f;
-    }
+        for (int i = 0; i < 16; ++i) o[nb][i] = 0.f;
     bool poison = false;
 
     // MFMA row l32 of a 32-key block stands for this key of it
@@ -277,21 +266,18 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         uint32_t v_at = lds_addr(&tiles[0][0]) + stage * (T::STAGE * 2) + v_lane;
         opaque(k_at);
         opaque(v_at);
-        f32x16 s[RB][KB];
+        f32x16 s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 const f16x8 kf = lds16((k_at ^ (32 * (k & 7))) + 256 * (k >> 3) + kb * (32 * HD * 2));
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    s[rb][kb] = mfma32(kf, qh[rb][k], k ? s[rb][kb] : f32x16{});
-                    if constexpr (F32) s[rb][kb] = mfma32(kf, ql[rb][k], s[rb][kb]);
-                }
+                s[kb] = mfma32(kf, qh[k], k ? s[kb] : f32x16{});
+                if constexpr (F32) s[kb] = mfma32(kf, ql[k], s[kb]);
             }
         }
         {
-            constexpr int N = KB * KS, PER = RB * (F32 ? 2 : 1), AHEAD = N < kAhead ? N : kAhead;
+            constexpr int N = KB * KS, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -300,87 +286,84 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             }
         }
         // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
-        f16x8 ph[RB][ST], pl[F32 ? RB : 1][F32 ? ST : 1];
+        f16x8 ph[ST], pl[F32 ? ST : 1];
+        float mb = m == -INFINITY ? 0.f : m;
+        float top = -INFINITY;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float mb = m[rb] == -INFINITY ? 0.f : m[rb];
-            float top = -INFINITY;
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {  // four registers: keys 32 kb + 16 (q/2) + 8 hh + 4 (q%2) ..
-                    f32x4 ks, lv;
-                    if constexpr (I8) {
-                        const int at = 32 * kb + 16 * (q >> 1) + 8 * hh + 4 * (q & 1);
-                        ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][at]);
-                        lv = *reinterpret_cast<const f32x4*>(&scales[stage][1][at]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = s[rb][kb][4 * q + e];
-                        if constexpr (I8)
-                            s[rb][kb][4 * q + e] = fmaf(x * ks[e], qs[rb], lv[e] - mb);
-                        else
-                            s[rb][kb][4 * q + e] = fmaf(x, qs[rb], -mb);
-                    }
+            for (int q = 0; q < 4; ++q) {  // four registers: keys 32 kb + 16 (q/2) + 8 hh + 4 (q%2) ..
+                f32x4 ks, lv;
+                if constexpr (I8) {
+                    const int at = 32 * kb + 16 * (q >> 1) + 8 * hh + 4 * (q & 1);
+                    ks = *reinterpret_cast<const f32x4*>(&scales[stage][0][at]);
+                    lv = *reinterpret_cast<const f32x4*>(&scales[stage][1][at]);
                 }
-            if constexpr (!WHOLE) {
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = t0 + 32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7);
-                        const bool on = p[2 * kb + (i >> 3)] >= 0 && key <= pos[rb] && key >= seen_lo[rb];
-                        if (!on) s[rb][kb][i] = -INFINITY;
-                    }
-            }
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rb][kb][i]);
-            if (__ballot(top > kMost || m[rb] == -INFINITY)) {
-                top = fmaxf(top, shfl_xor(top, 32));
-                float mn = m[rb];
-                if (mn == -INFINITY)
-                    mn = top > -INFINITY ? top - kLift : -INFINITY;  // mb = 0
-                else if (top > kMost)
-                    mn = mb + top - kLift;
-                const float f = m[rb] == -INFINITY ? 0.f : fast_exp2(m[rb] - mn);
-                const float delta = mn == -INFINITY ? 0.f : mn - mb;
-                m[rb] = mn;
-                l[rb] *= f;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[rb][nb] *= f;
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[rb][kb] -= delta;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p0 = fast_exp2(s[rb][kb][i]), p1 = fast_exp2(s[rb][kb][i + 1]);
-                    const f16x2 hi = __builtin_convertvector(f32x2{p0, p1}, f16x2);
-                    ph[rb][2 * kb + (i >> 3)][i & 7] = hi[0];
-                    ph[rb][2 * kb + (i >> 3)][(i & 7) + 1] = hi[1];
-                    if constexpr (F32) {
-                        const f16x2 lo = __builtin_convertvector(f32x2{p0 - (float)hi[0], p1 - (float)hi[1]}, f16x2);
-                        pl[rb][2 * kb + (i >> 3)][i & 7] = lo[0];
-                        pl[rb][2 * kb + (i >> 3)][(i & 7) + 1] = lo[1];
-                    }
-                    if constexpr (I8) {
-                        const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
-                        // (an unseen key's scale may be anything)
-                        sum = WHOLE || !(p0 == 0.f) ? fmaf(p0, iv[0], sum) : sum;
-                        sum = WHOLE || !(p1 == 0.f) ? fmaf(p1, iv[1], sum) : sum;
-                    } else if constexpr (F32) {
-                        sum += p0 + p1;
-                    } else {
-                        sum = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, sum, false);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const float x = s[kb][4 * q + e];
+                    if constexpr (I8)
+                        s[kb][4 * q + e] = fmaf(x * ks[e], qs, lv[e] - mb);
+                    else
+                        s[kb][4 * q + e] = fmaf(x, qs, -mb);
                 }
-            l[rb] += sum;
+            }
+        if constexpr (!WHOLE) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = t0 + 32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7);
+                    const bool on = p[2 * kb + (i >> 3)] >= 0 && key <= pos && key >= seen_lo;
+                    if (!on) s[kb][i] = -INFINITY;
+                }
         }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+        if (__ballot(top > kMost || m == -INFINITY)) {
+            top = fmaxf(top, shfl_xor(top, 32));
+            float mn = m;
+            if (mn == -INFINITY)
+                mn = top > -INFINITY ? top - kLift : -INFINITY;  // mb = 0
+            else if (top > kMost)
+                mn = mb + top - kLift;
+            const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            const float delta = mn == -INFINITY ? 0.f : mn - mb;
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) o[nb] *= f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] -= delta;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float p0 = fast_exp2(s[kb][i]), p1 = fast_exp2(s[kb][i + 1]);
+                const f16x2 hi = __builtin_convertvector(f32x2{p0, p1}, f16x2);
+                ph[2 * kb + (i >> 3)][i & 7] = hi[0];
+                ph[2 * kb + (i >> 3)][(i & 7) + 1] = hi[1];
+                if constexpr (F32) {
+                    const f16x2 lo = __builtin_convertvector(f32x2{p0 - (float)hi[0], p1 - (float)hi[1]}, f16x2);
+                    pl[2 * kb + (i >> 3)][i & 7] = lo[0];
+                    pl[2 * kb + (i >> 3)][(i & 7) + 1] = lo[1];
+                }
+                if constexpr (I8) {
+                    const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
+                    // (an unseen key's scale may be anything)
+                    sum = WHOLE || !(p0 == 0.f) ? fmaf(p0, iv[0], sum) : sum;
+                    sum = WHOLE || !(p1 == 0.f) ? fmaf(p1, iv[1], sum) : sum;
+                } else if constexpr (F32) {
+                    sum += p0 + p1;
+                } else {
+                    sum = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, sum, false);
+                }
+            }
+        l += sum;
         uint32_t bad = 0;
 #pragma unroll
         for (int st = 0; st < ST; ++st)
@@ -393,14 +376,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     u = uint4{finite2(u.x), finite2(u.y), finite2(u.z), finite2(u.w)};
                     vf = __builtin_bit_cast(f16x8, u);
                 }
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    o[rb][nb] = mfma32(vf, ph[rb][st], o[rb][nb]);
-                    if constexpr (F32) o[rb][nb] = mfma32(vf, pl[rb][st], o[rb][nb]);
-                }
+                o[nb] = mfma32(vf, ph[st], o[nb]);
+                if constexpr (F32) o[nb] = mfma32(vf, pl[st], o[nb]);
                 if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // few operands in flight: registers
             }
-        if constexpr (WHOLE && !I8 && RB == 1) {
+        if constexpr (WHOLE && !I8) {
             // the first operands are on their way during the first weights'
             // exponentials; the others' run beside the products
             constexpr int N = ST * NB, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
@@ -460,83 +440,78 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     }
 
     // ---- results
+    if constexpr (!I8) {
+        float z = 0.f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int row = w0 + 32 * rb + l32;
-        if constexpr (!I8) {
-            float z = 0.f;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int i = 0; i < 16; ++i) z = fmaf(o[nb][i], 0.f, z);
+        if (poison || __ballot(z != 0.f)) {
+            // rare, as in the rows kernel: V's infinities and NaN go to the rows that see them
+            const size_t step = (size_t)1 << pg.ps_log2;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) z = fmaf(o[rb][nb][i], 0.f, z);
-            if (poison || __ballot(z != 0.f)) {
-                // rare, as in the rows kernel: V's infinities and NaN go to the rows that see them
-                const size_t step = (size_t)1 << pg.ps_log2;
+            for (int nb = 0; nb < NB; ++nb) {
+                f32x16 add;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    f32x16 add;
+                for (int i = 0; i < 16; ++i) add[i] = 0.f;
+                pw.fill(a.p, k_lo);
+                for (int key = k_lo; key < k_hi; ++key) {
+                    if (key >= pw.end(a.p)) pw.fill(a.p, key);
+                    const int page = pw.at(a.p, key);
+                    if (page < 0 || key > pos || key < seen_lo) continue;
+                    const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
+                                   ((32 * nb + 4 * hh) << pg.ps_log2);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) add[i] = 0.f;
-                    pw.fill(a.p, k_lo);
-                    for (int key = k_lo; key < k_hi; ++key) {
-                        if (key >= pw.end(a.p)) pw.fill(a.p, key);
-                        const int page = pw.at(a.p, key);
-                        if (page < 0 || key > pos[rb] || key < seen_lo[rb]) continue;
-                        const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
-                                       ((32 * nb + 4 * hh) << pg.ps_log2);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float y = (float)*e;
-                            if (!(fabsf(y) < INFINITY)) add[i] += y;
-                            e += (i & 3) < 3 ? step : 5 * step;  // dims 32 nb + 8 (i/4) + 4 hh + i%4
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const float y = (float)*e;
+                        if (!(fabsf(y) < INFINITY)) add[i] += y;
+                        e += (i & 3) < 3 ? step : 5 * step;  // dims 32 nb + 8 (i/4) + 4 hh + i%4
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!(fabsf(add[i]) < INFINITY)) o[rb][nb][i] = add[i];
                 }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(fabsf(add[i]) < INFINITY)) o[nb][i] = add[i];
             }
         }
-        float sum = l[rb] + shfl_xor(l[rb], 32);
-        if (row >= n_rows) continue;
-        if (it.splits > 1) {
-            const size_t at = (size_t)(it.first + it.split * it.stride) * BM + (row - r0);
-            float* dst = a.part_o + at * HD;
+    }
+    float sum = l + shfl_xor(l, 32);
+    if (row >= n_rows) return;
+    if (it.splits > 1) {
+        const size_t at = (size_t)(it.first + it.split * it.stride) * BM + (row - r0);
+        float* dst = a.part_o + at * HD;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
-                        f32x4{o[rb][nb][4 * q], o[rb][nb][4 * q + 1], o[rb][nb][4 * q + 2], o[rb][nb][4 * q + 3]};
-            if (hh == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m[rb], sum};
-        } else {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            QT* dst = static_cast<QT*>(a.out) +
-                      ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD;
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
+                    f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]};
+        if (hh == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m, sum};
+    } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        QT* dst = static_cast<QT*>(a.out) +
+                  ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 y = f32x4{o[rb][nb][4 * q], o[rb][nb][4 * q + 1], o[rb][nb][4 * q + 2], o[rb][nb][4 * q + 3]} * inv;
-                    if constexpr (F32)
-                        *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) = y;
-                    else
-                        *reinterpret_cast<f16x4*>(dst + 32 * nb + 8 * q + 4 * hh) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
-                }
-        }
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 y = f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]} * inv;
+                if constexpr (F32)
+                    *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) = y;
+                else
+                    *reinterpret_cast<f16x4*>(dst + 32 * nb + 8 * q + 4 * hh) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+            }
     }
 }
 
-// Row blocks a wave and workgroups a CU, by what fits the registers.
-constexpr int chunk_rb(int, bool, bool) { return 1; }
+// Keys a tile and workgroups a CU, by what fits the registers.
 constexpr int chunk_bn(int hd, bool i8, bool f32) { return (hd == 256 && (f32 || !i8)) || (hd == 128 && f32) ? 32 : 64; }
 constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd <= 128 || (!f32 && !i8) ? 2 : 1; }
-int chunk_rows(int hd, bool i8, bool f32) { return hd <= 256 ? 128 * chunk_rb(hd, i8, f32) : 0; }
+int chunk_rows(int hd) { return hd <= 256 ? 128 : 0; }
 int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_rb(HD, I8, F32), chunk_bn(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_bn(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
 }
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
     auto by = [&](auto tag) {

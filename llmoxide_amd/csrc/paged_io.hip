@@ -709,6 +709,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
 // Heads a workgroup that makes its rows' angles once for them; short batches
 // take a head each, so that the heads run side by side.
 static int heads_a_group(uint32_t n_tokens) { return n_tokens <= 1024 ? 1 : 4; }
+// A grid that the launch can name: 256 threads a workgroup in 32 bits, and 16 bits across.
+static bool grid_fits(int64_t x, int64_t y) { return x < (1 << 24) && y < (1 << 16); }
 // Batches of few rows a sequence: whole granules are rare, and a block of rows
 // would be a row or two.
 static bool few_rows(const PagedGeom& g) { return g.max_new <= 4; }
@@ -720,21 +722,23 @@ static lmx_status launch_store_hd(const StoreArgs& a, int hd, hipStream_t st) {
         using L = RowLanes<HD>;
         if (few_rows(a.p.g)) {
             const int64_t units = (int64_t)a.p.g.n_tokens * (a.n_k + a.n_v + a.n_q);
-            const dim3 grid((unsigned)((units + 4 * L::RPI - 1) / (4 * L::RPI)));
-            hipLaunchKernelGGL((paged_store_tokens_kernel<SRC, I8, HD, PRO>), grid, dim3(256), 0, st, a);
+            const int64_t x = (units + 4 * L::RPI - 1) / (4 * L::RPI);
+            if (!grid_fits(x, 1)) return LMX_E_SHAPE;
+            hipLaunchKernelGGL((paged_store_tokens_kernel<SRC, I8, HD, PRO>), dim3((unsigned)x), dim3(256), 0, st, a);
         } else {
-            const dim3 grid((unsigned)row_blocks_bound(a.p.g, L::LOG2_R), a.g_k + a.g_v + a.g_q);
-            hipLaunchKernelGGL((paged_store_kernel<SRC, I8, HD, PRO>), grid, dim3(256), 0, st, a);
+            const int64_t x = row_blocks_bound(a.p.g, L::LOG2_R), y = a.g_k + a.g_v + a.g_q;
+            if (!grid_fits(x, y)) return LMX_E_SHAPE;
+            hipLaunchKernelGGL((paged_store_kernel<SRC, I8, HD, PRO>), dim3((unsigned)x, (unsigned)y), dim3(256), 0, st, a);
         }
+        LMX_CHECK_LAUNCH();
+        return LMX_OK;
     };
     switch (hd) {
-        case 64: go(std::integral_constant<int, 64>{}); break;
-        case 128: go(std::integral_constant<int, 128>{}); break;
-        case 256: go(std::integral_constant<int, 256>{}); break;
-        default: go(std::integral_constant<int, 512>{}); break;
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 128: return go(std::integral_constant<int, 128>{});
+        case 256: return go(std::integral_constant<int, 256>{});
+        default: return go(std::integral_constant<int, 512>{});
     }
-    LMX_CHECK_LAUNCH();
-    return LMX_OK;
 }
 
 lmx_status paged_append(const lmxp_pool* p, const lmxp_batch* b, const void* k_new, const void* v_new,
@@ -794,17 +798,18 @@ template <typename OUT, bool I8>
 static lmx_status launch_read(const ReadArgs& a, int hd, hipStream_t st) {
     auto go = [&](auto tag) {
         constexpr int HD = decltype(tag)::value;
-        const dim3 grid((unsigned)row_blocks_bound(a.p.g, RowLanes<HD>::LOG2_R), a.g_k + a.g_v);
-        hipLaunchKernelGGL((paged_read_kernel<OUT, I8, HD>), grid, dim3(256), 0, st, a);
+        const int64_t x = row_blocks_bound(a.p.g, RowLanes<HD>::LOG2_R), y = a.g_k + a.g_v;
+        if (!grid_fits(x, y)) return LMX_E_SHAPE;
+        hipLaunchKernelGGL((paged_read_kernel<OUT, I8, HD>), dim3((unsigned)x, (unsigned)y), dim3(256), 0, st, a);
+        LMX_CHECK_LAUNCH();
+        return LMX_OK;
     };
     switch (hd) {
-        case 64: go(std::integral_constant<int, 64>{}); break;
-        case 128: go(std::integral_constant<int, 128>{}); break;
-        case 256: go(std::integral_constant<int, 256>{}); break;
-        default: go(std::integral_constant<int, 512>{}); break;
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 128: return go(std::integral_constant<int, 128>{});
+        case 256: return go(std::integral_constant<int, 256>{});
+        default: return go(std::integral_constant<int, 512>{});
     }
-    LMX_CHECK_LAUNCH();
-    return LMX_OK;
 }
 
 lmx_status paged_read(const lmxp_pool* p, const lmxp_batch* b, void* k_out, void* v_out, lmx_dtype out_dt,

@@ -208,6 +208,22 @@ def test_counts_that_pass_32_bits_are_refused():
                                                  table_stride=1 << 25)) == S.E_SHAPE
 
 
+def test_launches_too_large_to_name_are_refused():
+    """2^24 workgroups and more, or 2^16 heads side by side."""
+    many = batch(n_seq=1 << 20, n_tokens=1 << 22, max_new=4)
+    assert append(p=pool(n_kv_heads=256), b=many) == S.E_SHAPE              # 2^22 rows x 512 heads / 16 a workgroup
+    assert prologue(p=pool(n_kv_heads=256), b=many, n_heads=256, out=1 << 44) == S.E_SHAPE
+    long = batch(n_tokens=1 << 28, max_new=1 << 28)
+    assert append(p=pool(head_dim=512), b=long) == S.E_SHAPE                # 16 rows a workgroup
+    assert read(p=pool(head_dim=512), b=long) == S.E_SHAPE
+    assert prologue(b=batch(n_tokens=8, max_new=8), n_heads=65536, out=1 << 44) == S.E_SHAPE
+    wide = batch(n_seq=1 << 20, n_tokens=1 << 20, max_new=1, max_ctx=4096, table_stride=256)
+    assert attn(p=pool(n_kv_heads=512), b=wide, n_heads=512, out=1 << 44) == S.E_SHAPE
+    d = paged.PagedAttnDesc(n_heads=512, window=0, q_head_stride=0, q_row_stride=0, scale=0.1)
+    assert paged.paged_lib().lmxp_attn_workspace_bytes(ctypes.byref(pool(n_kv_heads=512)), ctypes.byref(wide),
+                                                       ctypes.byref(d)) == 0
+
+
 # ---------------------------------------------------------- index arithmetic --
 WALK = r"""
 #include "paged_index.hpp"
@@ -269,6 +285,24 @@ int main() {
                 }
             }
             if (!garbage) CHECK(items <= row_tiles_bound(g, bm) * g.Hkv + target);
+        }
+        for (int log2_r = 4; log2_r <= 6; ++log2_r) {  // row blocks: every row once, cut at whole granules
+            int64_t blocks = 0;
+            for (int b = 0; b < g.n_seq; ++b) {
+                const PagedSeq s = paged_seq(g, cu[b], cu[b + 1], ctx[b]);
+                const int n = row_blocks(s, log2_r);
+                int next = 0;
+                for (int i = 0; i < n; ++i) {
+                    const RowBlock r = row_block(s, i, log2_r);
+                    CHECK(r.first == next && r.count > 0 && r.count <= 1 << log2_r);
+                    CHECK(i == 0 || ((s.ctx - s.n + r.first) & ((1 << log2_r) - 1)) == 0);
+                    next += r.count;
+                    if (garbage && i > 64) { next = s.n; break; }
+                }
+                CHECK(next == s.n);
+                blocks += n;
+            }
+            if (!garbage) CHECK(blocks <= row_blocks_bound(g, log2_r));
         }
         for (int i = 0; i < 50; ++i) {
             const int page = paged_page(g, (int)(rnd() << 8 ^ rnd()));
