@@ -666,8 +666,8 @@ struct Plan {
 static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     Plan p{};
     const int64_t most = (int64_t)g.max_new * g.G;  // rows of a sequence
-    const int cm = chunk_rows(hd);
-    const bool chunks = cm && most > kRowsMost;
+    const int cm = chunk_rows(hd, i8, f32);
+    const bool chunks = most > kRowsMost;
     if (!chunks || g.n_seq > 1) {
         const int64_t seq_rows = chunks ? kRowsMost : most;
         int64_t tiles = row_tiles_bound(g, kBM);

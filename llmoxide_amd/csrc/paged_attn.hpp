@@ -21,8 +21,8 @@ struct AttnPagedArgs {
     int lo_rows, hi_rows; // this kernel takes sequences with lo_rows < rows * G <= hi_rows
 };
 
-// paged_chunk.hip: rows of its workgroups (0: no kernel for this head_dim), and the launch.
-int chunk_rows(int hd);
+// paged_chunk.hip: rows of its workgroups, and the launch.
+int chunk_rows(int hd, bool i8, bool f32);
 int chunk_occ_of(int hd, bool i8, bool f32);  // workgroups a CU holds
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);
 

@@ -50,11 +50,11 @@ __device__ __forceinline__ f16x8 lds16(uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(at);
 }
 
-template <int HD, int BN>
+template <int HD, int BN, int DS>
 struct ChunkTile {
     static constexpr int KS = HD / 16;   // k-steps of QK
-    static constexpr int NB = HD / 32;   // 32-dim blocks of the output
-    static constexpr int BM = 128;  // rows a workgroup
+    static constexpr int NB = HD / 32 / DS;  // 32-dim blocks of the output, a wave
+    static constexpr int BM = 128 / DS;  // rows a workgroup
     static constexpr int KB = BN / 32;   // 32-key blocks a tile
     static constexpr int ST = BN / 16;   // k-steps of PV
     static constexpr int GR = BN / 16;   // 16-key granules a tile, each in one page
@@ -64,10 +64,11 @@ struct ChunkTile {
     static constexpr int STAGE = 2 * BN * HD;     // halfs: K then V
 };
 
-// BN: keys a tile.  OCC: workgroups a CU.
-template <int HD, bool I8, bool F32, int BN, int OCC>
+// BN: keys a tile.  DS: waves that share rows, each with its part of the
+// output's dims (the scores are made by all of them).  OCC: workgroups a CU.
+template <int HD, bool I8, bool F32, int BN, int DS, int OCC>
 __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) {
-    using T = ChunkTile<HD, BN>;
+    using T = ChunkTile<HD, BN, DS>;
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH, KB = T::KB, ST = T::ST, GR = T::GR, CV = T::CV;
     constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
@@ -93,7 +94,8 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int k_hi = imin(pos_of(r1) + 1, split_hi);  // one behind the last key
     const int n_t = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
     // the wave's: keys some row sees, keys all rows see
-    const int w0 = r0 + w * 32, w1 = imin(w0 + 32, n_rows) - 1;
+    const int w0 = r0 + w / DS * 32, w1 = imin(w0 + 32, n_rows) - 1;
+    const int nb0 = w % DS * NB;  // the wave's first block of dims
     const bool live = w0 <= r1;
     const int any_hi = live ? pos_of(w1) : -1, all_hi = live ? pos_of(w0) : -1;
     const int any_lo = live ? low_of(pos_of(w0)) : 0, all_lo = live ? low_of(pos_of(w1)) : 0;
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
 
     const uint32_t k_lane = krow * (HD * 2) + ((hh ^ swizzle<HD * 2>(krow)) * 16);
-    const uint32_t v_lane = BN * HD * 2 + l32 * (BN * 2) + ((hh ^ swizzle<BN * 2>(l32)) * 16);
+    const uint32_t v_lane = BN * HD * 2 + nb0 * (32 * BN * 2) + l32 * (BN * 2) + ((hh ^ swizzle<BN * 2>(l32)) * 16);
 
     // WHOLE: every row of the wave sees every key of the tile.
     auto compute = [&](auto whole_tag, int t0, const int (&p)[GR], int stage) {
@@ -460,12 +462,12 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     const int page = pw.at(a.p, key);
                     if (page < 0 || key > pos || key < seen_lo) continue;
                     const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
-                                   ((32 * nb + 4 * hh) << pg.ps_log2);
+                                   ((32 * (nb0 + nb) + 4 * hh) << pg.ps_log2);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float y = (float)*e;
                         if (!(fabsf(y) < INFINITY)) add[i] += y;
-                        e += (i & 3) < 3 ? step : 5 * step;  // dims 32 nb + 8 (i/4) + 4 hh + i%4
+                        e += (i & 3) < 3 ? step : 5 * step;  // dims 32 (nb0 + nb) + 8 (i/4) + 4 hh + i%4
                     }
                 }
 #pragma unroll
@@ -478,18 +480,18 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     if (row >= n_rows) return;
     if (it.splits > 1) {
         const size_t at = (size_t)(it.first + it.split * it.stride) * BM + (row - r0);
-        float* dst = a.part_o + at * HD;
+        float* dst = a.part_o + at * HD + 32 * nb0;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
                     f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]};
-        if (hh == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m, sum};
+        if (hh == 0 && nb0 == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m, sum};
     } else {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         QT* dst = static_cast<QT*>(a.out) +
-                  ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD;
+                  ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 32 * nb0;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -503,15 +505,16 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     }
 }
 
-// Keys a tile and workgroups a CU, by what fits the registers.
-constexpr int chunk_bn(int hd, bool i8, bool f32) { return (hd == 256 && (f32 || !i8)) || (hd == 128 && f32) ? 32 : 64; }
-constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd <= 128 || (!f32 && !i8) ? 2 : 1; }
-int chunk_rows(int hd) { return hd <= 256 ? 128 : 0; }
+// Keys a tile, waves to a row and workgroups a CU, by what fits the registers.
+constexpr int chunk_bn(int hd, bool i8, bool f32) { return hd == 512 || (hd == 256 && (f32 || !i8)) || (hd == 128 && f32) ? 32 : 64; }
+constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd <= 128 || (hd == 256 && !f32 && !i8) ? 2 : 1; }
+constexpr int chunk_ds(int hd, bool i8, bool f32) { return hd <= 256 ? 1 : i8 || f32 ? 4 : 2; }
+int chunk_rows(int hd, bool i8, bool f32) { return 128 / chunk_ds(hd, i8, f32); }
 int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_bn(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_bn(HD, I8, F32), chunk_ds(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
 }
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
     auto by = [&](auto tag) {
@@ -521,7 +524,8 @@ void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned it
     };
     if (hd == 64) by(std::integral_constant<int, 64>{});
     else if (hd == 128) by(std::integral_constant<int, 128>{});
-    else by(std::integral_constant<int, 256>{});
+    else if (hd == 256) by(std::integral_constant<int, 256>{});
+    else by(std::integral_constant<int, 512>{});
 }
 
 }  // namespace lmx

@@ -272,6 +272,16 @@ def test_attention_windows(window, store, hd, q16):
     check_attention(c, 4, q16=q16, window=window)
 
 
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("store", ["f16", "i8"])
+@pytest.mark.parametrize("hd,q16", [(256, True), (512, True), (512, False)])
+def test_attention_chunks_cut_along_their_keys(window, store, hd, q16):
+    """Chunks behind prefixes that several workgroups share, heads that several waves share."""
+    say("cut chunks", window, store, hd, q16)
+    c = po.PagedCase(23, new=[40, 3, 70], ctx=[1500, 700, 70], page=32, kv=1, hd=hd, store=store, pad=2)
+    check_attention(c, 3, q16=q16, window=window)
+
+
 @pytest.mark.parametrize("store", ["f16", "i8"])
 @pytest.mark.parametrize("new", [[1, 1], [90, 140]])
 def test_attention_scores_that_climb(store, new):
@@ -367,6 +377,23 @@ def test_attention_gives_infinities_to_the_rows_that_see_them():
         got = lmx.paged_attention(q, cache, batch, n_heads=1).cpu().numpy()
         assert np.all(np.isfinite(got[:17])) and np.all(got[17:, 5] == np.inf) and np.all(got[17:, 9] == -np.inf)
         assert np.all(np.isfinite(np.delete(got, [5, 9], 1)))
+
+
+@pytest.mark.parametrize("hd", [128, 256, 512])
+def test_attention_gives_infinities_to_their_dims(hd):
+    """Each part of a head that a wave has, in chunks and in single tokens."""
+    dims = [3, hd // 4 + 40, hd // 2 + 7, hd - 1]
+    for new in ([60], [2]):
+        c = po.PagedCase(28, new=new, ctx=[60], page=16, kv=1, hd=hd)
+        n = new[0]
+        pg, s = c.place(0, 59)
+        c.v[pg, 0, dims, s] = [np.inf, -np.inf, np.nan, np.inf]
+        cache, batch = on_gpu(c)
+        for dt in (torch.float32, torch.float16):
+            q = gpu(rows(c, 29, 1).reshape(n, -1)).to(dt)
+            got = lmx.paged_attention(q, cache, batch, n_heads=1).cpu().numpy()
+            assert np.all(np.isfinite(got[:-1])) and np.all(np.isfinite(np.delete(got, dims, 1)))
+            assert np.array_equal(got[-1, dims], [np.inf, -np.inf, np.nan, np.inf], equal_nan=True)
 
 
 @pytest.mark.parametrize("q16", [False, True])
