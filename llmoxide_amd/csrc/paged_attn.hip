@@ -20,6 +20,19 @@
 // (22 bits together); sums are fp32.  An 8-bit V's scale joins the exponent as
 // its logarithm, and the sum divides it out again, so that what f16 holds are
 // the weights that V's integers meet, row by row.
+//
+// Bound by HBM: every visible K and V byte once, 4 * G * hd operations for 4 * hd
+// bytes of f16 a position and kv head.  The waves share nothing and the
+// transposed V makes every load a whole operand, so nothing is staged in LDS.
+// Loads run one tile ahead in the registers that the
+// tile before leaves; with K's and V's waits counted apart and the four waves'
+// tiles side by side (V's 128-byte lines then meet in the caches) an 8-bit step
+// of 32 sequences fell from 145 to 110 us and one f16 token over 32k keys from
+// 38.9 to 33.9 us.  Measured (128-dim heads, 8 of them for 32 query heads):
+//   one token over 32768 f16 keys     33.8 us a call, 3.98 TB/s (25 us + merge 4)
+//   32 tokens, 8 bits, 527 MB         110 us, 4.8 TB/s (a copy reaches 5.1)
+//   one token over 512 keys           9.3 us a call, the launch and the host
+// Counters: profiles/paged_cache.md.
 #include <algorithm>
 
 #include "paged_attn.hpp"
@@ -479,6 +492,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
 }
 
 // Joins the splits of one query row: HD/4 columns x 1024/HD groups of splits.
+// Latency: 4-6 us for the partials of 32 heads, most of it the launch.
 // A workgroup for each row that a row tile can have (`rows` of them; tiles in
 // find_item's order with one split each).
 template <int HD, bool F32>
@@ -556,7 +570,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
 }
 
 // The same for row tiles with few splits and many rows (chunks): eight rows
-// at a time, HD/4 lanes (a wave at most) a row, 32 rows a workgroup.
+// at a time, HD/4 lanes (a wave at most) a row, 32 rows a workgroup.  512 rows
+// of 32 heads in 4 splits: 9 us for 38 MB.
 constexpr int kMergeRows = 32;
 template <int HD, bool F32>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a, int bm) {
@@ -625,12 +640,30 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
 // ------------------------------------------------------------------- host --
 // Items the rows kernel aims at: two rounds of the workgroups that the CUs hold
 // (two a CU up to head_dim 128, else one), so that uneven sequences level out.
-constexpr int rows_target(int hd) { return hd <= 128 ? 1024 : 512; }
-constexpr int kRowsLeast = 8;      // units a split has at least (512 keys)
+// Half as many: an 8-bit step of 32 sequences of 128-dim heads 112 -> 126 us, 4
+// of 256 dims 117 -> 129; twice as many 112 and 128.  512-dim items, whose
+// queries go through LDS first, come in one round: 16 sequences 139 us, in two
+// 158.
+constexpr int rows_target(int hd) { return hd <= 128 ? 1024 : hd == 256 ? 512 : 256; }
+// 64-key units a split has at least.  Shorter splits (4 units) cost one token
+// over 32k keys of 128 dims 29 -> 36 us and over 512 keys 9.7 -> 11.8 (a merge
+// that it has no need of), longer ones (16) 29 -> 29.5; a 512-dim head, whose
+// units take four times as long, gains: 32k keys, one kv head, 8 units 86 us, 4
+// 65, 2 68.
+constexpr int rows_least(int hd) { return hd <= 256 ? 8 : 4; }
 constexpr int kCus = 256;          // compute units of the target (MI355X)
-constexpr int kChunkLeast = 8;     // 64-key units a chunk's split has at least
-// Query rows a sequence may have per kv head for the rows kernel.
-constexpr int kRowsMost = 32;
+// The same for chunks; 512 rows on 4k keys take 64 us with 4, 8 and 16, eight
+// sequences of 64 rows 54, 54 and 56.5.
+constexpr int kChunkLeast = 8;
+// Query rows a sequence may have per kv head for the rows kernel: its tiles of
+// 16 each read the keys again, a chunk's tile of 128 wastes the rows that it
+// has too many.  Eight sequences of 2000-8000 positions, us on the rows and on
+// the chunk kernel (128 dims): 32 rows f16 46 and 50, 8 bits (f32 queries) 41
+// and 63; 48 rows 64 and 67, 54 and 72; 64 rows 79 and 64, 65 and 73; 128 rows
+// 135 and 58, 105 and 82.  256 dims, four sequences: 64 rows f16 94 and 105, 8
+// bits 74 and 121; 128 rows 138 and 124, 104 and 127.  512 dims: 48 rows f16 141
+// and 89, 8 bits 112 and 132.
+constexpr int rows_most(int hd, bool i8) { return hd == 256 ? (i8 ? 128 : 64) : i8 ? 64 : 32; }
 
 // One kernel's share of a call.
 struct Part {
@@ -667,20 +700,25 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     Plan p{};
     const int64_t most = (int64_t)g.max_new * g.G;  // rows of a sequence
     const int cm = chunk_rows(hd, i8, f32);
-    const bool chunks = most > kRowsMost;
+    const int few = rows_most(hd, i8);
+    const bool chunks = most > few;
     if (!chunks || g.n_seq > 1) {
-        const int64_t seq_rows = chunks ? kRowsMost : most;
+        const int64_t seq_rows = chunks ? few : most;
         int64_t tiles = row_tiles_bound(g, kBM);
-        if (chunks) tiles = std::min<int64_t>(tiles, (int64_t)g.n_seq * ((kRowsMost + kBM - 1) / kBM));
-        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, rows_target(hd), kRowsLeast);
-        if (chunks) p.rows.hi_rows = kRowsMost;
+        if (chunks) tiles = std::min<int64_t>(tiles, (int64_t)g.n_seq * (few / kBM));
+        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, rows_target(hd), rows_least(hd));
+        if (chunks) p.rows.hi_rows = few;
     }
     if (chunks) {
         const int64_t tiles = row_tiles_bound(g, cm);
-        // Splits where two or more of them a tile still start at once.
+        // Splits where two or more of them a tile still start at once: 512 rows on
+        // 4k keys 88 -> 58 us.  Where tiles fill the CUs once, splits cost more
+        // than their balance gives: a window of 1024 (256 dims) 114 -> 139 us, nine
+        // uneven sequences 276 -> 292, the worst one (six of 256 dims) gains 1085 ->
+        // 979.
         const int slots = kCus * chunk_occ_of(hd, i8, f32);
         p.chunk = make_part(g, hd, cm, tiles, most, 2 * tiles * g.Hkv <= slots, slots, kChunkLeast);
-        if (p.rows.on) p.chunk.lo_rows = kRowsMost;
+        if (p.rows.on) p.chunk.lo_rows = few;
     }
     return p;
 }

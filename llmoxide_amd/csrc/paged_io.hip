@@ -12,6 +12,19 @@
 // element.  Attention reads V's operand fragments straight from such columns,
 // which is what the transposed layout is for; the price is paid here, once a
 // row.
+//
+// Bound by HBM: the rows in, the pages out (8 bits: 1 + 4 / head_dim bytes a
+// value), nothing else.  Measured (8 kv heads; a copy reaches 5.13 TB/s):
+//   eight prompts to 8 bits and back, 228 MB, 128 dims   59 us, 3.87 TB/s (store
+//   22.9 us, read 20.1 us a kernel, the rest lies between the two)
+//   a read of 32768 8-bit positions to f16, 203 MB       46 us, 4.38 TB/s
+//   the prologue of six 8-bit chunks, 256 dims, 310 MB   86 us, 3.6 TB/s: loads
+//   and stores of one head wait on each other (78 us without the angles' sines,
+//   79.5 with; the next head's loads ahead of the stores, or four workgroups a
+//   CU, are not faster)
+//   one decode step of 16 sequences   4.0 us (append), 4.4 us (prologue) a kernel;
+//   a call 9.5 and 14.8 us, all of it the host's
+// Counters: profiles/paged_cache.md.
 #include <cmath>
 
 #include "lds_dma.hpp"
@@ -707,12 +720,15 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
 }
 
 // Heads a workgroup that makes its rows' angles once for them; short batches
-// take a head each, so that the heads run side by side.
+// take a head each, so that the heads run side by side.  3.4k rows of 32 heads:
+// 1, 2, 4, 8 heads 98, 82, 79, 82 us; 1024 rows one head 17.8, four 20.5; 2048
+// rows one head 25.6, four 23.9.
 static int heads_a_group(uint32_t n_tokens) { return n_tokens <= 1024 ? 1 : 4; }
 // A grid that the launch can name: 256 threads a workgroup in 32 bits, and 16 bits across.
 static bool grid_fits(int64_t x, int64_t y) { return x < (1 << 24) && y < (1 << 16); }
 // Batches of few rows a sequence: whole granules are rare, and a block of rows
-// would be a row or two.
+// would be a row or two.  One row: append 4.0 us a kernel against 6.2, prologue
+// 4.4 against 12.6; four rows: 15.4 us a prologue call on either.
 static bool few_rows(const PagedGeom& g) { return g.max_new <= 4; }
 
 template <bool PRO, typename SRC, bool I8>
@@ -821,7 +837,8 @@ lmx_status paged_read(const lmxp_pool* p, const lmxp_batch* b, void* k_out, void
     a.row_stride = row_stride ? row_stride : (size_t)p->n_kv_heads * p->head_dim;
     a.n_k = k_out ? (int)p->n_kv_heads : 0;
     a.n_v = v_out ? (int)p->n_kv_heads : 0;
-    a.hpw = b->n_tokens <= 1024 ? 1 : 2;  // the second head's loads go out beside the first's stores
+    // the second head's loads go out beside the first's stores (to 2048 rows no difference)
+    a.hpw = b->n_tokens <= 1024 ? 1 : 2;
     a.g_k = (a.n_k + a.hpw - 1) / a.hpw;
     a.g_v = (a.n_v + a.hpw - 1) / a.hpw;
     (void)hipGetLastError();

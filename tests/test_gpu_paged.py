@@ -278,7 +278,7 @@ def test_attention_windows(window, store, hd, q16):
 def test_attention_chunks_cut_along_their_keys(window, store, hd, q16):
     """Chunks behind prefixes that several workgroups share, heads that several waves share."""
     say("cut chunks", window, store, hd, q16)
-    c = po.PagedCase(23, new=[40, 3, 70], ctx=[1500, 700, 70], page=32, kv=1, hd=hd, store=store, pad=2)
+    c = po.PagedCase(23, new=[70, 3, 70], ctx=[1500, 700, 70], page=32, kv=1, hd=hd, store=store, pad=2)
     check_attention(c, 3, q16=q16, window=window)
 
 
