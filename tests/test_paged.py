@@ -337,3 +337,54 @@ def test_oracle_quantise():
     x[7] = np.inf
     q, s = quantise(x)
     assert np.isnan(s) and not q.any()
+
+
+@pytest.mark.parametrize("store", ["f16", "i8"])
+@pytest.mark.parametrize("window", [0, 9])
+def test_oracle_attention_is_the_textbooks(store, window):
+    """Each sequence's pages laid out side by side, against the contiguous form."""
+    from oracle import textbook
+    from tests import paged_oracle as po
+    c = po.PagedCase(3, new=[1, 5, 0, 17], ctx=[40, 5, 9, 30], page=16, kv=2, hd=64, store=store)
+    q = np.random.default_rng(4).standard_normal((c.tokens, 6, 64))
+    got = po.attend(c, q, heads=6, window=window)[0]
+    for b, (n, ctx) in enumerate(zip(c.new, c.ctx)):
+        if not n:
+            continue
+        kv = [[c.held(b, h, p) for h in range(2)] for p in range(ctx)]
+        k = np.array([[x[0] for x in row] for row in kv])
+        v = np.array([[x[1] for x in row] for row in kv])
+        rows = slice(int(c.cu[b]), int(c.cu[b]) + n)
+        want = textbook.attention(q[rows], k, v, n_heads=6, n_kv_heads=2, head_dim=64, base_pos=ctx - n, window=window)
+        assert np.abs(got[rows].reshape(n, -1) - want).max() < 1e-12
+
+
+@pytest.mark.parametrize("n_rot", [64, 32])
+def test_oracle_rotation_is_the_textbooks(n_rot):
+    from oracle import textbook
+    from tests.paged_oracle import rope_norm
+    x = np.random.default_rng(5).standard_normal(64)
+    want = x.copy()
+    want[:n_rot] = textbook.rope_neox(x[:n_rot], 77, 1e4)
+    assert np.abs(rope_norm(x, None, 77, n_rot=n_rot, eps=0, base=1e4) - want).max() < 1e-12
+    gain = np.linspace(0.5, 2, 64)
+    want = x / np.sqrt((x * x).mean() + 1e-6) * gain
+    assert np.abs(rope_norm(x, gain, 0, n_rot=n_rot, eps=1e-6, base=1e4) - want).max() < 1e-12
+
+
+@pytest.mark.parametrize("store", ["f16", "i8"])
+def test_oracle_append_is_read_where_it_belongs(store):
+    from tests import paged_oracle as po
+    c = po.PagedCase(6, new=[3, 0, 20], ctx=[18, 4, 20], page=16, kv=2, hd=64, store=store)
+    before = [x.copy() for x in (c.k, c.v)]
+    x = np.random.default_rng(7).standard_normal((2, c.tokens, 2, 64)).astype(np.float32)
+    c.k, c.v, c.k_scale, c.v_scale = po.append(c, x[0], x[1])
+    for row, b, pos, at in c.row_places():
+        for h in range(2):
+            for got, want in zip(c.held(b, h, pos), x[:, row, h]):
+                # half a step of f16 at 4, or of amax / 127
+                assert np.abs(got - want).max() <= (2.0 ** -9 if store == "f16" else 0.501 * np.abs(want).max() / 127)
+    own = {c.place(b, p) for row, b, p, _ in c.row_places()}
+    for now, was, slot in ((c.k, before[0], 2), (c.v, before[1], 3)):
+        off = np.moveaxis(now != was, slot, 1).any(axis=(2, 3))
+        assert {tuple(int(y) for y in t) for t in np.argwhere(off)} <= own
