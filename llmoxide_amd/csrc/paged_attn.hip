@@ -711,13 +711,15 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     }
     if (chunks) {
         const int64_t tiles = row_tiles_bound(g, cm);
-        // Splits where two or more of them a tile still start at once: 512 rows on
-        // 4k keys 88 -> 58 us.  Where tiles fill the CUs once, splits cost more
-        // than their balance gives: a window of 1024 (256 dims) 114 -> 139 us, nine
-        // uneven sequences 276 -> 292, the worst one (six of 256 dims) gains 1085 ->
-        // 979.
+        // Splits where two or more of them a tile still start at once (four in a
+        // window, whose tiles meet parts of few splits): 512 rows on 4k keys 88 ->
+        // 58 us, a prompt of 2048 with 8 heads of 256 120 -> 92, in a window of 1024
+        // 75 -> 91.  Where tiles fill the CUs once, splits cost more than their
+        // balance gives: two chunks in a window (256 dims) 114 -> 139 us, nine uneven
+        // sequences 276 -> 292, the worst one (six of 256 dims) gains 1085 -> 979.
         const int slots = kCus * chunk_occ_of(hd, i8, f32);
-        p.chunk = make_part(g, hd, cm, tiles, most, 2 * tiles * g.Hkv <= slots, slots, kChunkLeast);
+        const bool cut = (g.window ? 4 : 2) * row_tiles_least(g, cm) * g.Hkv <= slots;
+        p.chunk = make_part(g, hd, cm, tiles, most, cut, slots, kChunkLeast);
         if (p.rows.on) p.chunk.lo_rows = few;
     }
     return p;

@@ -103,9 +103,11 @@ LMX_FN SeqWork seq_work(const PagedGeom& g, const PagedSeq& s, int bm) {
 // that every row is written).
 LMX_FN int seq_splits(const SeqWork& w, int per) { return w.units > per ? (w.units + per - 1) / per : 1; }
 
-// Row tiles of all sequences together: an upper bound from the shapes alone.
+// Row tiles of all sequences together: an upper bound from the shapes alone,
+// and the least where every row of the batch is some sequence's.
+LMX_FN int64_t row_tiles_least(const PagedGeom& g, int bm) { return ((int64_t)g.n_tokens * g.G + bm - 1) / bm; }
 LMX_FN int64_t row_tiles_bound(const PagedGeom& g, int bm) {
-    const int64_t a = (int64_t)g.n_tokens * g.G / bm + g.n_seq;
+    const int64_t a = ((int64_t)g.n_tokens * g.G + (int64_t)g.n_seq * (bm - 1)) / bm;
     const int64_t b = (int64_t)g.n_tokens * ((g.G + bm - 1) / bm);
     return a < b ? a : b;
 }

@@ -284,7 +284,12 @@ int main() {
                     }
                 }
             }
-            if (!garbage) CHECK(items <= row_tiles_bound(g, bm) * g.Hkv + target);
+            if (!garbage) {
+                CHECK(items <= row_tiles_bound(g, bm) * g.Hkv + target);
+                int64_t tiles = 0;
+                for (int b = 0; b < g.n_seq; ++b) tiles += seq_work(g, paged_seq(g, cu[b], cu[b + 1], ctx[b]), bm).rt;
+                CHECK(tiles <= row_tiles_bound(g, bm) && (at == 0 || tiles >= row_tiles_least(g, bm)));
+            }
         }
         for (int log2_r = 4; log2_r <= 6; ++log2_r) {  // row blocks: every row once, cut at whole granules
             int64_t blocks = 0;
