@@ -195,7 +195,11 @@ def _rows(t, n_tokens: int, width: int, what: str) -> int:
     row, col = t.stride()
     if col != 1:
         raise ValueError(f"{what}'s rows must be contiguous")
-    return 0 if n_tokens == 1 or row == width else row
+    if n_tokens == 1 or row == width:
+        return 0
+    if not width < row < 1 << 32:
+        raise ValueError(f"{what}'s rows must not share memory, nor lie 2^32 elements apart")
+    return row
 
 
 def _kv_rows(k, v, cache: PagedCache, batch: PagedBatch, names=("k", "v")):

@@ -393,3 +393,15 @@ def test_oracle_append_is_read_where_it_belongs(store):
     for now, was, slot in ((c.k, before[0], 2), (c.v, before[1], 3)):
         off = np.moveaxis(now != was, slot, 1).any(axis=(2, 3))
         assert {tuple(int(y) for y in t) for t in np.argwhere(off)} <= own
+
+
+def test_rows_that_share_memory_are_refused():
+    """A row stride of 0 means dense to the library: broadcast rows must not reach it."""
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(1, 64)
+    assert paged._rows(torch.zeros(4, 64), 4, 64, "q") == 0 and paged._rows(x, 1, 64, "q") == 0
+    assert paged._rows(torch.zeros(4, 100)[:, 8:72], 4, 64, "q") == 100
+    for bad in (x.expand(4, 64), torch.zeros(200).as_strided((4, 64), (32, 1)), torch.zeros(4, 128)[:, ::2],
+                torch.empty_strided((2, 64), (1 << 32, 1), device="meta")):
+        with pytest.raises(ValueError):
+            paged._rows(bad, *bad.shape, "q")
