@@ -569,14 +569,15 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         *reinterpret_cast<f16x4*>(dst) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
 }
 
-// The same for row tiles with few splits and many rows (chunks): eight rows
-// at a time, HD/4 lanes (a wave at most) a row, 32 rows a workgroup.  512 rows
-// of 32 heads in 4 splits: 9 us for 38 MB.
+// The same for chunks' row tiles: few splits, many rows.  A workgroup takes 32
+// rows, a wave every fourth 8 of their dims, in the order that the chunk
+// kernel's lanes hold them (part_at), so that a load is 1 KB in a row.  512 rows
+// of 32 heads in 4 splits, 38 MB: 8.4 us, row by row 9.1 (and the chunk kernel 54 -> 52).
 constexpr int kMergeRows = 32;
 template <int HD, bool F32>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a, int bm) {
     using QT = std::conditional_t<F32, float, f16>;
-    constexpr int C = HD / 4 < 64 ? HD / 4 : 64, V = HD / 4 / C;  // lanes a row, float4s a lane
+    constexpr int V = HD / 32, U = V < 16 ? 16 / V : 1;  // float4s a lane; splits at once
     const PagedGeom& pg = a.p.g;
     const int per = bm / kMergeRows;
     Item it;
@@ -584,56 +585,53 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
     const int4 info = a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile];
     const int splits = imin(info.z, a.n_items);  // written by this call's split 0; in range whatever it holds
     if (splits <= 1) return;
-    const int col = threadIdx.x % C;
-    const int r_lo = blockIdx.x % per * kMergeRows;
-    for (int r = r_lo + threadIdx.x / C; r < r_lo + kMergeRows; r += 256 / C) {
-        const int row = it.tile * bm + r;
-        if (row >= it.s.n * pg.G) return;
-        float m = -INFINITY, l = 0.f;
-        f32x4 o[V];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
+    const int blk = blockIdx.x % per, r = blk * kMergeRows + (lane & 31), row = it.tile * bm + r;
+    if (row >= it.s.n * pg.G) return;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 4;
-        for (int s0 = 0; s0 < splits; s0 += U) {
-            f32x2 ml[U];
-            f32x4 x[U][V];
+    for (int v = 0; v < V; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < splits; s0 += U) {
+        f32x2 ml[U];
+        f32x4 x[U][V];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int sp = imin(s0 + u, splits - 1);
-                const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm + r;
-                ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+        for (int u = 0; u < U; ++u) {
+            const int sp = imin(s0 + u, splits - 1);
+            const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm;
+            ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + (at + r) * 2);
 #pragma unroll
-                for (int v = 0; v < V; ++v) x[u][v] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + 4 * (col + C * v));
+            for (int v = 0; v < V; ++v) x[u][v] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + part_at<HD>(blk, 4 * v + w, lane));
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < splits) mn = fmaxf(mn, ml[u][0]);
+        const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < splits) {
+                const float fu = fast_exp2(ml[u][0] - ref);
+                l = fmaf(ml[u][1], fu, l);
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;
             }
-            float mn = m;
+        m = mn;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    QT* dst = static_cast<QT*>(a.out) +
+              ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 4 * hh;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (s0 + u < splits) mn = fmaxf(mn, ml[u][0]);
-            const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
-            l *= f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] *= f;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (s0 + u < splits) {
-                    const float fu = fast_exp2(ml[u][0] - ref);
-                    l = fmaf(ml[u][1], fu, l);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;
-                }
-            m = mn;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        QT* dst = static_cast<QT*>(a.out) +
-                  ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 4 * col;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const f32x4 y = o[v] * inv;
-            if constexpr (F32)
-                *reinterpret_cast<f32x4*>(dst + 4 * C * v) = y;
-            else
-                *reinterpret_cast<f16x4*>(dst + 4 * C * v) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
-        }
+    for (int v = 0; v < V; ++v) {
+        const f32x4 y = o[v] * inv;
+        const int d = 8 * (4 * v + w);
+        if constexpr (F32)
+            *reinterpret_cast<f32x4*>(dst + d) = y;
+        else
+            *reinterpret_cast<f16x4*>(dst + d) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
     }
 }
 

@@ -11,7 +11,7 @@ struct AttnPagedArgs {
     void* out;
     size_t q_row_stride, q_head_stride;
     float c;              // scale * log2(e)
-    float* part_o;        // [items][bm][hd]   partial outputs, unnormalised
+    float* part_o;        // [items][bm][hd]   partial outputs, unnormalised (chunks: in part_at's order)
     float* part_ml;       // [items][bm][2]    (reference exponent, sum)
     int4* rows;           // [n_seq][Hkv][rt_max]  (first item, item stride, splits, 0)
     int n_items;          // workgroups, and slots in part_o
@@ -25,6 +25,13 @@ struct AttnPagedArgs {
 int chunk_rows(int hd, bool i8, bool f32);
 int chunk_occ_of(int hd, bool i8, bool f32);  // workgroups a CU holds
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);
+
+// Where a chunk's partial output keeps the dims 8c + 4 (lane / 32) .. of row
+// 32 blk + lane % 32 of its tile.
+template <int HD>
+__device__ __forceinline__ int part_at(int blk, int c, int lane) {
+    return ((blk * (HD / 8) + c) * 64 + lane) * 4;
+}
 
 // One work item: a row tile of one sequence and kv head, over one split.
 struct Item {

@@ -493,15 +493,15 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     float sum = l + shfl_xor(l, 32);
     if (row >= n_rows) return;
     if (it.splits > 1) {
-        const size_t at = (size_t)(it.first + it.split * it.stride) * BM + (row - r0);
-        float* dst = a.part_o + at * HD + 32 * nb0;
+        const size_t at = (size_t)(it.first + it.split * it.stride) * BM;
+        float* dst = a.part_o + at * HD;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
+                *reinterpret_cast<f32x4*>(dst + part_at<HD>(w / DS, 4 * (nb0 + nb) + q, lane)) =
                     f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]};
-        if (hh == 0 && nb0 == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m, sum};
+        if (hh == 0 && nb0 == 0) *reinterpret_cast<f32x2*>(a.part_ml + (at + row - r0) * 2) = f32x2{m, sum};
     } else {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         QT* dst = static_cast<QT*>(a.out) +
