@@ -63,6 +63,14 @@ __device__ __forceinline__ f16x8 lds16(uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) f16x8*>(at);
 }
 
+// lo: a of the lower 32 lanes, b of the lower in the upper lanes; hi: a of the
+// upper lanes in the lower, b of the upper.
+__device__ __forceinline__ void swap_halves(uint32_t a, uint32_t b, uint32_t& lo, uint32_t& hi) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    lo = r[0];
+    hi = r[1];
+}
+
 template <int HD, int BN, int DS>
 struct ChunkTile {
     static constexpr int KS = HD / 16;   // k-steps of QK
@@ -508,13 +516,29 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                   ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 32 * nb0;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
+            if constexpr (F32) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 y = f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]} * inv;
-                if constexpr (F32)
-                    *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) = y;
-                else
-                    *reinterpret_cast<f16x4*>(dst + 32 * nb + 8 * q + 4 * hh) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4*>(dst + 32 * nb + 8 * q + 4 * hh) =
+                        f32x4{o[nb][4 * q], o[nb][4 * q + 1], o[nb][4 * q + 2], o[nb][4 * q + 3]} * inv;
+            } else {
+                // the row's two lanes trade, so that each stores 8 dims: the lower
+                // those of q, the upper those of q + 1
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                    uint32_t x[2][2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float y0 = o[nb][4 * (q + e) + 2 * i] * inv, y1 = o[nb][4 * (q + e) + 2 * i + 1] * inv;
+                            x[e][i] = __builtin_bit_cast(uint32_t, f16x2{(f16)y0, (f16)y1});
+                        }
+                    uint4 y;
+                    swap_halves(x[0][0], x[1][0], y.x, y.z);
+                    swap_halves(x[0][1], x[1][1], y.y, y.w);
+                    *reinterpret_cast<uint4*>(dst + 32 * nb + 8 * (q + hh)) = y;
+                }
             }
     }
 }
