@@ -84,13 +84,18 @@ def paged_lib() -> ctypes.CDLL:
     return _lib
 
 
+_dts = None
+
+
 def _dt_of(dtype) -> int:
-    torch = _torch()
-    if dtype == torch.float32:
-        return F32
-    if dtype == torch.float16:
-        return F16
-    raise TypeError(f"unsupported dtype {dtype}")
+    global _dts
+    if _dts is None:
+        torch = _torch()
+        _dts = {torch.float32: F32, torch.float16: F16}
+    dt = _dts.get(dtype)
+    if dt is None:
+        raise TypeError(f"unsupported dtype {dtype}")
+    return dt
 
 
 class PagedCache:
@@ -176,7 +181,7 @@ def _place(cache: PagedCache, batch: PagedBatch, *ts) -> None:
     if batch.device.index != at or at != _current_device():
         raise ValueError("cache and batch must be on the current device")
     for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != at):
+        if t is not None and t.get_device() != at:  # -1: the CPU's
             raise ValueError("tensors must be on the cache's device")
 
 
@@ -184,6 +189,13 @@ def _place(cache: PagedCache, batch: PagedBatch, *ts) -> None:
 def _attn_desc(n_heads: int, window: int, head: int, row: int, scale: float):
     """(structure, reference) of an attention call's scalars."""
     d = PagedAttnDesc(n_heads, window, head, row, scale)
+    return d, ctypes.byref(d)
+
+
+@functools.lru_cache(maxsize=256)
+def _prologue_desc(*fields):
+    """The same of a prologue call's."""
+    d = PagedPrologueDesc(*fields)
     return d, ctypes.byref(d)
 
 
@@ -270,7 +282,8 @@ def paged_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: in
     dt, kv_stride = _kv_rows(k, v, cache, batch)
     if k is None or v is None or dt != F32 or q.dtype != torch.float32:
         raise TypeError("q, k and v are float32")
-    for g, n in ((q_gain, hd), (k_gain, hd), (rope_factors, (hd if n_rot is None else n_rot) // 2)):
+    n_rot = hd if n_rot is None else n_rot
+    for g, n in ((q_gain, hd), (k_gain, hd), (rope_factors, n_rot // 2)):
         if g is not None and (g.dtype != torch.float32 or g.numel() < n or not g.is_contiguous()):
             raise ValueError("gains are contiguous float32 [head_dim], factors [n_rot / 2]")
     if q_out is None:
@@ -280,11 +293,11 @@ def paged_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: in
     if _rows(q_out, batch.n_tokens, n_heads * hd, "q_out"):
         raise ValueError("q_out must be contiguous")
     _place(cache, batch, q, k, v, q_gain, k_gain, rope_factors, q_out)
-    d = PagedPrologueDesc(n_heads, hd if n_rot is None else n_rot, int(bool(v_norm)), head, q.stride(0) if
-                          batch.n_tokens > 1 else 0, kv_stride, rms_eps, rope_base)
+    dref = _prologue_desc(n_heads, n_rot, int(bool(v_norm)), head, q.stride(0) if batch.n_tokens > 1 else 0,
+                          kv_stride, float(rms_eps), float(rope_base))[1]
     _check("lmxp_prologue", paged_lib().lmxp_prologue(
-        cache.ref, batch.ref, ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(q_gain), _ptr(k_gain),
-        _ptr(rope_factors), _ptr(q_out), _dt_of(q_out.dtype), _stream(stream)))
+        cache.ref, batch.ref, dref, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_gain), _ptr(k_gain),
+        _ptr(rope_factors), q_out.data_ptr(), _dt_of(q_out.dtype), _stream(stream)))
     return q_out
 
 
