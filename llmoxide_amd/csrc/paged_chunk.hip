@@ -23,13 +23,14 @@
 // that 128 rows share.  Measured (a large matrix product reaches 1.18 PFLOP/s):
 //   prompt of 8192, 32 heads on 8 of 128 dims, f16   559-577 us, 950-983 TFLOP/s
 //   (MFMA busy 52% of the cycles; without its softmax, operand reads and copies
-//   the loop takes 400 us); 512 rows on 4k keys 58 us, 625 TFLOP/s with the merge
+//   the loop takes 400 us); 512 rows on 4k keys 56 us, 650 TFLOP/s with the merge
 //   8-bit pages and fp32 queries, nine sequences     277 us, 378 TFLOP/s, twice
 //   that with the queries' and weights' second parts
 //   256 dims, a window of 1024                       116 us, 512 TFLOP/s
 //   512 dims, 1024 rows of 16 heads on 2048 keys     157 us, 328 TFLOP/s
 // Steps on the way, prompt: 128-row tiles of two workgroups a CU, conflict-free
 // places and loops of one tile kind 859 -> 625 us; one base address a tile 578.
+// Waves of 64 rows (half the LDS reads a product, one workgroup a CU) take 677.
 // Counters: profiles/paged_cache.md.
 #include <algorithm>
 
