@@ -35,7 +35,7 @@
  * and tables that break the rules above give unspecified results for the
  * sequences that they belong to, but no access outside the buffers.  Several
  * sequences may share pages; a position that one call writes must be in one
- * sequence's pages only.
+ * sequence's pages only.  A call's other tensors do not overlap the pool.
  *
  * An 8-bit row head x is stored as scale = amax(|x|) / 127, rounded to f32,
  * and int = x / scale rounded to the nearest, ties to even, from the exact

@@ -274,7 +274,8 @@ def test_attention_windows(window, store, hd, q16):
 
 @pytest.mark.parametrize("window", [0, 200])
 @pytest.mark.parametrize("store", ["f16", "i8"])
-@pytest.mark.parametrize("hd,q16", [(256, True), (512, True), (512, False)])
+@pytest.mark.parametrize("hd,q16", [(64, True), (128, True), (128, False), (256, True), (256, False), (512, True),
+                                    (512, False)])
 def test_attention_chunks_cut_along_their_keys(window, store, hd, q16):
     """Chunks behind prefixes that several workgroups share, heads that several waves share."""
     say("cut chunks", window, store, hd, q16)
@@ -537,6 +538,23 @@ def test_calls_on_another_stream():
     gk, gv = lmx.paged_read(cache, batch, stream=side)
     side.synchronize()
     assert torch.equal(got, want) and torch.equal(gk, wk) and torch.equal(gv, wv)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap in time, a workspace each, on pages that both read."""
+    c = po.PagedCase(47, new=[200, 1, 1], ctx=[3000, 2500, 700], page=16, kv=2, hd=128, store="i8")
+    cache, batch = on_gpu(c)
+    qs = [gpu(rows(c, s, 4).reshape(c.tokens, -1)) for s in (48, 49)]
+    want = [lmx.paged_attention(q, cache, batch, n_heads=4) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    spaces = [lmx.Workspace() for _ in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        got = [lmx.paged_attention(q, cache, batch, n_heads=4, workspace=ws, stream=s)
+               for q, ws, s in zip(qs, spaces, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
 def test_a_workspace_serves_calls_of_other_shapes():
