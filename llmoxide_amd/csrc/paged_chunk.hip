@@ -2,8 +2,8 @@
 //
 // A workgroup takes a tile of 128 query rows of one kv head (row r: token
 // r / G, head r % G, so that all heads of a group share the tile's keys) and
-// walks its 64-key tiles; four waves of 32 rows share each K/V tile in
-// LDS.  As in the rows kernel the products are computed transposed,
+// walks its 64- or 32-key tiles; four waves of 32 rows share each K/V tile in
+// LDS (512-dim heads: two or four waves share 32 rows as well).  As in the rows kernel the products are computed transposed,
 //   S^T = K Q^T, O^T += V^T P^T   on v_mfma_f32_32x32x16_f16,
 // Q^T in registers for the whole walk.  The keys that MFMA row r of a 32-key
 // block stands for are chosen so that a lane's scores are 8 consecutive keys
@@ -43,10 +43,15 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-constexpr int kAhead = 6;  // operand reads in flight ahead of their product
+// Operand reads in flight ahead of their product (2, 3, 4, 6: 121, 116, 116, 116
+// us for a window of 1024 at 256 dims; 3 to 6 alike at 128).
+constexpr int kAhead = 6;
 
 // Weights are exp2(arg), arg = score - m, with m kLift below the largest score
-// that set it; a tile with an arg above kLift + kSlack moves m.
+// that set it; a tile with an arg above kMost moves m.  f16 queries, of 11 bits
+// themselves, take weights rounded once to f16's 11 (a second part would double
+// the second product), and least 2^-24 of the scale 2^6 of a weight at m; fp32
+// queries two parts of 22 bits together.
 template <bool F32>
 struct Lift {
     static constexpr float lift = F32 ? 10.f : 6.f, most = 14.f;
