@@ -138,7 +138,8 @@ lmx_status lmxp_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  * read from the pages: append them first.  A row that sees no position, or
  * whose every score is -infinity, gets zeros.  What a row does not see has no
  * part in its result, infinities and NaN included.  An 8-bit V scale below
- * 2^-90 (values below 1e-25) is taken as 2^-90.
+ * 2^-90 (values below 1e-25) is taken as 2^-90; beside one above 2^100 (values
+ * above 1e32) keys of far smaller scales may lose their part of the softmax.
  *   dt   LMX_F16: q and out are f16; the weights p are rounded to f16 before
  *        they meet V where chunks are long, the sums are fp32.
  *        LMX_F32: q and out are f32; q and p are carried as two f16 parts each

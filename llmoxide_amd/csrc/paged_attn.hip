@@ -18,8 +18,8 @@
 // tile and moved only when a score passes it by 2^4; weights are
 // exp2(s - m + 10) <= 2^14, so f16 holds them, with a residual in a second f16
 // (22 bits together); sums are fp32.  An 8-bit V's scale joins the exponent as
-// its logarithm, and the sum divides it out again, so that what f16 holds are
-// the weights that V's integers meet, row by row.
+// its logarithm, so that what f16 holds are the weights that V's integers meet,
+// row by row; the sum takes an exponential without it (log_v_scale).
 //
 // Bound by HBM: every visible K and V byte once, 4 * G * hd operations for 4 * hd
 // bytes of f16 a position and kv head.  The waves share nothing and the
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     constexpr int OP = HD + 4;  // floats a row of the exchange (16-byte rows, rows 4 banks apart)
     constexpr size_t kEx = 512 + 4 * 16 * OP * 4, kQ = QLDS ? (F32 ? 2 : 1) * KS * 64 * 16 : 0;
     __shared__ __align__(16) char smem[kEx > kQ ? kEx : kQ];
-    __shared__ __align__(16) float scales[I8 ? 4 : 1][3][64];  // a wave's: K's, log2 of V's, 1 / V's
+    __shared__ __align__(16) float scales[I8 ? 4 : 1][2][64];  // a wave's: K's, log2 of V's
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
 
@@ -255,10 +255,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     auto step = [&](int t0, int t1) {
         // ---- 8-bit scales: a lane prepares one key's, all read theirs back (wave's own LDS)
         if constexpr (I8) {
-            const float v = v_scale_of(t.vs);
             scales[w][0][lane] = t.ks;
-            scales[w][1][lane] = __builtin_amdgcn_logf(v);
-            scales[w][2][lane] = 1.f / v;
+            scales[w][1][lane] = log_v_scale(t.vs);
             wave_lds_order();
         }
         auto scale4 = [&](int what, int j) {  // of the lane's keys in block j
@@ -331,8 +329,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             float mn = m;
             if (top > m + (kSlack + kLift)) mn = top - kLift;
             const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            l = m == -INFINITY ? 0.f : moved<I8>(l, m - mn);
             m = mn;
-            l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
         }
@@ -342,13 +340,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
-            f32x4 iv;
-            if constexpr (I8) iv = scale4(2, j);
+            f32x4 lv;
+            if constexpr (I8) lv = scale4(1, j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = fast_exp2(s[j][i] - ms);
+                const float x = s[j][i] - ms, p = fast_exp2(x);
                 if constexpr (I8)
-                    sum += seen >> (4 * j + i) & 1 ? p * iv[i] : 0.f;
+                    sum += seen >> (4 * j + i) & 1 ? fast_exp2(x - lv[i]) : 0.f;
                 else
                     sum += p;
                 const int at = 4 * (j & 1) + i;
@@ -471,7 +469,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float f = fast_exp2(ex_m[16 * k + r] - ref);
-            sum = fmaf(ex_l[16 * k + r], f, sum);
+            sum += moved<I8>(ex_l[16 * k + r], ex_m[16 * k + r] - ref);
             const f32x4 x = *reinterpret_cast<const f32x4*>(&ex_o[(k * 16 + r) * OP + d]);
             y += x * f;
         }
@@ -495,7 +493,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
 // Latency: 4-6 us for the partials of 32 heads, most of it the launch.
 // A workgroup for each row that a row tile can have (`rows` of them; tiles in
 // find_item's order with one split each).
-template <int HD, bool F32>
+template <int HD, bool F32, bool I8>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int bm, int rows) {
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int C4 = HD / 4, NG = 256 / C4;
@@ -532,12 +530,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u][0]);
         const float ref = mn == -INFINITY ? 0.f : mn;
         const float f = fast_exp2(m - ref);
-        l *= f;
+        l = moved<I8>(l, m - ref);
         o *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float fu = fast_exp2(ml[u][0] - ref);
-            l = fmaf(ml[u][1], fu, l);
+            l += moved<I8>(ml[u][1], ml[u][0] - ref);
             if (s0 + u * NG < splits) o += x[u] * fu;
         }
         m = mn;
@@ -558,7 +556,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
         const float f = fast_exp2(ex_m[k] - ref);
-        sum = fmaf(ex_l[k], f, sum);
+        sum += moved<I8>(ex_l[k], ex_m[k] - ref);
         y += ex[k][col] * f;
     }
     y *= sum == 0.f ? 0.f : 1.f / sum;
@@ -574,7 +572,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
 // kernel's lanes hold them (part_at), so that a load is 1 KB in a row.  512 rows
 // of 32 heads in 4 splits, 38 MB: 8.4 us, row by row 9.1 (and the chunk kernel 54 -> 52).
 constexpr int kMergeRows = 32;
-template <int HD, bool F32>
+template <int HD, bool F32, bool I8>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a, int bm) {
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int V = HD / 32, U = V < 16 ? 16 / V : 1;  // float4s a lane; splits at once
@@ -608,14 +606,14 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
         for (int u = 0; u < U; ++u)
             if (s0 + u < splits) mn = fmaxf(mn, ml[u][0]);
         const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
-        l *= f;
+        l = moved<I8>(l, m - ref);
 #pragma unroll
         for (int v = 0; v < V; ++v) o[v] *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (s0 + u < splits) {
                 const float fu = fast_exp2(ml[u][0] - ref);
-                l = fmaf(ml[u][1], fu, l);
+                l += moved<I8>(ml[u][1], ml[u][0] - ref);
 #pragma unroll
                 for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;
             }
@@ -762,15 +760,25 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     if (r.splits) {
         if (chunk) {
             const dim3 mgrid((unsigned)r.merge);
-            if (f32) hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm);
-            else hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm);
+            if (i8) {
+                if (f32) hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, true, true>), mgrid, dim3(256), 0, st, a, r.bm);
+                else hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, false, true>), mgrid, dim3(256), 0, st, a, r.bm);
+            } else {
+                if (f32) hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, true, false>), mgrid, dim3(256), 0, st, a, r.bm);
+                else hipLaunchKernelGGL((paged_merge_tiles_kernel<HD, false, false>), mgrid, dim3(256), 0, st, a, r.bm);
+            }
             LMX_CHECK_LAUNCH();
             return LMX_OK;
         }
         const int rows = (int)std::min<int64_t>(r.bm, (int64_t)a.p.g.max_new * a.p.g.G);
         const dim3 mgrid((unsigned)r.merge);
-        if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
-        else hipLaunchKernelGGL((paged_merge_kernel<HD, false>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+        if (i8) {
+            if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+            else hipLaunchKernelGGL((paged_merge_kernel<HD, false, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+        } else {
+            if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true, false>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+            else hipLaunchKernelGGL((paged_merge_kernel<HD, false, false>), mgrid, dim3(256), 0, st, a, r.bm, rows);
+        }
         LMX_CHECK_LAUNCH();
     }
     return LMX_OK;

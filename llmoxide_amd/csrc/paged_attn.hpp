@@ -134,9 +134,26 @@ __device__ __forceinline__ uint32_t finite2(uint32_t x) {
     return x & ~(m | (m - (m >> 15)));
 }
 
-// A V scale as the attention kernels use it: at least 2^-90 (which only values
-// below 1e-24 notice), so that its logarithm and reciprocal are finite.
-__device__ __forceinline__ float v_scale_of(float s) { return s < 0x1p-90f ? 0x1p-90f : s; }
+// 8-bit values: a key's V scale joins its score's exponent as its logarithm, so
+// the running reference m is that of score + log2(scale).  In the sum of the
+// softmax a key counts exp2(score - m), without its scale, by an exponential of
+// its own.  (The weight divided by the scale would cost one multiplication, and
+// 1 to 7% less time, but beside a scale 2^130 times as large a weight lies below
+// f32's range where its key may have half of the sum.)  With scales of 2^-90 to
+// 2^100 that term is in range wherever it matters: no score is above m + 14 + 90,
+// and the largest is at least m + 6 - 100, 2^32 above what f32 loses.
+//
+// log2 of a V scale, of 2^-90 at least: finite, and values below 1e-24 are all
+// that notices.
+__device__ __forceinline__ float log_v_scale(float s) { return __builtin_amdgcn_logf(s < 0x1p-90f ? 0x1p-90f : s); }
+// A sum brought from one reference to another, d above it (d <= 0).  I8: a step
+// down to -240, as scales alone make it, in two factors that f32 holds; above
+// -120 the second is 1.
+template <bool I8>
+__device__ __forceinline__ float moved(float l, float d) {
+    if constexpr (I8) return l * fast_exp2(fmaxf(d, -120.f)) * fast_exp2(fminf(d + 120.f, 0.f));
+    return l * fast_exp2(d);
+}
 
 // Two int8 words -> f16: x's bytes 0, 1 (lo) and 2, 3 (hi) as f16 pairs.  A
 // byte b + 128 set under 0x6400 is the f16 1024 + b + 128: exact, so is the

@@ -16,8 +16,8 @@
 // f16 pages go from memory straight to LDS (the chunk permutation is made on
 // the addresses that the lanes read); 8-bit pages go through registers, where
 // they become f16 (exact), and their scales stay apart: K's multiplies the
-// score, V's joins the exponent as its logarithm, and the sum divides it out
-// again: weights are then weighed against each other with it, row by row.
+// score, V's joins the exponent as its logarithm, so that weights are weighed
+// against each other with it, row by row; the sum leaves it out.
 //
 // Bound by MFMA: 4 * hd operations a query row and key, for 4 * hd bytes a key
 // that 128 rows share.  Measured (a large matrix product reaches 1.18 PFLOP/s):
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH, KB = T::KB, ST = T::ST, GR = T::GR, CV = T::CV;
     constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
     __shared__ __align__(1024) f16 tiles[2][T::STAGE];
-    __shared__ __align__(16) float scales[I8 ? 2 : 1][3][BN];  // K's, log2 of V's, 1 / V's
+    __shared__ __align__(16) float scales[I8 ? 2 : 1][2][BN];  // K's, log2 of V's
 
     Item it;
     // longest first: eight uneven 8-bit sequences of 100-12000 positions 812 -> 757 us
@@ -263,11 +263,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             }
             if (lane < BN) {
                 if (w == 0) scales[stage][0][lane] = rs;
-                if (w == 1) {
-                    const float v = v_scale_of(rs);
-                    scales[stage][1][lane] = __builtin_amdgcn_logf(v);
-                    scales[stage][2][lane] = 1.f / v;
-                }
+                if (w == 1) scales[stage][1][lane] = log_v_scale(rs);
             }
         }
     };
@@ -360,9 +356,9 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             else if (top > kMost)
                 mn = mb + top - kLift;
             const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            l = m == -INFINITY ? 0.f : moved<I8>(l, m - mn);
             const float delta = mn == -INFINITY ? 0.f : mn - mb;
             m = mn;
-            l *= f;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) o[nb] *= f;
 #pragma unroll
@@ -383,10 +379,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     pl[2 * kb + (i >> 3)][(i & 7) + 1] = lo[1];
                 }
                 if constexpr (I8) {
-                    const float* iv = &scales[stage][2][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
+                    const float* lv = &scales[stage][1][32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7)];
                     // (an unseen key's scale may be anything)
-                    sum = WHOLE || !(p0 == 0.f) ? fmaf(p0, iv[0], sum) : sum;
-                    sum = WHOLE || !(p1 == 0.f) ? fmaf(p1, iv[1], sum) : sum;
+                    const float x0 = s[kb][i], x1 = s[kb][i + 1];
+                    sum += WHOLE || x0 != -INFINITY ? fast_exp2(x0 - lv[0]) : 0.f;
+                    sum += WHOLE || x1 != -INFINITY ? fast_exp2(x1 - lv[1]) : 0.f;
                 } else if constexpr (F32) {
                     sum += p0 + p1;
                 } else {
