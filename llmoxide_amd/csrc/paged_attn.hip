@@ -182,11 +182,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 float x[8];
                 load_f32<8>(qr + q_dim(s), x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_or_0(fabsf(x[j])));
             }
             m = max_groups(m);
             int e = 0;
-            if (m > 0.f && m < INFINITY) e = 15 - (__builtin_amdgcn_frexp_expf(m));
+            if (m > 0.f) e = 15 - (__builtin_amdgcn_frexp_expf(m));
             e = imin(imax(e, -120), 120);
             const float up = ldexpf(1.f, e);
             qscale = ldexpf(a.c, -e);
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 for (int j = 0; j < 8; ++j) {
                     const float y = have ? x[j] * up : 0.f;
                     hi[j] = (f16)y;
-                    lo[j] = (f16)(y - (float)hi[j]);
+                    lo[j] = (f16)finite_or_0(y - (float)hi[j]);
                 }
                 if constexpr (QLDS) {
                     if (w == 0) {
@@ -267,6 +267,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
             s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 sl = s[j];  // f16 pages: the products with q's second part
+            auto& s2 = I8 ? s[j] : sl;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 f16x8 kf;
@@ -278,12 +280,15 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 }
                 if constexpr (QLDS) {
                     s[j] = mfma16(kf, q_lds[k * 64 + lane], s[j]);
-                    if constexpr (F32) s[j] = mfma16(kf, q_lds[(KS + k) * 64 + lane], s[j]);
+                    if constexpr (F32) s2 = mfma16(kf, q_lds[(KS + k) * 64 + lane], s2);
                 } else {
                     s[j] = mfma16(kf, qh[k], s[j]);
-                    if constexpr (F32) s[j] = mfma16(kf, ql[k], s[j]);
+                    if constexpr (F32) s2 = mfma16(kf, ql[k], s2);
                 }
             }
+            if constexpr (F32 && !I8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[j][i] += second_part(s[j][i], sl[i]);
             if constexpr (I8) {
                 const f32x4 ks = scale4(0, j), lv = scale4(1, j);
 #pragma unroll

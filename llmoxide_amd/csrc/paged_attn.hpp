@@ -134,6 +134,12 @@ __device__ __forceinline__ uint32_t finite2(uint32_t x) {
     return x & ~(m | (m - (m >> 15)));
 }
 
+// f32 queries are two f16 parts, hi and lo.  Where K or q holds an infinity the
+// score is hi's alone: lo's product would be inf - inf, or 0 * inf, beside it.
+// (In f16 pages K may; the two products have a sum each there.)
+__device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.f; }
+__device__ __forceinline__ float second_part(float hi, float lo) { return fabsf(hi) < INFINITY ? lo : 0.f; }
+
 // 8-bit values: a key's V scale joins its score's exponent as its logarithm, so
 // the running reference m is that of score + log2(scale).  In the sum of the
 // softmax a key counts exp2(score - m), without its scale, by an exponential of

@@ -142,11 +142,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             float x[8];
             load_f32<8>(qr + 16 * k, x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[j]));
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_or_0(fabsf(x[j])));
         }
         m = fmaxf(m, shfl_xor(m, 32));
         int e = 0;  // the row's largest element to [2^14, 2^15), as in the rows kernel
-        if (m > 0.f && m < INFINITY) e = 15 - __builtin_amdgcn_frexp_expf(m);
+        if (m > 0.f) e = 15 - __builtin_amdgcn_frexp_expf(m);
         e = imin(imax(e, -120), 120);
         const float up = ldexpf(1.f, e);
         qs = ldexpf(a.c, -e);
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             for (int j = 0; j < 8; ++j) {
                 const float y = have ? x[j] * up : 0.f;
                 qh[k][j] = (f16)y;
-                ql[k][j] = (f16)(y - (float)(f16)y);
+                ql[k][j] = (f16)finite_or_0(y - (float)(f16)y);
             }
         }
     } else {
@@ -295,12 +295,17 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         f32x16 s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
+            f32x16 sl;  // f16 pages: the products with q's second part
+            auto& s2 = I8 ? s[kb] : sl;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 const f16x8 kf = lds16((k_at ^ (32 * (k & 7))) + 256 * (k >> 3) + kb * (32 * HD * 2));
                 s[kb] = mfma32(kf, qh[k], k ? s[kb] : f32x16{});
-                if constexpr (F32) s[kb] = mfma32(kf, ql[k], s[kb]);
+                if constexpr (F32) s2 = mfma32(kf, ql[k], I8 || k ? s2 : f32x16{});
             }
+            if constexpr (F32 && !I8)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] += second_part(s[kb][i], sl[i]);
         }
         {
             constexpr int N = KB * KS, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;

@@ -58,3 +58,53 @@ def test_small_values_beside_loud_ones(new):
         c.v_scale[pg, 0, s] = np.float32(2.0 ** (100 if p % 7 == 3 else -80 + p // 8))
         c.k_scale[pg, 0, s] *= np.float32(12 if p % 7 == 3 else 0.5)
     check_attention(c, 2, q16=False)
+
+
+# ------------------------------------------------------- infinities that are seen --
+def attend(c, q, dt, heads, **kw):
+    cache, batch = on_gpu(c)
+    return lmx.paged_attention(gpu(q.reshape(c.tokens, -1)).to(dt), cache, batch, n_heads=heads, **kw).float().cpu().numpy()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[2], [150]])
+def test_a_key_whose_score_is_minus_infinity_has_no_weight(new, hd, dt):
+    """Infinite elements of f16 keys against queries of both parts' signs: as a key of a
+    score so low that its weight is 0; nothing but such keys leaves zeros."""
+    say("minus infinity", new, hd, dt)
+    c = po.PagedCase(63, new=new, ctx=[600], page=16, kv=1, hd=hd)
+    q = rows(c, 64, 2)
+    q[..., 7] = np.abs(q[..., 7]) + 0.5
+    q[..., 9] = -np.abs(q[..., 9]) - 0.5
+    places = [c.place(0, p) for p in (0, 3, 17, 300, 430, 449)]
+    for x in (60000, np.inf):  # a score of -60000 / 2 / sqrt(512) and below: exp is 0
+        for i, (pg, s) in enumerate(places):
+            c.k[pg, 0, s] = 0
+            c.k[pg, 0, s, 7 if i % 2 else 9] = -x if i % 2 else x
+            if i > 3:
+                c.k[pg, 0, s, 9 if i % 2 else 7] = x if i % 2 else -x
+        got = attend(c, q, dt, 2)
+        if np.isfinite(x):
+            want = got
+    assert np.all(np.isfinite(want)) and np.array_equal(got, want)
+    c.k[:, 0, :, 7] = -np.inf
+    assert np.all(attend(c, q, dt, 2) == 0)
+
+
+@pytest.mark.parametrize("store", ["f16", "i8"])
+@pytest.mark.parametrize("new", [[2], [150]])
+def test_infinite_queries(store, new):
+    """A row that is infinite where every key is positive: every score is -inf, the row zero;
+    +inf: not a number.  The other heads and rows are as they are without it."""
+    c = po.PagedCase(65, new=new, ctx=[200], page=16, kv=1, hd=64, store=store)
+    c.k[:, 0, :, 5] = np.maximum(np.abs(c.k[:, 0, :, 5]), 1)
+    q = rows(c, 66, 3, 3e3)
+    base = attend(c, q, torch.float32, 3).reshape(c.tokens, 3, 64)
+    q[1, 0, 5], q[1, 2, 5] = -np.inf, np.inf
+    q[1, 0, 6] = 1e9
+    got = attend(c, q, torch.float32, 3).reshape(c.tokens, 3, 64)
+    assert np.all(got[1, 0] == 0) and np.all(np.isnan(got[1, 2]))
+    assert np.array_equal(got[:, 1], base[:, 1])
+    keep = np.arange(c.tokens) != 1
+    assert np.array_equal(got[keep], base[keep])
