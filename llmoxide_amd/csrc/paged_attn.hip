@@ -473,7 +473,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float f = fast_exp2(ex_m[16 * k + r] - ref);
+            const float f = join_weight(ex_m[16 * k + r] - ref);
             sum += moved<I8>(ex_l[16 * k + r], ex_m[16 * k + r] - ref);
             const f32x4 x = *reinterpret_cast<const f32x4*>(&ex_o[(k * 16 + r) * OP + d]);
             y += x * f;
@@ -534,12 +534,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
 #pragma unroll
         for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u][0]);
         const float ref = mn == -INFINITY ? 0.f : mn;
-        const float f = fast_exp2(m - ref);
+        const float f = join_weight(m - ref);
         l = moved<I8>(l, m - ref);
         o *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float fu = fast_exp2(ml[u][0] - ref);
+            const float fu = join_weight(ml[u][0] - ref);
             l += moved<I8>(ml[u][1], ml[u][0] - ref);
             if (s0 + u * NG < splits) o += x[u] * fu;
         }
@@ -560,7 +560,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        const float f = fast_exp2(ex_m[k] - ref);
+        const float f = join_weight(ex_m[k] - ref);
         sum += moved<I8>(ex_l[k], ex_m[k] - ref);
         y += ex[k][col] * f;
     }
@@ -610,14 +610,14 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (s0 + u < splits) mn = fmaxf(mn, ml[u][0]);
-        const float ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m - ref);
+        const float ref = mn == -INFINITY ? 0.f : mn, f = join_weight(m - ref);
         l = moved<I8>(l, m - ref);
 #pragma unroll
         for (int v = 0; v < V; ++v) o[v] *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (s0 + u < splits) {
-                const float fu = fast_exp2(ml[u][0] - ref);
+                const float fu = join_weight(ml[u][0] - ref);
                 l += moved<I8>(ml[u][1], ml[u][0] - ref);
 #pragma unroll
                 for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;

@@ -152,6 +152,10 @@ __device__ __forceinline__ float second_part(float hi, float lo) { return fabsf(
 // log2 of a V scale, of 2^-90 at least: finite, and values below 1e-24 are all
 // that notices.
 __device__ __forceinline__ float log_v_scale(float s) { return __builtin_amdgcn_logf(s < 0x1p-90f ? 0x1p-90f : s); }
+// The weight of a partial output in a join, d below the highest reference.  Never
+// 0, which would make NaN of an infinity among V: 2^-126 of a finite output is
+// far below the last place of the weights beside it.
+__device__ __forceinline__ float join_weight(float d) { return fmaxf(fast_exp2(d), 0x1p-126f); }
 // A sum brought from one reference to another, d above it (d <= 0).  I8: a step
 // down to -240, as scales alone make it, in two factors that f32 holds; above
 // -120 the second is 1.

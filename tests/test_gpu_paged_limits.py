@@ -108,3 +108,24 @@ def test_infinite_queries(store, new):
     assert np.array_equal(got[:, 1], base[:, 1])
     keep = np.arange(c.tokens) != 1
     assert np.array_equal(got[keep], base[keep])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("new", [[2], [150]])
+def test_infinite_values_of_small_weight_survive_a_join(new, dt):
+    """V's infinities at keys whose scores lie hundreds below the rest of the row's: those
+    of one wave's share, and of one split's."""
+    say("joined infinities", new, dt)
+    c = po.PagedCase(67, new=new, ctx=[64] if new == [2] else [1500], page=16, kv=1, hd=64)
+    low, at = (range(32, 64), 40) if new == [2] else (range(0, 1300), 700)
+    q = rows(c, 68, 2)
+    q[..., 3] = np.abs(q[..., 3]) + 1
+    for p in low:  # 4800 / 8 below in natural units
+        pg, s = c.place(0, p)
+        c.k[pg, 0, s, 3] = -4800
+    base = attend(c, q, dt, 2).reshape(c.tokens, 2, 64)
+    pg, s = c.place(0, at)
+    c.v[pg, 0, 11, s], c.v[pg, 0, 60, s] = np.inf, -np.inf
+    got = attend(c, q, dt, 2).reshape(c.tokens, 2, 64)
+    assert np.all(got[..., 11] == np.inf) and np.all(got[..., 60] == -np.inf)
+    assert np.array_equal(np.delete(got, [11, 60], 2), np.delete(base, [11, 60], 2))
