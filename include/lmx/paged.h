@@ -150,8 +150,12 @@ lmx_status lmxp_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *        overlapping q (LMX_E_SHAPE)
  * n_heads: a multiple of n_kv_heads.  The workspace (16-byte aligned) holds
  * partial results where a key range is split; every byte read from it was
- * written by the same call.  Calls that overlap in time (two streams, two
- * replayed graphs) need one each. */
+ * written by the same call.  A call that needs more than ws_bytes is refused
+ * with LMX_E_WORKSPACE; what one needs does not rise with its batch (only batches
+ * that leave compute units idle are split, so a long prompt needs less than a
+ * short chunk), which is why lmxp_attn_workspace_bytes answers for smaller ones
+ * too.  Calls that overlap in time (two streams, two replayed graphs) need one
+ * each. */
 typedef struct {
     uint32_t n_heads;
     uint32_t window;         /* 0: every earlier position                     */
@@ -160,7 +164,9 @@ typedef struct {
     float scale;
 } lmxp_attn_desc;
 
-/* Bytes lmxp_attn needs (0 for a description that it refuses). */
+/* Bytes that serve lmxp_attn with this pool and these n_heads on this batch and
+ * on every one whose n_seq, n_tokens, max_new and max_ctx are at most its own,
+ * for either dt and any window (0 for a description that lmxp_attn refuses). */
 size_t lmxp_attn_workspace_bytes(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_desc *d);
 
 lmx_status lmxp_attn(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_desc *d,

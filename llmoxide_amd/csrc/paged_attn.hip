@@ -666,6 +666,9 @@ constexpr int kChunkLeast = 8;
 // and 89, 8 bits 112 and 132.
 constexpr int rows_most(int hd, bool i8) { return hd == 256 ? (i8 ? 128 : 64) : i8 ? 64 : 32; }
 
+// Workgroups of the chunk kernel that start at once.
+static int chunk_slots(int hd, bool i8, bool f32) { return kCus * chunk_occ_of(hd, i8, f32); }
+
 // One kernel's share of a call.
 struct Part {
     bool on, splits;
@@ -697,19 +700,21 @@ static Part make_part(const PagedGeom& g, int hd, int bm, int64_t tiles, int64_t
 struct Plan {
     Part rows, chunk;
 };
+// The rows kernel's share; it grows with each of n_seq, n_tokens, max_new and max_ctx.
+static Part rows_part(const PagedGeom& g, int hd, bool i8) {
+    const int seq_rows = (int)std::min<int64_t>((int64_t)g.max_new * g.G, rows_most(hd, i8));
+    const int64_t tiles = std::min<int64_t>(row_tiles_bound(g, kBM), (int64_t)g.n_seq * ((seq_rows + kBM - 1) / kBM));
+    Part r = make_part(g, hd, kBM, tiles, seq_rows, true, rows_target(hd), rows_least(hd));
+    r.hi_rows = seq_rows;
+    return r;
+}
 static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     Plan p{};
     const int64_t most = (int64_t)g.max_new * g.G;  // rows of a sequence
     const int cm = chunk_rows(hd, i8, f32);
     const int few = rows_most(hd, i8);
     const bool chunks = most > few;
-    if (!chunks || g.n_seq > 1) {
-        const int64_t seq_rows = chunks ? few : most;
-        int64_t tiles = row_tiles_bound(g, kBM);
-        if (chunks) tiles = std::min<int64_t>(tiles, (int64_t)g.n_seq * (few / kBM));
-        p.rows = make_part(g, hd, kBM, tiles, seq_rows, true, rows_target(hd), rows_least(hd));
-        if (chunks) p.rows.hi_rows = few;
-    }
+    if (!chunks || g.n_seq > 1) p.rows = rows_part(g, hd, i8);
     if (chunks) {
         const int64_t tiles = row_tiles_bound(g, cm);
         // Splits where two or more of them a tile still start at once (four in a
@@ -718,7 +723,7 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
         // 75 -> 91.  Where tiles fill the CUs once, splits cost more than their
         // balance gives: two chunks in a window (256 dims) 114 -> 139 us, nine uneven
         // sequences 276 -> 292, the worst one (six of 256 dims) gains 1085 -> 979.
-        const int slots = kCus * chunk_occ_of(hd, i8, f32);
+        const int slots = chunk_slots(hd, i8, f32);
         const bool cut = (g.window ? 4 : 2) * row_tiles_least(g, cm) * g.Hkv <= slots;
         p.chunk = make_part(g, hd, cm, tiles, most, cut, slots, kChunkLeast);
         if (p.rows.on) p.chunk.lo_rows = few;
@@ -726,17 +731,46 @@ static Plan make_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     return p;
 }
 
-// The workspace that a call of either type needs; false where its launches could not name their work.
-bool paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, size_t* bytes) {
+// The most workspace that a plan of g or of any smaller geometry (n_seq, n_tokens,
+// max_new, max_ctx at most g's) asks for.  Chunks are cut only while their tiles
+// leave CUs idle, so their partials are largest at the most rows that are still
+// cut; a prompt of more rows needs none.
+static size_t most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
+    const int cm = chunk_rows(hd, i8, f32), slots = chunk_slots(hd, i8, f32);
+    PagedGeom c = g;
+    c.n_tokens = (int)std::min<int64_t>(g.n_tokens, (int64_t)(slots / (2 * g.Hkv)) * cm / g.G);
+    c.max_new = std::min(g.max_new, c.n_tokens);
+    const int64_t most = (int64_t)c.max_new * c.G;
+    size_t bytes = rows_part(g, hd, i8).bytes();
+    if (most > rows_most(hd, i8))
+        bytes += make_part(c, hd, cm, row_tiles_bound(c, cm), most, true, slots, kChunkLeast).bytes();
+    return bytes;
+}
+
+static PagedGeom attn_geom(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
     PagedGeom g = paged_args(p, b).g;
     g.G = (int)(d->n_heads / p->n_kv_heads);
-    *bytes = 0;
+    g.window = (int)d->window;
+    return g;
+}
+
+// The workspace that one call needs; false where launches of either type could not name their work.
+bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool is_f32, size_t* bytes) {
+    bool fits = true;
     for (bool f32 : {false, true}) {
-        const Plan pl = make_plan(g, (int)p->head_dim, p->store == LMXP_I8, f32);
-        if (!pl.rows.fits() || !pl.chunk.fits()) return false;
-        *bytes = std::max(*bytes, pl.rows.bytes() + pl.chunk.bytes());
+        const Plan pl = make_plan(attn_geom(p, b, d), (int)p->head_dim, p->store == LMXP_I8, f32);
+        fits = fits && pl.rows.fits() && pl.chunk.fits();
+        if (f32 == is_f32) *bytes = pl.rows.bytes() + pl.chunk.bytes();
     }
-    return true;
+    return fits;
+}
+// What serves calls of either type, with any window, on this batch and on every smaller one.
+size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
+    size_t need, bytes = 0;
+    if (!paged_attn_need(p, b, d, true, &need)) return 0;
+    for (bool f32 : {false, true})
+        bytes = std::max(bytes, most_workspace(attn_geom(p, b, d), (int)p->head_dim, p->store == LMXP_I8, f32));
+    return bytes;
 }
 
 template <int HD>
@@ -793,8 +827,7 @@ lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_d
                       void* out, void* ws, hipStream_t st) {
     AttnPagedArgs a{};
     a.p = paged_args(p, b);
-    a.p.g.G = (int)(d->n_heads / p->n_kv_heads);
-    a.p.g.window = (int)d->window;
+    a.p.g = attn_geom(p, b, d);
     a.q = q;
     a.out = out;
     a.q_head_stride = d->q_head_stride ? d->q_head_stride : p->head_dim;

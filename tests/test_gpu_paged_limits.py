@@ -129,3 +129,24 @@ def test_infinite_values_of_small_weight_survive_a_join(new, dt):
     got = attend(c, q, dt, 2).reshape(c.tokens, 2, 64)
     assert np.all(got[..., 11] == np.inf) and np.all(got[..., 60] == -np.inf)
     assert np.array_equal(np.delete(got, [11, 60], 2), np.delete(base, [11, 60], 2))
+
+
+# ---------------------------------------------------------------- the workspace --
+def test_a_workspace_sized_by_a_long_prompt_stays_where_it_is():
+    """A prompt that is not split, then a chunk and a token that are."""
+    kv, hd, ctx, page = 8, 64, 4200, 64
+    entries = -(-ctx // page)
+    cache = lmx.PagedCache(torch.randn(entries, kv, page, hd, device="cuda").half(),
+                           torch.randn(entries, kv, hd, page, device="cuda").half())
+    table = torch.arange(entries, dtype=torch.int32, device="cuda")[None]
+    ws, where, q = lmx.Workspace(), None, torch.randn(ctx, kv * hd, device="cuda").half()
+    for n in (ctx, 300, 1):
+        batch = lmx.PagedBatch(torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                               torch.tensor([ctx], dtype=torch.int32, device="cuda"), table, n_tokens=n, max_new=n, max_ctx=ctx)
+        out = lmx.paged_attention(q[-n:], cache, batch, n_heads=kv, workspace=ws)
+        where = where or ws.base
+        assert ws.base == where
+        if n == ctx:
+            whole = out
+    # the same rows: each within 2^-11 of weights and of the result, values below 6
+    assert (out[-1].float() - whole[-1].float()).abs().max() <= 6 * 3 * 2.0 ** -11
