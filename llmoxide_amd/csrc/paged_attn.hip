@@ -164,6 +164,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     const int r_last = imin(it.tile * kBM + kBM, it.s.n * pg.G) - 1;
     const int all_hi = it.s.ctx - it.s.n + (it.tile * kBM) / pg.G;                       // first row's position
     const int all_lo = pg.window ? imax(it.s.ctx - it.s.n + r_last / pg.G - pg.window + 1, 0) : 0;
+    // Keys that some row sees: up to the last row's position, from the first row's window.
+    const int any_hi = it.s.ctx - it.s.n + r_last / pg.G;
+    const int any_lo = pg.window ? imax(all_hi - pg.window + 1, 0) : 0;
 
     // Q: k-step s holds dims 32s + 8g (f16 tiles); an 8-bit tile's 16-byte load
     // spans two k-steps, so there k-step 2l + e holds dims 64l + 16g + 8e.
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     PageWindow pw;
     pw.row = a.p.table + (size_t)it.b * pg.table_stride;
 
-    bool poison = false;           // a masked tile's V held an infinity or a NaN
+    bool poison = false;           // V held an infinity or a NaN at a key that some row sees and some does not
 
     // Whether every row of the item sees all of the tile.
     auto all_seen = [&](const int (&pages)[T::GR], int t0) {
@@ -304,6 +307,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         load_k<HD, I8>(a, next, it.h, t1, t);
         const bool whole = all_seen(pages, t0);
         uint32_t seen = 0xffffffffu;  // bit 4j + i: the lane's key 4j + i
+        uint4 v_mask = {};            // f16, not whole: the lane's keys that some row sees
         if (!whole) {
             const int gran = I8 ? g : g >> 1;
             const int p0 = pages[0], p1 = pages[1];
@@ -313,6 +317,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 page = gran & 2 ? q : page;
             }
             const int key = t0 + QUART * g;
+            if constexpr (!I8) v_mask = page >= 0 ? keys8_mask(any_lo - key, any_hi - key) : uint4{};
             seen = 0;
 #pragma unroll
             for (int i = 0; i < QUART; ++i)
@@ -366,11 +371,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             // An infinity or NaN in V would meet the zero weights of rows that
             // do not see its key (0 * inf): in tiles that hold such a key,
             // these elements stay out of the product, and the rows that do see
-            // them get them after the loop.
+            // them get them after the loop.  What no row sees (slots behind the
+            // sequence, pages that are none) is cleared and asks for nothing.
             if (!whole) {
+                const uint4 on = v_mask;
                 uint32_t bad = 0;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
+                    t.v[d] = uint4{t.v[d].x & on.x, t.v[d].y & on.y, t.v[d].z & on.z, t.v[d].w & on.w};
                     bad |= nonfinite2(t.v[d].x) | nonfinite2(t.v[d].y) | nonfinite2(t.v[d].z) | nonfinite2(t.v[d].w);
                     t.v[d] = uint4{finite2(t.v[d].x), finite2(t.v[d].y), finite2(t.v[d].z), finite2(t.v[d].w)};
                 }

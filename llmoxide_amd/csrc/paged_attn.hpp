@@ -134,6 +134,14 @@ __device__ __forceinline__ uint32_t finite2(uint32_t x) {
     return x & ~(m | (m - (m >> 15)));
 }
 
+// Of eight f16, those lo .. hi (any integers) all ones.
+__device__ __forceinline__ uint4 keys8_mask(int lo, int hi) {
+    auto word = [&](int i) {
+        return (lo <= 2 * i && 2 * i <= hi ? 0xffffu : 0u) | (lo <= 2 * i + 1 && 2 * i + 1 <= hi ? 0xffff0000u : 0u);
+    };
+    return uint4{word(0), word(1), word(2), word(3)};
+}
+
 // f32 queries are two f16 parts, hi and lo.  Where K or q holds an infinity the
 // score is hi's alone: lo's product would be inf - inf, or 0 * inf, beside it.
 // (In f16 pages K may; the two products have a sum each there.)

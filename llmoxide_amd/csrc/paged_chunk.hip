@@ -426,7 +426,28 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 __builtin_amdgcn_sched_group_barrier(0x2, EACH, 0);
             }
         }
-        if constexpr (!I8 && !WHOLE) poison = poison || __ballot(bad != 0) != 0;
+        if constexpr (!I8 && !WHOLE) {
+            if (__ballot(bad != 0)) {
+                // Again, without the keys that no row of the wave sees (slots
+                // behind the sequence, pages that are none): they ask for
+                // nothing.  (Masked above, they cost a 256-dim window 107 -> 145 us.)
+                bad = 0;
+#pragma unroll 1
+                for (int st = 0; st < ST; ++st) {
+                    const int key = t0 + 16 * st + 8 * hh;
+                    int page = p[0];
+#pragma unroll
+                    for (int j = 1; j < GR; ++j) page = st == j ? p[j] : page;
+                    const uint4 on = page >= 0 ? keys8_mask(any_lo - key, any_hi - key) : uint4{};
+#pragma unroll 1
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const uint4 u = __builtin_bit_cast(uint4, lds16((v_at ^ (32 * st)) + nb * (32 * BN * 2)));
+                        bad |= nonfinite2(u.x & on.x) | nonfinite2(u.y & on.y) | nonfinite2(u.z & on.z) | nonfinite2(u.w & on.w);
+                    }
+                }
+                poison = poison || __ballot(bad != 0) != 0;
+            }
+        }
     };
 
     if (n_t > 0) {

@@ -150,3 +150,59 @@ def test_a_workspace_sized_by_a_long_prompt_stays_where_it_is():
             whole = out
     # the same rows: each within 2^-11 of weights and of the result, values below 6
     assert (out[-1].float() - whole[-1].float()).abs().max() <= 6 * 3 * 2.0 ** -11
+
+
+# ------------------------------------------------------ garbage that nobody sees --
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("name,new,ctx,window", [
+    ("a step", [1] * 8, [8190 - 7 * i for i in range(8)], 0), ("a chunk", [700], [8190], 0),
+    ("a chunk in a window", [700], [8190], 1000), ("a step in a window", [1, 1], [8190, 5001], 1000),
+])
+def test_garbage_in_unseen_slots_costs_nothing(name, new, ctx, window, dt):
+    """NaN and infinities in every slot that no row sees (behind the lengths, before the
+    windows, in pages of nobody) leave the bits and the time as they are.  (An infinity that
+    a row sees asks for a walk over its keys one by one, which takes many times as long.)"""
+    say("unseen garbage", name, dt)
+    page, kv, hd, heads = 16, 2, 128, 8
+    per = [-(-x // page) for x in ctx]
+    order = torch.randperm(sum(per) + 3, generator=torch.Generator().manual_seed(1)).int()
+    table = torch.full((len(ctx), max(per)), -1, dtype=torch.int32)
+    seen = torch.zeros(sum(per) + 3, page, dtype=torch.bool)
+    at = 0
+    for b, n in enumerate(per):
+        table[b, :n] = order[at:at + n]
+        at += n
+        lo = max(0, ctx[b] - new[b] - window + 1) if window else 0
+        p = torch.arange(lo, ctx[b])
+        seen[table[b, p // page].long(), p % page] = True
+    g = torch.Generator("cuda").manual_seed(2)
+    k = torch.randn(sum(per) + 3, kv, page, hd, device="cuda", generator=g).half()
+    v = torch.randn(sum(per) + 3, kv, hd, page, device="cuda", generator=g).half()
+    q = torch.randn(sum(new), heads * hd, device="cuda", generator=g).to(dt)
+    cu = torch.tensor([0] + new).cumsum(0).int().cuda()
+    batch = lmx.PagedBatch(cu, torch.tensor(ctx, dtype=torch.int32, device="cuda"), table.cuda(), n_tokens=sum(new),
+                           max_new=max(new), max_ctx=max(ctx))
+    ws = lmx.Workspace()
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda").half()
+
+    def run(k, v):
+        cache, times = lmx.PagedCache(k, v), []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                out = lmx.paged_attention(q, cache, batch, n_heads=heads, window=window, workspace=ws)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) / 5)
+        return out, min(times)
+
+    clean, fast = run(k, v)
+    hide = ~seen.cuda()
+    fill = bad[torch.arange(hide.numel(), device="cuda") % 3].view(hide.shape)
+    k = torch.where(hide[:, None, :, None], fill[:, None, :, None], k)
+    v = torch.where(hide[:, None, None, :], fill[:, None, None, :], v)
+    got, slow = run(k, v)
+    say(f"{fast * 1e3:.1f} us, with garbage {slow * 1e3:.1f}")
+    assert torch.equal(got, clean)
+    assert slow <= 1.5 * fast
