@@ -758,7 +758,7 @@ static size_t most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
 static PagedGeom attn_geom(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
     PagedGeom g = paged_args(p, b).g;
     g.G = (int)(d->n_heads / p->n_kv_heads);
-    g.window = (int)d->window;
+    g.window = d->window < b->max_ctx ? (int)d->window : 0;  // a wider one hides nothing
     return g;
 }
 

@@ -206,3 +206,18 @@ def test_garbage_in_unseen_slots_costs_nothing(name, new, ctx, window, dt):
     say(f"{fast * 1e3:.1f} us, with garbage {slow * 1e3:.1f}")
     assert torch.equal(got, clean)
     assert slow <= 1.5 * fast
+
+
+def test_a_window_that_hides_nothing_gives_the_bits_of_none():
+    kv, hd, n, page = 8, 64, 2500, 64
+    entries = -(-n // page)
+    cache = lmx.PagedCache(torch.randn(entries, kv, page, hd, device="cuda").half(),
+                           torch.randn(entries, kv, hd, page, device="cuda").half())
+    batch = lmx.PagedBatch(torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                           torch.tensor([n], dtype=torch.int32, device="cuda"),
+                           torch.arange(entries, dtype=torch.int32, device="cuda")[None], n_tokens=n, max_new=n, max_ctx=n)
+    q = torch.randn(n, kv * hd, device="cuda").half()
+    want = lmx.paged_attention(q, cache, batch, n_heads=kv)
+    for window in (n, n + 1, 1 << 20):
+        assert torch.equal(lmx.paged_attention(q, cache, batch, n_heads=kv, window=window), want)
+    assert not torch.equal(lmx.paged_attention(q, cache, batch, n_heads=kv, window=n - 1), want)

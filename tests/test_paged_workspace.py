@@ -59,3 +59,13 @@ def test_calls_take_the_workspace_of_a_larger_batch(seqs, ctx, small, dt, window
     call = dict(p=p, b=rows(*small, ctx), dt=dt, n_heads=32, window=window, out=FAR * 16, ws=FAKE + 8)
     assert attn(ws_bytes=0, **call) == S.E_WORKSPACE
     assert attn(ws_bytes=has, **call) == S.E_ALIGN
+
+
+@pytest.mark.parametrize("window", [0, 2500, 2501, 1 << 20])
+def test_a_window_that_hides_nothing_is_none(window):
+    """2500 rows of 8 heads of 256 are split without a window, and so behind one as long as
+    the sequence."""
+    b = rows(1, 2500, 2500, 2500)
+    call = dict(p=wide(hd=256), b=b, dt=lmx.F16, n_heads=8, out=FAR * 16, ws=FAKE + 8, window=window)
+    assert attn(ws_bytes=0, **call) == S.E_WORKSPACE
+    assert attn(ws_bytes=workspace(wide(hd=256), b, 8, window), **call) == S.E_ALIGN
