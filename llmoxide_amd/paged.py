@@ -171,7 +171,7 @@ class PagedBatch:
 _current_device = None
 
 
-def _place(cache: PagedCache, batch: PagedBatch, *ts) -> None:
+def _place(cache: PagedCache, batch: PagedBatch, *ts, stream=None, workspace=None) -> None:
     """All on the current device: the stream a call takes is that device's."""
     global _current_device
     if _current_device is None:
@@ -183,6 +183,15 @@ def _place(cache: PagedCache, batch: PagedBatch, *ts) -> None:
     for t in ts:
         if t is not None and t.get_device() != at:  # -1: the CPU's
             raise ValueError("tensors must be on the cache's device")
+    if stream is not None and getattr(stream, "device_index", at) != at:
+        raise ValueError("the stream must be one of the cache's device")
+    if workspace is not None:
+        if workspace.buf is not None:
+            held = workspace.buf.get_device()
+        else:  # where it will be allocated; no index: the current device
+            held = None if workspace.device is None else _torch().device(workspace.device).index
+        if held is not None and held != at:
+            raise ValueError("the workspace must be on the cache's device")
 
 
 @functools.lru_cache(maxsize=256)
@@ -230,7 +239,7 @@ def paged_append(k, v, cache: PagedCache, batch: PagedBatch, *, stream=None) -> 
     """Write the batch's rows ``k``, ``v`` [n_tokens, n_kv_heads * head_dim] (f32 or
     f16; columns of a wider tensor will do) into their pages.  Either may be None."""
     dt, stride = _kv_rows(k, v, cache, batch)
-    _place(cache, batch, k, v)
+    _place(cache, batch, k, v, stream=stream)
     _check("lmxp_append", paged_lib().lmxp_append(cache.ref, batch.ref, _ptr(k), _ptr(v), dt, stride,
                                                   _stream(stream)))
 
@@ -256,7 +265,7 @@ def paged_read(cache: PagedCache, batch: PagedBatch, *, dtype=None, k_out=None, 
     elif dtype is not None and any(t is not None and t.dtype != dtype for t in (k_out, v_out)):
         raise TypeError("dtype differs from the outputs'")
     dt, stride = _kv_rows(k_out, v_out, cache, batch, ("k_out", "v_out"))
-    _place(cache, batch, k_out, v_out)
+    _place(cache, batch, k_out, v_out, stream=stream)
     _check("lmxp_read", paged_lib().lmxp_read(cache.ref, batch.ref, _ptr(k_out), _ptr(v_out), dt, stride,
                                               _stream(stream)))
     return k_out, v_out
@@ -292,7 +301,7 @@ def paged_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: in
         raise TypeError("q_dtype differs from q_out's")
     if _rows(q_out, batch.n_tokens, n_heads * hd, "q_out"):
         raise ValueError("q_out must be contiguous")
-    _place(cache, batch, q, k, v, q_gain, k_gain, rope_factors, q_out)
+    _place(cache, batch, q, k, v, q_gain, k_gain, rope_factors, q_out, stream=stream)
     dref = _prologue_desc(n_heads, n_rot, int(bool(v_norm)), head, q.stride(0) if batch.n_tokens > 1 else 0,
                           kv_stride, float(rms_eps), float(rope_base))[1]
     _check("lmxp_prologue", paged_lib().lmxp_prologue(
@@ -322,7 +331,7 @@ def paged_attention(q, cache: PagedCache, batch: PagedBatch, *, n_heads: int, wi
         out = _new_out((batch.n_tokens, n_heads * hd), q.dtype, cache.device, stream)
     elif out.dtype != q.dtype or _rows(out, batch.n_tokens, n_heads * hd, "out"):
         raise ValueError("out is contiguous and of q's dtype")
-    _place(cache, batch, q, out)
+    _place(cache, batch, q, out, stream=stream, workspace=workspace)
     dref = _attn_desc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
                       1.0 / math.sqrt(hd) if scale is None else float(scale))[1]
     L = paged_lib()

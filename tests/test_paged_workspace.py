@@ -69,3 +69,32 @@ def test_a_window_that_hides_nothing_is_none(window):
     call = dict(p=wide(hd=256), b=b, dt=lmx.F16, n_heads=8, out=FAR * 16, ws=FAKE + 8, window=window)
     assert attn(ws_bytes=0, **call) == S.E_WORKSPACE
     assert attn(ws_bytes=workspace(wide(hd=256), b, 8, window), **call) == S.E_ALIGN
+
+
+def test_streams_and_workspaces_of_another_device_are_refused(monkeypatch):
+    """Stand-ins for what two GPUs would give: the check reads nothing but devices."""
+    torch = pytest.importorskip("torch")
+
+    class On:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+            self.device_index = index
+
+        def get_device(self):
+            return self.device.index
+
+    class Space:
+        def __init__(self, buf=None, device=None):
+            self.buf, self.device = buf, device
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    here, there = On(0), On(1)
+    paged._place(here, here, here, None, stream=here, workspace=Space(buf=here))
+    for device in (None, "cuda", "cuda:0", torch.device("cuda"), 0):
+        paged._place(here, here, workspace=Space(device=device))
+    for kw in (dict(stream=there), dict(workspace=Space(buf=there)), dict(workspace=Space(buf=there, device="cuda:0")),
+               dict(workspace=Space(device="cuda:1")), dict(workspace=Space(device=1))):
+        with pytest.raises(ValueError):
+            paged._place(here, here, here, **kw)
+    for args in ((here, there), (there, there), (here, here, there)):
+        with pytest.raises(ValueError):
+            paged._place(*args)
