@@ -221,3 +221,95 @@ def test_a_window_that_hides_nothing_gives_the_bits_of_none():
     for window in (n, n + 1, 1 << 20):
         assert torch.equal(lmx.paged_attention(q, cache, batch, n_heads=kv, window=window), want)
     assert not torch.equal(lmx.paged_attention(q, cache, batch, n_heads=kv, window=n - 1), want)
+
+
+# ----------------------------------------------------------- bounds and paddings --
+@pytest.mark.parametrize("store", ["f16", "i8"])
+@pytest.mark.parametrize("new", [[1, 2, 1], [3, 0, 70]])
+def test_rows_in_front_of_the_first_sequence(store, new):
+    """cu may begin above 0: rows before it belong to nobody, the others are as without them."""
+    lead, kv, hd, heads = 7, 2, 128, 4
+    c = po.PagedCase(90, new=new, ctx=[40, 90, 700], page=16, kv=kv, hd=hd, store=store)
+    n = c.tokens
+    x = {w: gpu(rows(c, 91 + i, h).reshape(n, -1)) for i, (w, h) in enumerate((("q", heads), ("k", kv), ("v", kv)))}
+
+    def padded(t):
+        return torch.cat([torch.full((lead, t.shape[1]), float("nan"), dtype=t.dtype, device="cuda"), t])
+
+    def run(pad):
+        cache, batch = on_gpu(c)
+        a = x
+        if pad:
+            a = {w: padded(t) for w, t in x.items()}
+            batch = lmx.PagedBatch(batch.cu + lead, batch.ctx_lens, batch.page_table, n_tokens=n + lead,
+                                   max_new=max(new), max_ctx=700)
+        outs = [torch.full((a["q"].shape[0], w), 3.0, device="cuda") for w in (heads * hd, heads * hd, kv * hd, kv * hd)]
+        lmx.paged_prologue(a["q"], a["k"], a["v"], cache, batch, n_heads=heads, q_out=outs[0])
+        lmx.paged_attention(outs[0], cache, batch, n_heads=heads, out=outs[1])
+        lmx.paged_read(cache, batch, k_out=outs[2])
+        lmx.paged_read(cache, batch, v_out=outs[3])
+        lmx.paged_append(a["v"], a["k"], cache, batch)
+        return outs, [cache.k, cache.v]
+    (outs, pools), (pad_outs, pad_pools) = run(False), run(True)
+    for a, b in zip(outs, pad_outs):
+        assert torch.equal(b[lead:], a) and torch.all(b[:lead] == 3)
+    assert all(torch.equal(a, b) for a, b in zip(pools, pad_pools))
+
+
+@pytest.mark.parametrize("store", ["f16", "i8"])
+@pytest.mark.parametrize("new", [[1], [40], [64, 2, 1]])
+@pytest.mark.parametrize("q16", [False, True])
+def test_bounds_above_what_a_batch_brings(store, new, q16):
+    """max_new, n_tokens and max_ctx as a captured graph keeps them, the batch far below:
+    the plan is that of the bounds, the result the batch's."""
+    c = po.PagedCase(94, new=new, ctx=[900, 70, 333][:len(new)], page=16, kv=2, hd=128, store=store, pad=300, extra_entries=400)
+    cache, small = on_gpu(c)
+    q = rows(c, 95, 8)
+    if q16:
+        q = q.astype(np.float16).astype(np.float32)
+    dt = torch.float16 if q16 else torch.float32
+    want, mag, prod, top = po.attend(c, q, heads=8)
+    bound = po.attend_bound(c, mag, prod, top, max(c.ctx), f32=not q16)
+    own = slice(0, c.rows)
+    for most, ctx in ((max(new), 900), (100, 4000), (c.tokens, 7000)):
+        batch = lmx.PagedBatch(small.cu, small.ctx_lens, small.page_table, n_tokens=c.tokens, max_new=most, max_ctx=ctx)
+        out = torch.full((c.tokens, 8 * 128), 5.0, dtype=dt, device="cuda")
+        lmx.paged_attention(gpu(q.reshape(c.tokens, -1)).to(dt), cache, batch, n_heads=8, out=out)
+        got = out.double().cpu().numpy().reshape(c.tokens, 8, 128)
+        assert np.all(np.abs(got[own] - want[own]) <= bound[own]), (most, ctx)
+        assert np.all(got[c.rows:] == 5)
+
+
+def test_a_graph_of_chunks_replays_with_shorter_ones():
+    """One capture for up to 96 rows a sequence, replayed with 96, 5, 1 and no rows."""
+    kv, hd, heads, page = 2, 128, 8, 16
+    c = po.PagedCase(96, new=[96, 96], ctx=[1500, 400], page=page, kv=kv, hd=hd, store="i8")
+    cache, batch = on_gpu(c)
+    twin, _ = on_gpu(c)
+    batch = lmx.PagedBatch(batch.cu, batch.ctx_lens, batch.page_table, n_tokens=192, max_new=96, max_ctx=1500)
+    q, k, v = (gpu(rows(c, 97 + i, h).reshape(192, -1)) for i, h in enumerate((heads, kv, kv)))
+    spaces = lmx.Workspace(), lmx.Workspace()
+
+    def path(cache, ws, out):
+        y = lmx.paged_prologue(q, k, v, cache, batch, n_heads=heads, q_dtype=torch.float16)
+        lmx.paged_attention(y, cache, batch, n_heads=heads, workspace=ws, out=out)
+    outs = [torch.zeros(192, heads * hd, device="cuda").half() for _ in range(2)]
+    for cc, ws, out in zip((cache, twin), spaces, outs):
+        path(cc, ws, out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        path(cache, spaces[0], outs[0])
+    for cu, ctx in (([0, 96, 192], [1500, 400]), ([0, 5, 101], [1300, 400]), ([3, 4, 5], [1400, 7]), ([2, 2, 98], [0, 96]),
+                    ([0, 0, 0], [5, 5])):
+        batch.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+        batch.ctx_lens.copy_(torch.tensor(ctx, dtype=torch.int32))
+        for out in outs:
+            out.fill_(4)
+        graph.replay()
+        path(twin, spaces[1], outs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(*outs) and torch.all(outs[0][:cu[0]] == 4) and torch.all(outs[0][cu[2]:] == 4)
+        assert torch.all(torch.isfinite(outs[0]))
+        assert torch.equal(cache.k, twin.k) and torch.equal(cache.v, twin.v)
