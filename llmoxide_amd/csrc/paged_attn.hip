@@ -536,7 +536,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
             const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm + row % bm;
             ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
             x[u] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + 4 * col);
-            if (s0 + u * NG >= splits) ml[u] = f32x2{-INFINITY, 0.f};
+            if (s0 + u * NG >= splits) {
+                ml[u] = f32x2{-INFINITY, 0.f};
+                x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         }
         float mn = m;
 #pragma unroll
@@ -549,7 +552,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         for (int u = 0; u < U; ++u) {
             const float fu = join_weight(ml[u][0] - ref);
             l += moved<I8>(ml[u][1], ml[u][0] - ref);
-            if (s0 + u * NG < splits) o += x[u] * fu;
+            o += x[u] * fu;
         }
         m = mn;
     }
