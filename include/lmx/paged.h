@@ -94,7 +94,8 @@ lmx_status lmxp_append(const lmxp_pool *p, const lmxp_batch *b, const void *k_ne
  * Read the batch's rows back from the pages: the inverse of lmxp_append for
  * the same batch.  (To read positions [a, e) of a sequence, give it e - a rows
  * and length e.)  k_out, v_out [n_tokens, row_stride] of out_dt (LMX_F32 or
- * LMX_F16; an 8-bit value is int * scale, rounded once); row_stride and
+ * LMX_F16; an 8-bit value is int * scale rounded to f32, and for LMX_F16 that to
+ * f16, which is one place off the nearest f16 once in some 17000); row_stride and
  * alignment as for lmxp_append.  Rows of positions in no page are written as
  * zeros.  Either output may be NULL. */
 lmx_status lmxp_read(const lmxp_pool *p, const lmxp_batch *b, void *k_out, void *v_out,
