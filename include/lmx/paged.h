@@ -141,10 +141,15 @@ lmx_status lmxp_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  * part in its result, infinities and NaN included.  An 8-bit V scale below
  * 2^-90 (values below 1e-25) is taken as 2^-90; beside one above 2^100 (values
  * above 1e32) keys of far smaller scales may lose their part of the softmax.
- *   dt   LMX_F16: q and out are f16; the weights p are rounded to f16 before
- *        they meet V where chunks are long, the sums are fp32.
+ *   dt   LMX_F16: q and out are f16, the sums fp32.  The weights p are rounded
+ *        to f16 (11 bits) before they meet V in sequences that bring many rows
+ *        (n_heads / n_kv_heads times its new rows above 32 to 128, by head_dim
+ *        and store; any number, where n_seq is 1 and max_new allows that many)
+ *        and carried as two f16 parts (22 bits) in the others.
+ *        A result is off by some 2.8e-4 of itself in the former and 2.1e-4 in
+ *        the latter (root mean square), its own rounding to f16 included.
  *        LMX_F32: q and out are f32; q and p are carried as two f16 parts each
- *        (22 bits).
+ *        (22 bits) whatever the lengths.
  *   q    head h of row i at q + i*q_row_stride + h*q_head_stride (elements,
  *        multiples of 8; 0: contiguous); 16-byte aligned
  *   out  [n_tokens, n_heads, head_dim] contiguous, 16-byte aligned, not

@@ -49,9 +49,13 @@ constexpr int kAhead = 6;
 
 // Weights are exp2(arg), arg = score - m, with m kLift below the largest score
 // that set it; a tile with an arg above kMost moves m.  f16 queries, of 11 bits
-// themselves, take weights rounded once to f16's 11 (a second part would double
-// the second product), and least 2^-24 of the scale 2^6 of a weight at m; fp32
-// queries two parts of 22 bits together.
+// themselves, take weights rounded once to f16's 11, and least 2^-24 of the scale
+// 2^6 of a weight at m; fp32 queries two parts of 22 bits together.  Two parts
+// for f16 queries as well double the second product: the prompt of 8192 588 ->
+// 793 us, 512 rows on 4k keys 57 -> 73, the 256-dim window 108 -> 148, 8-bit
+// chunks 361 -> 454.  The error of a result against 64 bits (root mean square, of
+// the result) is 2.7e-4, 2.9e-4, 2.8e-4 and 2.5e-4 with one part, 2.1e-4 with two,
+// as that of the exact result rounded to f16.
 template <bool F32>
 struct Lift {
     static constexpr float lift = F32 ? 10.f : 6.f, most = 14.f;

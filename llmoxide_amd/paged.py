@@ -317,7 +317,9 @@ def paged_attention(q, cache: PagedCache, batch: PagedBatch, *, n_heads: int, wi
     (f32 or f16; columns of a wider tensor will do) over the pages, where their own
     K and V already are.  Returns out [n_tokens, n_heads * head_dim] of q's dtype;
     ``window`` > 0 limits a row to its last ``window`` positions.  Rows of no
-    sequence are left as they are.  A ``workspace`` that served a batch serves all
+    sequence are left as they are.  With f16 ``q`` the softmax's weights have 11
+    bits where a sequence brings many rows (new rows times heads / kv heads above 32
+    to 128), 22 elsewhere and always with f32 ``q``.  A ``workspace`` that served a batch serves all
     whose ``n_seq``, ``n_tokens``, ``max_new`` and ``max_ctx`` are no larger without
     growing (and moving, which a captured graph would not notice)."""
     hd = cache.head_dim
