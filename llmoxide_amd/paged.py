@@ -339,8 +339,10 @@ def paged_attention(q, cache: PagedCache, batch: PagedBatch, *, n_heads: int, wi
     L = paged_lib()
     need = L.lmxp_attn_workspace_bytes(cache.ref, batch.ref, dref)
     ws_ptr, ws_bytes = None, 0
-    if need:
-        workspace = workspace or Workspace(device=cache.device)
+    if need and workspace is None:
+        held = _new_out((need,), _torch().uint8, cache.device, stream)  # for this call; nothing need be cleared
+        ws_ptr, ws_bytes = held.data_ptr(), need
+    elif need:
         if need > workspace.nbytes:
             workspace.ensure(need, stream)
         ws_ptr, ws_bytes = workspace.base, workspace.nbytes
