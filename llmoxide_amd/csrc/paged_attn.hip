@@ -29,9 +29,9 @@
 // tiles side by side (V's 128-byte lines then meet in the caches) an 8-bit step
 // of 32 sequences fell from 145 to 110 us and one f16 token over 32k keys from
 // 38.9 to 33.9 us.  Measured (128-dim heads, 8 of them for 32 query heads):
-//   one token over 32768 f16 keys     33.8 us a call, 3.98 TB/s (25 us + merge 4)
-//   32 tokens, 8 bits, 527 MB         110 us, 4.8 TB/s (a copy reaches 5.1)
-//   one token over 512 keys           9.3 us a call, the launch and the host
+//   one token over 32768 f16 keys     34.4 us a call, 3.9 TB/s (25 us + merge 4)
+//   32 tokens, 8 bits, 527 MB         112 us, 4.7 TB/s (a copy reaches 5.1)
+//   one token over 512 keys           9.6 us a call, the launch and the host
 // Counters: profiles/paged_cache.md.
 #include <algorithm>
 
@@ -674,7 +674,8 @@ constexpr int kChunkLeast = 8;
 // and 63; 48 rows 64 and 67, 54 and 72; 64 rows 79 and 64, 65 and 73; 128 rows
 // 135 and 58, 105 and 82.  256 dims, four sequences: 64 rows f16 94 and 105, 8
 // bits 74 and 121; 128 rows 138 and 124, 104 and 127.  512 dims: 48 rows f16 141
-// and 89, 8 bits 112 and 132.
+// and 89, 8 bits 112 and 132.  (Both kernels before 8-bit sums took an exponential
+// of their own, which costs the rows kernel 1% and the chunk kernel 4%.)
 constexpr int rows_most(int hd, bool i8) { return hd == 256 ? (i8 ? 128 : 64) : i8 ? 64 : 32; }
 
 // Workgroups of the chunk kernel that start at once.

@@ -21,13 +21,13 @@
 //
 // Bound by MFMA: 4 * hd operations a query row and key, for 4 * hd bytes a key
 // that 128 rows share.  Measured (a large matrix product reaches 1.18 PFLOP/s):
-//   prompt of 8192, 32 heads on 8 of 128 dims, f16   559-577 us, 950-983 TFLOP/s
+//   prompt of 8192, 32 heads on 8 of 128 dims, f16   560-575 us, 955-980 TFLOP/s
 //   (MFMA busy 52% of the cycles; without its softmax, operand reads and copies
-//   the loop takes 400 us); 512 rows on 4k keys 56 us, 650 TFLOP/s with the merge
-//   8-bit pages and fp32 queries, nine sequences     277 us, 378 TFLOP/s, twice
+//   the loop takes 400 us); 512 rows on 4k keys 57 us, 640 TFLOP/s with the merge
+//   8-bit pages and fp32 queries, nine sequences     297 us, 353 TFLOP/s, twice
 //   that with the queries' and weights' second parts
-//   256 dims, a window of 1024                       116 us, 512 TFLOP/s
-//   512 dims, 1024 rows of 16 heads on 2048 keys     157 us, 328 TFLOP/s
+//   256 dims, a window of 1024                       106 us, 558 TFLOP/s
+//   512 dims, 1024 rows of 16 heads on 2048 keys     158 us, 327 TFLOP/s
 // Steps on the way, prompt: 128-row tiles of two workgroups a CU, conflict-free
 // places and loops of one tile kind 859 -> 625 us; one base address a tile 578.
 // Waves of 64 rows (half the LDS reads a product, one workgroup a CU) take 677.
@@ -580,11 +580,11 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 // (two workgroups a CU leave 256, one 512) and the LDS.  With both sides
 // measured: f32 queries at 128 dims 64 keys and one workgroup 768 us, 32 keys and
 // two 386 (nine 8-bit sequences); f16 at 256 dims 64 keys and one 135 us, 32 keys
-// and two, though 129 registers spill, 119 (a window of 1024), two waves to a row
-// 139; 8 bits at 256 dims 64 keys and one 366, two waves to a row 585.  512 dims
-// (queries of 128 registers, outputs of 256) need waves that share rows: f16 two
-// 157 us, four 207; 8 bits, whose tiles pass the registers too, two 354, four
-// 263; f32 queries two 478, four 297.
+// and two, though registers spilled (129 then; 63 now), 119 (a window of 1024;
+// 106 now), two waves to a row 139; 8 bits at 256 dims 64 keys and one 366, two
+// waves to a row 585.  512 dims (queries of 128 registers, outputs of 256) need
+// waves that share rows: f16 two 157 us, four 207; 8 bits, whose tiles pass the
+// registers too, two 354, four 263; f32 queries two 478, four 297.
 constexpr int chunk_bn(int hd, bool i8, bool f32) { return hd == 512 || (hd == 256 && (f32 || !i8)) || (hd == 128 && f32) ? 32 : 64; }
 constexpr int chunk_occ(int hd, bool i8, bool f32) { return hd <= 128 || (hd == 256 && !f32 && !i8) ? 2 : 1; }
 constexpr int chunk_ds(int hd, bool i8, bool f32) { return hd <= 256 ? 1 : i8 || f32 ? 4 : 2; }

@@ -18,12 +18,12 @@
 //   eight prompts to 8 bits and back, 228 MB, 128 dims   59 us, 3.87 TB/s (store
 //   22.9 us, read 20.1 us a kernel, the rest lies between the two)
 //   a read of 32768 8-bit positions to f16, 203 MB       46 us, 4.38 TB/s
-//   the prologue of six 8-bit chunks, 256 dims, 310 MB   86 us, 3.6 TB/s: loads
-//   and stores of one head wait on each other (78 us without the angles' sines,
-//   79.5 with; the next head's loads ahead of the stores, or four workgroups a
-//   CU, are not faster)
-//   one decode step of 16 sequences   4.0 us (append), 4.4 us (prologue) a kernel;
-//   a call 9.5 and 14.8 us, all of it the host's
+//   the prologue of six 8-bit chunks, 256 dims, 310 MB   87 us, 3.6 TB/s: two
+//   thirds of the LDS cycles are conflicts of the angle table's stores (13% of
+//   the CU cycles); the next head's loads ahead of the stores, or four
+//   workgroups a CU, are not faster
+//   one decode step of 32 sequences (append) 4.0 us, of 16 (prologue) 4.6 us a
+//   kernel; a call 9.5 and 14.1 us, the host's
 // Counters: profiles/paged_cache.md.
 #include <cmath>
 
