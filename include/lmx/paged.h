@@ -149,7 +149,8 @@ lmx_status lmxp_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *        A result is off by some 2.8e-4 of itself in the former and 2.1e-4 in
  *        the latter (root mean square), its own rounding to f16 included.
  *        LMX_F32: q and out are f32; q and p are carried as two f16 parts each
- *        (22 bits) whatever the lengths.
+ *        (22 bits; an element of q below 2^-39 of its row's largest counts as
+ *        0) whatever the lengths.
  *   q    head h of row i at q + i*q_row_stride + h*q_head_stride (elements,
  *        multiples of 8; 0: contiguous); 16-byte aligned
  *   out  [n_tokens, n_heads, head_dim] contiguous, 16-byte aligned, not

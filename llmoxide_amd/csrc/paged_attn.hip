@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + ((size_t)item * kBM + r) * 2) = f32x2{mm, sum};
         } else {
             const int q = it.tile * kBM + r;
-            y *= sum == 0.f ? 0.f : 1.f / sum;
+            y = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : y * (1.f / sum);  // (y may hold infinities)
             QT* dst = static_cast<QT*>(a.out) +
                       ((size_t)(it.s.row0 + q / pg.G) * pg.Hkv * pg.G + it.h * pg.G + q % pg.G) * HD + d;
             if constexpr (F32)
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         sum += moved<I8>(ex_l[k], ex_m[k] - ref);
         y += ex[k][col] * f;
     }
-    y *= sum == 0.f ? 0.f : 1.f / sum;
+    y = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : y * (1.f / sum);
     QT* dst = static_cast<QT*>(a.out) + ((size_t)(s.row0 + row / pg.G) * pg.Hkv * pg.G + h * pg.G + row % pg.G) * HD + 4 * col;
     if constexpr (F32)
         *reinterpret_cast<f32x4*>(dst) = y;
@@ -635,12 +635,12 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(AttnPagedArgs a,
             }
         m = mn;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = 1.f / l;
     QT* dst = static_cast<QT*>(a.out) +
               ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 4 * hh;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const f32x4 y = o[v] * inv;
+        const f32x4 y = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o[v] * inv;
         const int d = 8 * (4 * v + w);
         if constexpr (F32)
             *reinterpret_cast<f32x4*>(dst + d) = y;

@@ -164,8 +164,8 @@ __device__ __forceinline__ float log_v_scale(float s) { return __builtin_amdgcn_
 // 0, which would make NaN of an infinity among V: 2^-126 of a finite output is
 // far below the last place of the weights beside it.
 __device__ __forceinline__ float join_weight(float d) { return fmaxf(fast_exp2(d), 0x1p-126f); }
-// A sum brought from one reference to another, d above it (d <= 0).  I8: a step
-// down to -240, as scales alone make it, in two factors that f32 holds; above
+// A sum brought to a reference -d above its own (d <= 0).  I8: a step down to
+// -240, as scales alone make it, in two factors that f32 holds; above
 // -120 the second is 1.
 template <bool I8>
 __device__ __forceinline__ float moved(float l, float d) {

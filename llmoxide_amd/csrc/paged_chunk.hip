@@ -545,6 +545,10 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         if (hh == 0 && nb0 == 0) *reinterpret_cast<f32x2*>(a.part_ml + (at + row - r0) * 2) = f32x2{m, sum};
     } else {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if constexpr (!I8)
+            if (sum == 0.f)  // (o may hold infinities)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) o[nb] = f32x16{};
         QT* dst = static_cast<QT*>(a.out) +
                   ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD + 32 * nb0;
 #pragma unroll

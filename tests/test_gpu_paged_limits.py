@@ -313,3 +313,19 @@ def test_a_graph_of_chunks_replays_with_shorter_ones():
         assert torch.equal(*outs) and torch.all(outs[0][:cu[0]] == 4) and torch.all(outs[0][cu[2]:] == 4)
         assert torch.all(torch.isfinite(outs[0]))
         assert torch.equal(cache.k, twin.k) and torch.equal(cache.v, twin.v)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("new,ctx", [([2], [60]), ([2], [2000]), ([150], [150]), ([150], [2000])])
+@pytest.mark.parametrize("hd", [64, 512])
+def test_rows_of_no_weight_are_zero_whatever_the_values(new, ctx, hd, dt):
+    """Every score -infinity, infinities and NaN among V: zeros, in one walk and in splits."""
+    say("no weight", new, ctx, hd, dt)
+    c = po.PagedCase(98, new=new, ctx=ctx, page=16, kv=1, hd=hd)
+    q = rows(c, 99, 2)
+    q[..., 7] = np.abs(q[..., 7]) + 0.5
+    c.k[:, 0, :, 7] = -np.inf
+    for p, x in ((1, np.inf), (40, -np.inf), (ctx[0] - 1, np.nan)):
+        pg, s = c.place(0, p)
+        c.v[pg, 0, 5 * p % hd, s] = x
+    assert np.all(attend(c, q, dt, 2) == 0)
