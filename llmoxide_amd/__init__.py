@@ -24,6 +24,8 @@ this module                reference dispatch it mirrors
                            (qwen35.rs:968-986)
 ``paged_append`` and the   the paged KV cache (include/lmx/paged.h), in
 other ``paged_`` calls     :mod:`llmoxide_amd.paged`
+``spec_plan`` and the      steps with drafted tokens over it
+other ``spec_`` calls      (include/lmx/spec.h), in :mod:`llmoxide_amd.spec`
 =========================  ==================================================
 
 Tensors are torch tensors on a ROCm device (torch provides device memory and
@@ -709,3 +711,5 @@ class KvManager:
 
 from .paged import (PagedBatch, PagedCache, paged_append, paged_attention,  # noqa: E402
                     paged_prologue, paged_read)
+from .spec import (PageTables, SpecTree, StepPlan, Verified, rope_scaling, spec_attention,  # noqa: E402
+                   spec_keep, spec_plan, spec_prologue, spec_tree, spec_verify)

@@ -125,8 +125,9 @@ __device__ __forceinline__ void load_v(const AttnPagedArgs& a, const int (&pages
     for (int l = 0; l < T::VL; ++l) t.v[l] = *reinterpret_cast<const uint4*>(vc + l * vstep);
 }
 
-// F32: q and out are f32 and q has a residual part.
-template <int HD, bool I8, bool F32>
+// F32: q and out are f32 and q has a residual part.  SEEN: rows see each other by
+// a mask, and all of them what lies before them (in their windows).
+template <int HD, bool I8, bool F32, bool SEEN>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(AttnPagedArgs a) {
     using T = Tile<HD, I8>;
     using QT = std::conditional_t<F32, float, f16>;
@@ -160,13 +161,17 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
     const int pos = have ? it.s.ctx - it.s.n + tok : -1;
     const int seen_lo = pg.window ? imax(pos - pg.window + 1, 0) : 0;
+    Sight sight;
+    if constexpr (SEEN) sight = sight_of(a, it.s, have, tok);
     // Keys that every row of the tile sees need no mask.
     const int r_last = imin(it.tile * kBM + kBM, it.s.n * pg.G) - 1;
-    const int all_hi = it.s.ctx - it.s.n + (it.tile * kBM) / pg.G;                       // first row's position
-    const int all_lo = pg.window ? imax(it.s.ctx - it.s.n + r_last / pg.G - pg.window + 1, 0) : 0;
+    const int p_first = it.s.ctx - it.s.n + (SEEN ? 0 : (it.tile * kBM) / pg.G);  // the first row's position, or the least
+    const int p_last = SEEN ? it.s.ctx - 1 : it.s.ctx - it.s.n + r_last / pg.G;   // the last row's, or the largest
+    const int all_hi = SEEN ? p_first - 1 : p_first;
+    const int all_lo = pg.window ? imax(p_last - pg.window + 1, 0) : 0;
     // Keys that some row sees: up to the last row's position, from the first row's window.
-    const int any_hi = it.s.ctx - it.s.n + r_last / pg.G;
-    const int any_lo = pg.window ? imax(all_hi - pg.window + 1, 0) : 0;
+    const int any_hi = p_last;
+    const int any_lo = pg.window ? imax(p_first - pg.window + 1, 0) : 0;
 
     // Q: k-step s holds dims 32s + 8g (f16 tiles); an 8-bit tile's 16-byte load
     // spans two k-steps, so there k-step 2l + e holds dims 64l + 16g + 8e.
@@ -319,9 +324,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             const int key = t0 + QUART * g;
             if constexpr (!I8) v_mask = page >= 0 ? keys8_mask(any_lo - key, any_hi - key) : uint4{};
             seen = 0;
+            if constexpr (SEEN) {
+                if (page >= 0) seen = (uint32_t)sight.from(key) & ((1u << QUART) - 1);
+            } else {
 #pragma unroll
-            for (int i = 0; i < QUART; ++i)
-                seen |= (uint32_t)(page >= 0 && key + i <= pos && key + i >= seen_lo) << i;
+                for (int i = 0; i < QUART; ++i)
+                    seen |= (uint32_t)(page >= 0 && key + i <= pos && key + i >= seen_lo) << i;
+            }
 #pragma unroll
             for (int j = 0; j < T::NB; ++j)
 #pragma unroll
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 if (key >= key_hi) break;
                 if (key >= pw.end(a.p)) pw.fill(a.p, key);
                 const int page = pw.at(a.p, key);
-                if (page < 0 || key > pos || key < seen_lo) continue;
+                if (page < 0 || (SEEN ? !sight.sees(key) : key > pos || key < seen_lo)) continue;
                 const f16* e = reinterpret_cast<const f16*>(a.p.v) +
                                v_offset(a.p, page, it.h, key & ((1 << pg.ps_log2) - 1)) + ((4 * g) << pg.ps_log2);
 #pragma unroll
@@ -800,12 +809,16 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     const dim3 grid((unsigned)r.items);
     if (chunk) {
         launch_chunk(a, HD, i8, f32, grid.x, st);
-    } else if (i8) {
-        if (f32) hipLaunchKernelGGL((paged_rows_kernel<HD, true, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((paged_rows_kernel<HD, true, false>), grid, dim3(256), 0, st, a);
     } else {
-        if (f32) hipLaunchKernelGGL((paged_rows_kernel<HD, false, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((paged_rows_kernel<HD, false, false>), grid, dim3(256), 0, st, a);
+        auto go = [&](auto i8_tag, auto f32_tag) {
+            constexpr bool I8 = decltype(i8_tag)::value, F32 = decltype(f32_tag)::value;
+            if (a.seen) hipLaunchKernelGGL((paged_rows_kernel<HD, I8, F32, true>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((paged_rows_kernel<HD, I8, F32, false>), grid, dim3(256), 0, st, a);
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        if (i8) f32 ? go(yes, yes) : go(yes, no);
+        else f32 ? go(no, yes) : go(no, no);
     }
     LMX_CHECK_LAUNCH();
     if (r.splits) {
@@ -835,9 +848,14 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     return LMX_OK;
 }
 
-lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const void* q, lmx_dtype dt,
-                      void* out, void* ws, hipStream_t st) {
+// seen NULL: causal.
+static lmx_status attend(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const uint64_t* seen,
+                         uint32_t words, const int32_t* at, const void* q, lmx_dtype dt, void* out, void* ws,
+                         hipStream_t st) {
     AttnPagedArgs a{};
+    a.seen = seen;
+    a.words = (int)words;
+    a.at = at;
     a.p = paged_args(p, b);
     a.p.g = attn_geom(p, b, d);
     a.q = q;
@@ -859,6 +877,15 @@ lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_d
         case 256: return go(std::integral_constant<int, 256>{});
         default: return go(std::integral_constant<int, 512>{});
     }
+}
+lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const void* q, lmx_dtype dt,
+                      void* out, void* ws, hipStream_t st) {
+    return attend(p, b, d, nullptr, 0, nullptr, q, dt, out, ws, st);
+}
+lmx_status paged_attn_seen(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const uint64_t* seen,
+                           uint32_t words, const int32_t* pos, const void* q, lmx_dtype dt, void* out, void* ws,
+                           hipStream_t st) {
+    return attend(p, b, d, seen, words, pos, q, dt, out, ws, st);
 }
 
 }  // namespace lmx

@@ -19,12 +19,50 @@ struct AttnPagedArgs {
     int least;            // units a split has at least
     int rt_max;           // entries of `rows` a (sequence, head)
     int lo_rows, hi_rows; // this kernel takes sequences with lo_rows < rows * G <= hi_rows
+    // rows that see each other by a mask only
+    const uint64_t* seen; // [n_tokens][words]
+    int words;
+    const int32_t* at;    // [n_tokens] positions; read in a window
 };
+
+// What one query row sees where a mask says so (SEEN kernels): of the positions
+// before its sequence's rows those from lo on, of the rows those whose bit is set.
+struct Sight {
+    const uint64_t* bits;  // of the row; NULL: it sees nothing
+    int words, lo, first, n;  // first: position of the sequence's row 0, n: its rows
+    // Of the 64 positions from t0 on, those that it sees (pages apart).
+    __device__ __forceinline__ uint64_t from(int t0) const {
+        if (!bits) return 0;
+        auto below = [](int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
+        uint64_t m = below(first - t0) & ~below(lo - t0);
+        const int j = t0 - first;  // the sequence's row at t0: two words hold the 64 rows from there on
+        if (j > -64 && j < n) {
+            const int w = j >> 6, sh = j & 63;
+            const uint64_t x = w >= 0 ? bits[imin(w, words - 1)] : 0;
+            const uint64_t y = w + 1 < words ? bits[w + 1] : 0;
+            m |= (sh ? x >> sh | y << (64 - sh) : x) & below(n - j);
+        }
+        return m;
+    }
+    __device__ __forceinline__ bool sees(int key) const { return from(key) & 1; }
+};
+// Row `row` (of the sequence's, `have`: it is one) and the lowest position that it sees.
+__device__ __forceinline__ Sight sight_of(const AttnPagedArgs& a, const PagedSeq& s, bool have, int row) {
+    Sight r;
+    r.bits = have ? a.seen + (size_t)(s.row0 + row) * a.words : nullptr;
+    r.words = a.words;
+    r.first = imax(s.ctx - s.n, 0);
+    r.n = imin(s.n, 64 * a.words);
+    r.lo = 0;
+    if (a.p.g.window && have)
+        r.lo = imax(imin(imax(a.at[s.row0 + row], r.first), s.ctx - 1) - a.p.g.window + 1, 0);
+    return r;
+}
 
 // paged_chunk.hip: rows of its workgroups, and the launch.
 int chunk_rows(int hd, bool i8, bool f32);
 int chunk_occ_of(int hd, bool i8, bool f32);  // workgroups a CU holds
-void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);
+void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st);  // a.seen: by a mask
 
 // Where a chunk's partial output keeps the dims 8c + 4 (lane / 32) .. of row
 // 32 blk + lane % 32 of its tile.

@@ -97,7 +97,8 @@ struct ChunkTile {
 
 // BN: keys a tile.  DS: waves that share rows, each with its part of the
 // output's dims (the scores are made by all of them).  OCC: workgroups a CU.
-template <int HD, bool I8, bool F32, int BN, int DS, int OCC>
+// SEEN: rows see each other by a mask, and all what lies before them.
+template <int HD, bool I8, bool F32, int BN, int DS, int OCC, bool SEEN>
 __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) {
     using T = ChunkTile<HD, BN, DS>;
     using QT = std::conditional_t<F32, float, f16>;
@@ -122,21 +123,26 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     auto low_of = [&](int pos) { return pg.window ? imax(pos - pg.window + 1, 0) : 0; };
     const int split_lo = it.splits > 1 ? it.w.lo + it.split * it.per * kUnit : it.w.lo;
     const int split_hi = it.splits > 1 ? split_lo + it.per * kUnit : 0x7fffffff;
-    const int k_lo = imax(low_of(pos_of(r0)) & ~(BN - 1), split_lo);
-    const int k_hi = imin(pos_of(r1) + 1, split_hi);  // one behind the last key
+    // a tile's first and last position (by a mask: the least and the largest)
+    auto least = [&](int r) { return SEEN ? first_pos : pos_of(r); };
+    auto most = [&](int r) { return SEEN ? it.s.ctx - 1 : pos_of(r); };
+    const int k_lo = imax(low_of(least(r0)) & ~(BN - 1), split_lo);
+    const int k_hi = imin(most(r1) + 1, split_hi);  // one behind the last key
     const int n_t = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
     // the wave's: keys some row sees, keys all rows see
     const int w0 = r0 + w / DS * 32, w1 = imin(w0 + 32, n_rows) - 1;
     const int nb0 = w % DS * NB;  // the wave's first block of dims
     const bool live = w0 <= r1;
-    const int any_hi = live ? pos_of(w1) : -1, all_hi = live ? pos_of(w0) : -1;
-    const int any_lo = live ? low_of(pos_of(w0)) : 0, all_lo = live ? low_of(pos_of(w1)) : 0;
+    const int any_hi = live ? most(w1) : -1, all_hi = live ? least(w0) - SEEN : -1;
+    const int any_lo = live ? low_of(least(w0)) : 0, all_lo = live ? low_of(most(w1)) : 0;
 
     f16x8 qh[KS], ql[F32 ? KS : 1];
     const int row = w0 + l32;
     const bool have = row < n_rows;
     const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
     const int pos = have ? first_pos + tok : -1, seen_lo = low_of(pos);
+    Sight sight;
+    if constexpr (SEEN) sight = sight_of(a, it.s, have, tok);
     float qs = a.c;  // what a score is multiplied by
     const QT* qr = static_cast<const QT*>(a.q) + (size_t)(it.s.row0 + tok) * a.q_row_stride + head * a.q_head_stride + 8 * hh;
     if constexpr (F32) {
@@ -344,12 +350,14 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 }
             }
         if constexpr (!WHOLE) {
+            uint64_t seen = 0;  // bit k: key t0 + 8 hh + k
+            if constexpr (SEEN) seen = sight.from(t0 + 8 * hh);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int key = t0 + 32 * kb + 16 * (i >> 3) + 8 * hh + (i & 7);
-                    const bool on = p[2 * kb + (i >> 3)] >= 0 && key <= pos && key >= seen_lo;
+                    const int at = 32 * kb + 16 * (i >> 3) + (i & 7), key = t0 + 8 * hh + at;
+                    const bool on = p[2 * kb + (i >> 3)] >= 0 && (SEEN ? seen >> at & 1 : key <= pos && key >= seen_lo);
                     if (!on) s[kb][i] = -INFINITY;
                 }
         }
@@ -515,7 +523,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 for (int key = k_lo; key < k_hi; ++key) {
                     if (key >= pw.end(a.p)) pw.fill(a.p, key);
                     const int page = pw.at(a.p, key);
-                    if (page < 0 || key > pos || key < seen_lo) continue;
+                    if (page < 0 || (SEEN ? !sight.sees(key) : key > pos || key < seen_lo)) continue;
                     const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
                                    ((32 * (nb0 + nb) + 4 * hh) << pg.ps_log2);
 #pragma unroll
@@ -597,7 +605,10 @@ int chunk_occ_of(int hd, bool i8, bool f32) { return chunk_occ(hd, i8, f32); }
 
 template <int HD, bool I8, bool F32>
 static void go_chunk(const AttnPagedArgs& a, unsigned items, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_bn(HD, I8, F32), chunk_ds(HD, I8, F32), chunk_occ(HD, I8, F32)>), dim3(items), dim3(256), 0, st, a);
+    auto launch = [&](auto seen) {
+        hipLaunchKernelGGL((paged_chunk_kernel<HD, I8, F32, chunk_bn(HD, I8, F32), chunk_ds(HD, I8, F32), chunk_occ(HD, I8, F32), decltype(seen)::value>), dim3(items), dim3(256), 0, st, a);
+    };
+    a.seen ? launch(std::true_type{}) : launch(std::false_type{});
 }
 void launch_chunk(const AttnPagedArgs& a, int hd, bool i8, bool f32, unsigned items, hipStream_t st) {
     auto by = [&](auto tag) {

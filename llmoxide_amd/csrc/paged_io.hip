@@ -28,6 +28,7 @@
 #include <cmath>
 
 #include "lds_dma.hpp"
+#include "lmx/spec.h"
 #include "paged.hpp"
 
 namespace lmx {
@@ -203,7 +204,13 @@ struct StoreArgs {
     int n_rot, v_norm, q_out_f16;
     float eps;
     double scale_pow[8];  // s^(2^k), s = base^(-2/n_rot): pair i turns by pos * s^i
+    // prologue at given positions only
+    const int32_t* at;    // [n_tokens]; NULL: the slots' positions
+    int interleaved;      // pairs (2i, 2i + 1)
+    float turn_scale;     // of cos and sin
 };
+// What a store does to its rows on the way.
+enum Pro { kPlain, kPrologue, kPrologueAt };
 
 // sin and cos of theta (double): the multiple of pi/2 is taken off in double,
 // what is left (|r| <= pi/4) goes through its Taylor series in f32: the terms
@@ -247,6 +254,23 @@ __device__ __forceinline__ void turn_row(f32x4 (&e)[2], const float (&c)[4], con
         e[0][j] = p * c[j] - q * s[j];
         e[1][j] = q * c[j] + p * s[j];
     }
+}
+// Neighbouring dims turn, those below 2 * half: pairs 2 li, 2 li + 1 of the first
+// half and as many of the second are the lane's own.
+template <int HD, typename F>
+__device__ __forceinline__ void turn_pairs(f32x4 (&e)[2], int li, int half, const F& turn_at) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * li + HD / 4 * v + j;
+            if (i < half) {
+                const float2 t = turn_at(i);
+                const float p = e[v][2 * j], q = e[v][2 * j + 1];
+                e[v][2 * j] = p * t.x - q * t.y;
+                e[v][2 * j + 1] = q * t.x + p * t.y;
+            }
+        }
 }
 // The first 2 * half dims turn: partners lie in other lanes as a rule, so the
 // row goes through LDS (rs: the row's floats).  turn_at(i): (cos, sin) of pair i.
@@ -296,7 +320,7 @@ __device__ __forceinline__ double freq_of(const StoreArgs& a, int i) {
 
 // Rows of prompts.  PRO: norm and rotate on the way, and take the query heads
 // too.
-template <typename SRC, bool I8, int HD, bool PRO>
+template <typename SRC, bool I8, int HD, Pro PRO>
 __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
     using L = RowLanes<HD>;
     using VT = VTile<HD, I8>;
@@ -344,10 +368,13 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
         int rl2 = 0;
         while ((1 << rl2) < n_rows) ++rl2;
         const int row = tid & ((1 << rl2) - 1);
-        const double pos = (double)__shfl(at.pos, row, 64);
+        int stands = __shfl(at.pos, row, 64);
+        if (PRO == kPrologueAt && a.at) stands = a.at[r0 + imin(row, n_rows - 1)];
+        const double pos = (double)stands;
         for (int i = tid >> rl2; i < half; i += 256 >> rl2) {
             float c, s;
             turn_of(pos * freq_s[i], c, s);
+            if (PRO == kPrologueAt) c *= a.turn_scale, s *= a.turn_scale;
             turn[row * H2 + i] = make_float2(c, s);
         }
         __syncthreads();
@@ -365,7 +392,9 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
             if constexpr (PRO) {
                 const float* gain = is_v ? nullptr : is_k ? a.k_gain : a.q_gain;
                 if (is_v ? a.v_norm != 0 : gain != nullptr) norm_row<LPR, HD>(e, gain, a.eps, li);
-                if (!is_v && half == H2) {
+                if (PRO == kPrologueAt && a.interleaved) {
+                    if (!is_v) turn_pairs<HD>(e, li, half, [&](int i) { return turn[rl * H2 + i]; });
+                } else if (!is_v && half == H2) {
                     const f32x4* t = reinterpret_cast<const f32x4*>(&turn[rl * H2 + 4 * li]);
                     const f32x4 t0 = t[0], t1 = t[1];
                     turn_row(e, {t0[0], t0[2], t1[0], t1[2]}, {t0[1], t0[3], t1[1], t1[3]});
@@ -465,7 +494,7 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
 
 // Single tokens: a row head is LPR lanes of a wave, from load to store; no LDS
 // but for a partial turn, V's column element by element.
-template <typename SRC, bool I8, int HD, bool PRO>
+template <typename SRC, bool I8, int HD, Pro PRO>
 __global__ __launch_bounds__(256) void paged_store_tokens_kernel(StoreArgs a) {
     using L = RowLanes<HD>;
     using DT = std::conditional_t<I8, int8_t, f16>;
@@ -502,19 +531,29 @@ __global__ __launch_bounds__(256) void paged_store_tokens_kernel(StoreArgs a) {
             e[0] = n[0];
             e[1] = n[1];
         }
-        if (half == H2) {
+        int stands = at.pos;
+        if (PRO == kPrologueAt && a.at) stands = a.at[row];
+        auto turn = [&](int i) {  // pair i's
+            float2 t;
+            turn_of((double)stands * freq_of(a, i), t.x, t.y);
+            if (PRO == kPrologueAt) t.x *= a.turn_scale, t.y *= a.turn_scale;
+            return t;
+        };
+        if (PRO == kPrologueAt && a.interleaved) {
+            if (!is_v) turn_pairs<HD>(e, li, half, turn);
+        } else if (half == H2) {
             float c[4], s[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) turn_of((double)at.pos * freq_of(a, 4 * li + j), c[j], s[j]);
+            for (int j = 0; j < 4; ++j) {
+                const float2 t = turn(4 * li + j);
+                c[j] = t.x;
+                s[j] = t.y;
+            }
             if (!is_v) turn_row(e, c, s);
         } else if (half) {
             n[0] = e[0];
             n[1] = e[1];
-            turn_part<HD>(n, rows_s[w] + sub * HD, li, half, [&](int i) {
-                float2 t;
-                turn_of((double)at.pos * freq_of(a, i), t.x, t.y);
-                return t;
-            });
+            turn_part<HD>(n, rows_s[w] + sub * HD, li, half, turn);
             if (!is_v) {
                 e[0] = n[0];
                 e[1] = n[1];
@@ -731,7 +770,7 @@ static bool grid_fits(int64_t x, int64_t y) { return x < (1 << 24) && y < (1 << 
 // 4.4 against 12.6; four rows: 15.4 us a prologue call on either.
 static bool few_rows(const PagedGeom& g) { return g.max_new <= 4; }
 
-template <bool PRO, typename SRC, bool I8>
+template <Pro PRO, typename SRC, bool I8>
 static lmx_status launch_store_hd(const StoreArgs& a, int hd, hipStream_t st) {
     auto go = [&](auto tag) {
         constexpr int HD = decltype(tag)::value;
@@ -773,13 +812,14 @@ lmx_status paged_append(const lmxp_pool* p, const lmxp_batch* b, const void* k_n
     const bool i8 = p->store == LMXP_I8;
     const int hd = (int)p->head_dim;
     if (src_dt == LMX_F32)
-        return i8 ? launch_store_hd<false, float, true>(a, hd, st) : launch_store_hd<false, float, false>(a, hd, st);
-    return i8 ? launch_store_hd<false, f16, true>(a, hd, st) : launch_store_hd<false, f16, false>(a, hd, st);
+        return i8 ? launch_store_hd<kPlain, float, true>(a, hd, st) : launch_store_hd<kPlain, float, false>(a, hd, st);
+    return i8 ? launch_store_hd<kPlain, f16, true>(a, hd, st) : launch_store_hd<kPlain, f16, false>(a, hd, st);
 }
 
-lmx_status paged_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
-                          const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
-                          const float* factors, void* q_out, lmx_dtype q_out_dt, hipStream_t st) {
+// The arguments of a prologue.
+static StoreArgs prologue_args(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
+                               const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
+                               const float* factors, void* q_out, lmx_dtype q_out_dt) {
     StoreArgs a{};
     a.p = paged_args(p, b);
     a.k_new = k_new;
@@ -804,10 +844,31 @@ lmx_status paged_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_pr
     a.g_k = (a.n_k + a.hpw - 1) / a.hpw;
     a.g_v = (a.n_v + a.hpw - 1) / a.hpw;
     a.g_q = (a.n_q + a.hpw - 1) / a.hpw;
+    return a;
+}
+
+lmx_status paged_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
+                          const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
+                          const float* factors, void* q_out, lmx_dtype q_out_dt, hipStream_t st) {
+    const StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt);
     (void)hipGetLastError();
     const int hd = (int)p->head_dim;
-    return p->store == LMXP_I8 ? launch_store_hd<true, float, true>(a, hd, st)
-                               : launch_store_hd<true, float, false>(a, hd, st);
+    return p->store == LMXP_I8 ? launch_store_hd<kPrologue, float, true>(a, hd, st)
+                               : launch_store_hd<kPrologue, float, false>(a, hd, st);
+}
+
+lmx_status paged_prologue_at(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const lmxs_rope* r,
+                             const int32_t* pos, const float* q, const float* k_new, const float* v_new,
+                             const float* q_gain, const float* k_gain, const float* factors, void* q_out,
+                             lmx_dtype q_out_dt, hipStream_t st) {
+    StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt);
+    a.at = pos;
+    a.interleaved = (int)r->interleaved;
+    a.turn_scale = r->turn_scale;
+    (void)hipGetLastError();
+    const int hd = (int)p->head_dim;
+    return p->store == LMXP_I8 ? launch_store_hd<kPrologueAt, float, true>(a, hd, st)
+                               : launch_store_hd<kPrologueAt, float, false>(a, hd, st);
 }
 
 template <typename OUT, bool I8>

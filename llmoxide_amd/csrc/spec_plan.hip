@@ -1,0 +1,261 @@
+// Pages and row maps of a step from its requests' lengths, and positions and
+// sight of its rows from their parents.
+//
+// The list of free pages is a stack: given-back pages go on top, then requests
+// take from the top in order, so a request's first page lies at a place that
+// sums over the requests before it name.  One workgroup makes these sums (1024
+// requests at a time) and moves the pages, a thread an entry, whatever request
+// it is of; the order of everything is that of the sums, none of arrivals.
+//
+// Bound by latency: a step's entries and rows are a few KB, read once through
+// four dependent steps (lengths, sums, free list, table).
+#include "spec.hpp"
+
+namespace lmx {
+
+struct PlanArgs {
+    int n_seq, n_tokens, ps_log2, stride, n_pages, trim;
+    int rows_here;  // 1: the plan's workgroup maps the rows too
+    const int32_t* lens;
+    const int32_t* fresh;
+    int32_t* table;
+    int32_t* held;
+    int32_t* free_pages;
+    int32_t* n_free;
+    int32_t* cu;
+    int32_t* ctx;
+    int64_t* slots;
+    int32_t* pos;
+};
+
+constexpr int kPlan = 1024;  // threads, and requests at a time
+
+struct Request {
+    int len, rows, total, need, held;
+};
+__device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
+    Request r;
+    r.len = imax(a.lens[b], 0);
+    r.rows = imin(imax(a.fresh[b], 0), a.n_tokens);
+    r.held = imin(imax(a.held[b], 0), a.stride);
+    const int64_t room = (int64_t)a.stride << a.ps_log2, total = (int64_t)r.len + r.rows;
+    r.total = (int)(total < room ? total : room < kMost ? room : kMost);
+    r.total = imin(r.total, kMost);
+    r.need = (int)(((int64_t)r.total + (1 << a.ps_log2) - 1) >> a.ps_log2);
+    return r;
+}
+
+// Inclusive scan over the workgroup; `sums` (16 words of LDS) may be used again
+// afterwards.
+__device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    x = wave_scan_sat(x);
+    if (lane == 63) sums[w] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int k = 0; k < kPlan / 64; ++k) {
+        if (k == w) before = total;
+        total = add_sat(total, sums[k]);
+    }
+    __syncthreads();
+    return add_sat(x, before);
+}
+// Of 1024 rising numbers, the last at or below i (the first one is).
+__device__ __forceinline__ int last_at(const int* start, int i) {
+    int at = 0;
+#pragma unroll
+    for (int step = kPlan / 2; step > 0; step >>= 1) at += start[at + step] <= i ? step : 0;
+    return at;
+}
+
+// Row j of request b, whose rows begin behind `len` positions.
+__device__ __forceinline__ void map_row(const PlanArgs& a, int row, int b, int len, int j) {
+    const int64_t p = (int64_t)len + j, e = p >> a.ps_log2;
+    int page = -1;
+    if (e < a.stride) page = a.table[(size_t)b * a.stride + e];
+    if (a.slots)
+        a.slots[row] = (uint32_t)page < (uint32_t)a.n_pages ? ((int64_t)page << a.ps_log2) + (p & ((1 << a.ps_log2) - 1)) : -1;
+    if (a.pos) a.pos[row] = (int32_t)(p < 0x7fffffff ? p : 0x7fffffff);
+}
+__device__ __forceinline__ void map_none(const PlanArgs& a, int row) {
+    if (a.slots) a.slots[row] = -1;
+    if (a.pos) a.pos[row] = -1;
+}
+
+__global__ __launch_bounds__(kPlan) void spec_plan_kernel(PlanArgs a) {
+    __shared__ int sums[kPlan / 64];
+    __shared__ int start[kPlan], from[kPlan];        // of entries: a request's first, and its place in the table
+    __shared__ int row_start[kPlan], row_len[kPlan];  // of rows
+    const int tid = threadIdx.x;
+    int top = imin(imax(a.n_free[0], 0), a.n_pages);  // free pages
+
+    if (a.trim)
+        for (int hi = a.n_seq; hi > 0; hi -= kPlan) {  // the last requests first
+            const int b = hi - 1 - tid;
+            int n = 0, last = 0, total;
+            if (b >= 0) {
+                const Request r = load_request(a, b);
+                n = imax(r.held - r.need, 0);
+                last = r.held - 1;
+            }
+            const int upto = block_scan(n, sums, total);
+            if (total == 0) continue;  // uniform
+            start[tid] = upto - n;
+            from[tid] = last;
+            __syncthreads();
+            for (int i0 = 0; i0 < total; i0 += kPlan) {
+                const int i = i0 + tid;
+                int id = -1, back;
+                if (i < total) {
+                    const int t = last_at(start, i);
+                    int32_t* at = a.table + (size_t)(hi - 1 - t) * a.stride + (from[t] - (i - start[t]));
+                    id = *at;
+                    *at = -1;
+                }
+                const bool page = (uint32_t)id < (uint32_t)a.n_pages;
+                const int rank = block_scan(page, sums, back);
+                const int to = top + rank - 1;
+                if (page && to < a.n_pages) a.free_pages[to] = id;
+                top = imin(top + back, a.n_pages);
+            }
+        }
+    __syncthreads();
+
+    int rows = 0, taken = 0;  // of the requests before
+    for (int c0 = 0; c0 < a.n_seq; c0 += kPlan) {
+        const int b = c0 + tid;
+        Request r{0, 0, 0, 0, 0};
+        int had = 0, want = 0, all_rows, all_want;
+        if (b < a.n_seq) {
+            r = load_request(a, b);
+            had = a.trim ? imin(r.held, r.need) : r.held;
+            want = imax(r.need - had, 0);
+        }
+        const int rows_upto = block_scan(r.rows, sums, all_rows);
+        const int want_upto = block_scan(want, sums, all_want);
+        if (b < a.n_seq) {
+            a.cu[b + 1] = imin(add_sat(rows, rows_upto), a.n_tokens);
+            a.ctx[b] = r.total;
+            a.held[b] = had + imin(imax(top - add_sat(taken, want_upto - want), 0), want);
+        }
+        start[tid] = want_upto - want;
+        from[tid] = had;
+        row_start[tid] = rows_upto - r.rows;
+        row_len[tid] = r.len;
+        __syncthreads();
+        for (int i = tid; i < all_want; i += kPlan) {
+            const int t = last_at(start, i), at = top - 1 - add_sat(taken, i);
+            a.table[(size_t)(c0 + t) * a.stride + from[t] + (i - start[t])] = at >= 0 ? a.free_pages[at] : -1;
+        }
+        if (a.rows_here) {
+            __syncthreads();
+            for (int i = tid; i < all_rows && rows + i < a.n_tokens; i += kPlan) {
+                const int t = last_at(row_start, i);
+                map_row(a, rows + i, c0 + t, row_len[t], i - row_start[t]);
+            }
+        }
+        rows = add_sat(rows, all_rows);
+        taken = add_sat(taken, all_want);
+        __syncthreads();
+    }
+    if (a.rows_here)
+        for (int row = rows + tid; row < a.n_tokens; row += kPlan) map_none(a, row);
+    if (tid == 0) {
+        a.cu[0] = 0;
+        a.n_free[0] = imax(top - taken, 0);
+        a.n_free[1] = imax(taken - top, 0);
+    }
+}
+
+// The map of many rows: a thread a row.
+__global__ __launch_bounds__(256) void spec_rows_kernel(PlanArgs a) {
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row >= a.n_tokens) return;
+    if (row >= a.cu[a.n_seq]) return map_none(a, row);
+    int lo = 0, hi = a.n_seq;  // the last request that begins at or below the row
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    map_row(a, row, lo, imax(a.lens[lo], 0), row - a.cu[lo]);
+}
+
+// Rows that the plan's workgroup maps itself.
+constexpr int kRowsHere = 4096;
+
+lmx_status spec_plan(const lmxs_plan_desc* d, const int32_t* lens, const int32_t* new_rows, int32_t* table, int32_t* held,
+                     int32_t* free_pages, int32_t* n_free, int32_t* cu, int32_t* ctx, int64_t* slots, int32_t* pos,
+                     hipStream_t st) {
+    PlanArgs a{};
+    a.n_seq = (int)d->n_seq;
+    a.n_tokens = (int)d->n_tokens;
+    while ((1u << a.ps_log2) < d->page_size) ++a.ps_log2;
+    a.stride = (int)d->table_stride;
+    a.n_pages = (int)d->n_pages;
+    a.trim = (int)d->trim;
+    a.lens = lens;
+    a.fresh = new_rows;
+    a.table = table;
+    a.held = held;
+    a.free_pages = free_pages;
+    a.n_free = n_free;
+    a.cu = cu;
+    a.ctx = ctx;
+    a.slots = slots;
+    a.pos = pos;
+    const bool map = slots || pos;
+    a.rows_here = map && a.n_tokens <= kRowsHere;
+    (void)hipGetLastError();
+    hipLaunchKernelGGL(spec_plan_kernel, dim3(1), dim3(kPlan), 0, st, a);
+    LMX_CHECK_LAUNCH();
+    if (map && !a.rows_here) {
+        hipLaunchKernelGGL(spec_rows_kernel, dim3((unsigned)((a.n_tokens + 255) / 256)), dim3(256), 0, st, a);
+        LMX_CHECK_LAUNCH();
+    }
+    return LMX_OK;
+}
+
+// ------------------------------------------------------------------- trees --
+// A workgroup takes a request.  A thread walks from its row up to the root and
+// gathers one word of the ancestors on the way: a tree of 64 drafts is some ten
+// steps deep, and its parents are in LDS.  (Doubling the reach of every row's
+// sight a step would need a copy of all words a step.)
+__global__ __launch_bounds__(256) void spec_tree_kernel(int n_tokens, int words, int window, const int32_t* cu,
+                                                        const int32_t* ctx, const int32_t* parent, int32_t* pos,
+                                                        uint64_t* seen) {
+    __shared__ int up[LMXS_MAX_ROWS];
+    const SpecRows s = spec_rows(cu, blockIdx.x, n_tokens, 64 * words);
+    for (int i = threadIdx.x; i < s.n; i += 256) {
+        const int p = parent[s.row0 + i];
+        up[i] = p >= 0 && p < i ? p : -1;
+    }
+    const int first = imax(ctx[blockIdx.x] - s.n, 0);
+    __syncthreads();
+    for (int x = threadIdx.x; x < s.n * words; x += 256) {
+        const int row = x / words, w = x % words;
+        uint64_t bits = 0;
+        int depth = 0;
+        for (int p = row;;) {
+            if (p >> 6 == w && (!window || depth < window)) bits |= 1ull << (p & 63);
+            p = up[p];
+            if (p < 0) break;
+            ++depth;
+        }
+        if (seen) seen[(size_t)(s.row0 + row) * words + w] = bits;
+        if (pos && w == 0) pos[s.row0 + row] = first + depth;
+    }
+}
+
+lmx_status spec_tree(const lmxp_batch* b, const int32_t* parent, uint32_t words, uint32_t window, int32_t* pos,
+                     uint64_t* seen, hipStream_t st) {
+    (void)hipGetLastError();
+    hipLaunchKernelGGL(spec_tree_kernel, dim3(b->n_seq), dim3(256), 0, st, (int)b->n_tokens, (int)words, (int)window,
+                       b->cu, b->ctx_lens, parent, pos, seen);
+    LMX_CHECK_LAUNCH();
+    return LMX_OK;
+}
+
+}  // namespace lmx

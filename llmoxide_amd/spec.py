@@ -1,0 +1,470 @@
+"""Steps with drafted tokens over the paged KV cache (include/lmx/spec.h): pages and
+row maps from the requests' lengths, trees, the prologue at their positions,
+attention by their masks, verification of the drafts and the keeping of what was
+accepted.
+
+=====================  ======================================================
+this module            what it does
+=====================  ======================================================
+``spec_plan``          page table, row offsets, lengths and slots of a step
+``spec_tree``          positions of a tree's rows, and who sees whom
+``spec_prologue``      ``paged_prologue`` at given positions, either order of
+                       pairs, with scaled turns
+``spec_attention``     ``paged_attention`` of rows that see each other by a mask
+``spec_verify``        which drafts the target accepts, and the next token
+``spec_keep``          the accepted rows to consecutive slots, in all layers
+=====================  ======================================================
+
+The reference decodes one token at a time (docs/limitations.md:21).  A request's
+rows are its last accepted token, whose K and V the cache lacks, and drafted tokens
+behind it; ``parent`` names the row that each continues.  One step of a loop::
+
+    step = spec_plan(tables, lens, new_rows, out=step, trim=True)
+    tree = spec_tree(parent, batch, out=tree)             # batch of step and tables
+    for layer in layers:
+        q = spec_prologue(..., layer.cache, batch, pos=tree.pos)
+        o = spec_attention(q, layer.cache, batch, tree.seen)
+    got = spec_verify(p, tokens, u, r, step.cu, max_new=..., parent=parent, lens=lens)
+    spec_keep([layer.cache for layer in layers], batch, got.path, got.accepted)
+
+All of it is read on the device, so the loop can be one captured graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import NamedTuple, Optional, Sequence
+
+from . import F32, Workspace, _check, _need_cuda, _ptr, _stream, _torch, lib
+from . import paged as _paged
+from .paged import BatchDesc, PagedAttnDesc, PagedBatch, PagedCache, PagedPrologueDesc, PoolDesc, _new_out, _rows
+
+#: Most rows of a request in a tree, an attention, a verification and a keeping.
+MAX_ROWS = 1024
+
+_U32, _VP = ctypes.c_uint32, ctypes.c_void_p
+
+
+class SpecPlanDesc(ctypes.Structure):
+    """lmxs_plan_desc."""
+    _fields_ = [("n_seq", _U32), ("n_tokens", _U32), ("page_size", _U32), ("table_stride", _U32), ("n_pages", _U32),
+                ("trim", _U32)]
+
+
+class SpecRope(ctypes.Structure):
+    """lmxs_rope."""
+    _fields_ = [("interleaved", _U32), ("turn_scale", ctypes.c_float)]
+
+
+class SpecVerifyDesc(ctypes.Structure):
+    """lmxs_verify_desc."""
+    _fields_ = [("n_seq", _U32), ("n_tokens", _U32), ("max_new", _U32), ("vocab", _U32), ("p_stride", _U32),
+                ("q_stride", _U32), ("greedy", _U32)]
+
+
+_PP, _PB = ctypes.POINTER(PoolDesc), ctypes.POINTER(BatchDesc)
+_PR, _PA = ctypes.POINTER(PagedPrologueDesc), ctypes.POINTER(PagedAttnDesc)
+_PS, _PO, _PV = ctypes.POINTER(SpecPlanDesc), ctypes.POINTER(SpecRope), ctypes.POINTER(SpecVerifyDesc)
+_I, _SZ = ctypes.c_int, ctypes.c_size_t
+# Every symbol include/lmx/spec.h declares.
+SIGNATURES = {
+    "lmxs_plan": (_I, [_PS] + [_VP] * 11),
+    "lmxs_tree": (_I, [_PB, _VP, _U32, _U32, _VP, _VP, _VP]),
+    "lmxs_prologue": (_I, [_PP, _PB, _PR, _PO] + [_VP] * 8 + [_I, _VP]),
+    "lmxs_attn": (_I, [_PP, _PB, _PA, _VP, _U32, _VP, _VP, _I, _VP, _VP, _SZ, _VP]),
+    "lmxs_verify_workspace_bytes": (_SZ, [_PV]),
+    "lmxs_verify": (_I, [_PV] + [_VP] * 5 + [_I] + [_VP] * 7 + [_SZ, _VP]),
+    "lmxs_keep": (_I, [_PP, _U32, _PB, _VP, _U32, _VP, _VP]),
+}
+
+_lib = None
+
+
+def spec_lib() -> ctypes.CDLL:
+    """The library with lmx/spec.h's signatures set; raises if it is missing."""
+    global _lib
+    if _lib is None:
+        L = lib()
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        _lib = L
+    return _lib
+
+
+def _ints(what: str, *ts, size=None) -> None:
+    """int32 tensors, contiguous and on the GPU, of ``size`` elements each."""
+    torch = _torch()
+    for t in ts:
+        if t is None:
+            continue
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what} is int32")
+        _need_cuda(t)
+        if size is not None and t.numel() != size:
+            raise ValueError(f"{what} has {size} elements, not {t.numel()}")
+
+
+class _At(NamedTuple):
+    """What _place looks at of a cache and a batch."""
+    device: object
+
+
+def _here(device, *ts, stream=None, workspace=None) -> None:
+    """Tensors, stream and workspace of ``device``, which has to be the current one."""
+    at = _At(device)
+    _paged._place(at, at, *ts, stream=stream, workspace=workspace)
+
+
+# ------------------------------------------------------------------- pages --
+class PageTables:
+    """Who has which page: int32 device tensors ``page_table`` [n_seq, entries],
+    ``held`` [n_seq] (entries in use), ``free_pages`` [n_pages] (the first
+    ``n_free[0]`` of them are free) and ``n_free`` [2] (free pages; entries that the
+    last plan lacked)."""
+
+    def __init__(self, page_table, held, free_pages, n_free, *, page_size: int):
+        if page_table.dim() != 2:
+            raise ValueError("page_table is [n_seq, entries]")
+        n_seq = page_table.shape[0]
+        _ints("page_table", page_table)
+        _ints("held", held, size=n_seq)
+        _ints("free_pages", free_pages)
+        _ints("n_free", n_free, size=2)
+        for t in (held, free_pages, n_free):
+            if t.device != page_table.device:
+                raise ValueError("the tables are on one device")
+        self.page_table, self.held, self.free_pages, self.n_free = page_table, held, free_pages, n_free
+        self.n_seq, self.entries, self.n_pages, self.page_size = n_seq, page_table.shape[1], free_pages.numel(), page_size
+        self.device = page_table.device
+
+    @classmethod
+    def empty(cls, n_pages: int, *, page_size: int, n_seq: int, entries: int, device=None) -> "PageTables":
+        """Tables of requests that hold nothing; page 0 is handed out first."""
+        torch = _torch()
+        device = device or torch.device("cuda")
+
+        def full(shape, x):
+            return torch.full(shape, x, dtype=torch.int32, device=device)
+
+        free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        n_free = full((2,), 0)
+        n_free[0] = n_pages
+        return cls(full((n_seq, entries), -1), full((n_seq,), 0), free, n_free, page_size=page_size)
+
+
+class StepPlan(NamedTuple):
+    """What a plan writes: ``cu`` [n_seq + 1] and ``ctx_lens`` [n_seq] (a
+    PagedBatch's), ``slots`` int64 [n_tokens] (page * page_size + slot, or -1) and
+    ``pos`` int32 [n_tokens]; the last two may be None."""
+    cu: object
+    ctx_lens: object
+    slots: object
+    pos: object
+
+    @classmethod
+    def empty(cls, tables: PageTables, *, n_tokens: int, rows: bool = True, stream=None) -> "StepPlan":
+        """Tensors for a plan to write; without ``rows`` slots and pos are left out."""
+        torch = _torch()
+
+        def new(n, dtype=torch.int32):
+            return _new_out((n,), dtype, tables.device, stream)
+
+        return cls(new(tables.n_seq + 1), new(tables.n_seq), new(n_tokens, torch.int64) if rows else None,
+                   new(n_tokens) if rows else None)
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_desc(*fields):
+    d = SpecPlanDesc(*fields)
+    return d, ctypes.byref(d)
+
+
+def spec_plan(tables: PageTables, lens, new_rows, *, n_tokens: Optional[int] = None, trim: bool = False,
+              out: Optional[StepPlan] = None, stream=None) -> StepPlan:
+    """The step's pages and row maps: requests with ``lens`` [n_seq] positions cached
+    and ``new_rows`` [n_seq] to come take from the free list the pages that they
+    lack, in order; with ``trim`` those beyond what a request needs go back first
+    (all of one with length 0 and no rows).  Pages that the list lacks are left out,
+    counted in ``tables.n_free[1]`` and asked for again by the next plan.
+    ``n_tokens`` is the rows of the maps (``out``'s where that is given)."""
+    torch = _torch()
+    if out is None:
+        if n_tokens is None:
+            raise ValueError("n_tokens or out must be given")
+        out = StepPlan.empty(tables, n_tokens=n_tokens, stream=stream)
+    else:
+        _ints("cu", out.cu, size=tables.n_seq + 1)
+        _ints("ctx_lens", out.ctx_lens, size=tables.n_seq)
+        _ints("pos", out.pos)
+        if out.slots is not None and out.slots.dtype != torch.int64:
+            raise TypeError("slots is int64")
+        _need_cuda(out.slots)
+        sizes = {t.numel() for t in (out.slots, out.pos) if t is not None}
+        if n_tokens is None:
+            n_tokens = next(iter(sizes), 1)
+        if sizes - {n_tokens}:
+            raise ValueError(f"slots and pos have {n_tokens} elements")
+    _ints("lens", lens, size=tables.n_seq)
+    _ints("new_rows", new_rows, size=tables.n_seq)
+    _here(tables.device, lens, new_rows, *out, stream=stream)
+    d = _plan_desc(tables.n_seq, n_tokens, tables.page_size, tables.entries, tables.n_pages, int(bool(trim)))[1]
+    _check("lmxs_plan", spec_lib().lmxs_plan(
+        d, lens.data_ptr(), new_rows.data_ptr(), tables.page_table.data_ptr(), tables.held.data_ptr(),
+        tables.free_pages.data_ptr(), tables.n_free.data_ptr(), out.cu.data_ptr(), out.ctx_lens.data_ptr(),
+        _ptr(out.slots), _ptr(out.pos), _stream(stream)))
+    return out
+
+
+# ------------------------------------------------------------------- trees --
+class SpecTree(NamedTuple):
+    """``pos`` int32 [n_tokens] and ``seen`` int64 [n_tokens, words]: bit j of row i's
+    words (64 rows a word, lowest first) says that it sees row j of its request."""
+    pos: object
+    seen: object
+
+
+def spec_tree(parent, batch: PagedBatch, *, window: int = 0, out: Optional[SpecTree] = None, stream=None) -> SpecTree:
+    """Positions and sight of the batch's rows from ``parent`` int32 [n_tokens], the
+    row of the request that each continues (earlier than its own; -1: a root).  With
+    ``window`` > 0 ancestors that far behind are not seen.  Rows of no request are
+    left as they are."""
+    torch = _torch()
+    _ints("parent", parent, size=batch.n_tokens)
+    words = -(-batch.max_new // 64)
+    if out is None:
+        out = SpecTree(_new_out((batch.n_tokens,), torch.int32, batch.device, stream),
+                       _new_out((batch.n_tokens, words), torch.int64, batch.device, stream))
+    else:
+        _ints("pos", out.pos, size=batch.n_tokens)
+        words = _words(out.seen, batch)
+    _here(batch.device, parent, *out, stream=stream)
+    _check("lmxs_tree", spec_lib().lmxs_tree(batch.ref, parent.data_ptr(), words, window, out.pos.data_ptr(),
+                                             out.seen.data_ptr(), _stream(stream)))
+    return out
+
+
+def _words(seen, batch: PagedBatch) -> int:
+    """Words a row of a mask."""
+    _need_cuda(seen)
+    if seen.dtype != _torch().int64 or seen.dim() != 2 or seen.shape[0] != batch.n_tokens:
+        raise ValueError(f"seen is int64 [{batch.n_tokens}, words]")
+    return seen.shape[1]
+
+
+# ---------------------------------------------------- prologue and attention --
+@functools.lru_cache(maxsize=256)
+def _rope_desc(interleaved: int, turn_scale: float):
+    d = SpecRope(interleaved, turn_scale)
+    return d, ctypes.byref(d)
+
+
+def rope_scaling(n_rot: int, *, kind: str, factor: float, rope_base: float = 1e6, trained_ctx: int = 0,
+                 fast: float = 32.0, slow: float = 1.0):
+    """(rope_factors [n_rot / 2] as a list, turn_scale) that stretch a rotation
+    trained on ``trained_ctx`` positions ``factor`` times, for ``spec_prologue``
+    (and, with turn_scale 1, ``paged_prologue``):
+
+    * ``linear``  every angle divided by ``factor``
+    * ``bands``   pairs that turn more than ``fast`` times in trained_ctx positions
+                  keep their angle, those below ``slow`` turns are divided, and in
+                  between 1 / divisor goes linearly in the turns
+    * ``yarn``    the same with the divisor's reciprocal linear in the pair's index
+                  between the two borders, and sine and cosine times
+                  0.1 ln(factor) + 1
+    """
+    if kind not in ("linear", "bands", "yarn"):
+        raise ValueError(f"unknown scaling {kind!r}")
+    if n_rot < 2 or n_rot % 2 or not factor > 0 or not rope_base > 1:
+        raise ValueError("n_rot is even, factor positive and rope_base above 1")
+    half = n_rot // 2
+    if kind == "linear":
+        return [float(factor)] * half, 1.0
+    if trained_ctx < 1 or not fast > slow > 0:
+        raise ValueError("trained_ctx is positive, and fast above slow above 0")
+
+    def pair(turns):  # index, as a real number, of the pair that turns so often
+        return half * math.log(trained_ctx / (2 * math.pi * turns)) / math.log(rope_base)
+
+    out = []
+    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), n_rot - 1)
+    for j in range(half):
+        if kind == "yarn":
+            keep = 1 - min(max((j - lo) / max(hi - lo, 0.001), 0.0), 1.0)
+        else:
+            turns = trained_ctx / (2 * math.pi) * rope_base ** (-j / half)
+            keep = min(max((turns - slow) / (fast - slow), 0.0), 1.0)
+        out.append(1 / (keep + (1 - keep) / factor))
+    return out, 0.1 * math.log(factor) + 1 if kind == "yarn" and factor > 1 else 1.0
+
+
+def spec_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: int, pos=None,
+                  n_rot: Optional[int] = None, interleaved: bool = False, turn_scale: float = 1.0,
+                  v_norm: bool = False, rms_eps: float = 1e-6, rope_base: float = 1e6, q_gain=None, k_gain=None,
+                  rope_factors=None, q_head_stride: Optional[int] = None, q_dtype=None, q_out=None, stream=None):
+    """``paged_prologue`` with the rows' positions ``pos`` int32 [n_tokens] apart from
+    their slots (None: the slots'), pairs of neighbouring dims where ``interleaved``
+    (else half a rotation apart), and sine and cosine times ``turn_scale``."""
+    torch = _torch()
+    hd = cache.head_dim
+    head = q_head_stride or hd
+    # the last head's columns behind its head_dim need not exist
+    width = q.shape[-1] if q.dim() == 2 else -1
+    if not (n_heads - 1) * head + hd <= width <= n_heads * head:
+        raise ValueError(f"q is [{batch.n_tokens}, {n_heads * head}], not {list(q.shape)}")
+    _rows(q, batch.n_tokens, width, "q")
+    if k is None or v is None:
+        raise ValueError("k and v must be given")
+    dt, kv_stride = _paged._kv_rows(k, v, cache, batch)
+    if dt != F32 or q.dtype != torch.float32:
+        raise TypeError("q, k and v are float32")
+    n_rot = hd if n_rot is None else n_rot
+    for g, n in ((q_gain, hd), (k_gain, hd), (rope_factors, n_rot // 2)):
+        if g is not None and (g.dtype != torch.float32 or g.numel() < n or not g.is_contiguous()):
+            raise ValueError("gains are contiguous float32 [head_dim], factors [n_rot / 2]")
+    _ints("pos", pos, size=batch.n_tokens)
+    if q_out is None:
+        q_out = _new_out((batch.n_tokens, n_heads * hd), q_dtype or torch.float32, cache.device, stream)
+    elif q_dtype is not None and q_out.dtype != q_dtype:
+        raise TypeError("q_dtype differs from q_out's")
+    if _rows(q_out, batch.n_tokens, n_heads * hd, "q_out"):
+        raise ValueError("q_out must be contiguous")
+    _paged._place(cache, batch, q, k, v, pos, q_gain, k_gain, rope_factors, q_out, stream=stream)
+    d = _paged._prologue_desc(n_heads, n_rot, int(bool(v_norm)), head, q.stride(0) if batch.n_tokens > 1 else 0,
+                              kv_stride, float(rms_eps), float(rope_base))[1]
+    r = _rope_desc(int(bool(interleaved)), float(turn_scale))[1]
+    _check("lmxs_prologue", spec_lib().lmxs_prologue(
+        cache.ref, batch.ref, d, r, _ptr(pos), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_gain), _ptr(k_gain),
+        _ptr(rope_factors), q_out.data_ptr(), _paged._dt_of(q_out.dtype), _stream(stream)))
+    return q_out
+
+
+def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: int, pos=None, window: int = 0,
+                   scale: Optional[float] = None, q_head_stride: Optional[int] = None, out=None,
+                   workspace: Optional[Workspace] = None, stream=None):
+    """``paged_attention`` of rows that see each other by a mask: each the positions
+    before its request's rows (with ``window`` > 0 those above its ``pos`` less the
+    window) and the request's rows whose bits are set in its ``seen`` int64
+    [n_tokens, words]; one that sees nothing gets zeros.  Types, precision and
+    workspaces are ``paged_attention``'s."""
+    hd = cache.head_dim
+    head = q_head_stride or hd
+    width = q.shape[-1] if q.dim() == 2 else -1
+    if not (n_heads - 1) * head + hd <= width <= n_heads * head:
+        raise ValueError(f"q is [{batch.n_tokens}, {n_heads * head}], not {list(q.shape)}")
+    _rows(q, batch.n_tokens, width, "q")
+    dt = _paged._dt_of(q.dtype)
+    words = _words(seen, batch)
+    _ints("pos", pos, size=batch.n_tokens)
+    if out is None:
+        out = _new_out((batch.n_tokens, n_heads * hd), q.dtype, cache.device, stream)
+    elif out.dtype != q.dtype or _rows(out, batch.n_tokens, n_heads * hd, "out"):
+        raise ValueError("out is contiguous and of q's dtype")
+    _paged._place(cache, batch, q, seen, pos, out, stream=stream, workspace=workspace)
+    d = _paged._attn_desc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
+                          1.0 / math.sqrt(hd) if scale is None else float(scale))[1]
+    L = spec_lib()
+    ws_ptr, ws_bytes = _space(_paged.paged_lib().lmxp_attn_workspace_bytes(cache.ref, batch.ref, d), workspace,
+                              cache.device, stream)
+    _check("lmxs_attn", L.lmxs_attn(cache.ref, batch.ref, d, seen.data_ptr(), words, _ptr(pos), q.data_ptr(), dt,
+                                    out.data_ptr(), _ptr_of(ws_ptr), ws_bytes, _stream(stream)))
+    return out
+
+
+def _space(need: int, workspace: Optional[Workspace], device, stream):
+    """(pointer or tensor held for this call, bytes) of ``need`` bytes of workspace;
+    nothing need be cleared."""
+    if not need:
+        return None, 0
+    if workspace is None:
+        return _new_out((need,), _torch().uint8, device, stream), need
+    if need > workspace.nbytes:
+        workspace.ensure(need, stream)
+    return workspace.base, workspace.nbytes
+
+
+def _ptr_of(x):
+    return x if x is None or isinstance(x, int) else x.data_ptr()
+
+
+# ------------------------------------------------------------ verification --
+class Verified(NamedTuple):
+    """``path`` int32 [n_seq, max_new] (accepted rows within the request, 0 first, then
+    -1), ``accepted`` int32 [n_seq] (their number) and ``token`` int32 [n_seq]."""
+    path: object
+    accepted: object
+    token: object
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_desc(*fields):
+    d = SpecVerifyDesc(*fields)
+    return d, ctypes.byref(d), spec_lib().lmxs_verify_workspace_bytes(ctypes.byref(d))
+
+
+def spec_verify(p, tokens, u, r, cu, *, max_new: int, parent=None, q=None, lens=None, greedy: bool = False,
+                out: Optional[Verified] = None, workspace: Optional[Workspace] = None, stream=None) -> Verified:
+    """Which drafted rows the target accepts, and the token behind them, distributed as
+    the target's own samples.  ``p`` [n_tokens, vocab] (f32 or f16) is the target's
+    distribution behind each row, ``tokens`` int32 [n_tokens] the rows' tokens, ``cu``
+    the step's row offsets; ``parent`` as ``spec_tree``'s (None: chains).  ``q``
+    [n_tokens, vocab] is what each row's children were drawn from; None: they were
+    chosen.  ``u`` f32 [n_tokens] decides each row's test, ``r`` f32 [n_seq] the last
+    token, both uniform in [0, 1).  With ``greedy`` a child passes if it is the
+    largest p's index (p may be logits; u, r and q are not read, u and r may be
+    None).  ``lens`` int32 [n_seq], where given, has the accepted rows added."""
+    torch = _torch()
+    dt = _paged._dt_of(p.dtype)
+    if p.dim() != 2:
+        raise ValueError("p is [n_tokens, vocab]")
+    n_tokens, vocab = p.shape
+    n_seq = cu.numel() - 1
+    p_stride, q_stride = _rows(p, n_tokens, vocab, "p"), 0
+    if q is not None:
+        if q.dtype != p.dtype:
+            raise TypeError("q is of p's dtype")
+        q_stride = _rows(q, n_tokens, vocab, "q")
+    _ints("cu", cu)
+    _ints("tokens", tokens, size=n_tokens)
+    _ints("parent", parent, size=n_tokens)
+    _ints("lens", lens, size=n_seq)
+    for t, n, what in ((u, n_tokens, "u"), (r, n_seq, "r")):
+        if t is None and greedy:
+            continue
+        if t is None or t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what} is contiguous float32 [{n}]")
+    if out is None:
+        out = Verified(_new_out((n_seq, max_new), torch.int32, p.device, stream),
+                       _new_out((n_seq,), torch.int32, p.device, stream),
+                       _new_out((n_seq,), torch.int32, p.device, stream))
+    else:
+        _ints("path", out.path, size=n_seq * max_new)
+        _ints("accepted", out.accepted, size=n_seq)
+        _ints("token", out.token, size=n_seq)
+    _here(p.device, p, tokens, u, r, cu, parent, q, lens, *out, stream=stream, workspace=workspace)
+    _, d, need = _verify_desc(n_seq, n_tokens, max_new, vocab, p_stride, q_stride, int(bool(greedy)))
+    ws_ptr, ws_bytes = _space(need, workspace, p.device, stream)
+    _check("lmxs_verify", spec_lib().lmxs_verify(
+        d, cu.data_ptr(), tokens.data_ptr(), _ptr(parent), p.data_ptr(), _ptr(q), dt, _ptr(u), _ptr(r),
+        out.path.data_ptr(), out.accepted.data_ptr(), out.token.data_ptr(), _ptr(lens), _ptr_of(ws_ptr), ws_bytes,
+        _stream(stream)))
+    return out
+
+
+def spec_keep(caches: Sequence[PagedCache], batch: PagedBatch, path, accepted, *, stream=None) -> None:
+    """Moves the accepted rows' K and V to the slots behind the cached positions, in
+    all ``caches`` (layers of one geometry) at once: row ``path[b][j]`` of request b to
+    where its row j is.  ``batch`` is the step's, ``path`` and ``accepted`` are
+    ``spec_verify``'s."""
+    if not caches:
+        raise ValueError("caches is empty")
+    _ints("path", path)
+    _ints("accepted", accepted, size=batch.n_seq)
+    if path.dim() != 2 or path.shape[0] != batch.n_seq:
+        raise ValueError(f"path is [{batch.n_seq}, entries]")
+    for c in caches:
+        _paged._place(c, batch, path, accepted, stream=stream)
+    pools = (PoolDesc * len(caches))(*[c.desc for c in caches])
+    _check("lmxs_keep", spec_lib().lmxs_keep(pools, len(caches), batch.ref, path.data_ptr(), path.shape[1],
+                                             accepted.data_ptr(), _stream(stream)))

@@ -14,6 +14,7 @@ use std::ffi::{c_char, c_void, CStr};
 use std::fmt;
 
 pub mod paged;
+pub mod spec;
 
 /// `lmx_stream`: binary-compatible with `hipStream_t`.
 pub type HipStream = *mut c_void;
