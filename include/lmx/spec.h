@@ -52,8 +52,8 @@ extern "C" {
  * A call that takes pages and one with the lengths before it that trims them
  * leave table and list as they were.
  *   lens, new_rows  device int32 [n_seq]
- *   page_table      int32 [n_seq, table_stride]; entries from held[b] on are
- *                   written where they are taken, and no other ones read
+ *   page_table      int32 [n_seq, table_stride]; what lies from held[b] on is not
+ *                   read, and written where the request needs it
  *   held            int32 [n_seq], updated
  *   free_pages      int32 [n_pages]; n_free[0] of them are free.  What lies
  *                   behind them is not read and stays.
@@ -149,7 +149,8 @@ lmx_status lmxs_attn(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_de
  *             equals, NaN none of them); so the token.  p may be logits; q, u
  *             and r are not read.  -1 where every p is NaN.
  *   cu        device int32 [n_seq + 1], as lmxp_batch's
- *   tokens    int32 [n_tokens]; one outside [0, vocab) never passes
+ *   tokens    int32 [n_tokens]; one outside [0, vocab) never passes and changes
+ *             nothing
  *   parent    int32 [n_tokens], or NULL: each row continues the one before it
  *   p, q      [n_tokens, vocab] of dt (LMX_F32 or LMX_F16), rows p_stride,
  *             q_stride elements apart; entries that are not above 0 and finite
@@ -187,12 +188,12 @@ lmx_status lmxs_verify(const lmxs_verify_desc *d, const int32_t *cu, const int32
  * path rises and path[b][j] >= j, as lmxs_verify writes it; an entry that does
  * not, and one that is no row of the request, is not moved, nor one from or to a
  * position in no page.
- *   pools     host array of n_pools pools (a layer each) of one geometry and
- *             store, whose pages the batch's table names
+ *   pools     host array of n_pools pointers to pools (a layer each) of one
+ *             geometry and store, whose pages the batch's table names
  *   b         the step's batch, its lengths with all of its rows
  *   path      int32 [n_seq, path_stride], path_stride at least max_new
  *   accepted  int32 [n_seq] */
-lmx_status lmxs_keep(const lmxp_pool *pools, uint32_t n_pools, const lmxp_batch *b,
+lmx_status lmxs_keep(const lmxp_pool *const *pools, uint32_t n_pools, const lmxp_batch *b,
                      const int32_t *path, uint32_t path_stride, const int32_t *accepted,
                      lmx_stream stream);
 

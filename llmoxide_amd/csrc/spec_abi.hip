@@ -23,7 +23,7 @@ bool spec_verify_fits(const lmxs_verify_desc* d);
 lmx_status spec_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32_t* tokens, const int32_t* parent,
                        const void* p, const void* q, lmx_dtype dt, const float* u, const float* r, int32_t* path,
                        int32_t* accepted, int32_t* token, int32_t* lens, void* ws, hipStream_t st);
-lmx_status spec_keep(const lmxp_pool* pools, uint32_t n_pools, const lmxp_batch* b, const int32_t* path,
+lmx_status spec_keep(const lmxp_pool* const* pools, uint32_t n_pools, const lmxp_batch* b, const int32_t* path,
                      uint32_t path_stride, const int32_t* accepted, hipStream_t st);
 
 // A call's arrays: one that is written may overlap none of the others.
@@ -174,24 +174,26 @@ lmx_status lmxs_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32
                        (hipStream_t)stream);
 }
 
-lmx_status lmxs_keep(const lmxp_pool* pools, uint32_t n_pools, const lmxp_batch* b, const int32_t* path,
+lmx_status lmxs_keep(const lmxp_pool* const* pools, uint32_t n_pools, const lmxp_batch* b, const int32_t* path,
                      uint32_t path_stride, const int32_t* accepted, lmx_stream stream) {
     if (!pools) return LMX_E_NULL;
     if (n_pools == 0 || n_pools > 65536) return LMX_E_SHAPE;
     for (uint32_t i = 0; i < n_pools; ++i) {
-        const lmx_status s = check_pool(pools + i);
+        const lmx_status s = check_pool(pools[i]);
         if (s != LMX_OK) return s;
-        if (pools[i].n_pages != pools->n_pages || pools[i].page_size != pools->page_size || pools[i].store != pools->store ||
-            pools[i].n_kv_heads != pools->n_kv_heads || pools[i].head_dim != pools->head_dim)
+        const lmxp_pool &x = *pools[i], &y = *pools[0];
+        if (x.n_pages != y.n_pages || x.page_size != y.page_size || x.store != y.store || x.n_kv_heads != y.n_kv_heads ||
+            x.head_dim != y.head_dim)
             return LMX_E_SHAPE;
     }
-    const lmx_status s = check_batch(pools, b);
+    const lmxp_pool* const p = pools[0];
+    const lmx_status s = check_batch(p, b);
     if (s != LMX_OK) return s;
     if (!path || !accepted) return LMX_E_NULL;
     if (b->max_new > LMXS_MAX_ROWS || path_stride < b->max_new || path_stride >= (1u << 30)) return LMX_E_SHAPE;
     if (!aligned(path, 4) || !aligned(accepted, 4)) return LMX_E_ALIGN;
     // pieces of 16 bytes of K and elements of V, 256 a workgroup, and 64 layers a launch at most
-    const uint64_t pieces = (uint64_t)pools->n_kv_heads * (pools->head_dim + pools->head_dim / 8 + 2);
+    const uint64_t pieces = (uint64_t)p->n_kv_heads * (p->head_dim + p->head_dim / 8 + 2);
     if ((uint64_t)b->n_seq * ((pieces + 255) / 256) * 64 >= (1u << 24)) return LMX_E_SHAPE;
     return spec_keep(pools, n_pools, b, path, path_stride, accepted, (hipStream_t)stream);
 }

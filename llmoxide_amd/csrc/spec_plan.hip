@@ -45,28 +45,42 @@ __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
     return r;
 }
 
-// Inclusive scan over the workgroup; `sums` (16 words of LDS) may be used again
-// afterwards.
-__device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
+// Inclusive scans over the workgroup of three counts that only its first `waves`
+// waves have; `sums` (48 words of LDS) may be used again afterwards.
+struct Three {
+    int x[3];
+};
+__device__ __forceinline__ Three block_scan(Three v, int waves, int* sums, Three& total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    x = wave_scan_sat(x);
-    if (lane == 63) sums[w] = x;
-    __syncthreads();
-    int before = 0;
-    total = 0;
+    if (w < waves) {
 #pragma unroll
-    for (int k = 0; k < kPlan / 64; ++k) {
-        if (k == w) before = total;
-        total = add_sat(total, sums[k]);
+        for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int y = __shfl_up(v.x[i], d, 64);
+                v.x[i] = lane >= d ? add_sat(v.x[i], y) : v.x[i];
+            }
+        if (lane == 63)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sums[3 * w + i] = v.x[i];
     }
     __syncthreads();
-    return add_sat(x, before);
-}
-// Of 1024 rising numbers, the last at or below i (the first one is).
-__device__ __forceinline__ int last_at(const int* start, int i) {
-    int at = 0;
+    Three before{{0, 0, 0}};
+    total = before;
+    for (int k = 0; k < waves; ++k) {
+        if (k == w) before = total;
 #pragma unroll
-    for (int step = kPlan / 2; step > 0; step >>= 1) at += start[at + step] <= i ? step : 0;
+        for (int i = 0; i < 3; ++i) total.x[i] = add_sat(total.x[i], sums[3 * k + i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v.x[i] = add_sat(v.x[i], before.x[i]);
+    return v;
+}
+// Of `n` rising numbers (n a power of two), the last at or below i (the first one is).
+__device__ __forceinline__ int last_at(const int* start, int n, int i) {
+    int at = 0;
+    for (int step = n >> 1; step > 0; step >>= 1) at += start[at + step] <= i ? step : 0;
     return at;
 }
 
@@ -84,75 +98,89 @@ __device__ __forceinline__ void map_none(const PlanArgs& a, int row) {
     if (a.pos) a.pos[row] = -1;
 }
 
+// Up to kPlan requests, a thread each, and the sums over them.
+enum { kBack, kWant, kRows };
+struct Chunk {
+    Request r;
+    int had, want, back;
+    Three upto, all;
+};
+__device__ __forceinline__ Chunk load_chunk(const PlanArgs& a, int c0, int waves, int* sums) {
+    Chunk c;
+    c.r = Request{0, 0, 0, 0, 0};
+    if (c0 + (int)threadIdx.x < a.n_seq) c.r = load_request(a, c0 + threadIdx.x);
+    c.back = a.trim ? imax(c.r.held - c.r.need, 0) : 0;
+    c.had = c.r.held - c.back;
+    c.want = imax(c.r.need - c.had, 0);
+    c.upto = block_scan(Three{{c.back, c.want, c.r.rows}}, waves, sums, c.all);
+    return c;
+}
+
 __global__ __launch_bounds__(kPlan) void spec_plan_kernel(PlanArgs a) {
-    __shared__ int sums[kPlan / 64];
+    __shared__ int sums[3 * kPlan / 64];
     __shared__ int start[kPlan], from[kPlan];        // of entries: a request's first, and its place in the table
     __shared__ int row_start[kPlan], row_len[kPlan];  // of rows
     const int tid = threadIdx.x;
     int top = imin(imax(a.n_free[0], 0), a.n_pages);  // free pages
+    const int waves = imin((a.n_seq + 63) / 64, kPlan / 64);
+    int size = 1;  // of `start` and `row_start`: places of requests, rounded up
+    while (size < a.n_seq && size < kPlan) size <<= 1;
 
+    Chunk c = load_chunk(a, 0, waves, sums);
     if (a.trim)
-        for (int hi = a.n_seq; hi > 0; hi -= kPlan) {  // the last requests first
-            const int b = hi - 1 - tid;
-            int n = 0, last = 0, total;
-            if (b >= 0) {
-                const Request r = load_request(a, b);
-                n = imax(r.held - r.need, 0);
-                last = r.held - 1;
-            }
-            const int upto = block_scan(n, sums, total);
+        for (int c0 = (a.n_seq - 1) / kPlan * kPlan; c0 >= 0; c0 -= kPlan) {  // the last requests first
+            if (a.n_seq > kPlan) c = load_chunk(a, c0, waves, sums);
+            const int total = c.all.x[kBack];
             if (total == 0) continue;  // uniform
-            start[tid] = upto - n;
-            from[tid] = last;
+            // place k of start: the request k from behind
+            if (tid < size) {
+                start[size - 1 - tid] = total - c.upto.x[kBack];
+                from[size - 1 - tid] = c.r.held - 1;
+            }
             __syncthreads();
             for (int i0 = 0; i0 < total; i0 += kPlan) {
                 const int i = i0 + tid;
-                int id = -1, back;
+                int id = -1;
                 if (i < total) {
-                    const int t = last_at(start, i);
-                    int32_t* at = a.table + (size_t)(hi - 1 - t) * a.stride + (from[t] - (i - start[t]));
+                    const int t = last_at(start, size, i);
+                    int32_t* at = a.table + (size_t)(c0 + size - 1 - t) * a.stride + (from[t] - (i - start[t]));
                     id = *at;
                     *at = -1;
                 }
                 const bool page = (uint32_t)id < (uint32_t)a.n_pages;
-                const int rank = block_scan(page, sums, back);
-                const int to = top + rank - 1;
+                Three back;
+                const Three rank = block_scan(Three{{page, 0, 0}}, kPlan / 64, sums, back);
+                const int to = top + rank.x[0] - 1;
                 if (page && to < a.n_pages) a.free_pages[to] = id;
-                top = imin(top + back, a.n_pages);
+                top = imin(top + back.x[0], a.n_pages);
             }
         }
     __syncthreads();
 
     int rows = 0, taken = 0;  // of the requests before
     for (int c0 = 0; c0 < a.n_seq; c0 += kPlan) {
-        const int b = c0 + tid;
-        Request r{0, 0, 0, 0, 0};
-        int had = 0, want = 0, all_rows, all_want;
+        if (c0) c = load_chunk(a, c0, waves, sums);  // (the first chunk is at hand)
+        const int b = c0 + tid, all_rows = c.all.x[kRows], all_want = c.all.x[kWant];
         if (b < a.n_seq) {
-            r = load_request(a, b);
-            had = a.trim ? imin(r.held, r.need) : r.held;
-            want = imax(r.need - had, 0);
+            a.cu[b + 1] = imin(add_sat(rows, c.upto.x[kRows]), a.n_tokens);
+            a.ctx[b] = c.r.total;
+            a.held[b] = c.had + imin(imax(top - add_sat(taken, c.upto.x[kWant] - c.want), 0), c.want);
         }
-        const int rows_upto = block_scan(r.rows, sums, all_rows);
-        const int want_upto = block_scan(want, sums, all_want);
-        if (b < a.n_seq) {
-            a.cu[b + 1] = imin(add_sat(rows, rows_upto), a.n_tokens);
-            a.ctx[b] = r.total;
-            a.held[b] = had + imin(imax(top - add_sat(taken, want_upto - want), 0), want);
+        if (tid < size) {
+            start[tid] = c.upto.x[kWant] - c.want;
+            from[tid] = c.had;
+            row_start[tid] = c.upto.x[kRows] - c.r.rows;
+            row_len[tid] = c.r.len;
         }
-        start[tid] = want_upto - want;
-        from[tid] = had;
-        row_start[tid] = rows_upto - r.rows;
-        row_len[tid] = r.len;
         __syncthreads();
         for (int i = tid; i < all_want; i += kPlan) {
-            const int t = last_at(start, i), at = top - 1 - add_sat(taken, i);
+            const int t = last_at(start, size, i), at = top - 1 - add_sat(taken, i);
             a.table[(size_t)(c0 + t) * a.stride + from[t] + (i - start[t])] = at >= 0 ? a.free_pages[at] : -1;
         }
         if (a.rows_here) {
             __syncthreads();
             for (int i = tid; i < all_rows && rows + i < a.n_tokens; i += kPlan) {
-                const int t = last_at(row_start, i);
+                const int t = last_at(row_start, size, i);
                 map_row(a, rows + i, c0 + t, row_len[t], i - row_start[t]);
             }
         }

@@ -1,13 +1,13 @@
 // Which drafted rows a target model accepts, and the token behind them.
 //
-// Two launches.  The walk: a workgroup a request, with all of its rows' p(c),
-// q(c) and u in LDS, so that accepting and refusing chosen drafts reads no
-// memory at all; only sums over the vocabulary that a second sibling asks for
+// The walk has all rows' p(c), q(c) and u in LDS, so that accepting and refusing
+// reads no memory; only sums over the vocabulary that a second sibling asks for
 // (drafts that were sampled), or the largest scores (greedy), are passes over a
-// row of p, by the whole workgroup.  The sample: the last row's distribution in
-// chunks of 4096 entries, a workgroup each; the one that finishes last adds the
-// chunks up, finds the one where the sum passes r times the whole, and goes
-// through it.
+// row of p, by one workgroup of the request.  Then the last row's distribution is
+// weighed, 256 entries a sum, by a workgroup for 4096 entries; and one wave adds
+// the sums up, finds the one where the running sum passes r times the whole, and
+// goes through its 256 entries.  Chosen drafts and chains need no passes: there
+// every workgroup that weighs walks by itself, which saves a launch.
 //
 // What is left of p after refusals needs one number: with w = p - a q wherever
 // that is above 0, and W its sum, the next refusal's w / W - q is, times W,
@@ -17,15 +17,17 @@
 // in the running sum, which is where a 32-bit sum's own rounding lies.  Each is
 // made in an order that the shapes alone decide.
 //
-// Bound by HBM in the sample (the last rows once: 4 or 8 bytes an entry), by
-// latency elsewhere.
+// Bound by latency: the last rows (4 or 8 bytes an entry) are 4 MB for 8 requests.
+#include <type_traits>
+
 #include "spec.hpp"
 
 namespace lmx {
 
-constexpr int kChunk = 4096;   // entries of the vocabulary a workgroup of the sample
+constexpr int kGroup = 256;            // entries of the vocabulary a sum
+constexpr int kGroups = 16;            // sums a workgroup makes, four a wave
 
-// What the walk leaves for the sample.
+// Where the walk ended.
 struct Last {
     int row;       // of the batch; -1: the request has none
     int at;        // of the request
@@ -35,7 +37,8 @@ struct Last {
 };
 
 struct VerifyArgs {
-    int n_seq, n_tokens, max_new, vocab, n_chunks;
+    int n_seq, n_tokens, max_new, vocab;
+    int n_groups, n_blocks;  // sums a request, workgroups that make them
     size_t p_stride, q_stride;
     const int32_t* cu;
     const int32_t* tokens;
@@ -48,9 +51,8 @@ struct VerifyArgs {
     int32_t* accepted;
     int32_t* token;
     int32_t* lens;
-    double* sums;   // [n_seq][n_chunks]
+    double* sums;   // [n_seq][n_groups]
     Last* last;     // [n_seq]
-    int* done;      // [n_seq] chunks whose sums are there
 };
 
 // A probability; what is not above 0 and finite is 0.
@@ -62,87 +64,203 @@ __device__ __forceinline__ int parent_of(const VerifyArgs& a, int row0, int i) {
     return p >= 0 && p < i ? p : -1;
 }
 
+// Four consecutive entries of a row, which need not be aligned to more than one.
+template <typename T>
+struct Four {
+    typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+template <typename T>
+__device__ __forceinline__ f32x4 four(const T* p) {
+    const typename Four<T>::type x = *reinterpret_cast<const typename Four<T>::type*>(p);
+    return f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+}
+// Entries t .. t+3 of a row of n, `none` behind its end.
+template <typename T>
+__device__ __forceinline__ f32x4 four_of(const T* p, int t, int n, float none) {
+    if (t + 4 <= n) return four(p + t);
+    f32x4 x = {none, none, none, none};
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (t + j < n) x[j] = (float)p[t + j];
+    return x;
+}
+
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
     return x;
 }
-// Sum over a workgroup of NT threads, in every thread.  ex: NT / 64 doubles.
-template <int NT>
-__device__ __forceinline__ double block_sum(double x, double* ex) {
-    x = wave_sum(x);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) ex[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double s = 0.0;
+// Sum of the lanes before this one.
+__device__ __forceinline__ double wave_before(double x) {
+    const int lane = __lane_id();
+    double y = x;
 #pragma unroll
-    for (int k = 0; k < NT / 64; ++k) s += ex[k];
-    return s;
+    for (int d = 1; d < 64; d <<= 1) {
+        const double z = __shfl_up(y, d, 64);
+        y += lane >= d ? z : 0.0;
+    }
+    const double z = __shfl_up(y, 1, 64);
+    return lane ? z : 0.0;
+}
+__device__ __forceinline__ double lane_value(double x, int lane) { return __shfl(x, lane, 64); }
+
+// CHAIN: sampled, each row the next one's parent.
+enum Drafts { CHOSEN, CHAIN, SAMPLED, GREEDY };
+
+// A request's rows in LDS.
+struct Rows {
+    int up[LMXS_MAX_ROWS], tok[LMXS_MAX_ROWS];  // parent (-1: none), token (-1: none, or no parent)
+    float p[LMXS_MAX_ROWS], q[LMXS_MAX_ROWS], u[LMXS_MAX_ROWS];
+};
+
+template <typename T, Drafts D, int NT>
+__device__ __forceinline__ void load_rows(const VerifyArgs& a, const SpecRows& s, Rows& r) {
+    const T* const p = static_cast<const T*>(a.p);
+    const T* const q = static_cast<const T*>(a.q);
+    for (int i = threadIdx.x; i < s.n; i += NT) {
+        const int above = parent_of(a, s.row0, i), t = a.tokens[s.row0 + i];
+        const bool on = above >= 0 && (uint32_t)t < (uint32_t)a.vocab;
+        r.up[i] = above;
+        r.tok[i] = on ? t : -1;
+        if (D != GREEDY && on) {
+            r.p[i] = (float)p[(size_t)(s.row0 + above) * a.p_stride + t];
+            if (D != CHOSEN) r.q[i] = (float)q[(size_t)(s.row0 + above) * a.q_stride + t];
+            r.u[i] = a.u[s.row0 + i];
+        }
+    }
+    __syncthreads();
 }
 
-enum Drafts { CHOSEN, SAMPLED, GREEDY };
+// The walk, by every wave for itself over the same LDS (so that passes' barriers
+// meet).  mass(row, c): sum of (p - c q)+; best_of(row): its largest entry's index.
+// path: where to note the accepted rows, or NULL.
+struct Walk {
+    int cur, count, children, best;
+    double a;
+};
+template <Drafts D, typename M, typename B>
+__device__ __forceinline__ Walk walk(const SpecRows& s, const Rows& r, int32_t* path, const M& mass, const B& best_of) {
+    const int lane = threadIdx.x & 63;
+    Walk w{0, s.n ? 1 : 0, 0, -1, 0.0};
+    double W = 1.0;
+    bool known = D != GREEDY;  // SAMPLED: W is that of w.a; GREEDY: best is cur's
+    for (int from = 1;;) {
+        int i = -1;
+        for (int c0 = from & ~63; c0 < s.n && i < 0; c0 += 64) {
+            const int k = c0 + lane;
+            const uint64_t hit = __ballot(k >= from && k < s.n && r.up[k < s.n ? k : 0] == w.cur);
+            if (hit) i = c0 + __builtin_ctzll(hit);
+        }
+        if (i < 0) break;
+        from = i + 1;
+        ++w.children;
+        const int t = r.tok[i];
+        bool pass = false;
+        if constexpr (D == GREEDY) {
+            if (!known) w.best = best_of(w.cur);
+            known = true;
+            pass = t >= 0 && t == w.best;
+        } else if (t >= 0) {
+            double x = prob(r.p[i]);
+            if constexpr (D != CHOSEN) {
+                if (!known) W = mass(w.cur, w.a);
+                known = true;
+                const double y = prob(r.q[i]);
+                x = fmax(x - w.a * y, 0.0);
+                pass = (double)r.u[i] * W * y < x;
+                if (!pass) {
+                    w.a += W;
+                    known = false;
+                }
+            } else {
+                bool twice = false;  // an earlier sibling was the same token
+                for (int c0 = (w.cur + 1) & ~63; c0 < i; c0 += 64) {
+                    const int k = c0 + lane;
+                    twice = twice || __ballot(k < i && k > w.cur && r.up[k < s.n ? k : 0] == w.cur && r.tok[k < s.n ? k : 0] == t);
+                }
+                if (twice) x = 0.0;
+                pass = (double)r.u[i] * W < x;
+                if (!pass) W -= x;
+            }
+        }
+        if (pass) {
+            if (path && threadIdx.x == 0) path[w.count] = i;
+            ++w.count;
+            w.cur = i;
+            w.children = 0;
+            w.a = 0.0;
+            W = 1.0;
+            known = D != GREEDY;
+        }
+    }
+    if (D == GREEDY && s.n && !known) w.best = best_of(w.cur);
+    return w;
+}
+// What the walk found, by the request's first workgroup.
+template <Drafts D, int NT>
+__device__ __forceinline__ void write_walk(const VerifyArgs& a, int b, const SpecRows& s, const Walk& w) {
+    int32_t* path = a.path + (size_t)b * a.max_new;
+    for (int j = w.count + threadIdx.x; j < a.max_new; j += NT) path[j] = -1;
+    if (threadIdx.x == 0) {
+        if (w.count) path[0] = 0;
+        a.accepted[b] = w.count;
+        if (a.lens) a.lens[b] += w.count;
+        if (D == GREEDY || !s.n) a.token[b] = w.best;
+        if (D != GREEDY) a.last[b] = Last{s.n ? s.row0 + w.cur : -1, w.cur, w.children, 0, w.a};
+    }
+}
 
+// ---- drafts that ask for passes over the vocabulary: a workgroup a request
 template <typename T, Drafts D>
-__global__ __launch_bounds__(D == CHOSEN ? 256 : 1024) void spec_walk_kernel(VerifyArgs a) {
-    constexpr int NT = D == CHOSEN ? 256 : 1024;
-    __shared__ int up[LMXS_MAX_ROWS], tok[LMXS_MAX_ROWS];
-    __shared__ float ps[LMXS_MAX_ROWS], qs[LMXS_MAX_ROWS], us[LMXS_MAX_ROWS];
+__global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
+    constexpr int NT = 1024, U = 4;  // fours a thread has on the way
+    __shared__ Rows rows;
     __shared__ double ex[NT / 64];
     __shared__ float ex_x[NT / 64];
     __shared__ int ex_t[NT / 64];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
-    const T* const p = static_cast<const T*>(a.p);
-    const T* const q = static_cast<const T*>(a.q);
-
-    for (int i = tid; i < s.n; i += NT) {
-        const int above = parent_of(a, s.row0, i), t = a.tokens[s.row0 + i];
-        const bool on = above >= 0 && (uint32_t)t < (uint32_t)a.vocab;
-        up[i] = above;
-        tok[i] = on ? t : -1;
-        if (D != GREEDY && on) {
-            ps[i] = (float)p[(size_t)(s.row0 + above) * a.p_stride + t];
-            if (D == SAMPLED) qs[i] = (float)q[(size_t)(s.row0 + above) * a.q_stride + t];
-            us[i] = a.u[s.row0 + i];
-        }
-    }
-    __syncthreads();
-
-    // Sum of (p - c q)+ over a row.
+    load_rows<T, D, NT>(a, s, rows);
     auto mass = [&](int row, double c) {
-        const T* pr = p + (size_t)(s.row0 + row) * a.p_stride;
-        const T* qr = q + (size_t)(s.row0 + row) * a.q_stride;
-        constexpr int U = 8;
+        const T* pr = static_cast<const T*>(a.p) + (size_t)(s.row0 + row) * a.p_stride;
+        const T* qr = static_cast<const T*>(a.q) + (size_t)(s.row0 + row) * a.q_stride;
         double sum = 0.0;
-        for (int t0 = tid; t0 < a.vocab; t0 += U * NT) {
-            float x[U], y[U];
+        for (int t0 = 4 * tid; t0 < a.vocab; t0 += 4 * U * NT) {
+            f32x4 x[U], y[U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const int t = t0 + k * NT < a.vocab ? t0 + k * NT : t0;
-                x[k] = t0 + k * NT < a.vocab ? (float)pr[t] : 0.f;
-                y[k] = (float)qr[t];
-            }
+            for (int k = 0; k < U; ++k) x[k] = four_of(pr, t0 + 4 * k * NT, a.vocab, 0.f);
 #pragma unroll
-            for (int k = 0; k < U; ++k) sum += fmax(prob(x[k]) - c * prob(y[k]), 0.0);
+            for (int k = 0; k < U; ++k) y[k] = four_of(qr, t0 + 4 * k * NT, a.vocab, 0.f);
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum += fmax(prob(x[k][j]) - c * prob(y[k][j]), 0.0);
         }
-        return block_sum<NT>(sum, ex);
+        sum = wave_sum(sum);
+        __syncthreads();
+        if (lane == 0) ex[tid >> 6] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < NT / 64; ++k) sum += ex[k];
+        return sum;
     };
-    // Index of a row's largest score, the lowest of equals; -1 where all are NaN.
+    // The largest score's index, the lowest of equals; -1 where all are NaN.
     auto best_of = [&](int row) {
-        const T* pr = p + (size_t)(s.row0 + row) * a.p_stride;
-        constexpr int U = 8;
+        const T* pr = static_cast<const T*>(a.p) + (size_t)(s.row0 + row) * a.p_stride;
         float top = -INFINITY;
         int at = 0x7fffffff;
         auto take = [&](float x, int t) {
             if (x > top || (x == top && t < at)) top = x, at = t;
         };
-        for (int t0 = tid; t0 < a.vocab; t0 += U * NT) {
-            float x[U];
+        for (int t0 = 4 * tid; t0 < a.vocab; t0 += 4 * U * NT) {
+            f32x4 x[U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) x[k] = (float)pr[t0 + k * NT < a.vocab ? t0 + k * NT : t0];
+            for (int k = 0; k < U; ++k) x[k] = four_of(pr, t0 + 4 * k * NT, a.vocab, __builtin_nanf(""));
 #pragma unroll
             for (int k = 0; k < U; ++k)
-                if (t0 + k * NT < a.vocab) take(x[k], t0 + k * NT);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) take(x[k][j], t0 + 4 * k * NT + j);
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) take(__shfl_xor(top, m, 64), __shfl_xor(at, m, 64));
@@ -153,284 +271,236 @@ __global__ __launch_bounds__(D == CHOSEN ? 256 : 1024) void spec_walk_kernel(Ver
         for (int k = 0; k < NT / 64; ++k) take(ex_x[k], ex_t[k]);
         return at == 0x7fffffff ? -1 : at;
     };
-
-    // Every wave walks by itself, over the same LDS: the passes' barriers meet.
-    int cur = 0, count = s.n ? 1 : 0, children = 0;
-    double c = 0.0, W = 1.0;
-    bool known = D != GREEDY;  // SAMPLED: W is that of c; GREEDY: best is cur's
-    int best = -1;
-    for (int from = 1;;) {
-        int i = -1;
-        for (int c0 = from & ~63; c0 < s.n && i < 0; c0 += 64) {
-            const int k = c0 + lane;
-            const uint64_t hit = __ballot(k >= from && k < s.n && up[k < s.n ? k : 0] == cur);
-            if (hit) i = c0 + __builtin_ctzll(hit);
-        }
-        if (i < 0) break;
-        from = i + 1;
-        ++children;
-        const int t = tok[i];
-        bool pass = false;
-        if constexpr (D == GREEDY) {
-            if (!known) best = best_of(cur);
-            known = true;
-            pass = t >= 0 && t == best;
-        } else if (t >= 0) {
-            double w = prob(ps[i]);
-            if constexpr (D == SAMPLED) {
-                if (!known) W = mass(cur, c);
-                known = true;
-                const double y = prob(qs[i]);
-                w = fmax(w - c * y, 0.0);
-                pass = (double)us[i] * W * y < w;
-                if (!pass) {
-                    c += W;
-                    known = false;
-                }
-            } else {
-                bool twice = false;  // an earlier sibling was the same token
-                for (int c0 = (cur + 1) & ~63; c0 < i; c0 += 64) {
-                    const int k = c0 + lane;
-                    twice = twice || __ballot(k < i && k > cur && up[k < s.n ? k : 0] == cur && tok[k < s.n ? k : 0] == t);
-                }
-                if (twice) w = 0.0;
-                pass = (double)us[i] * W < w;
-                if (!pass) W -= w;
-            }
-        }
-        if (pass) {
-            if (tid == 0) a.path[(size_t)b * a.max_new + count] = i;
-            ++count;
-            cur = i;
-            children = 0;
-            c = 0.0;
-            W = 1.0;
-            known = D != GREEDY;
-        }
-    }
-    if (D == GREEDY && s.n && !known) best = best_of(cur);
-    for (int j = count + tid; j < a.max_new; j += NT) a.path[(size_t)b * a.max_new + j] = -1;
-    if (tid == 0) {
-        if (count) a.path[(size_t)b * a.max_new] = 0;
-        a.accepted[b] = count;
-        if (a.lens) a.lens[b] += count;
-        if (D == GREEDY || !s.n) a.token[b] = best;
-        if (D != GREEDY) {
-            a.last[b] = Last{s.n ? s.row0 + cur : -1, cur, children, 0, c};
-            a.done[b] = 0;
-        }
-    }
+    const Walk w = walk<D>(s, rows, a.path + (size_t)b * a.max_new, mass, best_of);
+    write_walk<D, NT>(a, b, s, w);
 }
 
-// The weight of entry t: what is left of p behind the refused drafts.
+// ---- the last row's weights
+//
+// Weights behind the walk: (p - a q)+, or p, of which the tokens of refused children
+// are taken by their readers.
 template <typename T, bool Q>
 struct Weights {
     const T* p;
     const T* q;
     double a;
-    const uint32_t* gone;  // bits of the chunk's entries that chosen drafts took
-    __device__ __forceinline__ double at(int t, int in_chunk) const {
-        const double x = prob((float)p[t]);
-        if constexpr (Q) return fmax(x - a * prob((float)q[t]), 0.0);
-        return gone && (gone[in_chunk >> 5] >> (in_chunk & 31) & 1) ? 0.0 : x;
+    int vocab;
+    __device__ __forceinline__ void load(int t, f32x4& x, f32x4& y) const {
+        x = four_of(p, t, vocab, 0.f);
+        if (Q) y = four_of(q, t, vocab, 0.f);
+    }
+    __device__ __forceinline__ double of(float x, float y) const {
+        return Q ? fmax(prob(x) - a * prob(y), 0.0) : prob(x);
     }
 };
-
 template <typename T, bool Q>
-__global__ __launch_bounds__(256) void spec_sample_kernel(VerifyArgs a) {
-    constexpr int PER = kChunk / 256;
-    __shared__ double ex[4], ex_scan[4];
-    __shared__ uint32_t gone[kChunk / 32];
-    __shared__ int found, finishing;
-    const int b = blockIdx.x / a.n_chunks, mine = blockIdx.x % a.n_chunks, tid = threadIdx.x, lane = tid & 63;
+__device__ __forceinline__ Weights<T, Q> weights_of(const VerifyArgs& a, int row, double c) {
+    // (behind a leaf a is 0 and q says nothing: p is read in its place)
+    const T* const p = static_cast<const T*>(a.p) + (size_t)row * a.p_stride;
+    return Weights<T, Q>{p, Q && c != 0.0 ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride : p, c, a.vocab};
+}
+
+// WALK: the workgroup walks for itself (CHOSEN, CHAIN); else the walk is there.
+template <typename T, Drafts D>
+__global__ __launch_bounds__(256) void spec_weigh_kernel(VerifyArgs a) {
+    constexpr bool WALK = D == CHOSEN || D == CHAIN, Q = D != CHOSEN;
+    constexpr int W = kGroups / 4;  // sums a wave
+    __shared__ std::conditional_t<WALK, Rows, int> rows;
+    const int b = blockIdx.x / a.n_blocks, block = blockIdx.x % a.n_blocks;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Last l;
+    SpecRows s;
+    if constexpr (WALK) {
+        s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
+        load_rows<T, D, 256>(a, s, rows);
+        const Walk k = walk<D>(s, rows, block ? nullptr : a.path + (size_t)b * a.max_new,
+                               [](int, double) { return 0.0; }, [](int) { return -1; });
+        if (block == 0) write_walk<D, 256>(a, b, s, k);
+        l = Last{s.n ? s.row0 + k.cur : -1, k.cur, k.children, 0, k.a};
+    } else {
+        l = a.last[b];
+    }
+    if (l.row < 0) return;
+    const Weights<T, Q> wt = weights_of<T, Q>(a, l.row, l.a);
+    const int g0 = block * kGroups + w * W;
+    f32x4 x[W], y[W];
+#pragma unroll
+    for (int g = 0; g < W; ++g) wt.load((g0 + g) * kGroup + 4 * lane, x[g], y[g]);
+    if constexpr (D == CHOSEN) {
+        if (l.children)
+            for (int c0 = (l.at + 1) & ~63; c0 < s.n; c0 += 64) {
+                const int k = c0 + lane, j = k < s.n ? k : 0;
+                const bool mine = k > l.at && k < s.n && rows.up[j] == l.at;
+                const int t = mine ? rows.tok[j] : -1;
+                for (uint64_t left = __ballot(t >= g0 * kGroup && t < (g0 + W) * kGroup); left; left &= left - 1) {
+                    const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(left)) - g0 * kGroup;
+#pragma unroll
+                    for (int g = 0; g < W; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (at == g * kGroup + 4 * lane + e) x[g][e] = 0.f;
+                }
+            }
+    }
+    double sum[W];
+#pragma unroll
+    for (int g = 0; g < W; ++g) {
+        sum[g] = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[g] += wt.of(x[g][e], Q ? y[g][e] : 0.f);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1)
+#pragma unroll
+        for (int g = 0; g < W; ++g) sum[g] += __shfl_xor(sum[g], m, 64);
+    if (lane < W && g0 + lane < a.n_groups) {
+        double x0 = sum[0];
+#pragma unroll
+        for (int g = 1; g < W; ++g) x0 = lane == g ? sum[g] : x0;
+        a.sums[(size_t)b * a.n_groups + g0 + lane] = x0;
+    }
+}
+
+// The token: a wave a request.
+template <typename T, Drafts D>
+__global__ __launch_bounds__(64) void spec_find_kernel(VerifyArgs a) {
+    constexpr bool Q = D != CHOSEN;
+    const int b = blockIdx.x, lane = threadIdx.x;
     const Last l = a.last[b];
     if (l.row < 0) return;
-    const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
-    // (behind a leaf a is 0 and q says nothing: p is read in its place)
-    const T* const pr = static_cast<const T*>(a.p) + (size_t)l.row * a.p_stride;
-    Weights<T, Q> w{pr, Q && l.a != 0.0 ? static_cast<const T*>(a.q) + (size_t)l.row * a.q_stride : pr, l.a, nullptr};
-    const bool some_gone = !Q && l.children > 0;
+    const double* const sums = a.sums + (size_t)b * a.n_groups;
+    const double r = fmax((double)a.r[b], 0.0);
+    Weights<T, Q> wt = weights_of<T, Q>(a, l.row, l.a);
+    bool drop = D == CHOSEN && l.children > 0;
 
-    // The chunk's entries that refused drafts took.
-    auto mark = [&](int chunk) {
-        w.gone = some_gone ? gone : nullptr;
-        if (!some_gone) return;
-        __syncthreads();
-        if (tid < kChunk / 32) gone[tid] = 0;
-        __syncthreads();
-        for (int i = l.at + 1 + tid; i < s.n; i += 256) {
-            if (parent_of(a, s.row0, i) != l.at) continue;
-            const uint32_t t = (uint32_t)a.tokens[s.row0 + i] - (uint32_t)chunk * kChunk;
-            if (t < kChunk) atomicOr(&gone[t >> 5], 1u << (t & 31));
-        }
-        __syncthreads();
+    // Of 64 lanes' values, those of which `some` count: the first whose running sum
+    // passes the target, or else the last that counts, or else -1.
+    auto choose = [&](bool passes, bool some) {
+        const uint64_t p = __ballot(passes && some), s = __ballot(some);
+        return p ? (int)__builtin_ctzll(p) : s ? 63 - (int)__builtin_clzll(s) : -1;
     };
-    auto chunk_sum = [&](int chunk) {
-        const int t0 = chunk * kChunk, n = imin(kChunk, a.vocab - t0);
-        double x[PER], sum = 0.0;
+    // The entry of group g at which the running sum, `before` at its start, passes the target.
+    auto search = [&](int g, double before, double target) {
+        const int t0 = g * kGroup + 4 * lane;
+        f32x4 x, y = {};
+        wt.load(t0, x, y);
+        if (drop) {
+            const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
+            for (int c0 = l.at + 1; c0 < s.n; c0 += 64) {
+                const int k = c0 + lane;
+                const bool mine = k < s.n && parent_of(a, s.row0, k) == l.at;
+                const int t = mine ? a.tokens[s.row0 + k] : -1;
+                for (uint64_t left = __ballot(t >= g * kGroup && t < (g + 1) * kGroup); left; left &= left - 1) {
+                    const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(left));
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int i = tid + 256 * k;
-            x[k] = i < n ? w.at(t0 + i, i) : 0.0;
-        }
-#pragma unroll
-        for (int k = 0; k < PER; ++k) sum += x[k];
-        return block_sum<256>(sum, ex);
-    };
-    // Sum over the threads before this one, and of all.
-    auto scan = [&](double x, double& total) {
-        double y = x;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double z = __shfl_up(y, d, 64);
-            y += lane >= d ? z : 0.0;
-        }
-        __syncthreads();
-        if (lane == 63) ex_scan[tid >> 6] = y;
-        __syncthreads();
-        double before = 0.0;
-        total = 0.0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k == (tid >> 6)) before = total;
-            total += ex_scan[k];
-        }
-        return before + y - x;
-    };
-    // The least entry of the chunk whose sum, with `before`, passes the target; the
-    // last one with a weight where rounding keeps the sum below it; -1: no weight.
-    auto search = [&](int chunk, double before, double target) {
-        const int t0 = chunk * kChunk, n = imin(kChunk, a.vocab - t0);
-        double x[PER], sum = 0.0, total;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int i = tid * PER + k;
-            x[k] = i < n ? w.at(t0 + i, i) : 0.0;
-            sum += x[k];
-        }
-        double run = before + scan(sum, total);
-        int hit = 0x7fffffff, any = -1;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            run += x[k];
-            if (x[k] > 0.0) {
-                any = t0 + tid * PER + k;
-                if (run > target && hit == 0x7fffffff) hit = any;
+                    for (int e = 0; e < 4; ++e)
+                        if (at == t0 + e) x[e] = 0.f;
+                }
             }
         }
-        if (tid == 0) found = 0x7fffffff;
-        __syncthreads();
-        if (hit != 0x7fffffff) atomicMin(&found, hit);
-        __syncthreads();
-        const int first = found;
-        if (first != 0x7fffffff) return first;
-        __syncthreads();
-        if (tid == 0) found = -1;
-        __syncthreads();
-        if (any >= 0) atomicMax(&found, any);
-        __syncthreads();
-        return found;
+        double v[4], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[e] = wt.of(x[e], y[e]);
+        double run = before + wave_before(sum);
+        int hit = -1, any = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            run += v[e];
+            if (v[e] > 0.0) {
+                any = t0 + e;
+                if (run > target && hit < 0) hit = any;
+            }
+        }
+        const int at = choose(hit >= 0, any >= 0);
+        return at < 0 ? -1 : __builtin_amdgcn_readlane(hit >= 0 ? hit : any, at);
     };
 
-    mark(mine);
-    const double sum = chunk_sum(mine);
-    if (tid == 0) {
-        __hip_atomic_store(&a.sums[(size_t)b * a.n_chunks + mine], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        finishing = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.n_chunks - 1;
+    // ---- the sums: a run of them a lane
+    const int per = (a.n_groups + 63) / 64, first = lane * per;
+    constexpr int U = 8;
+    double part = 0.0;
+    for (int k0 = 0; k0 < per; k0 += U) {
+        double v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) v[k] = k0 + k < per && first + k0 + k < a.n_groups ? sums[first + k0 + k] : 0.0;
+#pragma unroll
+        for (int k = 0; k < U; ++k) part += v[k];
     }
-    __syncthreads();
-    if (!finishing) return;  // uniform
-    __threadfence();
-
-    // ---- the last workgroup of the request: every sum is there
-    const int per = (a.n_chunks + 255) / 256;
-    double part = 0.0, total;
-    auto chunk_at = [&](int c) {
-        return __hip_atomic_load(&a.sums[(size_t)b * a.n_chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    };
-    for (int k = 0; k < per; ++k)
-        if (tid * per + k < a.n_chunks) part += chunk_at(tid * per + k);
-    const double before = scan(part, total);
-    const double r = fmax((double)a.r[b], 0.0);
+    const double before = wave_before(part), total = lane_value(before + part, 63);
     int token = -1;
     if (total > 0.0) {
         const double target = r * total;
-        double run = before;
-        int hit = 0x7fffffff, any = -1;
-        for (int k = 0; k < per; ++k)
-            if (tid * per + k < a.n_chunks) {
-                const double x = chunk_at(tid * per + k);
-                run += x;
-                if (x > 0.0) {
-                    any = tid * per + k;
-                    if (run > target && hit == 0x7fffffff) hit = any;
-                }
-            }
-        if (tid == 0) found = 0x7fffffff;
-        __syncthreads();
-        if (hit != 0x7fffffff) atomicMin(&found, hit);
-        __syncthreads();
-        int chunk = found;
-        if (chunk == 0x7fffffff) {  // (r of 1, or rounding): the last chunk with a weight
-            __syncthreads();
-            if (tid == 0) found = -1;
-            __syncthreads();
-            if (any >= 0) atomicMax(&found, any);
-            __syncthreads();
-            chunk = found;
-        }
-        // the sum of the chunks before it
-        double x = 0.0;
-        for (int k = 0; k < per; ++k)
-            if (tid * per + k < chunk) x += chunk_at(tid * per + k);
-        const double below = block_sum<256>(x, ex);
-        mark(chunk);
-        token = search(chunk, below, target);
-    } else {
-        // Nothing is left (the drafts had all of p): from p itself, by this
-        // workgroup alone, twice through the row.
-        w.a = 0.0;
-        w.gone = nullptr;
-        double all = 0.0;
-        for (int c = 0; c < a.n_chunks; ++c) all += chunk_sum(c);
-        const double target = r * all;
-        double run = 0.0;
-        for (int c = 0; c < a.n_chunks; ++c) {
-            const double x = chunk_sum(c);
+        const int at = choose(before + part > target, part > 0.0);
+        // that lane's run, by all lanes alike
+        const int g1 = at * per;
+        double run = lane_value(before, at), below = run;
+        int group = -1;
+        for (int k = 0; k < per && g1 + k < a.n_groups; ++k) {
+            const double x = sums[g1 + k];
             if (x > 0.0) {
-                const int t = search(c, run, target);
-                if (t >= 0) token = t;
+                group = g1 + k;
+                below = run;
                 if (run + x > target) break;  // uniform
             }
             run += x;
         }
+        token = search(group, below, target);
+    } else {
+        // Nothing is left (the drafts had all of p): from p itself, twice through the row.
+        wt.a = 0.0;
+        drop = false;
+        double all = 0.0;
+        for (int g = 0; g < a.n_groups; ++g) {
+            f32x4 x, y = {};
+            wt.load(g * kGroup + 4 * lane, x, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) all += prob(x[e]);
+        }
+        all = wave_sum(all);
+        const double target = r * all;
+        double run = 0.0;
+        for (int g = 0; all > 0.0 && g < a.n_groups; ++g) {
+            f32x4 x, y = {};
+            wt.load(g * kGroup + 4 * lane, x, y);
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += prob(x[e]);
+            sum = wave_sum(sum);
+            if (sum > 0.0) token = search(g, run, target);
+            if (run + sum > target) break;  // uniform
+            run += sum;
+        }
     }
-    if (tid == 0) a.token[b] = token;
+    if (lane == 0) a.token[b] = token;
 }
 
 // ------------------------------------------------------------------- host --
 static size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
-static int chunks_of(const lmxs_verify_desc* d) { return (int)((d->vocab + kChunk - 1) / kChunk); }
+static int groups_of(const lmxs_verify_desc* d) { return (int)((d->vocab + kGroup - 1) / kGroup); }
+static int blocks_of(const lmxs_verify_desc* d) { return (groups_of(d) + kGroups - 1) / kGroups; }
 size_t spec_verify_workspace(const lmxs_verify_desc* d) {
     if (d->greedy) return 0;
-    return align16((size_t)d->n_seq * chunks_of(d) * sizeof(double)) + d->n_seq * sizeof(Last) +
-           align16((size_t)d->n_seq * sizeof(int));
+    return align16((size_t)d->n_seq * groups_of(d) * sizeof(double)) + align16(d->n_seq * sizeof(Last));
 }
 // A launch names its workgroups' threads in 32 bits.
-bool spec_verify_fits(const lmxs_verify_desc* d) { return (uint64_t)d->n_seq * chunks_of(d) < (1u << 24); }
+bool spec_verify_fits(const lmxs_verify_desc* d) { return (uint64_t)d->n_seq * blocks_of(d) < (1u << 24); }
 
-template <typename T>
-static void launch(const VerifyArgs& a, bool greedy, hipStream_t st) {
-    const dim3 seqs((unsigned)a.n_seq), chunks((unsigned)(a.n_seq * a.n_chunks));
-    if (greedy) {
-        hipLaunchKernelGGL((spec_walk_kernel<T, GREEDY>), seqs, dim3(1024), 0, st, a);
-    } else if (a.q) {
-        hipLaunchKernelGGL((spec_walk_kernel<T, SAMPLED>), seqs, dim3(1024), 0, st, a);
-        hipLaunchKernelGGL((spec_sample_kernel<T, true>), chunks, dim3(256), 0, st, a);
-    } else {
-        hipLaunchKernelGGL((spec_walk_kernel<T, CHOSEN>), seqs, dim3(256), 0, st, a);
-        hipLaunchKernelGGL((spec_sample_kernel<T, false>), chunks, dim3(256), 0, st, a);
+template <typename T, Drafts D>
+static void launch(const VerifyArgs& a, hipStream_t st) {
+    const dim3 seqs((unsigned)a.n_seq), blocks((unsigned)(a.n_seq * a.n_blocks));
+    if constexpr (D == SAMPLED || D == GREEDY)
+        hipLaunchKernelGGL((spec_walk_kernel<T, D>), seqs, dim3(1024), 0, st, a);
+    if constexpr (D != GREEDY) {
+        hipLaunchKernelGGL((spec_weigh_kernel<T, D>), blocks, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((spec_find_kernel<T, D>), seqs, dim3(64), 0, st, a);
     }
+}
+template <typename T>
+static void launch_by(const VerifyArgs& a, bool greedy, hipStream_t st) {
+    if (greedy) launch<T, GREEDY>(a, st);
+    else if (!a.q) launch<T, CHOSEN>(a, st);
+    else if (!a.parent) launch<T, CHAIN>(a, st);  // one child a row: no second sibling asks for a sum
+    else launch<T, SAMPLED>(a, st);
 }
 
 lmx_status spec_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32_t* tokens, const int32_t* parent,
@@ -441,7 +511,8 @@ lmx_status spec_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32
     a.n_tokens = (int)d->n_tokens;
     a.max_new = (int)d->max_new;
     a.vocab = (int)d->vocab;
-    a.n_chunks = chunks_of(d);
+    a.n_groups = groups_of(d);
+    a.n_blocks = blocks_of(d);
     a.p_stride = d->p_stride ? d->p_stride : d->vocab;
     a.q_stride = d->q_stride ? d->q_stride : d->vocab;
     a.cu = cu;
@@ -455,14 +526,11 @@ lmx_status spec_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32
     a.accepted = accepted;
     a.token = token;
     a.lens = lens;
-    char* at = static_cast<char*>(ws);
-    a.sums = reinterpret_cast<double*>(at);
-    at += align16((size_t)d->n_seq * a.n_chunks * sizeof(double));
-    a.last = reinterpret_cast<Last*>(at);
-    a.done = reinterpret_cast<int*>(at + d->n_seq * sizeof(Last));
+    a.sums = static_cast<double*>(ws);
+    a.last = reinterpret_cast<Last*>(static_cast<char*>(ws) + align16((size_t)d->n_seq * a.n_groups * sizeof(double)));
     (void)hipGetLastError();
-    if (dt == LMX_F32) launch<float>(a, d->greedy != 0, st);
-    else launch<f16>(a, d->greedy != 0, st);
+    if (dt == LMX_F32) launch_by<float>(a, d->greedy != 0, st);
+    else launch_by<f16>(a, d->greedy != 0, st);
     LMX_CHECK_LAUNCH();
     return LMX_OK;
 }

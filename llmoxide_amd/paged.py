@@ -126,6 +126,7 @@ class PagedCache:
         self.desc = PoolDesc(self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, store,
                              _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale))
         self.ref = ctypes.byref(self.desc)
+        self.at, self.address = k.get_device(), ctypes.addressof(self.desc)
 
     @classmethod
     def empty(cls, n_pages: int, *, page_size: int, n_kv_heads: int, head_dim: int, dtype=None,

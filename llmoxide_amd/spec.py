@@ -75,7 +75,7 @@ SIGNATURES = {
     "lmxs_attn": (_I, [_PP, _PB, _PA, _VP, _U32, _VP, _VP, _I, _VP, _VP, _SZ, _VP]),
     "lmxs_verify_workspace_bytes": (_SZ, [_PV]),
     "lmxs_verify": (_I, [_PV] + [_VP] * 5 + [_I] + [_VP] * 7 + [_SZ, _VP]),
-    "lmxs_keep": (_I, [_PP, _U32, _PB, _VP, _U32, _VP, _VP]),
+    "lmxs_keep": (_I, [ctypes.POINTER(_VP), _U32, _PB, _VP, _U32, _VP, _VP]),
 }
 
 _lib = None
@@ -93,17 +93,22 @@ def spec_lib() -> ctypes.CDLL:
     return _lib
 
 
-def _ints(what: str, *ts, size=None) -> None:
-    """int32 tensors, contiguous and on the GPU, of ``size`` elements each."""
-    torch = _torch()
-    for t in ts:
-        if t is None:
-            continue
-        if t.dtype != torch.int32:
-            raise TypeError(f"{what} is int32")
-        _need_cuda(t)
-        if size is not None and t.numel() != size:
-            raise ValueError(f"{what} has {size} elements, not {t.numel()}")
+_i32 = None
+
+
+def _ints(what: str, t, size, at: int) -> None:
+    """``t``: int32, contiguous, on device ``at``, of ``size`` elements (None: any)."""
+    global _i32
+    if _i32 is None:
+        _i32 = _torch().int32
+    if t.dtype != _i32:
+        raise TypeError(f"{what} is int32")
+    if t.get_device() != at or at < 0:
+        raise ValueError(f"{what} must be on the GPU, on the device of the call's other tensors")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    if size is not None and t.numel() != size:
+        raise ValueError(f"{what} has {size} elements, not {t.numel()}")
 
 
 class _At(NamedTuple):
@@ -117,6 +122,20 @@ def _here(device, *ts, stream=None, workspace=None) -> None:
     _paged._place(at, at, *ts, stream=stream, workspace=workspace)
 
 
+class _Held:
+    """Tensors that a call writes, checked when they are put together; the calls read
+    their addresses from ``ptrs``.  Unpacks to the tensors."""
+    __slots__ = ("ts", "ptrs", "device", "at")
+
+    def __init__(self, *ts):
+        first = next(t for t in ts if t is not None)
+        self.ts, self.ptrs = ts, tuple(_ptr(t) for t in ts)
+        self.device, self.at = first.device, first.get_device()
+
+    def __iter__(self):
+        return iter(self.ts)
+
+
 # ------------------------------------------------------------------- pages --
 class PageTables:
     """Who has which page: int32 device tensors ``page_table`` [n_seq, entries],
@@ -127,17 +146,15 @@ class PageTables:
     def __init__(self, page_table, held, free_pages, n_free, *, page_size: int):
         if page_table.dim() != 2:
             raise ValueError("page_table is [n_seq, entries]")
-        n_seq = page_table.shape[0]
-        _ints("page_table", page_table)
-        _ints("held", held, size=n_seq)
-        _ints("free_pages", free_pages)
-        _ints("n_free", n_free, size=2)
-        for t in (held, free_pages, n_free):
-            if t.device != page_table.device:
-                raise ValueError("the tables are on one device")
+        n_seq, at = page_table.shape[0], page_table.get_device()
+        _ints("page_table", page_table, None, at)
+        _ints("held", held, n_seq, at)
+        _ints("free_pages", free_pages, None, at)
+        _ints("n_free", n_free, 2, at)
         self.page_table, self.held, self.free_pages, self.n_free = page_table, held, free_pages, n_free
         self.n_seq, self.entries, self.n_pages, self.page_size = n_seq, page_table.shape[1], free_pages.numel(), page_size
-        self.device = page_table.device
+        self.device, self.at = page_table.device, at
+        self.ptrs = tuple(t.data_ptr() for t in (page_table, held, free_pages, n_free))
 
     @classmethod
     def empty(cls, n_pages: int, *, page_size: int, n_seq: int, entries: int, device=None) -> "PageTables":
@@ -154,14 +171,26 @@ class PageTables:
         return cls(full((n_seq, entries), -1), full((n_seq,), 0), free, n_free, page_size=page_size)
 
 
-class StepPlan(NamedTuple):
-    """What a plan writes: ``cu`` [n_seq + 1] and ``ctx_lens`` [n_seq] (a
+class StepPlan(_Held):
+    """What a plan writes: int32 ``cu`` [n_seq + 1] and ``ctx_lens`` [n_seq] (a
     PagedBatch's), ``slots`` int64 [n_tokens] (page * page_size + slot, or -1) and
-    ``pos`` int32 [n_tokens]; the last two may be None."""
-    cu: object
-    ctx_lens: object
-    slots: object
-    pos: object
+    ``pos`` int32 [n_tokens]; each of the last two may be None."""
+    __slots__ = ("n_seq", "n_tokens")
+
+    def __init__(self, cu, ctx_lens, slots=None, pos=None):
+        super().__init__(cu, ctx_lens, slots, pos)
+        self.n_seq = ctx_lens.numel()
+        _ints("ctx_lens", ctx_lens, None, self.at)
+        _ints("cu", cu, self.n_seq + 1, self.at)
+        self.n_tokens = next((t.numel() for t in (slots, pos) if t is not None), None)
+        if pos is not None:
+            _ints("pos", pos, self.n_tokens, self.at)
+        if slots is not None:
+            _need_cuda(slots)
+            if slots.dtype != _torch().int64 or slots.get_device() != self.at:
+                raise TypeError("slots is int64, on the device of cu")
+
+    cu, ctx_lens, slots, pos = (property(lambda self, i=i: self.ts[i]) for i in range(4))
 
     @classmethod
     def empty(cls, tables: PageTables, *, n_tokens: int, rows: bool = True, stream=None) -> "StepPlan":
@@ -188,41 +217,39 @@ def spec_plan(tables: PageTables, lens, new_rows, *, n_tokens: Optional[int] = N
     lack, in order; with ``trim`` those beyond what a request needs go back first
     (all of one with length 0 and no rows).  Pages that the list lacks are left out,
     counted in ``tables.n_free[1]`` and asked for again by the next plan.
-    ``n_tokens`` is the rows of the maps (``out``'s where that is given)."""
-    torch = _torch()
+    ``n_tokens`` is the rows of the batch (``out``'s maps have as many)."""
+    if n_tokens is None:
+        n_tokens = out and out.n_tokens
+        if n_tokens is None:
+            raise ValueError("n_tokens, or an out with maps, must be given")
     if out is None:
-        if n_tokens is None:
-            raise ValueError("n_tokens or out must be given")
         out = StepPlan.empty(tables, n_tokens=n_tokens, stream=stream)
-    else:
-        _ints("cu", out.cu, size=tables.n_seq + 1)
-        _ints("ctx_lens", out.ctx_lens, size=tables.n_seq)
-        _ints("pos", out.pos)
-        if out.slots is not None and out.slots.dtype != torch.int64:
-            raise TypeError("slots is int64")
-        _need_cuda(out.slots)
-        sizes = {t.numel() for t in (out.slots, out.pos) if t is not None}
-        if n_tokens is None:
-            n_tokens = next(iter(sizes), 1)
-        if sizes - {n_tokens}:
-            raise ValueError(f"slots and pos have {n_tokens} elements")
-    _ints("lens", lens, size=tables.n_seq)
-    _ints("new_rows", new_rows, size=tables.n_seq)
-    _here(tables.device, lens, new_rows, *out, stream=stream)
-    d = _plan_desc(tables.n_seq, n_tokens, tables.page_size, tables.entries, tables.n_pages, int(bool(trim)))[1]
-    _check("lmxs_plan", spec_lib().lmxs_plan(
-        d, lens.data_ptr(), new_rows.data_ptr(), tables.page_table.data_ptr(), tables.held.data_ptr(),
-        tables.free_pages.data_ptr(), tables.n_free.data_ptr(), out.cu.data_ptr(), out.ctx_lens.data_ptr(),
-        _ptr(out.slots), _ptr(out.pos), _stream(stream)))
+    elif out.n_seq != tables.n_seq or out.n_tokens not in (None, n_tokens):
+        raise ValueError("out is of other requests or rows")
+    at = tables.at
+    _ints("lens", lens, tables.n_seq, at)
+    _ints("new_rows", new_rows, tables.n_seq, at)
+    _here(tables.device, out.cu, stream=stream)
+    d = _plan_desc(tables.n_seq, n_tokens, tables.page_size, tables.entries, tables.n_pages, 1 if trim else 0)[1]
+    _check("lmxs_plan", spec_lib().lmxs_plan(d, lens.data_ptr(), new_rows.data_ptr(), *tables.ptrs, *out.ptrs,
+                                             _stream(stream)))
     return out
 
 
 # ------------------------------------------------------------------- trees --
-class SpecTree(NamedTuple):
+class SpecTree(_Held):
     """``pos`` int32 [n_tokens] and ``seen`` int64 [n_tokens, words]: bit j of row i's
     words (64 rows a word, lowest first) says that it sees row j of its request."""
-    pos: object
-    seen: object
+    __slots__ = ("words",)
+
+    def __init__(self, pos, seen):
+        super().__init__(pos, seen)
+        self.words = _words(seen, pos.numel())
+        _ints("pos", pos, None, self.at)
+        if seen.get_device() != self.at:
+            raise ValueError("pos and seen are on one device")
+
+    pos, seen = (property(lambda self, i=i: self.ts[i]) for i in range(2))
 
 
 def spec_tree(parent, batch: PagedBatch, *, window: int = 0, out: Optional[SpecTree] = None, stream=None) -> SpecTree:
@@ -230,26 +257,25 @@ def spec_tree(parent, batch: PagedBatch, *, window: int = 0, out: Optional[SpecT
     row of the request that each continues (earlier than its own; -1: a root).  With
     ``window`` > 0 ancestors that far behind are not seen.  Rows of no request are
     left as they are."""
-    torch = _torch()
-    _ints("parent", parent, size=batch.n_tokens)
-    words = -(-batch.max_new // 64)
+    n_tokens = batch.n_tokens
     if out is None:
-        out = SpecTree(_new_out((batch.n_tokens,), torch.int32, batch.device, stream),
-                       _new_out((batch.n_tokens, words), torch.int64, batch.device, stream))
-    else:
-        _ints("pos", out.pos, size=batch.n_tokens)
-        words = _words(out.seen, batch)
-    _here(batch.device, parent, *out, stream=stream)
-    _check("lmxs_tree", spec_lib().lmxs_tree(batch.ref, parent.data_ptr(), words, window, out.pos.data_ptr(),
-                                             out.seen.data_ptr(), _stream(stream)))
+        torch = _torch()
+        out = SpecTree(_new_out((n_tokens,), torch.int32, batch.device, stream),
+                       _new_out((n_tokens, -(-batch.max_new // 64)), torch.int64, batch.device, stream))
+    elif out.pos.numel() != n_tokens:
+        raise ValueError("out is of other rows")
+    _ints("parent", parent, n_tokens, out.at)
+    _here(batch.device, parent, stream=stream)
+    pos, seen = out.ptrs
+    _check("lmxs_tree", spec_lib().lmxs_tree(batch.ref, parent.data_ptr(), out.words, window, pos, seen, _stream(stream)))
     return out
 
 
-def _words(seen, batch: PagedBatch) -> int:
+def _words(seen, n_tokens: int) -> int:
     """Words a row of a mask."""
     _need_cuda(seen)
-    if seen.dtype != _torch().int64 or seen.dim() != 2 or seen.shape[0] != batch.n_tokens:
-        raise ValueError(f"seen is int64 [{batch.n_tokens}, words]")
+    if seen.dtype != _torch().int64 or seen.dim() != 2 or seen.shape[0] != n_tokens:
+        raise ValueError(f"seen is int64 [{n_tokens}, words]")
     return seen.shape[1]
 
 
@@ -323,14 +349,15 @@ def spec_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: int
     for g, n in ((q_gain, hd), (k_gain, hd), (rope_factors, n_rot // 2)):
         if g is not None and (g.dtype != torch.float32 or g.numel() < n or not g.is_contiguous()):
             raise ValueError("gains are contiguous float32 [head_dim], factors [n_rot / 2]")
-    _ints("pos", pos, size=batch.n_tokens)
+    if pos is not None:
+        _ints("pos", pos, batch.n_tokens, cache.at)
     if q_out is None:
         q_out = _new_out((batch.n_tokens, n_heads * hd), q_dtype or torch.float32, cache.device, stream)
     elif q_dtype is not None and q_out.dtype != q_dtype:
         raise TypeError("q_dtype differs from q_out's")
     if _rows(q_out, batch.n_tokens, n_heads * hd, "q_out"):
         raise ValueError("q_out must be contiguous")
-    _paged._place(cache, batch, q, k, v, pos, q_gain, k_gain, rope_factors, q_out, stream=stream)
+    _paged._place(cache, batch, q, k, v, q_gain, k_gain, rope_factors, q_out, stream=stream)
     d = _paged._prologue_desc(n_heads, n_rot, int(bool(v_norm)), head, q.stride(0) if batch.n_tokens > 1 else 0,
                               kv_stride, float(rms_eps), float(rope_base))[1]
     r = _rope_desc(int(bool(interleaved)), float(turn_scale))[1]
@@ -355,13 +382,14 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
         raise ValueError(f"q is [{batch.n_tokens}, {n_heads * head}], not {list(q.shape)}")
     _rows(q, batch.n_tokens, width, "q")
     dt = _paged._dt_of(q.dtype)
-    words = _words(seen, batch)
-    _ints("pos", pos, size=batch.n_tokens)
+    words = _words(seen, batch.n_tokens)
+    if pos is not None:
+        _ints("pos", pos, batch.n_tokens, cache.at)
     if out is None:
         out = _new_out((batch.n_tokens, n_heads * hd), q.dtype, cache.device, stream)
     elif out.dtype != q.dtype or _rows(out, batch.n_tokens, n_heads * hd, "out"):
         raise ValueError("out is contiguous and of q's dtype")
-    _paged._place(cache, batch, q, seen, pos, out, stream=stream, workspace=workspace)
+    _paged._place(cache, batch, q, seen, out, stream=stream, workspace=workspace)
     d = _paged._attn_desc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
                           1.0 / math.sqrt(hd) if scale is None else float(scale))[1]
     L = spec_lib()
@@ -389,12 +417,26 @@ def _ptr_of(x):
 
 
 # ------------------------------------------------------------ verification --
-class Verified(NamedTuple):
-    """``path`` int32 [n_seq, max_new] (accepted rows within the request, 0 first, then
-    -1), ``accepted`` int32 [n_seq] (their number) and ``token`` int32 [n_seq]."""
-    path: object
-    accepted: object
-    token: object
+class Verified(_Held):
+    """int32 ``path`` [n_seq, max_new] (accepted rows within the request, 0 first, then
+    -1), ``accepted`` [n_seq] (their number) and ``token`` [n_seq]."""
+    __slots__ = ()
+
+    def __init__(self, path, accepted, token):
+        super().__init__(path, accepted, token)
+        if path.dim() != 2:
+            raise ValueError("path is [n_seq, max_new]")
+        _ints("path", path, None, self.at)
+        _ints("accepted", accepted, path.shape[0], self.at)
+        _ints("token", token, path.shape[0], self.at)
+
+    path, accepted, token = (property(lambda self, i=i: self.ts[i]) for i in range(3))
+
+    @classmethod
+    def empty(cls, n_seq: int, max_new: int, device, stream=None) -> "Verified":
+        """Tensors for a verification to write."""
+        i32 = _torch().int32
+        return cls(*(_new_out(shape, i32, device, stream) for shape in ((n_seq, max_new), (n_seq,), (n_seq,))))
 
 
 @functools.lru_cache(maxsize=256)
@@ -425,30 +467,27 @@ def spec_verify(p, tokens, u, r, cu, *, max_new: int, parent=None, q=None, lens=
         if q.dtype != p.dtype:
             raise TypeError("q is of p's dtype")
         q_stride = _rows(q, n_tokens, vocab, "q")
-    _ints("cu", cu)
-    _ints("tokens", tokens, size=n_tokens)
-    _ints("parent", parent, size=n_tokens)
-    _ints("lens", lens, size=n_seq)
-    for t, n, what in ((u, n_tokens, "u"), (r, n_seq, "r")):
-        if t is None and greedy:
-            continue
-        if t is None or t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{what} is contiguous float32 [{n}]")
+    at = p.get_device()
+    _ints("cu", cu, None, at)
+    _ints("tokens", tokens, n_tokens, at)
+    if parent is not None:
+        _ints("parent", parent, n_tokens, at)
+    if lens is not None:
+        _ints("lens", lens, n_seq, at)
+    if not greedy or u is not None or r is not None:
+        for t, n, what in ((u, n_tokens, "u"), (r, n_seq, "r")):
+            if t is None or t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"{what} is contiguous float32 [{n}]")
     if out is None:
-        out = Verified(_new_out((n_seq, max_new), torch.int32, p.device, stream),
-                       _new_out((n_seq,), torch.int32, p.device, stream),
-                       _new_out((n_seq,), torch.int32, p.device, stream))
-    else:
-        _ints("path", out.path, size=n_seq * max_new)
-        _ints("accepted", out.accepted, size=n_seq)
-        _ints("token", out.token, size=n_seq)
-    _here(p.device, p, tokens, u, r, cu, parent, q, lens, *out, stream=stream, workspace=workspace)
-    _, d, need = _verify_desc(n_seq, n_tokens, max_new, vocab, p_stride, q_stride, int(bool(greedy)))
+        out = Verified.empty(n_seq, max_new, p.device, stream)
+    elif out.path.shape != (n_seq, max_new):
+        raise ValueError("out is of other requests or rows")
+    _here(p.device, u, r, q, out.path, stream=stream, workspace=workspace)
+    _, d, need = _verify_desc(n_seq, n_tokens, max_new, vocab, p_stride, q_stride, 1 if greedy else 0)
     ws_ptr, ws_bytes = _space(need, workspace, p.device, stream)
     _check("lmxs_verify", spec_lib().lmxs_verify(
-        d, cu.data_ptr(), tokens.data_ptr(), _ptr(parent), p.data_ptr(), _ptr(q), dt, _ptr(u), _ptr(r),
-        out.path.data_ptr(), out.accepted.data_ptr(), out.token.data_ptr(), _ptr(lens), _ptr_of(ws_ptr), ws_bytes,
-        _stream(stream)))
+        d, cu.data_ptr(), tokens.data_ptr(), _ptr(parent), p.data_ptr(), _ptr(q), dt, _ptr(u), _ptr(r), *out.ptrs,
+        _ptr(lens), _ptr_of(ws_ptr), ws_bytes, _stream(stream)))
     return out
 
 
@@ -459,12 +498,16 @@ def spec_keep(caches: Sequence[PagedCache], batch: PagedBatch, path, accepted, *
     ``spec_verify``'s."""
     if not caches:
         raise ValueError("caches is empty")
-    _ints("path", path)
-    _ints("accepted", accepted, size=batch.n_seq)
-    if path.dim() != 2 or path.shape[0] != batch.n_seq:
-        raise ValueError(f"path is [{batch.n_seq}, entries]")
+    first = caches[0]
+    at, n_seq = first.at, batch.n_seq
+    _ints("path", path, None, at)
+    _ints("accepted", accepted, n_seq, at)
+    if path.dim() != 2 or path.shape[0] != n_seq:
+        raise ValueError(f"path is [{n_seq}, entries]")
+    _paged._place(first, batch, stream=stream)
     for c in caches:
-        _paged._place(c, batch, path, accepted, stream=stream)
-    pools = (PoolDesc * len(caches))(*[c.desc for c in caches])
+        if c.at != at:
+            raise ValueError("the caches are on one device")
+    pools = (_VP * len(caches))(*[c.address for c in caches])
     _check("lmxs_keep", spec_lib().lmxs_keep(pools, len(caches), batch.ref, path.data_ptr(), path.shape[1],
                                              accepted.data_ptr(), _stream(stream)))

@@ -45,5 +45,5 @@ extern "C" {
     pub fn lmxs_attn(p: *const LmxpPool, b: *const LmxpBatch, d: *const LmxpAttnDesc, seen: *const u64, words: u32, pos: *const i32, q: *const c_void, dt: i32, out: *mut c_void, ws: *mut c_void, ws_bytes: usize, stream: HipStream) -> i32;
     pub fn lmxs_verify_workspace_bytes(d: *const LmxsVerifyDesc) -> usize;
     pub fn lmxs_verify(d: *const LmxsVerifyDesc, cu: *const i32, tokens: *const i32, parent: *const i32, p: *const c_void, q: *const c_void, dt: i32, u: *const f32, r: *const f32, path: *mut i32, accepted: *mut i32, token: *mut i32, lens: *mut i32, ws: *mut c_void, ws_bytes: usize, stream: HipStream) -> i32;
-    pub fn lmxs_keep(pools: *const LmxpPool, n_pools: u32, b: *const LmxpBatch, path: *const i32, path_stride: u32, accepted: *const i32, stream: HipStream) -> i32;
+    pub fn lmxs_keep(pools: *const *const LmxpPool, n_pools: u32, b: *const LmxpBatch, path: *const i32, path_stride: u32, accepted: *const i32, stream: HipStream) -> i32;
 }

@@ -48,7 +48,7 @@ def to_rust(ctype):
     const = "const" in ctype
     words = [w for w in re.findall(r"\w+|\*", ctype) if w != "const"]
     t = C_TYPES.get(words[0]) or "".join(p.capitalize() for p in words[0].split("_"))
-    return ("*const " if const else "*mut ") + t if "*" in words else t
+    return ("*const " if const else "*mut ") * words.count("*") + t  # const: all of a pointer's levels
 
 
 def test_rust_mirror_matches():
@@ -143,7 +143,9 @@ def attn(p=None, b=None, seen=FAKE + BIG, words=1, pos=FAKE + 2 * BIG, q=FAKE, o
 
 
 def keep(p=None, b=None, n=1, path=FAKE, stride=8, accepted=FAKE):
-    return spec.spec_lib().lmxs_keep(ctypes.byref(p or pool()), n, ctypes.byref(b or batch()), path, stride, accepted, None)
+    p = p or pool()
+    pools = (ctypes.c_void_p * max(1, min(n, 4)))(*[ctypes.addressof(p)] * max(1, min(n, 4)))
+    return spec.spec_lib().lmxs_keep(pools, n, ctypes.byref(b or batch()), path, stride, accepted, None)
 
 
 @pytest.mark.parametrize("call", [prologue, attn, keep])
@@ -215,7 +217,8 @@ def test_bad_keepings_are_refused(kw, code):
 def test_layers_of_different_geometry_are_refused():
     for kw in (dict(n_pages=9), dict(page_size=32), dict(n_kv_heads=1), dict(head_dim=64),
                dict(store=paged.STORE_I8, k_scale=FAKE, v_scale=FAKE)):
-        pools = (paged.PoolDesc * 2)(pool(), pool(**kw))
+        two = pool(), pool(**kw)
+        pools = (ctypes.c_void_p * 2)(*map(ctypes.addressof, two))
         assert spec.spec_lib().lmxs_keep(pools, 2, ctypes.byref(batch()), FAKE, 8, FAKE, None) == S.E_SHAPE
 
 
@@ -226,6 +229,7 @@ def test_null_descriptions_are_refused():
     assert L.lmxs_verify(None, *[FAKE] * 5, 0, *[FAKE] * 7, 0, None) == S.E_NULL
     assert L.lmxs_verify_workspace_bytes(None) == 0
     assert L.lmxs_keep(None, 1, ctypes.byref(batch()), FAKE, 8, FAKE, None) == S.E_NULL
+    assert L.lmxs_keep((ctypes.c_void_p * 1)(None), 1, ctypes.byref(batch()), FAKE, 8, FAKE, None) == S.E_NULL
 
 
 def test_verification_workspace():
