@@ -124,8 +124,15 @@ lmx_status lmxs_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *   seen   uint64 [n_tokens, words], 8-byte aligned; words 1 to 16, 64 * words
  *          at least max_new
  *   pos    int32 [n_tokens]; may be NULL without a window
- * Types, layouts, precision and workspace are lmxp_attn's;
- * lmxp_attn_workspace_bytes gives its size. */
+ * Types, layouts and precision are lmxp_attn's, with f16 weights of 11 bits where
+ * the batch's max_new * n_heads / n_kv_heads is above 32 to 128 (by head_dim and
+ * store).  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
+ * what serves this batch and every one whose n_seq, n_tokens, max_new and max_ctx
+ * are at most its own, for either dt and any window (0 for a description that is
+ * refused). */
+size_t lmxs_attn_workspace_bytes(const lmxp_pool *p, const lmxp_batch *b,
+                                 const lmxp_attn_desc *d);
+
 lmx_status lmxs_attn(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_desc *d,
                      const uint64_t *seen, uint32_t words, const int32_t *pos, const void *q,
                      lmx_dtype dt, void *out, void *ws, size_t ws_bytes, lmx_stream stream);

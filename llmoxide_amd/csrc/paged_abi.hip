@@ -11,8 +11,8 @@ lmx_status paged_read(const lmxp_pool* p, const lmxp_batch* b, void* k_out, void
 lmx_status paged_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
                           const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
                           const float* factors, void* q_out, lmx_dtype q_out_dt, hipStream_t st);
-size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d);
-bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool f32, size_t* bytes);
+size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool seen);
+bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool f32, bool seen, size_t* bytes);
 lmx_status paged_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const void* q, lmx_dtype dt,
                       void* out, void* ws, hipStream_t st);
 
@@ -87,7 +87,7 @@ lmx_status lmxp_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_pro
 
 size_t lmxp_attn_workspace_bytes(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
     QLayout l;
-    return check_attn(p, b, d, &l) == LMX_OK ? paged_attn_workspace(p, b, d) : 0;
+    return check_attn(p, b, d, &l) == LMX_OK ? paged_attn_workspace(p, b, d, false) : 0;
 }
 
 lmx_status lmxp_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const void* q, lmx_dtype dt,
@@ -95,7 +95,7 @@ lmx_status lmxp_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_de
     lmx_status s = check_attn_call(p, b, d, q, dt, out);
     if (s != LMX_OK) return s;
     size_t need;
-    if (!paged_attn_need(p, b, d, dt == LMX_F32, &need)) return LMX_E_SHAPE;
+    if (!paged_attn_need(p, b, d, dt == LMX_F32, false, &need)) return LMX_E_SHAPE;
     if (need && (!ws || ws_bytes < need)) return LMX_E_WORKSPACE;
     if (need && !at16(ws)) return LMX_E_ALIGN;
     return paged_attn(p, b, d, q, dt, out, ws, (hipStream_t)stream);

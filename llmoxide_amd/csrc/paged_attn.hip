@@ -592,6 +592,82 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnPagedArgs a, int b
         *reinterpret_cast<f16x4*>(dst) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
 }
 
+// The same for rows of masks: a wave a row, HD/4 columns x 256/HD groups of splits
+// (two float4s a lane at 512 dims), joined across the lanes; four rows a workgroup.
+// 32 sequences of up to 64 rows, 8 bits: KERNEL_MERGE_FIGURE.
+template <int HD, bool F32, bool I8>
+__global__ __launch_bounds__(256) void paged_merge_rows_kernel(AttnPagedArgs a, int bm, int per) {
+    using QT = std::conditional_t<F32, float, f16>;
+    constexpr int C4 = HD < 256 ? HD / 4 : 64, NG = 64 / C4, V = HD / 4 / C4, U = 4 / V;
+    const PagedGeom& pg = a.p.g;
+    Item it;
+    if (!find_item(a, blockIdx.x / per, bm, false, false, it)) return;
+    const int lane = threadIdx.x & 63, r = blockIdx.x % per * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = it.tile * bm + r;
+    if (r >= bm || row >= it.s.n * pg.G || it.tile >= a.rt_max) return;
+    const int4 info = a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile];
+    const int splits = imin(info.z, a.n_items);  // written by this call's split 0; in range whatever it holds
+    if (splits <= 1) return;
+    const int col = lane % C4, grp = lane / C4;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = grp; s0 < splits; s0 += NG * U) {
+        f32x2 ml[U];
+        f32x4 x[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int sp = s0 + u * NG < splits ? s0 + u * NG : s0;
+            const size_t at = (size_t)imin(imax(info.x + sp * info.y, 0), a.n_items - 1) * bm + r;
+            ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[u][v] = *reinterpret_cast<const f32x4*>(a.part_o + at * HD + 4 * (col + C4 * v));
+            if (s0 + u * NG >= splits) {
+                ml[u] = f32x2{-INFINITY, 0.f};
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u][0]);
+        const float ref = mn == -INFINITY ? 0.f : mn, f = join_weight(m - ref);
+        l = moved<I8>(l, m - ref);
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float fu = join_weight(ml[u][0] - ref);
+            l += moved<I8>(ml[u][1], ml[u][0] - ref);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += x[u][v] * fu;
+        }
+        m = mn;
+    }
+#pragma unroll
+    for (int d = C4; d < 64; d <<= 1) {  // the groups (then V is 1)
+        const float m2 = shfl_xor(m, d), l2 = shfl_xor(l, d), mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+        const float f = join_weight(m - ref), f2 = join_weight(m2 - ref);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[0][j] = o[0][j] * f + shfl_xor(o[0][j], d) * f2;
+        l = moved<I8>(l, m - ref) + moved<I8>(l2, m2 - ref);
+        m = mn;
+    }
+    if (grp) return;
+    const float inv = 1.f / l;
+    QT* dst = static_cast<QT*>(a.out) + ((size_t)(it.s.row0 + row / pg.G) * pg.Hkv * pg.G + it.h * pg.G + row % pg.G) * HD;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const f32x4 y = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o[v] * inv;
+        const int d = 4 * (col + C4 * v);
+        if constexpr (F32)
+            *reinterpret_cast<f32x4*>(dst + d) = y;
+        else
+            *reinterpret_cast<f16x4*>(dst + d) = f16x4{(f16)y[0], (f16)y[1], (f16)y[2], (f16)y[3]};
+    }
+}
+
 // The same for chunks' row tiles: few splits, many rows.  A workgroup takes 32
 // rows, a wave every fourth 8 of their dims, in the order that the chunk
 // kernel's lanes hold them (part_at), so that a load is 1 KB in a row.  512 rows
@@ -696,6 +772,7 @@ struct Part {
     int bm, lo_rows, hi_rows, target, least, rt_max;
     int64_t items;  // workgroups: an upper bound of its items
     int64_t merge;  // workgroups of its merge
+    int slots, fine;  // rows of masks: AttnPagedArgs'
     size_t o_bytes, ml_bytes, rows_bytes;
     size_t bytes() const { return o_bytes + ml_bytes + rows_bytes; }
     // 256 threads a workgroup are counted in 32 bits
@@ -768,6 +845,71 @@ static size_t most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
     return bytes;
 }
 
+// ---- rows of masks.  A step's sequences bring about as many rows each, so that one
+// kernel takes them all, and there is no launch for rows that turn out to be none's.
+//
+// Query rows a sequence may have per kv head for the rows kernel.  Eight sequences
+// of 2000-8000 positions, 16 heads on 4, us on the rows and on the chunk kernel:
+//   128 dims  f16            16 rows  31 and 31, 20 rows  49 and 32, 32 rows  50 and 31
+//             f16, f32 q.    16 rows  31 and 37, 20 rows  51 and 38
+//             8 bits         48 rows  38 and 40, 64 rows  42 and 40 (32 sequences of up to 64: 84 and 117)
+//             8 bits, f32 q. 64 rows  45 and 53, 96 rows  60 and 55
+//   64 dims   f16            16 rows  19 and 22, 20 rows  27 and 21;  f32 q.  19 and 27, 28 and 27
+//             8 bits         64 rows  29 and 31, 96 rows  36 and 31;  f32 q.  31 and 37, 38 and 38
+//   256 dims  f16            16 rows  64 and 59, 20 rows  96 and 63;  f32 q.  68 and 80, 98 and 82
+//             8 bits         96 rows 106 and 124, 128 rows 127 and 125
+//             8 bits, f32 q. 64 rows 104 and 101
+//   512 dims  f16             4 rows 211 and 114 (one sequence 56 and 71);  f32 q. 258 and 132 (67 and 89)
+//             8 bits          4 rows 150 and 104 (45 and 78);  f32 q. 16 rows 161 and 212, 20 rows 303 and 214
+constexpr int seen_most(int hd, bool i8, bool f32, int n_seq) {
+    if (hd == 512) return n_seq > 1 && !(i8 && f32) ? 0 : kBM;
+    if (!i8) return kBM;
+    return hd == 256 && !f32 ? 96 : 64;
+}
+// 64-key units a split has at least where the work is short: one sequence of 6 rows
+// (16 heads on 8, f32) on 518, 2048, 8192 and 32768 keys, splits of 2 units 12.0,
+// 13.1, 19.9 and 46.8 us, of 4 units 13.3, 14.6, 17.2 and 37.1, of 8 units 14.6,
+// 18.0, 18.7 and 38.5; so about half of target of them, up to 8 units.  No split of
+// up to 8 units in all: 300 keys of 64 dims 7.9 and 10.7 us, 32 8-bit sequences 9.9
+// and 14.9.  (Even splits: 32 8-bit sequences 92 -> 84 us.)
+constexpr int seen_fine(int hd) { return rows_least(hd) / 4; }
+static Part seen_rows_part(const PagedGeom& g, int hd, int most) {
+    const int rows = (int)std::min<int64_t>((int64_t)g.max_new * g.G, most);
+    const int64_t tiles = std::min<int64_t>(row_tiles_bound(g, kBM), (int64_t)g.n_seq * ((rows + kBM - 1) / kBM));
+    Part r = make_part(g, hd, kBM, tiles, rows, true, rows_target(hd), rows_least(hd));
+    r.least = r.splits ? 1 : r.least;
+    r.fine = r.splits ? seen_fine(hd) : 0;
+    r.merge = r.splits ? tiles * g.Hkv * ((std::min(kBM, rows) + 3) / 4) : 0;
+    return r;
+}
+static Part seen_chunk_part(const PagedGeom& g, int hd, bool i8, bool f32) {
+    const int cm = chunk_rows(hd, i8, f32), slots = chunk_slots(hd, i8, f32);
+    const bool cut = (g.window ? 4 : 2) * row_tiles_least(g, cm) * g.Hkv <= slots;
+    Part r = make_part(g, hd, cm, row_tiles_bound(g, cm), (int64_t)g.max_new * g.G, cut, slots, kChunkLeast);
+    r.slots = slots;
+    return r;
+}
+static Plan seen_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
+    Plan p{};
+    const int most = seen_most(hd, i8, f32, g.n_seq);
+    if ((int64_t)g.max_new * g.G > most) p.chunk = seen_chunk_part(g, hd, i8, f32);
+    else p.rows = seen_rows_part(g, hd, most);
+    return p;
+}
+// The most of any smaller geometry, as most_workspace: of few rows, or of chunks.
+static size_t seen_most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
+    size_t bytes = seen_rows_part(g, hd, seen_most(hd, i8, f32, 1)).bytes();
+    if ((int64_t)g.max_new * g.G > seen_most(hd, i8, f32, g.n_seq)) {
+        const int cm = chunk_rows(hd, i8, f32), slots = chunk_slots(hd, i8, f32);
+        PagedGeom c = g;
+        c.n_tokens = (int)std::min<int64_t>(g.n_tokens, (int64_t)(slots / (2 * g.Hkv)) * cm / g.G);
+        c.max_new = std::min(g.max_new, c.n_tokens);
+        if (c.n_tokens > 0)
+            bytes = std::max(bytes, make_part(c, hd, cm, row_tiles_bound(c, cm), (int64_t)c.max_new * c.G, true, slots, kChunkLeast).bytes());
+    }
+    return bytes;
+}
+
 static PagedGeom attn_geom(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
     PagedGeom g = paged_args(p, b).g;
     g.G = (int)(d->n_heads / p->n_kv_heads);
@@ -775,22 +917,27 @@ static PagedGeom attn_geom(const lmxp_pool* p, const lmxp_batch* b, const lmxp_a
     return g;
 }
 
+static Plan plan_of(const PagedGeom& g, int hd, bool i8, bool f32, bool seen) {
+    return seen ? seen_plan(g, hd, i8, f32) : make_plan(g, hd, i8, f32);
+}
 // The workspace that one call needs; false where launches of either type could not name their work.
-bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool is_f32, size_t* bytes) {
+bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool is_f32, bool seen, size_t* bytes) {
     bool fits = true;
     for (bool f32 : {false, true}) {
-        const Plan pl = make_plan(attn_geom(p, b, d), (int)p->head_dim, p->store == LMXP_I8, f32);
+        const Plan pl = plan_of(attn_geom(p, b, d), (int)p->head_dim, p->store == LMXP_I8, f32, seen);
         fits = fits && pl.rows.fits() && pl.chunk.fits();
         if (f32 == is_f32) *bytes = pl.rows.bytes() + pl.chunk.bytes();
     }
     return fits;
 }
 // What serves calls of either type, with any window, on this batch and on every smaller one.
-size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
+size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool seen) {
     size_t need, bytes = 0;
-    if (!paged_attn_need(p, b, d, true, &need)) return 0;
+    if (!paged_attn_need(p, b, d, true, seen, &need)) return 0;
+    const PagedGeom g = attn_geom(p, b, d);
+    const bool i8 = p->store == LMXP_I8;
     for (bool f32 : {false, true})
-        bytes = std::max(bytes, most_workspace(attn_geom(p, b, d), (int)p->head_dim, p->store == LMXP_I8, f32));
+        bytes = std::max(bytes, seen ? seen_most_workspace(g, (int)p->head_dim, i8, f32) : most_workspace(g, (int)p->head_dim, i8, f32));
     return bytes;
 }
 
@@ -806,6 +953,9 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
     a.rt_max = r.splits ? r.rt_max : 0;
     a.lo_rows = r.lo_rows;
     a.hi_rows = r.hi_rows;
+    a.slots = r.slots;
+    a.even = a.seen != nullptr;
+    a.fine = r.fine;
     const dim3 grid((unsigned)r.items);
     if (chunk) {
         launch_chunk(a, HD, i8, f32, grid.x, st);
@@ -836,6 +986,18 @@ static lmx_status launch_part(AttnPagedArgs a, const Part& r, bool chunk, bool i
         }
         const int rows = (int)std::min<int64_t>(r.bm, (int64_t)a.p.g.max_new * a.p.g.G);
         const dim3 mgrid((unsigned)r.merge);
+        if (a.seen) {
+            auto go = [&](auto i8_tag, auto f32_tag) {
+                hipLaunchKernelGGL((paged_merge_rows_kernel<HD, decltype(f32_tag)::value, decltype(i8_tag)::value>), mgrid, dim3(256),
+                                   0, st, a, r.bm, (rows + 3) / 4);
+            };
+            const std::true_type yes;
+            const std::false_type no;
+            if (i8) f32 ? go(yes, yes) : go(yes, no);
+            else f32 ? go(no, yes) : go(no, no);
+            LMX_CHECK_LAUNCH();
+            return LMX_OK;
+        }
         if (i8) {
             if (f32) hipLaunchKernelGGL((paged_merge_kernel<HD, true, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
             else hipLaunchKernelGGL((paged_merge_kernel<HD, false, true>), mgrid, dim3(256), 0, st, a, r.bm, rows);
@@ -864,7 +1026,7 @@ static lmx_status attend(const lmxp_pool* p, const lmxp_batch* b, const lmxp_att
     a.q_row_stride = d->q_row_stride ? d->q_row_stride : a.q_head_stride * d->n_heads;
     a.c = d->scale * kLog2e;
     const bool i8 = p->store == LMXP_I8, f32 = dt == LMX_F32;
-    const Plan pl = make_plan(a.p.g, (int)p->head_dim, i8, f32);
+    const Plan pl = plan_of(a.p.g, (int)p->head_dim, i8, f32, seen != nullptr);
     (void)hipGetLastError();
     auto go = [&](auto tag) {
         constexpr int HD = decltype(tag)::value;

@@ -23,13 +23,18 @@ struct AttnPagedArgs {
     const uint64_t* seen; // [n_tokens][words]
     int words;
     const int32_t* at;    // [n_tokens] positions; read in a window
+    int slots;            // items are no more than start at once, where that can be (0: whatever target gives)
+    int even;             // a sequence's splits are of about one length
+    int fine;             // short work: half of target splits, of this many units to four times as many (0: none)
 };
 
 // What one query row sees where a mask says so (SEEN kernels): of the positions
 // before its sequence's rows those from lo on, of the rows those whose bit is set.
 struct Sight {
     const uint64_t* bits;  // of the row; NULL: it sees nothing
+    uint64_t word0;        // the first of them: of trees of up to 64 rows the only one
     int words, lo, first, n;  // first: position of the sequence's row 0, n: its rows
+    __device__ __forceinline__ uint64_t word(int i) const { return i == 0 ? word0 : i > 0 && i < words ? bits[i] : 0; }
     // Of the 64 positions from t0 on, those that it sees (pages apart).
     __device__ __forceinline__ uint64_t from(int t0) const {
         if (!bits) return 0;
@@ -38,8 +43,7 @@ struct Sight {
         const int j = t0 - first;  // the sequence's row at t0: two words hold the 64 rows from there on
         if (j > -64 && j < n) {
             const int w = j >> 6, sh = j & 63;
-            const uint64_t x = w >= 0 ? bits[imin(w, words - 1)] : 0;
-            const uint64_t y = w + 1 < words ? bits[w + 1] : 0;
+            const uint64_t x = word(w), y = word(w + 1);
             m |= (sh ? x >> sh | y << (64 - sh) : x) & below(n - j);
         }
         return m;
@@ -50,6 +54,7 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const AttnPagedArgs& a, const PagedSeq& s, bool have, int row) {
     Sight r;
     r.bits = have ? a.seen + (size_t)(s.row0 + row) * a.words : nullptr;
+    r.word0 = have ? *r.bits : 0;
     r.words = a.words;
     r.first = imax(s.ctx - s.n, 0);
     r.n = imin(s.n, 64 * a.words);
@@ -130,7 +135,13 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
             load_work(a, c0 + lane, bm, s2, w2);
             work += (float)w2.rt * (float)w2.units;
         }
-        o.per = units_per_split(wave_sum64(work) * (float)Hkv, a.target, a.least);
+        const float all = wave_sum64(work) * (float)Hkv;
+        o.per = units_per_split(all, a.target, a.least);
+        if (a.fine) o.per = imax(o.per, imin(units_per_split(all, a.target / 2, a.fine), 4 * a.fine));
+        // (every sequence's last split adds an item that its length does not fill)
+        if (a.slots && a.p.g.n_seq <= 64)
+            for (int k = 0; k < 8 && wave_sum64((float)(w.rt * Hkv * seq_splits(w, o.per))) > (float)a.slots; ++k)
+                o.per += imax(o.per >> 4, 1);
     }
     int base = 0;
     for (int c0 = 0;; ) {
@@ -144,6 +155,7 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
             o.s = PagedSeq{get(s.row0), get(s.n), get(s.ctx)};
             o.w = SeqWork{get(w.rt), get(w.lo), get(w.units)};
             o.splits = seq_splits(o.w, o.per);
+            if (a.even) o.per = (o.w.units + o.splits - 1) / o.splits;  // as many splits, of about one length
             const int first = base + get(upto) - get(n);
             // item order within a sequence: split, then row tile, then kv head
             // (with 8 heads every XCD keeps to one, and the row tiles that

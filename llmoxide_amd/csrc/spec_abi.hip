@@ -14,7 +14,8 @@ lmx_status paged_prologue_at(const lmxp_pool* p, const lmxp_batch* b, const lmxp
                              const int32_t* pos, const float* q, const float* k_new, const float* v_new,
                              const float* q_gain, const float* k_gain, const float* factors, void* q_out,
                              lmx_dtype q_out_dt, hipStream_t st);
-bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool f32, size_t* bytes);
+bool paged_attn_need(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool f32, bool seen, size_t* bytes);
+size_t paged_attn_workspace(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, bool seen);
 lmx_status paged_attn_seen(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const uint64_t* seen,
                            uint32_t words, const int32_t* pos, const void* q, lmx_dtype dt, void* out, void* ws,
                            hipStream_t st);
@@ -125,6 +126,11 @@ lmx_status lmxs_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_pro
                              (hipStream_t)stream);
 }
 
+size_t lmxs_attn_workspace_bytes(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d) {
+    QLayout l;
+    return check_attn(p, b, d, &l) == LMX_OK && b->max_new <= LMXS_MAX_ROWS ? paged_attn_workspace(p, b, d, true) : 0;
+}
+
 lmx_status lmxs_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_desc* d, const uint64_t* seen,
                      uint32_t words, const int32_t* pos, const void* q, lmx_dtype dt, void* out, void* ws,
                      size_t ws_bytes, lmx_stream stream) {
@@ -137,7 +143,7 @@ lmx_status lmxs_attn(const lmxp_pool* p, const lmxp_batch* b, const lmxp_attn_de
     if (overlap(seen, 8ull * b->n_tokens * words, out, bytes)) return LMX_E_SHAPE;
     if (pos && overlap(pos, 4ull * b->n_tokens, out, bytes)) return LMX_E_SHAPE;
     size_t need;
-    if (!paged_attn_need(p, b, d, dt == LMX_F32, &need)) return LMX_E_SHAPE;
+    if (!paged_attn_need(p, b, d, dt == LMX_F32, true, &need)) return LMX_E_SHAPE;
     if (need && (!ws || ws_bytes < need)) return LMX_E_WORKSPACE;
     if (need && !at16(ws)) return LMX_E_ALIGN;
     return paged_attn_seen(p, b, d, seen, words, pos, q, dt, out, ws, (hipStream_t)stream);

@@ -72,6 +72,7 @@ SIGNATURES = {
     "lmxs_plan": (_I, [_PS] + [_VP] * 11),
     "lmxs_tree": (_I, [_PB, _VP, _U32, _U32, _VP, _VP, _VP]),
     "lmxs_prologue": (_I, [_PP, _PB, _PR, _PO] + [_VP] * 8 + [_I, _VP]),
+    "lmxs_attn_workspace_bytes": (_SZ, [_PP, _PB, _PA]),
     "lmxs_attn": (_I, [_PP, _PB, _PA, _VP, _U32, _VP, _VP, _I, _VP, _VP, _SZ, _VP]),
     "lmxs_verify_workspace_bytes": (_SZ, [_PV]),
     "lmxs_verify": (_I, [_PV] + [_VP] * 5 + [_I] + [_VP] * 7 + [_SZ, _VP]),
@@ -393,8 +394,7 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
     d = _paged._attn_desc(n_heads, window, head, q.stride(0) if batch.n_tokens > 1 else 0,
                           1.0 / math.sqrt(hd) if scale is None else float(scale))[1]
     L = spec_lib()
-    ws_ptr, ws_bytes = _space(_paged.paged_lib().lmxp_attn_workspace_bytes(cache.ref, batch.ref, d), workspace,
-                              cache.device, stream)
+    ws_ptr, ws_bytes = _space(L.lmxs_attn_workspace_bytes(cache.ref, batch.ref, d), workspace, cache.device, stream)
     _check("lmxs_attn", L.lmxs_attn(cache.ref, batch.ref, d, seen.data_ptr(), words, _ptr(pos), q.data_ptr(), dt,
                                     out.data_ptr(), _ptr_of(ws_ptr), ws_bytes, _stream(stream)))
     return out
