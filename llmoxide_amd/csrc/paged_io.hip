@@ -769,13 +769,24 @@ static bool grid_fits(int64_t x, int64_t y) { return x < (1 << 24) && y < (1 << 
 // would be a row or two.  One row: append 4.0 us a kernel against 6.2, prologue
 // 4.4 against 12.6; four rows: 15.4 us a prologue call on either.
 static bool few_rows(const PagedGeom& g) { return g.max_new <= 4; }
+// The same for steps of trees, by the batch's rows: blocks of a few heads make every
+// row's angles again in each of their many workgroups, single rows V's columns
+// element by element.  Single rows and blocks (of one, two and four heads), us, 32
+// heads on 8 of 128 dims: 64 rows 4.7 and 6.9, 512 rows 10.2 and 15.1 (two heads),
+// 1024 rows 16.4 and 18.6, 2048 rows 26.2 and 26.0 (four); 256 dims (16 heads on 8): 128
+// rows 8.9 and 10.2, 256 rows 14.2 and 14.4, 512 rows 24.7 and 15.8; 512 dims (16 on
+// 4): 512 rows 19.4 and 19.1; 8 bits alike.
+static bool few_rows_at(const PagedGeom& g, int hd) { return g.n_tokens <= (hd <= 128 ? 1024 : hd == 256 ? 256 : 512); }
+// Heads a workgroup of the blocks then: 1024 rows of 256 dims two 17.6 to 26.9 us (as
+// one chunk, as eight), four 21.6 and 22.4; 2048 rows 42 and 39.
+static int heads_a_group_at(uint32_t n_tokens) { return n_tokens <= 1024 ? 2 : 4; }
 
 template <Pro PRO, typename SRC, bool I8>
 static lmx_status launch_store_hd(const StoreArgs& a, int hd, hipStream_t st) {
     auto go = [&](auto tag) {
         constexpr int HD = decltype(tag)::value;
         using L = RowLanes<HD>;
-        if (few_rows(a.p.g)) {
+        if (few_rows(a.p.g) || (PRO == kPrologueAt && few_rows_at(a.p.g, HD))) {
             const int64_t units = (int64_t)a.p.g.n_tokens * (a.n_k + a.n_v + a.n_q);
             const int64_t x = (units + 4 * L::RPI - 1) / (4 * L::RPI);
             if (!grid_fits(x, 1)) return LMX_E_SHAPE;
@@ -819,7 +830,7 @@ lmx_status paged_append(const lmxp_pool* p, const lmxp_batch* b, const void* k_n
 // The arguments of a prologue.
 static StoreArgs prologue_args(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
                                const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
-                               const float* factors, void* q_out, lmx_dtype q_out_dt) {
+                               const float* factors, void* q_out, lmx_dtype q_out_dt, int heads) {
     StoreArgs a{};
     a.p = paged_args(p, b);
     a.k_new = k_new;
@@ -840,7 +851,7 @@ static StoreArgs prologue_args(const lmxp_pool* p, const lmxp_batch* b, const lm
     a.eps = d->rms_eps;
     double s = d->n_rot ? std::pow((double)d->rope_base, -2.0 / (double)d->n_rot) : 1.0;
     for (int k = 0; k < 8; ++k, s *= s) a.scale_pow[k] = s;
-    a.hpw = heads_a_group(b->n_tokens);
+    a.hpw = heads;
     a.g_k = (a.n_k + a.hpw - 1) / a.hpw;
     a.g_v = (a.n_v + a.hpw - 1) / a.hpw;
     a.g_q = (a.n_q + a.hpw - 1) / a.hpw;
@@ -850,7 +861,8 @@ static StoreArgs prologue_args(const lmxp_pool* p, const lmxp_batch* b, const lm
 lmx_status paged_prologue(const lmxp_pool* p, const lmxp_batch* b, const lmxp_prologue_desc* d, const float* q,
                           const float* k_new, const float* v_new, const float* q_gain, const float* k_gain,
                           const float* factors, void* q_out, lmx_dtype q_out_dt, hipStream_t st) {
-    const StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt);
+    const StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt,
+                                      heads_a_group(b->n_tokens));
     (void)hipGetLastError();
     const int hd = (int)p->head_dim;
     return p->store == LMXP_I8 ? launch_store_hd<kPrologue, float, true>(a, hd, st)
@@ -861,7 +873,8 @@ lmx_status paged_prologue_at(const lmxp_pool* p, const lmxp_batch* b, const lmxp
                              const int32_t* pos, const float* q, const float* k_new, const float* v_new,
                              const float* q_gain, const float* k_gain, const float* factors, void* q_out,
                              lmx_dtype q_out_dt, hipStream_t st) {
-    StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt);
+    StoreArgs a = prologue_args(p, b, d, q, k_new, v_new, q_gain, k_gain, factors, q_out, q_out_dt,
+                                heads_a_group_at(b->n_tokens));
     a.at = pos;
     a.interleaved = (int)r->interleaved;
     a.turn_scale = r->turn_scale;

@@ -117,9 +117,12 @@ class _At(NamedTuple):
     device: object
 
 
+_at = functools.lru_cache(maxsize=64)(_At)
+
+
 def _here(device, *ts, stream=None, workspace=None) -> None:
     """Tensors, stream and workspace of ``device``, which has to be the current one."""
-    at = _At(device)
+    at = _at(device)
     _paged._place(at, at, *ts, stream=stream, workspace=workspace)
 
 
@@ -135,6 +138,13 @@ class _Held:
 
     def __iter__(self):
         return iter(self.ts)
+
+    @classmethod
+    def _made(cls, device, at, *ts):
+        """Of tensors that a call allocated itself: nothing to check."""
+        self = object.__new__(cls)
+        self.ts, self.ptrs, self.device, self.at = ts, tuple([t.data_ptr() for t in ts]), device, at
+        return self
 
 
 # ------------------------------------------------------------------- pages --
@@ -261,8 +271,10 @@ def spec_tree(parent, batch: PagedBatch, *, window: int = 0, out: Optional[SpecT
     n_tokens = batch.n_tokens
     if out is None:
         torch = _torch()
-        out = SpecTree(_new_out((n_tokens,), torch.int32, batch.device, stream),
-                       _new_out((n_tokens, -(-batch.max_new // 64)), torch.int64, batch.device, stream))
+        words = -(-batch.max_new // 64)
+        out = SpecTree._made(batch.device, batch.device.index, _new_out((n_tokens,), torch.int32, batch.device, stream),
+                             _new_out((n_tokens, words), torch.int64, batch.device, stream))
+        out.words = words
     elif out.pos.numel() != n_tokens:
         raise ValueError("out is of other rows")
     _ints("parent", parent, n_tokens, out.at)
@@ -436,7 +448,9 @@ class Verified(_Held):
     def empty(cls, n_seq: int, max_new: int, device, stream=None) -> "Verified":
         """Tensors for a verification to write."""
         i32 = _torch().int32
-        return cls(*(_new_out(shape, i32, device, stream) for shape in ((n_seq, max_new), (n_seq,), (n_seq,))))
+        path = _new_out((n_seq, max_new), i32, device, stream)
+        return cls._made(path.device, path.get_device(), path, _new_out((n_seq,), i32, device, stream),
+                         _new_out((n_seq,), i32, device, stream))
 
 
 @functools.lru_cache(maxsize=256)

@@ -776,3 +776,41 @@ def test_a_loop_of_steps_writes_what_the_model_says(store, captured):
             k2, v2 = lmx.paged_read(c, own)
             assert torch.equal(v, v2)
             assert (k - k2).abs().max() <= 2.0 ** -6 * k2.abs().max()  # one step of 8 bits, or of f16
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("hd,n_rot,store", [(128, 128, "f16"), (128, 40, "i8"), (256, 256, "i8"), (512, 512, "f16")])
+def test_prologue_in_blocks_of_rows_is_that_of_single_rows(hd, n_rot, store, interleaved):
+    """A batch of many rows and the same rows in small batches.  The arithmetic is the
+    same but for where a product is fused into the sum behind it, so that each is
+    within test_prologue's bound of the exact result, and the two within twice that."""
+    say("prologue blocks", hd, n_rot, store, interleaved)
+    c = po.PagedCase(50, new=[700, 1, 400], ctx=[900, 30, 400], page=32, kv=2, hd=hd, store=store, pad=3)
+    heads = 3
+    q, k, v = (gpu(rows(c, 51 + i, h).reshape(c.tokens, -1)) for i, h in enumerate((heads, 2, 2)))
+    gain = gpu((1 + 0.1 * np.random.default_rng(1).standard_normal(hd)).astype(np.float32))
+    pos = ints(np.random.default_rng(2).integers(0, 1 << 20, c.tokens))
+    kw = dict(n_heads=heads, n_rot=n_rot, interleaved=interleaved, turn_scale=1.1, q_gain=gain, k_gain=gain)
+    cache, batch = on_gpu(c)
+    want = torch.zeros(c.tokens, heads * hd, device="cuda")
+    lmx.spec_prologue(q, k, v, cache, batch, pos=pos, q_out=want, **kw)
+    small, _ = on_gpu(c)
+    got = torch.zeros_like(want)
+    for b, n in enumerate(c.new):
+        for j in range(0, n, 100):
+            m = min(100, n - j)
+            at = slice(int(c.cu[b]) + j, int(c.cu[b]) + j + m)
+            part = lmx.PagedBatch(ints([0, m]), ints([c.ctx[b] - n + j + m]), ints(c.table[b:b + 1]), n_tokens=m, max_new=m,
+                                  max_ctx=max(c.ctx))
+            lmx.spec_prologue(q[at], k[at], v[at], small, part, pos=pos[at], q_out=got[at], **kw)
+    rel = 2 * (hd + 34) * 2.0 ** -24 * 1.1  # test_prologue's, of a row head's largest element
+    big = want.view(c.tokens, heads, hd).abs().amax(-1, keepdim=True)
+    assert ((got - want).view(c.tokens, heads, hd).abs() <= 2 * rel * big).all()
+    for name in ("k", "v"):
+        x, y = (getattr(p, name).float() for p in (cache, small))
+        if store == "i8":  # the scales by the same bound; an int where the quotient lies beside a half
+            sx, sy = (getattr(p, name + "_scale") for p in (cache, small))
+            assert ((sx - sy).abs() <= 4 * rel * sx).all() and (x - y).abs().max() <= 1
+        else:  # a place of f16 where the value lies beside a half
+            top = x.abs().amax(-1 if name == "k" else -2, keepdim=True)
+            assert ((x - y).abs() <= 2 * rel * top + 2.0 ** -10 * x.abs() + 2.0 ** -24).all()
