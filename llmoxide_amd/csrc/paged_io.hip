@@ -327,7 +327,8 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
     using DT = std::conditional_t<I8, int8_t, f16>;
     constexpr int R = L::R, NI = L::NI, LPR = L::LPR, H2 = HD / 2;
     // a workgroup holds V's rows, or the angles (cos, sin) of its rows
-    constexpr int kTurn = PRO ? R * H2 * 8 : 0, kBytes = VT::BYTES > kTurn ? VT::BYTES : kTurn;
+    constexpr int TS = PRO == kPrologueAt ? H2 + 2 : H2;  // pairs from row to row of the angles
+    constexpr int kTurn = PRO ? R * TS * 8 : 0, kBytes = VT::BYTES > kTurn ? VT::BYTES : kTurn;
     __shared__ __align__(16) char smem[kBytes];
     __shared__ __align__(16) float rows_s[PRO ? 4 : 1][PRO ? 512 : 4];
     __shared__ double freq_s[PRO ? H2 : 1];
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
             float c, s;
             turn_of(pos * freq_s[i], c, s);
             if (PRO == kPrologueAt) c *= a.turn_scale, s *= a.turn_scale;
-            turn[row * H2 + i] = make_float2(c, s);
+            turn[row * TS + i] = make_float2(c, s);
         }
         __syncthreads();
     }
@@ -393,13 +394,13 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
                 const float* gain = is_v ? nullptr : is_k ? a.k_gain : a.q_gain;
                 if (is_v ? a.v_norm != 0 : gain != nullptr) norm_row<LPR, HD>(e, gain, a.eps, li);
                 if (PRO == kPrologueAt && a.interleaved) {
-                    if (!is_v) turn_pairs<HD>(e, li, half, [&](int i) { return turn[rl * H2 + i]; });
+                    if (!is_v) turn_pairs<HD>(e, li, half, [&](int i) { return turn[rl * TS + i]; });
                 } else if (!is_v && half == H2) {
-                    const f32x4* t = reinterpret_cast<const f32x4*>(&turn[rl * H2 + 4 * li]);
+                    const f32x4* t = reinterpret_cast<const f32x4*>(&turn[rl * TS + 4 * li]);
                     const f32x4 t0 = t[0], t1 = t[1];
                     turn_row(e, {t0[0], t0[2], t1[0], t1[2]}, {t0[1], t0[3], t1[1], t1[3]});
                 } else if (!is_v && half) {
-                    turn_part<HD>(e, rows_s[w] + sub * HD, li, half, [&](int i) { return turn[rl * H2 + i]; });
+                    turn_part<HD>(e, rows_s[w] + sub * HD, li, half, [&](int i) { return turn[rl * TS + i]; });
                 }
                 if (is_q) {
                     if (rl < n_rows) {
