@@ -11,17 +11,6 @@ namespace lmx {
 constexpr int kMost = (1 << 30) - 1;
 __device__ __forceinline__ int add_sat(int a, int b) { return imin(a + b, kMost); }
 
-// Inclusive scan over the wave's lanes with add_sat.
-__device__ __forceinline__ int wave_scan_sat(int x) {
-    const int lane = __lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d, 64);
-        x = lane >= d ? add_sat(x, y) : x;
-    }
-    return x;
-}
-
 // A request's rows of the batch, forced into range.
 struct SpecRows {
     int row0, n;

@@ -8,7 +8,8 @@
 // it is of; the order of everything is that of the sums, none of arrivals.
 //
 // Bound by latency: a step's entries and rows are a few KB, read once through
-// four dependent steps (lengths, sums, free list, table).
+// four dependent steps (lengths, sums, free list, table).  Eight requests of 64 rows
+// 6.5 us; with the launch and the host 19 us, a plan and its trees 23.
 #include "spec.hpp"
 
 namespace lmx {
@@ -211,8 +212,9 @@ __global__ __launch_bounds__(256) void spec_rows_kernel(PlanArgs a) {
     map_row(a, row, lo, imax(a.lens[lo], 0), row - a.cu[lo]);
 }
 
-// Rows that the plan's workgroup maps itself.
-constexpr int kRowsHere = 4096;
+// Rows that the plan's workgroup maps itself.  Here and in a kernel of their own, us a
+// plan: 4096 rows 6.5 and 8.9, 8192 rows 8.4 and 9.2, 16384 rows 10.1 and 9.1.
+constexpr int kRowsHere = 8192;
 
 lmx_status spec_plan(const lmxs_plan_desc* d, const int32_t* lens, const int32_t* new_rows, int32_t* table, int32_t* held,
                      int32_t* free_pages, int32_t* n_free, int32_t* cu, int32_t* ctx, int64_t* slots, int32_t* pos,
@@ -247,14 +249,22 @@ lmx_status spec_plan(const lmxs_plan_desc* d, const int32_t* lens, const int32_t
 }
 
 // ------------------------------------------------------------------- trees --
-// A workgroup takes a request.  A thread walks from its row up to the root and
-// gathers one word of the ancestors on the way: a tree of 64 drafts is some ten
-// steps deep, and its parents are in LDS.  (Doubling the reach of every row's
-// sight a step would need a copy of all words a step.)
+// A workgroup takes a request.  A row's ancestors among the 64 rows of its own word
+// come from a walk up the parents, which lie in LDS: at most 63 steps, some ten in a
+// tree of 64 drafts.  The words before are those of its first ancestor there, and so
+// on: at most 15 more steps, whatever the depth (1024 rows in a chain 26 us,
+// eight trees of 1024 13; with a walk up to the root for each word 2940 and 444).
+//
+// Bound by latency: eight trees of 64 rows 3.4 us, 4 KB.
+struct Above {
+    int next, n;    // the row's first ancestor in an earlier word (-1: none); bits set
+    uint64_t bits;  // the row and its ancestors in its own word
+};
 __global__ __launch_bounds__(256) void spec_tree_kernel(int n_tokens, int words, int window, const int32_t* cu,
                                                         const int32_t* ctx, const int32_t* parent, int32_t* pos,
                                                         uint64_t* seen) {
     __shared__ int up[LMXS_MAX_ROWS];
+    __shared__ Above above[LMXS_MAX_ROWS];
     const SpecRows s = spec_rows(cu, blockIdx.x, n_tokens, 64 * words);
     for (int i = threadIdx.x; i < s.n; i += 256) {
         const int p = parent[s.row0 + i];
@@ -262,18 +272,33 @@ __global__ __launch_bounds__(256) void spec_tree_kernel(int n_tokens, int words,
     }
     const int first = imax(ctx[blockIdx.x] - s.n, 0);
     __syncthreads();
-    for (int x = threadIdx.x; x < s.n * words; x += 256) {
-        const int row = x / words, w = x % words;
-        uint64_t bits = 0;
-        int depth = 0;
-        for (int p = row;;) {
-            if (p >> 6 == w && (!window || depth < window)) bits |= 1ull << (p & 63);
-            p = up[p];
-            if (p < 0) break;
-            ++depth;
+    for (int i = threadIdx.x; i < s.n; i += 256) {
+        Above x{up[i], 1, 1ull << (i & 63)};
+        while (x.next >= 0 && x.next >> 6 == i >> 6) {
+            x.bits |= 1ull << (x.next & 63);
+            ++x.n;
+            x.next = up[x.next];
         }
-        if (seen) seen[(size_t)(s.row0 + row) * words + w] = bits;
-        if (pos && w == 0) pos[s.row0 + row] = first + depth;
+        above[i] = x;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < s.n; i += 256) {
+        int depth = -1;  // of the row, less those still to come
+        int p = i;
+        for (int w = words - 1; w >= 0; --w) {
+            uint64_t bits = 0;
+            if (p >= 0 && p >> 6 == w) {
+                const Above x = above[p];
+                bits = x.bits;
+                // ancestors come before: those behind the window are the lowest bits
+                if (window)
+                    for (int drop = imin(depth + 1 + x.n - window, x.n); drop > 0; --drop) bits &= bits - 1;
+                depth += x.n;
+                p = x.next;
+            }
+            if (seen) seen[(size_t)(s.row0 + i) * words + w] = bits;
+        }
+        if (pos) pos[s.row0 + i] = first + depth;
     }
 }
 
