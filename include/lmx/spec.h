@@ -124,9 +124,10 @@ lmx_status lmxs_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *   seen   uint64 [n_tokens, words], 8-byte aligned; words 1 to 16, 64 * words
  *          at least max_new
  *   pos    int32 [n_tokens]; may be NULL without a window
- * Types, layouts and precision are lmxp_attn's, with f16 weights of 11 bits where
- * the batch's max_new * n_heads / n_kv_heads is above 32 to 128 (by head_dim and
- * store).  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
+ * Types, layouts and precision are lmxp_attn's, but for where f16 q and out take
+ * weights of 11 bits: in all of a batch whose max_new * n_heads / n_kv_heads is above
+ * 16 (LMXP_F16) or 64 (LMXP_I8; 96 at 256 dims), and at 512 dims in every batch of
+ * several requests.  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
  * what serves this batch and every one whose n_seq, n_tokens, max_new and max_ctx
  * are at most its own, for either dt and any window (0 for a description that is
  * refused). */
@@ -196,8 +197,9 @@ lmx_status lmxs_verify(const lmxs_verify_desc *d, const int32_t *cu, const int32
  * path rises and path[b][j] >= j, as lmxs_verify writes it; an entry that does
  * not, and one that is no row of the request, is not moved, nor one from or to a
  * position in no page.
- *   pools     host array of n_pools pointers to pools (a layer each) of one
- *             geometry and store, whose pages the batch's table names
+ *   pools     host array of n_pools (1 to 1024) pointers to pools (a layer each) of
+ *             one geometry and store, whose pages the batch's table names; their K
+ *             and V do not overlap
  *   b         the step's batch, its lengths with all of its rows
  *   path      int32 [n_seq, path_stride], path_stride at least max_new
  *   accepted  int32 [n_seq] */

@@ -183,7 +183,7 @@ lmx_status lmxs_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32
 lmx_status lmxs_keep(const lmxp_pool* const* pools, uint32_t n_pools, const lmxp_batch* b, const int32_t* path,
                      uint32_t path_stride, const int32_t* accepted, lmx_stream stream) {
     if (!pools) return LMX_E_NULL;
-    if (n_pools == 0 || n_pools > 65536) return LMX_E_SHAPE;
+    if (n_pools == 0 || n_pools > 1024) return LMX_E_SHAPE;
     for (uint32_t i = 0; i < n_pools; ++i) {
         const lmx_status s = check_pool(pools[i]);
         if (s != LMX_OK) return s;
@@ -195,6 +195,17 @@ lmx_status lmxs_keep(const lmxp_pool* const* pools, uint32_t n_pools, const lmxp
     const lmxp_pool* const p = pools[0];
     const lmx_status s = check_batch(p, b);
     if (s != LMX_OK) return s;
+    // A layer's moves are in order only within one pool: none may share memory.
+    const uintptr_t bytes = (uintptr_t)p->n_pages * p->n_kv_heads * p->page_size * p->head_dim * (p->store == LMXP_I8 ? 1 : 2);
+    auto near = [&](const void* x, const void* y) {
+        const uintptr_t u = (uintptr_t)x, v = (uintptr_t)y;
+        return (u > v ? u - v : v - u) < bytes;
+    };
+    for (uint32_t i = 1; i < n_pools; ++i)
+        for (uint32_t j = 0; j < i; ++j) {
+            const lmxp_pool &x = *pools[i], &y = *pools[j];
+            if (near(x.k, y.k) || near(x.v, y.v) || near(x.k, y.v) || near(x.v, y.k)) return LMX_E_SHAPE;
+        }
     if (!path || !accepted) return LMX_E_NULL;
     if (b->max_new > LMXS_MAX_ROWS || path_stride < b->max_new || path_stride >= (1u << 30)) return LMX_E_SHAPE;
     if (!aligned(path, 4) || !aligned(accepted, 4)) return LMX_E_ALIGN;

@@ -9,7 +9,9 @@
 //
 // Bound by latency (four dependent loads: lengths, path, table, rows) and, in many
 // layers, by V's sectors: it lies transposed, so that a position's dims are 2 bytes
-// each in a page's 32 to 512 bytes a dim.
+// each in a page's 32 to 512 bytes a dim.  Sixteen requests' paths through trees of 32
+// rows, 36 layers of 8 heads of 128 dims, f16 (24 MB read and written): 12 us, 2 TB/s;
+// one request, 8 layers: 3.7 us, 7 with the launch and the host.
 #include "spec.hpp"
 
 namespace lmx {

@@ -386,8 +386,10 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
     """``paged_attention`` of rows that see each other by a mask: each the positions
     before its request's rows (with ``window`` > 0 those above its ``pos`` less the
     window) and the request's rows whose bits are set in its ``seen`` int64
-    [n_tokens, words]; one that sees nothing gets zeros.  Types, precision and
-    workspaces are ``paged_attention``'s."""
+    [n_tokens, words]; one that sees nothing gets zeros.  Types and workspaces are
+    ``paged_attention``'s, and its precision, but that with f16 ``q`` the weights have
+    11 bits where the batch's max_new * heads / kv heads is above 16 (f16 pages) or 64
+    (8 bits; 96 at 256 dims), and at 512 dims in every batch of several requests."""
     hd = cache.head_dim
     head = q_head_stride or hd
     width = q.shape[-1] if q.dim() == 2 else -1
@@ -507,7 +509,7 @@ def spec_verify(p, tokens, u, r, cu, *, max_new: int, parent=None, q=None, lens=
 
 def spec_keep(caches: Sequence[PagedCache], batch: PagedBatch, path, accepted, *, stream=None) -> None:
     """Moves the accepted rows' K and V to the slots behind the cached positions, in
-    all ``caches`` (layers of one geometry) at once: row ``path[b][j]`` of request b to
+    all ``caches`` (layers of one geometry, each its own memory) at once: row ``path[b][j]`` of request b to
     where its row j is.  ``batch`` is the step's, ``path`` and ``accepted`` are
     ``spec_verify``'s."""
     if not caches:

@@ -814,3 +814,279 @@ def test_prologue_in_blocks_of_rows_is_that_of_single_rows(hd, n_rot, store, int
         else:  # a place of f16 where the value lies beside a half
             top = x.abs().amax(-1 if name == "k" else -2, keepdim=True)
             assert ((x - y).abs() <= 2 * rel * top + 2.0 ** -10 * x.abs() + 2.0 ** -24).all()
+
+
+# --------------------------------------------- calls that tests above do not make --
+@pytest.mark.parametrize("kind", ["tree", "chain", "forest"])
+@pytest.mark.parametrize("window", [63, 64, 65, 130, 1000, 1 << 29])
+def test_windows_of_trees_that_end_in_earlier_words(kind, window):
+    say("tree window", kind, window)
+    c = po.PagedCase(2, new=[1024, 200, 64], ctx=[1030, 200, 99], page=16, kv=1, hd=64)
+    _, batch = on_gpu(c)
+    trees = [np.array([-1] + [max(i - (1 + i % 3), 0) for i in range(1, n)]) for n in c.new] if kind == "tree" else \
+        trees_of(c, 3, kind)
+    got = lmx.spec_tree(ints(np.concatenate(trees)), batch, window=window)
+    for b, t in enumerate(trees):
+        depth, sees = so.tree(t, window)
+        at = slice(int(c.cu[b]), int(c.cu[b + 1]))
+        assert np.array_equal(got.pos[at].cpu().numpy(), c.ctx[b] - c.new[b] + depth)
+        assert np.array_equal(got.seen[at].cpu().numpy(), so.words_of(sees, 16))
+
+
+def far_pages(store, hd):
+    """A pool whose K and V pass 2^31 elements and 2^32 bytes each, its pages' number, and
+    two tables of two requests: the first pages and the last ones."""
+    dt = torch.float16 if store == "f16" else torch.int8
+    page, kv = 256, 8
+    per = page * kv * hd
+    n_pages = ((1 << 32) + (1 << 28)) // (per * (2 if store == "f16" else 1)) + 12
+    cache = lmx.PagedCache.empty(n_pages, page_size=page, n_kv_heads=kv, head_dim=hd, dtype=dt)
+    for x in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        if x is not None:
+            x.zero_()
+    ids = np.arange(12).reshape(2, 6)
+    return cache, n_pages, ints(ids), ints(n_pages - 1 - ids)
+
+
+@pytest.mark.parametrize("store,hd,new", [("f16", 128, 7), ("f16", 128, 60), ("i8", 64, 7), ("i8", 64, 100), ("f16", 512, 3)])
+def test_pages_beyond_32_bits_of_offset(store, hd, new):
+    """The same requests in the first pages of a pool and in the last: the same bits
+    come out of every call, and land where they belong."""
+    say("far pages", store, hd, new)
+    torch.manual_seed(5)
+    cache, n_pages, near, far = far_pages(store, hd)
+    kv, heads, first, n_seq = 8, 16, [1300, 255], 2
+    results = []
+    for table in (near, far):
+        for n, at in ((np.array(first), 0), (np.array([new, new]), 1)):
+            torch.manual_seed(6 + at)
+            T = int(n.sum())
+            ctx = n if at == 0 else n + first
+            batch = lmx.PagedBatch(ints(np.concatenate([[0], np.cumsum(n)])), ints(ctx), table, n_tokens=T,
+                                   max_new=int(n.max()), max_ctx=int(ctx.max()))
+            q, k, v = (torch.randn(T, h * hd, device="cuda") for h in (heads, kv, kv))
+            if at == 0:
+                lmx.paged_append(k, v, cache, batch)
+        parent = ints(np.concatenate([[-1] + [max(i - 2, 0) for i in range(1, new)]] * n_seq))
+        tree = lmx.spec_tree(parent, batch)
+        q = lmx.spec_prologue(q, k, v, cache, batch, n_heads=heads, pos=tree.pos, q_dtype=torch.float16)
+        out = lmx.spec_attention(q, cache, batch, tree.seen, n_heads=heads)
+        path = np.full((n_seq, new), -1)
+        path[:, :(new + 1) // 2] = np.arange(0, new, 2)
+        lmx.spec_keep([cache], batch, ints(path), ints([min((new + 1) // 2, 4)] * n_seq))
+        k2, v2 = lmx.paged_read(cache, lmx.PagedBatch(ints([0, *np.cumsum(ctx)]), ints(ctx), table, n_tokens=int(ctx.sum()),
+                                                      max_new=int(ctx.max()), max_ctx=int(ctx.max())))
+        results.append((q, out, k2, v2))
+    assert results[0][1].abs().max() > 0
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+    assert not cache.k[20:n_pages - 20].any() and not cache.v[20:n_pages - 20].any()
+
+
+def test_distributions_beyond_32_bits_of_offset():
+    """The last of 1100 rows of 2^21 entries: their own words, not those that 32 bits reach."""
+    say("far rows")
+    vocab, T = 1 << 21, 1100
+    p = torch.zeros(T, vocab, dtype=torch.float16, device="cuda")
+    tokens = np.zeros(T, np.int32)
+    rng = np.random.default_rng(8)
+    best = rng.integers(0, vocab, T)
+    p[torch.arange(T, device="cuda"), gpu(best)] = 1
+    new = [1000, 100]
+    cu = ints([0, 1000, 1100])
+    for b, at in ((0, 0), (1, 1000)):  # chains that are right up to a wrong token
+        n = new[b]
+        tokens[at + 1:at + n] = best[at:at + n - 1]
+        tokens[at + n - 2] += 1 if tokens[at + n - 2] == 0 else -1
+    u, r = torch.full((T,), 0.5, device="cuda"), torch.tensor([0.25, 0.75], device="cuda")
+    for kw in (dict(), dict(greedy=True), dict(q=p)):
+        got = lmx.spec_verify(p, ints(tokens), u, r, cu, max_new=1000, **kw)
+        assert got.accepted.tolist() == [998, 98]
+        if "q" not in kw:
+            assert got.token.tolist() == [int(best[997]), int(best[1097])]
+        else:  # the draft was p itself and is refused for a token it never gives: nothing left, p's own
+            assert got.token.tolist() == [int(best[997]), int(best[1097])]
+
+
+class Captured:
+    """Every call of a step, with inputs that `fill` changes and outputs of its own."""
+
+    def __init__(self, drafts, ws):
+        self.c = po.PagedCase(60, new=[20, 3, 9], ctx=[900, 70, 9], page=16, kv=2, hd=128, store="i8", pad=4, spare=60)
+        c, vocab = self.c, 5000
+        self.cache, _ = on_gpu(c)
+        self.kept = [x.clone() for x in (self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale)]
+        table = np.full((3, 80), -1)
+        for b, row in enumerate(c.table):
+            table[b, :-(-c.ctx[b] // 16)] = row[:-(-c.ctx[b] // 16)]
+        held = [-(-x // 16) for x in c.ctx]
+        used = {int(x) for b in range(3) for x in table[b, :held[b]]}
+        free = [x for x in range(c.n_pages) if x not in used]
+        self.start = [ints(table), ints(held), ints(free + [0] * (c.n_pages - len(free))), ints([len(free), 0])]
+        self.tables = lmx.PageTables(*[x.clone() for x in self.start], page_size=16)
+        self.T, self.most = 48, 16
+        self.step = lmx.StepPlan.empty(self.tables, n_tokens=self.T)
+        self.batch = lmx.PagedBatch(self.step.cu, self.step.ctx_lens, self.tables.page_table, n_tokens=self.T,
+                                    max_new=self.most, max_ctx=80 * 16)
+        self.lens, self.new = ints([0] * 3), ints([0] * 3)
+        self.parent, self.tokens = ints([-1] * self.T), ints([0] * self.T)
+        self.q, self.k, self.v = (torch.zeros(self.T, h * 128, device="cuda") for h in (8, 2, 2))
+        self.p, self.draft = (torch.zeros(self.T, vocab, device="cuda") for _ in range(2))
+        self.u, self.r = torch.zeros(self.T, device="cuda"), torch.zeros(3, device="cuda")
+        self.tree = spec.SpecTree(ints([0] * self.T), torch.zeros(self.T, 1, dtype=torch.int64, device="cuda"))
+        self.turned, self.out = (torch.zeros(self.T, 8 * 128, device="cuda") for _ in range(2))
+        self.got = spec.Verified(ints(np.zeros((3, self.most))), ints([0] * 3), ints([0] * 3))
+        self.drafts, self.ws = drafts, ws
+
+    def fill(self, seed):
+        g, rng = torch.Generator("cuda").manual_seed(seed), np.random.default_rng(seed)
+        for x, y in zip((self.tables.page_table, self.tables.held, self.tables.free_pages, self.tables.n_free), self.start):
+            x.copy_(y)
+        for x, y in zip((self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale), self.kept):
+            x.copy_(y)
+        new = rng.integers(0, 17, 3)
+        self.lens.copy_(ints([int(rng.integers(0, x + 1)) for x in self.c.ctx]))
+        self.new.copy_(ints(new))
+        self.parent.copy_(ints([int(rng.integers(-1, 4)) for _ in range(self.T)]))
+        self.tokens.copy_(ints(rng.integers(0, 4, self.T)))  # the likely ones, and one that is not
+        for x in (self.q, self.k, self.v):
+            x.normal_(generator=g)
+        for x in (self.u, self.r):
+            x.uniform_(generator=g)
+        for x in (self.p, self.draft):
+            x.uniform_(generator=g)
+            x[:, :3] *= 5000
+            x.div_(x.sum(1, keepdim=True))
+        self.step.slots.fill_(9)
+        for x in (self.out, self.turned):
+            x.fill_(3)
+
+    def run(self):
+        lmx.spec_plan(self.tables, self.lens, self.new, out=self.step, trim=True)
+        lmx.spec_tree(self.parent, self.batch, out=self.tree)
+        lmx.spec_prologue(self.q, self.k, self.v, self.cache, self.batch, n_heads=8, pos=self.tree.pos, q_out=self.turned)
+        lmx.spec_attention(self.turned, self.cache, self.batch, self.tree.seen, n_heads=8, out=self.out, workspace=self.ws)
+        kw = dict(q=self.draft) if self.drafts == "sampled" else dict(greedy=True) if self.drafts == "greedy" else {}
+        lmx.spec_verify(self.p, self.tokens, self.u, self.r, self.step.cu, max_new=self.most, parent=self.parent,
+                        lens=self.lens, out=self.got, workspace=self.ws, **kw)
+        lmx.spec_keep([self.cache], self.batch, self.got.path, self.got.accepted)
+
+    def results(self):
+        rows_ = int(self.step.cu[-1])
+        return [x.clone() for x in (*self.step, self.lens, self.tables.page_table, self.tables.held, self.tables.n_free,
+                                    self.tree.pos[:rows_], self.tree.seen[:rows_], self.turned, self.out, *self.got,
+                                    self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale)]
+
+    def capture(self):
+        self.fill(99)
+        self.run()
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.run()
+
+    def same(self, want):
+        return all(torch.equal(x, y) for x, y in zip(self.results(), want))
+
+
+def test_graphs_that_share_a_workspace_replay_as_eager_steps():
+    """Three graphs, of drafts of each kind, over one workspace; eager steps of another
+    program in between."""
+    ws = lmx.Workspace(1 << 24)
+    steps = {d: Captured(d, ws) for d in ("sampled", "best", "greedy")}
+    other = Captured("sampled", None)
+    for s in steps.values():
+        s.capture()
+    for seed in range(6):
+        for d, s in steps.items():
+            say("graph", d, seed)
+            s.fill(seed)
+            s.run()
+            torch.cuda.synchronize()
+            want = s.results()
+            other.fill(seed + 50)
+            s.fill(seed)
+            s.graph.replay()
+            other.run()  # eager work behind the replay
+            assert s.same(want)
+            torch.cuda.synchronize()
+            s.fill(seed)
+            s.graph.replay()
+            assert s.same(want)
+
+
+def test_steps_on_two_streams_at_once():
+    """Each with its own tables, cache and workspace."""
+    steps = [Captured("sampled", lmx.Workspace(1 << 24)), Captured("best", None)]
+    wants = []
+    for i, s in enumerate(steps):
+        s.fill(i)
+        s.run()
+        torch.cuda.synchronize()
+        wants.append(s.results())
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(5):
+        for i, s in enumerate(steps):
+            s.fill(i)
+        torch.cuda.synchronize()
+        for s, st in zip(steps, streams):
+            with torch.cuda.stream(st):
+                s.run()
+        torch.cuda.synchronize()
+        for s, want in zip(steps, wants):
+            assert s.same(want)
+
+
+def test_verification_on_a_stream_without_a_workspace():
+    """What the call allocates belongs to the stream that uses it."""
+    c = verify_case(70, [9, 30], 50000, "tree", "sampled")
+    args = (gpu(c["p"]), gpu(c["tok"]), gpu(c["u"]), gpu(c["r"]), gpu(c["cu"]))
+    kw = dict(max_new=30, parent=ints(np.concatenate(c["trees"])), q=gpu(c["q"]))
+    want = lmx.spec_verify(*args, **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = lmx.spec_verify(*args, stream=side, **kw)
+        torch.empty(1 << 20, dtype=torch.uint8, device="cuda").fill_(255)  # of the other stream
+        side.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_what_python_refuses():
+    c = po.PagedCase(71, new=[4, 2], ctx=[40, 9], page=16, kv=1, hd=64)
+    cache, batch = on_gpu(c)
+    parent, seen = ints([-1, 0, 1, 1, -1, 0]), torch.full((6, 1), -1, dtype=torch.int64, device="cuda")
+    q, kv = torch.randn(6, 128, device="cuda"), torch.randn(6, 64, device="cuda")
+    p, tok, u, r, cu = torch.rand(6, 30, device="cuda"), ints([0] * 6), torch.rand(6, device="cuda"), torch.rand(2, device="cuda"), batch.cu
+    path, accepted = ints([[0, -1, -1, -1]] * 2), ints([1, 1])
+    good = dict(n_heads=2)
+    bad = [
+        lambda: lmx.spec_tree(parent.cpu(), batch), lambda: lmx.spec_tree(parent.long(), batch),
+        lambda: lmx.spec_tree(parent[:5], batch), lambda: lmx.spec_tree(ints([0] * 12)[::2], batch),
+        lambda: lmx.spec_tree(parent, batch, out=spec.SpecTree(ints([0] * 7), torch.zeros(7, 1, dtype=torch.int64, device="cuda"))),
+        lambda: spec.SpecTree(ints([0] * 6), seen.int()), lambda: spec.SpecTree(ints([0] * 6), seen.view(-1)),
+        lambda: lmx.spec_prologue(q, kv, kv, cache, batch, pos=parent.float(), **good),
+        lambda: lmx.spec_prologue(q, kv, kv, cache, batch, pos=parent.cpu(), **good),
+        lambda: lmx.spec_prologue(q.half(), kv, kv, cache, batch, **good),
+        lambda: lmx.spec_prologue(q, kv, None, cache, batch, **good),
+        lambda: lmx.spec_prologue(q, kv, kv, cache, batch, n_heads=3),
+        lambda: lmx.spec_attention(q, cache, batch, seen[:5], **good), lambda: lmx.spec_attention(q, cache, batch, seen.cpu(), **good),
+        lambda: lmx.spec_attention(q, cache, batch, seen.int(), **good), lambda: lmx.spec_attention(q.double(), cache, batch, seen, **good),
+        lambda: lmx.spec_attention(q, cache, batch, seen, window=5, **good),  # a window asks for positions
+        lambda: lmx.spec_attention(q, cache, batch, seen, out=q.half(), **good),
+        lambda: lmx.spec_verify(p.double(), tok, u, r, cu, max_new=4), lambda: lmx.spec_verify(p, tok, u, None, cu, max_new=4),
+        lambda: lmx.spec_verify(p, tok, u[:5], r, cu, max_new=4), lambda: lmx.spec_verify(p, tok, u, r.half(), cu, max_new=4),
+        lambda: lmx.spec_verify(p, tok.cpu(), u, r, cu, max_new=4), lambda: lmx.spec_verify(p, tok, u, r, cu, max_new=7),
+        lambda: lmx.spec_verify(p, tok, u, r, cu, max_new=0), lambda: lmx.spec_verify(p[0], tok, u, r, cu, max_new=4),
+        lambda: lmx.spec_verify(p, tok, u, r, cu, max_new=4, q=p.half()), lambda: lmx.spec_verify(p, tok, u, r, cu, max_new=4, lens=ints([0])),
+        lambda: lmx.spec_verify(p, tok, u, r, cu, max_new=4, out=lmx.Verified.empty(2, 3, p.device)),
+        lambda: lmx.spec_keep([cache], batch, path.long(), accepted), lambda: lmx.spec_keep([cache], batch, path[:1], accepted),
+        lambda: lmx.spec_keep([cache], batch, path[:, :2].contiguous(), accepted), lambda: lmx.spec_keep([cache], batch, path, accepted[:1]),
+        lambda: lmx.spec_keep([cache, cache], batch, path, accepted),  # one pool twice
+    ]
+    before = [cache.k.clone(), cache.v.clone()]
+    for i, call in enumerate(bad):
+        say("refused", i)
+        with pytest.raises((TypeError, ValueError, RuntimeError, lmx.LmxError)):
+            call()
+    assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])

@@ -3,6 +3,7 @@ call here returns before anything is enqueued), and what pins the oracle."""
 import ctypes
 import math
 import os
+import random
 import re
 import subprocess
 
@@ -13,6 +14,7 @@ import llmoxide_amd as lmx
 from llmoxide_amd import paged, spec
 from tests import spec_oracle as so
 from tests.test_paged import BAD_BATCHES, BAD_POOLS, FAKE, FAR, S, batch, pool
+from tests.test_paged_workspace import SHAPES, rows as batch_of, wide
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "lmx", "spec.h")
@@ -340,3 +342,122 @@ def test_rope_scaling():
             lmx.rope_scaling(64, **bad)
     with pytest.raises(ValueError):
         lmx.rope_scaling(7, kind="linear", factor=2)
+
+
+# -------------------------------------------------- what calls may rely on --
+def test_a_pool_twice_among_the_layers_is_refused():
+    """A layer's moves are ordered within one pool only."""
+    far = dict(k=FAKE + BIG, v=FAKE + 2 * BIG)
+    one = pool()
+
+    def call(*pools):
+        return spec.spec_lib().lmxs_keep((ctypes.c_void_p * len(pools))(*map(ctypes.addressof, pools)), len(pools),
+                                         ctypes.byref(batch()), FAKE + 2, 8, FAKE, None)
+    assert call(one, pool(**far)) == S.E_ALIGN  # the next check's
+    for other in (one, pool(), pool(**dict(far, v=one.v)), pool(**dict(far, k=one.k)), pool(**dict(far, k=one.v)),
+                  pool(**dict(far, v=one.k + 16))):
+        assert call(one, pool(**far), other) == S.E_SHAPE
+
+
+def seen_workspace(p, b, heads, window=0):
+    d = paged.PagedAttnDesc(n_heads=heads, window=window, q_head_stride=0, q_row_stride=0, scale=0.1)
+    return spec.spec_lib().lmxs_attn_workspace_bytes(ctypes.byref(p), ctypes.byref(b), ctypes.byref(d))
+
+
+@pytest.mark.parametrize("kv,group,hd", SHAPES + [(2, 16, 512), (16, 1, 512), (1, 40, 64)])
+@pytest.mark.parametrize("store", [paged.STORE_F16, paged.STORE_I8])
+def test_the_workspace_of_a_batch_serves_every_smaller_one(kv, group, hd, store):
+    rng = random.Random(kv * hd + store)
+    p = wide(kv=kv, hd=hd, store=store)
+
+    def most(hi):
+        return max(1, min(hi, int(2 ** rng.uniform(0, 14))))
+    for _ in range(400):
+        tokens = most(1 << 14)
+        big = (most(40), tokens, most(min(tokens, 1024)), most(1 << 14))
+        tokens = most(tokens)
+        small = (most(big[0]), tokens, most(min(tokens, big[2])), most(big[3]))
+        window = rng.choice([0, 1, 100, 1 << 20])
+        has = seen_workspace(p, batch_of(*big), kv * group)
+        assert seen_workspace(p, batch_of(*small), kv * group, window) <= has, (small, big, window)
+
+
+@pytest.mark.parametrize("hd,seqs,small", [
+    (128, 1, (1, 1, 1)), (128, 1, (1, 6, 6)), (128, 1, (1, 300, 300)), (64, 40, (33, 544, 512)), (256, 40, (8, 64, 9)),
+    (512, 1, (1, 4, 4)), (512, 9, (2, 40, 39)), (512, 9, (1, 2, 2)),
+])
+@pytest.mark.parametrize("store", [paged.STORE_F16, paged.STORE_I8])
+@pytest.mark.parametrize("dt", [lmx.F32, lmx.F16])
+@pytest.mark.parametrize("window", [0, 4000])
+def test_calls_take_the_workspace_of_a_larger_batch(hd, seqs, small, store, dt, window):
+    """Each small batch is cut between workgroups: its call needs a workspace, and goes on
+    past its size to the next check (the alignment), which refuses it."""
+    p = wide(kv=2, hd=hd, store=store)
+    has = seen_workspace(p, batch_of(seqs, 1024, 1024, 32768), 8)
+    call = dict(p=p, b=batch_of(*small, 8192), dt=dt, n_heads=8, window=window, words=16, out=FAR * 64, ws=FAKE + 8)
+    assert attn(ws_bytes=0, **call) == S.E_WORKSPACE
+    assert attn(ws_bytes=has, **call) == S.E_ALIGN
+
+
+def test_streams_and_workspaces_of_another_device_are_refused(monkeypatch):
+    """Stand-ins for what two GPUs would give: the check reads nothing but devices."""
+    torch = pytest.importorskip("torch")
+
+    class On:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+            self.device_index = index
+
+        def get_device(self):
+            return self.device.index
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    here, there = On(0), On(1)
+    spec._here(here.device, here, None, stream=here, workspace=lmx.Workspace(device="cuda:0"))
+    for device, ts, kw in ((there.device, (there,), {}), (here.device, (there,), {}), (here.device, (here,), dict(stream=there)),
+                           (here.device, (here,), dict(workspace=lmx.Workspace(device="cuda:1")))):
+        with pytest.raises(ValueError):
+            spec._here(device, *ts, **kw)
+
+
+class Fake:
+    """A tensor's looks, of device 0."""
+
+    def __init__(self, *shape, dtype=None, at=0, contiguous=True):
+        import torch
+        self.shape, self.dtype, self.at, self.flat = shape, dtype or torch.int32, at, contiguous
+        self.device = torch.device("cuda", at) if at >= 0 else torch.device("cpu")
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def get_device(self):
+        return self.at
+
+    def is_contiguous(self):
+        return self.flat
+
+    def data_ptr(self):
+        return FAKE
+
+
+def test_python_tables_and_plans_refuse_what_does_not_fit():
+    torch = pytest.importorskip("torch")
+
+    def tables(**kw):  # name: shape, or looks
+        shapes = dict(table=(3, 5), held=(3,), free=(9,), n_free=(2,))
+        return spec.PageTables(*[Fake(*(kw[n] if isinstance(kw.get(n), tuple) else s),
+                                      **(kw[n] if isinstance(kw.get(n), dict) else {})) for n, s in shapes.items()],
+                               page_size=16)
+    assert (tables().n_seq, tables().entries, tables().n_pages) == (3, 5, 9)
+    for kw, error in ((dict(table=(15,)), ValueError), (dict(held=(4,)), ValueError), (dict(n_free=(1,)), ValueError),
+                      (dict(free=dict(dtype=torch.int64)), TypeError), (dict(held=dict(at=1)), ValueError),
+                      (dict(table=dict(at=-1)), ValueError), (dict(table=dict(contiguous=False)), ValueError)):
+        with pytest.raises(error):
+            tables(**kw)
+    with pytest.raises(ValueError):
+        spec.spec_plan(tables(), Fake(3), Fake(3))  # no rows given
+    with pytest.raises(ValueError):
+        spec.spec_keep([], None, None, None)
