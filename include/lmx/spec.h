@@ -171,8 +171,9 @@ lmx_status lmxs_attn(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_de
  *   accepted  int32 [n_seq], written: their number, 0 for a request of no rows
  *   token     int32 [n_seq], written; -1 for a request of no rows
  *   lens      int32 [n_seq] or NULL: accepted is added to it
- * The workspace (16-byte aligned) is needed unless greedy; every byte read from
- * it was written by the same call.  Outputs overlap nothing. */
+ * The workspace (16-byte aligned) is needed for large vocabularies unless greedy, where
+ * lmxs_verify_workspace_bytes is not 0; every byte read from it was written by the same
+ * call.  Outputs overlap nothing. */
 typedef struct {
     uint32_t n_seq;
     uint32_t n_tokens;

@@ -4,10 +4,11 @@
 // reads no memory; only sums over the vocabulary that a second sibling asks for
 // (drafts that were sampled), or the largest scores (greedy), are passes over a
 // row of p, by one workgroup of the request.  Then the last row's distribution is
-// weighed, 256 entries a sum, by a workgroup for 4096 entries; and one wave adds
-// the sums up, finds the one where the running sum passes r times the whole, and
-// goes through its 256 entries.  Chosen drafts and chains need no passes: there
-// every workgroup that weighs walks by itself, which saves a launch.
+// weighed, 256 entries a sum; and one wave adds the sums up, finds the one where the
+// running sum passes r times the whole, and goes through its 256 entries.  Up to 32768
+// entries all of this is one launch, a workgroup a request.  Longer rows are weighed by
+// a workgroup for 4096 entries; chosen drafts and chains, which need no passes, are
+// then walked by every workgroup that weighs, which saves a launch.
 //
 // What is left of p after refusals needs one number: with w = p - a q wherever
 // that is above 0, and W its sum, the next refusal's w / W - q is, times W,
@@ -17,7 +18,11 @@
 // in the running sum, which is where a 32-bit sum's own rounding lies.  Each is
 // made in an order that the shapes alone decide.
 //
-// Bound by latency: the last rows (4 or 8 bytes an entry) are 4 MB for 8 requests.
+// Bound by latency: the last rows (4 or 8 bytes an entry) are 8 MB for 16 requests of
+// 131072 entries, chosen drafts: 8.8 us from a graph (weights 8.3, token 4.5 by
+// themselves), 15 from the host.  A pass takes a workgroup 8.5 us for 100003 entries of
+// p and q (94 GB/s of one CU): eight sampled trees of up to 24 rows 40 us, of which the
+// walk and its passes 36.
 #include <type_traits>
 
 #include "spec.hpp"
@@ -26,6 +31,7 @@ namespace lmx {
 
 constexpr int kGroup = 256;            // entries of the vocabulary a sum
 constexpr int kGroups = 16;            // sums a workgroup makes, four a wave
+constexpr int kOne = 1 << 15;          // most entries that one workgroup goes through
 
 // Where the walk ended.
 struct Last {
@@ -56,7 +62,10 @@ struct VerifyArgs {
 };
 
 // A probability; what is not above 0 and finite is 0.
-__device__ __forceinline__ double prob(float x) { return x > 0.f && x < INFINITY ? (double)x : 0.0; }
+__device__ __forceinline__ double prob(float x) {
+    const bool on = __builtin_bit_cast(uint32_t, x) - 1u < 0x7f7fffffu;  // the bits of 0 < x < inf
+    return (double)(on ? x : 0.f);
+}
 
 // A row's parent within the request, -1 for a root.
 __device__ __forceinline__ int parent_of(const VerifyArgs& a, int row0, int i) {
@@ -206,15 +215,213 @@ __device__ __forceinline__ void write_walk(const VerifyArgs& a, int b, const Spe
         a.accepted[b] = w.count;
         if (a.lens) a.lens[b] += w.count;
         if (D == GREEDY || !s.n) a.token[b] = w.best;
-        if (D != GREEDY) a.last[b] = Last{s.n ? s.row0 + w.cur : -1, w.cur, w.children, 0, w.a};
+        if (D != GREEDY && a.last) a.last[b] = Last{s.n ? s.row0 + w.cur : -1, w.cur, w.children, 0, w.a};
     }
 }
 
-// ---- drafts that ask for passes over the vocabulary: a workgroup a request
+// ---- the last row's weights
+//
+// Weights behind the walk: (p - a q)+, or p, of which the tokens of refused children
+// are taken by their readers.
+template <typename T, bool Q>
+struct Weights {
+    const T* p;
+    const T* q;
+    double a;
+    int vocab;
+    __device__ __forceinline__ void load(int t, f32x4& x, f32x4& y) const {
+        x = four_of(p, t, vocab, 0.f);
+        if (Q) y = four_of(q, t, vocab, 0.f);
+    }
+    __device__ __forceinline__ double of(float x, float y) const {
+        return Q ? fmax(prob(x) - a * prob(y), 0.0) : prob(x);
+    }
+};
+template <typename T, bool Q>
+__device__ __forceinline__ Weights<T, Q> weights_of(const VerifyArgs& a, int row, double c) {
+    // (behind a leaf a is 0 and q says nothing: p is read in its place)
+    const T* const p = static_cast<const T*>(a.p) + (size_t)row * a.p_stride;
+    return Weights<T, Q>{p, Q && c != 0.0 ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride : p, c, a.vocab};
+}
+
+// Where the walk's children are: child(k) is the token of row k if it continues row
+// `at`, else -1; `drop`: their tokens weigh nothing.
+template <typename C>
+struct Refused {
+    bool drop;
+    int at, n;
+    const C& child;
+    // The lanes' entries 4 lane .. of W groups from g0 on that are such tokens: 0.
+    template <int W>
+    __device__ __forceinline__ void clear(int g0, f32x4 (&x)[W]) const {
+        if (!drop) return;
+        const int lane = __lane_id();
+        for (int c0 = (at + 1) & ~63; c0 < n; c0 += 64) {
+            const int t = child(c0 + lane);
+            for (uint64_t left = __ballot(t >= g0 * kGroup && t < (g0 + W) * kGroup); left; left &= left - 1) {
+                const int e0 = __builtin_amdgcn_readlane(t, __builtin_ctzll(left)) - g0 * kGroup;
+#pragma unroll
+                for (int g = 0; g < W; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e0 == g * kGroup + 4 * lane + e) x[g][e] = 0.f;
+            }
+        }
+    }
+};
+
+// A wave's W sums from group g0 on, of whose weights x and y are loaded.
+template <int W, typename T, bool Q, typename C>
+__device__ __forceinline__ void weigh(const Weights<T, Q>& wt, const Refused<C>& refused, int g0, int n_groups,
+                                      f32x4 (&x)[W], const f32x4 (&y)[W], double* sums) {
+    const int lane = __lane_id();
+    refused.clear(g0, x);
+    double sum[W];
+#pragma unroll
+    for (int g = 0; g < W; ++g) {
+        sum[g] = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[g] += wt.of(x[g][e], Q ? y[g][e] : 0.f);
+    }
+    // Over the lanes: while there are several sums a lane hands half of them to its
+    // partner, so that lane l ends with sum l % W.
+#pragma unroll
+    for (int m = 1, n = W; m < 64; m <<= 1) {
+        if (n > 1) {
+            n >>= 1;
+#pragma unroll
+            for (int g = 0; g < n; ++g) {
+                // (sum 2g is the even lanes')
+                const double give = lane & m ? sum[2 * g] : sum[2 * g + 1], keep = lane & m ? sum[2 * g + 1] : sum[2 * g];
+                sum[g] = keep + __shfl_xor(give, m, 64);
+            }
+        } else {
+            sum[0] += __shfl_xor(sum[0], m, 64);
+        }
+    }
+    if (lane < W && g0 + lane < n_groups) sums[g0 + lane] = sum[0];
+}
+
+// The token, from the groups' sums, by a wave.
+template <typename T, bool Q, typename C>
+__device__ __forceinline__ int find_token(Weights<T, Q> wt, Refused<C> refused, int n_groups, const double* sums, double r) {
+    const int lane = __lane_id();
+    // Of 64 lanes' values, those of which `some` count: the first whose running sum
+    // passes the target, or else the last that counts, or else -1.
+    auto choose = [&](bool passes, bool some) {
+        const uint64_t p = __ballot(passes && some), s = __ballot(some);
+        return p ? (int)__builtin_ctzll(p) : s ? 63 - (int)__builtin_clzll(s) : -1;
+    };
+    // The entry of group g at which the running sum, `before` at its start, passes the target.
+    auto search = [&](int g, double before, double target) {
+        const int t0 = g * kGroup + 4 * lane;
+        f32x4 x[1], y = {};
+        wt.load(t0, x[0], y);
+        refused.clear(g, x);
+        double v[4], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[e] = wt.of(x[0][e], y[e]);
+        double run = before + wave_before(sum);
+        int hit = -1, any = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            run += v[e];
+            if (v[e] > 0.0) {
+                any = t0 + e;
+                if (run > target && hit < 0) hit = any;
+            }
+        }
+        const int at = choose(hit >= 0, any >= 0);
+        return at < 0 ? -1 : __builtin_amdgcn_readlane(hit >= 0 ? hit : any, at);
+    };
+
+    // ---- the sums: a run of them a lane
+    const int per = (n_groups + 63) / 64, first = lane * per;
+    constexpr int U = 8;
+    double part = 0.0;
+    for (int k0 = 0; k0 < per; k0 += U) {
+        double v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) v[k] = k0 + k < per && first + k0 + k < n_groups ? sums[first + k0 + k] : 0.0;
+#pragma unroll
+        for (int k = 0; k < U; ++k) part += v[k];
+    }
+    const double before = wave_before(part), total = lane_value(before + part, 63);
+    int token = -1;
+    if (total > 0.0) {
+        const double target = r * total;
+        const int at = choose(before + part > target, part > 0.0);
+        // that lane's run, by all lanes alike
+        const int g1 = at * per;
+        double run = lane_value(before, at), below = run;
+        int group = -1;
+        for (int k = 0; k < per && g1 + k < n_groups; ++k) {
+            const double x = sums[g1 + k];
+            if (x > 0.0) {
+                group = g1 + k;
+                below = run;
+                if (run + x > target) break;  // uniform
+            }
+            run += x;
+        }
+        token = search(group, below, target);
+    } else {
+        // Nothing is left (the drafts had all of p): from p itself, twice through the row.
+        wt.a = 0.0;
+        refused.drop = false;
+        double all = 0.0;
+        for (int g = 0; g < n_groups; ++g) {
+            f32x4 x, y = {};
+            wt.load(g * kGroup + 4 * lane, x, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) all += prob(x[e]);
+        }
+        all = wave_sum(all);
+        const double target = r * all;
+        double run = 0.0;
+        for (int g = 0; all > 0.0 && g < n_groups; ++g) {
+            f32x4 x, y = {};
+            wt.load(g * kGroup + 4 * lane, x, y);
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += prob(x[e]);
+            sum = wave_sum(sum);
+            if (sum > 0.0) token = search(g, run, target);
+            if (run + sum > target) break;  // uniform
+            run += sum;
+        }
+    }
+    return token;
+}
+
+// ---- a request in one workgroup, from its rows to its token
 template <typename T, Drafts D>
+__device__ __forceinline__ void token_here(const VerifyArgs& a, int b, const SpecRows& s, const Rows& rows, const Walk& k,
+                                           double* sums) {
+    constexpr bool Q = D != CHOSEN;
+    constexpr int W = Q ? 4 : 8;  // groups of a wave on the way
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Weights<T, Q> wt = weights_of<T, Q>(a, s.row0 + k.cur, k.a);
+    auto child = [&](int i) { return i > k.cur && i < s.n && rows.up[i < s.n ? i : 0] == k.cur ? rows.tok[i] : -1; };
+    const Refused<decltype(child)> refused{D == CHOSEN && k.children > 0, k.cur, s.n, child};
+    for (int g0 = w * W; g0 < a.n_groups; g0 += 16 * W) {
+        f32x4 x[W], y[W];
+#pragma unroll
+        for (int g = 0; g < W; ++g) wt.load((g0 + g) * kGroup + 4 * lane, x[g], y[g]);
+        weigh<W>(wt, refused, g0, a.n_groups, x, y, sums);
+    }
+    __syncthreads();
+    if (w) return;
+    const int token = find_token(wt, refused, a.n_groups, sums, fmax((double)a.r[b], 0.0));
+    if (lane == 0) a.token[b] = token;
+}
+
+// A workgroup a request: the walk, and where TOKEN what follows from it.
+template <typename T, Drafts D, bool TOKEN>
 __global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
     constexpr int NT = 1024, U = 4;  // fours a thread has on the way
     __shared__ Rows rows;
+    __shared__ double sums[TOKEN ? kOne / kGroup : 1];
     __shared__ double ex[NT / 64];
     __shared__ float ex_x[NT / 64];
     __shared__ int ex_t[NT / 64];
@@ -302,33 +509,13 @@ __global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
     };
     const Walk w = walk<D>(s, rows, a.path + (size_t)b * a.max_new, mass, best_of);
     write_walk<D, NT>(a, b, s, w);
+    if constexpr (TOKEN)
+        if (s.n) token_here<T, D>(a, b, s, rows, w, sums);  // uniform
 }
 
-// ---- the last row's weights
+// ---- the last row's weights and the token, where a workgroup of the request would
+// take too long
 //
-// Weights behind the walk: (p - a q)+, or p, of which the tokens of refused children
-// are taken by their readers.
-template <typename T, bool Q>
-struct Weights {
-    const T* p;
-    const T* q;
-    double a;
-    int vocab;
-    __device__ __forceinline__ void load(int t, f32x4& x, f32x4& y) const {
-        x = four_of(p, t, vocab, 0.f);
-        if (Q) y = four_of(q, t, vocab, 0.f);
-    }
-    __device__ __forceinline__ double of(float x, float y) const {
-        return Q ? fmax(prob(x) - a * prob(y), 0.0) : prob(x);
-    }
-};
-template <typename T, bool Q>
-__device__ __forceinline__ Weights<T, Q> weights_of(const VerifyArgs& a, int row, double c) {
-    // (behind a leaf a is 0 and q says nothing: p is read in its place)
-    const T* const p = static_cast<const T*>(a.p) + (size_t)row * a.p_stride;
-    return Weights<T, Q>{p, Q && c != 0.0 ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride : p, c, a.vocab};
-}
-
 // WALK: the workgroup walks for itself (CHOSEN, CHAIN); else the walk is there.
 template <typename T, Drafts D>
 __global__ __launch_bounds__(256) void spec_weigh_kernel(VerifyArgs a) {
@@ -338,7 +525,7 @@ __global__ __launch_bounds__(256) void spec_weigh_kernel(VerifyArgs a) {
     const int b = blockIdx.x / a.n_blocks, block = blockIdx.x % a.n_blocks;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Last l;
-    SpecRows s;
+    SpecRows s{0, 0};
     if constexpr (WALK) {
         s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
         load_rows<T, D, 256>(a, s, rows);
@@ -355,160 +542,42 @@ __global__ __launch_bounds__(256) void spec_weigh_kernel(VerifyArgs a) {
     f32x4 x[W], y[W];
 #pragma unroll
     for (int g = 0; g < W; ++g) wt.load((g0 + g) * kGroup + 4 * lane, x[g], y[g]);
-    if constexpr (D == CHOSEN) {
-        if (l.children)
-            for (int c0 = (l.at + 1) & ~63; c0 < s.n; c0 += 64) {
-                const int k = c0 + lane, j = k < s.n ? k : 0;
-                const bool mine = k > l.at && k < s.n && rows.up[j] == l.at;
-                const int t = mine ? rows.tok[j] : -1;
-                for (uint64_t left = __ballot(t >= g0 * kGroup && t < (g0 + W) * kGroup); left; left &= left - 1) {
-                    const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(left)) - g0 * kGroup;
-#pragma unroll
-                    for (int g = 0; g < W; ++g)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (at == g * kGroup + 4 * lane + e) x[g][e] = 0.f;
-                }
-            }
-    }
-    double sum[W];
-#pragma unroll
-    for (int g = 0; g < W; ++g) {
-        sum[g] = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[g] += wt.of(x[g][e], Q ? y[g][e] : 0.f);
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1)
-#pragma unroll
-        for (int g = 0; g < W; ++g) sum[g] += __shfl_xor(sum[g], m, 64);
-    if (lane < W && g0 + lane < a.n_groups) {
-        double x0 = sum[0];
-#pragma unroll
-        for (int g = 1; g < W; ++g) x0 = lane == g ? sum[g] : x0;
-        a.sums[(size_t)b * a.n_groups + g0 + lane] = x0;
-    }
+    auto child = [&](int i) {
+        if constexpr (WALK) return i > l.at && i < s.n && rows.up[i < s.n ? i : 0] == l.at ? rows.tok[i] : -1;
+        else return -1;
+    };
+    const Refused<decltype(child)> refused{D == CHOSEN && l.children > 0, l.at, s.n, child};
+    weigh<W>(wt, refused, g0, a.n_groups, x, y, a.sums + (size_t)b * a.n_groups);
 }
 
 // The token: a wave a request.
 template <typename T, Drafts D>
 __global__ __launch_bounds__(64) void spec_find_kernel(VerifyArgs a) {
     constexpr bool Q = D != CHOSEN;
-    const int b = blockIdx.x, lane = threadIdx.x;
+    const int b = blockIdx.x;
     const Last l = a.last[b];
     if (l.row < 0) return;
-    const double* const sums = a.sums + (size_t)b * a.n_groups;
-    const double r = fmax((double)a.r[b], 0.0);
-    Weights<T, Q> wt = weights_of<T, Q>(a, l.row, l.a);
-    bool drop = D == CHOSEN && l.children > 0;
-
-    // Of 64 lanes' values, those of which `some` count: the first whose running sum
-    // passes the target, or else the last that counts, or else -1.
-    auto choose = [&](bool passes, bool some) {
-        const uint64_t p = __ballot(passes && some), s = __ballot(some);
-        return p ? (int)__builtin_ctzll(p) : s ? 63 - (int)__builtin_clzll(s) : -1;
-    };
-    // The entry of group g at which the running sum, `before` at its start, passes the target.
-    auto search = [&](int g, double before, double target) {
-        const int t0 = g * kGroup + 4 * lane;
-        f32x4 x, y = {};
-        wt.load(t0, x, y);
-        if (drop) {
-            const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
-            for (int c0 = l.at + 1; c0 < s.n; c0 += 64) {
-                const int k = c0 + lane;
-                const bool mine = k < s.n && parent_of(a, s.row0, k) == l.at;
-                const int t = mine ? a.tokens[s.row0 + k] : -1;
-                for (uint64_t left = __ballot(t >= g * kGroup && t < (g + 1) * kGroup); left; left &= left - 1) {
-                    const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(left));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at == t0 + e) x[e] = 0.f;
-                }
-            }
-        }
-        double v[4], sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += v[e] = wt.of(x[e], y[e]);
-        double run = before + wave_before(sum);
-        int hit = -1, any = -1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            run += v[e];
-            if (v[e] > 0.0) {
-                any = t0 + e;
-                if (run > target && hit < 0) hit = any;
-            }
-        }
-        const int at = choose(hit >= 0, any >= 0);
-        return at < 0 ? -1 : __builtin_amdgcn_readlane(hit >= 0 ? hit : any, at);
-    };
-
-    // ---- the sums: a run of them a lane
-    const int per = (a.n_groups + 63) / 64, first = lane * per;
-    constexpr int U = 8;
-    double part = 0.0;
-    for (int k0 = 0; k0 < per; k0 += U) {
-        double v[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) v[k] = k0 + k < per && first + k0 + k < a.n_groups ? sums[first + k0 + k] : 0.0;
-#pragma unroll
-        for (int k = 0; k < U; ++k) part += v[k];
-    }
-    const double before = wave_before(part), total = lane_value(before + part, 63);
-    int token = -1;
-    if (total > 0.0) {
-        const double target = r * total;
-        const int at = choose(before + part > target, part > 0.0);
-        // that lane's run, by all lanes alike
-        const int g1 = at * per;
-        double run = lane_value(before, at), below = run;
-        int group = -1;
-        for (int k = 0; k < per && g1 + k < a.n_groups; ++k) {
-            const double x = sums[g1 + k];
-            if (x > 0.0) {
-                group = g1 + k;
-                below = run;
-                if (run + x > target) break;  // uniform
-            }
-            run += x;
-        }
-        token = search(group, below, target);
-    } else {
-        // Nothing is left (the drafts had all of p): from p itself, twice through the row.
-        wt.a = 0.0;
-        drop = false;
-        double all = 0.0;
-        for (int g = 0; g < a.n_groups; ++g) {
-            f32x4 x, y = {};
-            wt.load(g * kGroup + 4 * lane, x, y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) all += prob(x[e]);
-        }
-        all = wave_sum(all);
-        const double target = r * all;
-        double run = 0.0;
-        for (int g = 0; all > 0.0 && g < a.n_groups; ++g) {
-            f32x4 x, y = {};
-            wt.load(g * kGroup + 4 * lane, x, y);
-            double sum = 0.0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum += prob(x[e]);
-            sum = wave_sum(sum);
-            if (sum > 0.0) token = search(g, run, target);
-            if (run + sum > target) break;  // uniform
-            run += sum;
-        }
-    }
-    if (lane == 0) a.token[b] = token;
+    const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
+    auto child = [&](int k) { return k > l.at && k < s.n && parent_of(a, s.row0, k) == l.at ? a.tokens[s.row0 + k] : -1; };
+    const Refused<decltype(child)> refused{D == CHOSEN && l.children > 0, l.at, s.n, child};
+    const int token = find_token(weights_of<T, Q>(a, l.row, l.a), refused, a.n_groups, a.sums + (size_t)b * a.n_groups,
+                                 fmax((double)a.r[b], 0.0));
+    if (threadIdx.x == 0) a.token[b] = token;
 }
 
 // ------------------------------------------------------------------- host --
 static size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 static int groups_of(const lmxs_verify_desc* d) { return (int)((d->vocab + kGroup - 1) / kGroup); }
 static int blocks_of(const lmxs_verify_desc* d) { return (groups_of(d) + kGroups - 1) / kGroups; }
+// One launch, a workgroup a request, or two and three with many, us (a step's calls
+// from a graph; from the host, which then waits for no launch): 16 requests of 32 rows
+// and 32000 entries, chosen drafts 7.8 and 7.9 (9.0 and 11.1 from the host), sampled
+// chains 12.9 and 10.2 (12.9 and 11.2; one request 9.8 and 7.2, 9.9 and 11.3), sampled
+// trees 21.3 and 21.4; 65536 entries 10.2 and 8.2, 15.3 and 8.9, 19.4 and 15.4; 4096
+// entries 6.5 and 7.8, 7.3 and 8.5, 14.9 and 18.4.
+static bool one_workgroup(const lmxs_verify_desc* d) { return d->vocab <= kOne; }
 size_t spec_verify_workspace(const lmxs_verify_desc* d) {
-    if (d->greedy) return 0;
+    if (d->greedy || one_workgroup(d)) return 0;
     return align16((size_t)d->n_seq * groups_of(d) * sizeof(double)) + align16(d->n_seq * sizeof(Last));
 }
 // A launch names its workgroups' threads in 32 bits.
@@ -517,8 +586,13 @@ bool spec_verify_fits(const lmxs_verify_desc* d) { return (uint64_t)d->n_seq * b
 template <typename T, Drafts D>
 static void launch(const VerifyArgs& a, hipStream_t st) {
     const dim3 seqs((unsigned)a.n_seq), blocks((unsigned)(a.n_seq * a.n_blocks));
+    if constexpr (D != GREEDY)
+        if (!a.last) {
+            hipLaunchKernelGGL((spec_walk_kernel<T, D, true>), seqs, dim3(1024), 0, st, a);
+            return;
+        }
     if constexpr (D == SAMPLED || D == GREEDY)
-        hipLaunchKernelGGL((spec_walk_kernel<T, D>), seqs, dim3(1024), 0, st, a);
+        hipLaunchKernelGGL((spec_walk_kernel<T, D, false>), seqs, dim3(1024), 0, st, a);
     if constexpr (D != GREEDY) {
         hipLaunchKernelGGL((spec_weigh_kernel<T, D>), blocks, dim3(256), 0, st, a);
         hipLaunchKernelGGL((spec_find_kernel<T, D>), seqs, dim3(64), 0, st, a);
@@ -555,8 +629,10 @@ lmx_status spec_verify(const lmxs_verify_desc* d, const int32_t* cu, const int32
     a.accepted = accepted;
     a.token = token;
     a.lens = lens;
-    a.sums = static_cast<double*>(ws);
-    a.last = reinterpret_cast<Last*>(static_cast<char*>(ws) + align16((size_t)d->n_seq * a.n_groups * sizeof(double)));
+    if (spec_verify_workspace(d)) {
+        a.sums = static_cast<double*>(ws);
+        a.last = reinterpret_cast<Last*>(static_cast<char*>(ws) + align16((size_t)d->n_seq * a.n_groups * sizeof(double)));
+    }
     (void)hipGetLastError();
     if (dt == LMX_F32) launch_by<float>(a, d->greedy != 0, st);
     else launch_by<f16>(a, d->greedy != 0, st);

@@ -449,10 +449,11 @@ class Verified(_Held):
     @classmethod
     def empty(cls, n_seq: int, max_new: int, device, stream=None) -> "Verified":
         """Tensors for a verification to write."""
-        i32 = _torch().int32
-        path = _new_out((n_seq, max_new), i32, device, stream)
-        return cls._made(path.device, path.get_device(), path, _new_out((n_seq,), i32, device, stream),
-                         _new_out((n_seq,), i32, device, stream))
+        rows = n_seq * max_new
+        # (one allocation and its parts: 3.5 us, three of them 5.9)
+        path, accepted, token = _new_out((rows + 2 * n_seq,), _torch().int32, device, stream).split_with_sizes(
+            (rows, n_seq, n_seq))
+        return cls._made(path.device, path.get_device(), path.view(n_seq, max_new), accepted, token)
 
 
 @functools.lru_cache(maxsize=256)

@@ -482,7 +482,8 @@ def check_verify(c, *, greedy=False, views=False, ws=None):
 
 
 @pytest.mark.parametrize("new,vocab", [([1], 1), ([5], 7), ([4, 0, 9, 1], 31), ([33, 64, 2], 4096), ([70, 3], 4097),
-                                       ([6] * 40, 100), ([8, 5], 20011), ([12], 131072)])
+                                       ([6] * 40, 100), ([8, 5], 20011), ([12], 131072),
+                                       ([3, 0, 9], 32768), ([33, 1, 20], 32769), ([4] * 20, 40000)])
 @pytest.mark.parametrize("kind", ["chain", "tree"])
 @pytest.mark.parametrize("drafts", ["best", "sampled"])
 @pytest.mark.parametrize("dt", [np.float32, np.float16])
@@ -496,23 +497,25 @@ def test_verify(new, vocab, kind, drafts, dt):
 
 
 @pytest.mark.parametrize("drafts", ["best", "sampled"])
-def test_verify_siblings(drafts):
+@pytest.mark.parametrize("vocab", [50, 33000])  # one workgroup a request, and many
+def test_verify_siblings(drafts, vocab):
     """All rows are children of the root: refusals one after another, tokens that come
     twice, tokens that are none, draws of 0 and just below 1."""
     for seed in range(6):
-        c = verify_case(seed, [40, 1000, 3], 50, "tree", drafts)
+        c = verify_case(seed, [40, 1000 if vocab == 50 else 70, 3], vocab, "tree", drafts)
         c["trees"] = [np.array([-1] + [0] * (n - 1)) for n in c["new"]]
         c["u"][:] = np.where(np.random.default_rng(seed).random(c["u"].shape) < 0.9, np.float32(1 - 2 ** -24), 0.3)
         c["tok"][::7] = -1
-        c["tok"][3::11] = 50
+        c["tok"][3::11] = vocab
         c["tok"][5::13] = 1 << 30
         c["r"][:] = [0, 1 - 2 ** -24, 0.5]
         check_verify(c)
 
 
-def test_verify_of_rows_with_nothing_left():
+@pytest.mark.parametrize("vocab", [9000, 40000])
+def test_verify_of_rows_with_nothing_left(vocab):
     """Refused drafts that had all of p, rows of zeros, negative, infinite and NaN entries."""
-    c = verify_case(3, [4, 3, 2, 2, 3], 9000, "tree", "best")
+    c = verify_case(3, [4, 3, 2, 2, 3], vocab, "tree", "best")
     c["trees"] = [np.array([-1] + [0] * (n - 1)) for n in c["new"]]
     p = c["p"]
     p[:] = 0
@@ -548,9 +551,10 @@ def test_verify_greedy_of_logits():
     assert accepted.tolist()[0] >= 2 and token[1] == -1 and accepted[1] == 1 and accepted[2] >= 2
 
 
-def test_verify_of_rows_out_of_range():
+@pytest.mark.parametrize("vocab", [100, 40000])
+def test_verify_of_rows_out_of_range(vocab):
     """Offsets that name rows beyond the batch, and more rows than max_new: in bounds."""
-    c = verify_case(5, [4, 4], 100, "chain", "best")
+    c = verify_case(5, [4, 4], vocab, "chain", "best")
     out = lmx.spec_verify(gpu(c["p"]), gpu(c["tok"]), gpu(c["u"]), gpu(c["r"]), ints([-3, 1 << 30, 2]), max_new=2)
     assert out.path.shape == (2, 2) and out.accepted.tolist()[1] == 0
 
@@ -911,9 +915,9 @@ def test_distributions_beyond_32_bits_of_offset():
 class Captured:
     """Every call of a step, with inputs that `fill` changes and outputs of its own."""
 
-    def __init__(self, drafts, ws):
+    def __init__(self, drafts, ws, vocab=5000):
         self.c = po.PagedCase(60, new=[20, 3, 9], ctx=[900, 70, 9], page=16, kv=2, hd=128, store="i8", pad=4, spare=60)
-        c, vocab = self.c, 5000
+        c = self.c
         self.cache, _ = on_gpu(c)
         self.kept = [x.clone() for x in (self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale)]
         table = np.full((3, 80), -1)
@@ -989,12 +993,13 @@ class Captured:
         return all(torch.equal(x, y) for x, y in zip(self.results(), want))
 
 
-def test_graphs_that_share_a_workspace_replay_as_eager_steps():
+@pytest.mark.parametrize("vocab", [5000, 40000])
+def test_graphs_that_share_a_workspace_replay_as_eager_steps(vocab):
     """Three graphs, of drafts of each kind, over one workspace; eager steps of another
     program in between."""
     ws = lmx.Workspace(1 << 24)
-    steps = {d: Captured(d, ws) for d in ("sampled", "best", "greedy")}
-    other = Captured("sampled", None)
+    steps = {d: Captured(d, ws, vocab) for d in ("sampled", "best", "greedy")}
+    other = Captured("sampled", None, vocab)
     for s in steps.values():
         s.capture()
     for seed in range(6):
@@ -1017,7 +1022,7 @@ def test_graphs_that_share_a_workspace_replay_as_eager_steps():
 
 def test_steps_on_two_streams_at_once():
     """Each with its own tables, cache and workspace."""
-    steps = [Captured("sampled", lmx.Workspace(1 << 24)), Captured("best", None)]
+    steps = [Captured("sampled", lmx.Workspace(1 << 24), 40000), Captured("best", None)]
     wants = []
     for i, s in enumerate(steps):
         s.fill(i)

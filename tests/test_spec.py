@@ -198,10 +198,11 @@ def verify(cu=FAKE, tokens=FAKE + BIG, parent=FAKE + 2 * BIG, p=FAKE + 3 * BIG, 
     (dict(dt=3), S.E_UNSUPPORTED), (dict(n_seq=0), S.E_SHAPE), (dict(n_tokens=0), S.E_SHAPE), (dict(max_new=0), S.E_SHAPE),
     (dict(max_new=41), S.E_SHAPE), (dict(n_tokens=5000, max_new=1025), S.E_SHAPE), (dict(vocab=0), S.E_SHAPE),
     (dict(vocab=(1 << 24) + 1), S.E_SHAPE), (dict(p_stride=999), S.E_SHAPE), (dict(q_stride=1), S.E_SHAPE),
-    (dict(greedy=2), S.E_SHAPE), (dict(n_seq=1 << 20, vocab=1 << 20), S.E_SHAPE), (dict(ws=None), S.E_WORKSPACE),
-    (dict(ws_bytes=100), S.E_WORKSPACE), (dict(ws=FAKE + 11 * BIG + 8), S.E_ALIGN), (dict(p=FAKE + 3 * BIG + 2), S.E_ALIGN),
+    (dict(greedy=2), S.E_SHAPE), (dict(n_seq=1 << 20, vocab=1 << 20), S.E_SHAPE),
+    (dict(ws=None, vocab=40000), S.E_WORKSPACE), (dict(ws_bytes=100, vocab=40000), S.E_WORKSPACE),
+    (dict(ws=FAKE + 11 * BIG + 8, vocab=40000), S.E_ALIGN), (dict(p=FAKE + 3 * BIG + 2), S.E_ALIGN),
     (dict(lens=FAKE + 3), S.E_ALIGN), (dict(path=FAKE + 5 * BIG), S.E_SHAPE), (dict(lens=FAKE + 8 * BIG), S.E_SHAPE),
-    (dict(token=FAKE + 3 * BIG + 159996), S.E_SHAPE), (dict(ws=FAKE + 9 * BIG), S.E_SHAPE),
+    (dict(token=FAKE + 3 * BIG + 159996), S.E_SHAPE), (dict(ws=FAKE + 9 * BIG, vocab=40000), S.E_SHAPE),
 ])
 def test_bad_verifications_are_refused(kw, code):
     assert verify(**kw) == code
@@ -240,7 +241,8 @@ def test_verification_workspace():
         d.update(kw)
         return spec.spec_lib().lmxs_verify_workspace_bytes(ctypes.byref(spec.SpecVerifyDesc(**d)))
     assert need(greedy=1) == 0 and need(vocab=0) == 0
-    assert 0 < need() <= need(vocab=100000) <= need(vocab=100000, n_seq=8)
+    assert need() == need(vocab=32768) == 0  # one workgroup a request
+    assert 0 < need(vocab=32769) <= need(vocab=100000) <= need(vocab=100000, n_seq=8)
 
 
 # -------------------------------------------------------------- the oracle --
