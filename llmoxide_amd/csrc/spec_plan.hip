@@ -8,8 +8,8 @@
 // it is of; the order of everything is that of the sums, none of arrivals.
 //
 // Bound by latency: a step's entries and rows are a few KB, read once through
-// four dependent steps (lengths, sums, free list, table).  Eight requests of 64 rows
-// 6.5 us; with the launch and the host 19 us, a plan and its trees 23.
+// four dependent steps (lengths, sums, free list, table).  Sixteen requests of 32
+// rows 6.6 us, 64 requests with 10500 rows 6.7 and 2.5 for the map.
 #include "spec.hpp"
 
 namespace lmx {
@@ -255,7 +255,7 @@ lmx_status spec_plan(const lmxs_plan_desc* d, const int32_t* lens, const int32_t
 // on: at most 15 more steps, whatever the depth (1024 rows in a chain 26 us,
 // eight trees of 1024 13; with a walk up to the root for each word 2940 and 444).
 //
-// Bound by latency: eight trees of 64 rows 3.4 us, 4 KB.
+// Bound by latency: sixteen trees of 32 rows 3.4 us, 8 KB.
 struct Above {
     int next, n;    // the row's first ancestor in an earlier word (-1: none); bits set
     uint64_t bits;  // the row and its ancestors in its own word
