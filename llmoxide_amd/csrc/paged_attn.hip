@@ -137,7 +137,16 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     constexpr int OP = HD + 4;  // floats a row of the exchange (16-byte rows, rows 4 banks apart)
     constexpr size_t kEx = 512 + 4 * 16 * OP * 4, kQ = QLDS ? (F32 ? 2 : 1) * KS * 64 * 16 : 0;
     __shared__ __align__(16) char smem[kEx > kQ ? kEx : kQ];
-    __shared__ __align__(16) float scales[I8 ? 4 : 1][2][64];  // a wave's: K's, log2 of V's
+    // By masks, f16 q and out have one part of the weights, as in the chunk kernel (a
+    // result's error against 64 bits is 2.2e-4 of itself with one, 2.1e-4 with two):
+    // a third of the products and 48 of a tile's 700 operations.
+    constexpr bool TWO = F32 || !SEEN;
+    // By masks, 8 bits: one exponential a key, exp2(score - m), is the sum's, and times
+    // V's scale the weight.  Scales of 2^-90 to 2^100 keep both in range as above.  Both
+    // together: 32 sequences of 4 to 64 rows 79 -> 74 us a kernel; eight of 512 dims, whose
+    // registers then suffice, 150 -> 74 us a call, f16 pages 211 -> 97.
+    constexpr bool LEAN = I8 && SEEN;
+    __shared__ __align__(16) float scales[I8 ? 4 : 1][LEAN ? 3 : 2][64];  // a wave's: K's, log2 of V's, LEAN: V's
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
 
@@ -263,8 +272,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     auto step = [&](int t0, int t1) {
         // ---- 8-bit scales: a lane prepares one key's, all read theirs back (wave's own LDS)
         if constexpr (I8) {
-            scales[w][0][lane] = t.ks;
+            scales[w][0][lane] = LEAN && !F32 ? t.ks * a.c : t.ks;
             scales[w][1][lane] = log_v_scale(t.vs);
+            if constexpr (LEAN) scales[w][2][lane] = least_v_scale(t.vs);
             wave_lds_order();
         }
         auto scale4 = [&](int what, int j) {  // of the lane's keys in block j
@@ -272,6 +282,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         };
         // ---- scores
         f32x4 s[T::NB];
+        f32x4 lv[LEAN ? T::NB : 1], vs[LEAN ? T::NB : 1];  // of the lane's keys: log2 of V's scale, and the scale
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
             s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -297,7 +308,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             if constexpr (F32 && !I8)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[j][i] += second_part(s[j][i], sl[i]);
-            if constexpr (I8) {
+            if constexpr (LEAN) {
+                s[j] *= scale4(0, j);
+                if constexpr (F32) s[j] *= qscale;
+                lv[j] = scale4(1, j);
+                vs[j] = scale4(2, j);
+            } else if constexpr (I8) {
                 const f32x4 ks = scale4(0, j), lv = scale4(1, j);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[j][i] = fmaf(s[j][i] * ks[i], qscale, lv[i]);
@@ -335,14 +351,17 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             for (int j = 0; j < T::NB; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (!(seen >> (4 * j + i) & 1)) s[j][i] = -INFINITY;
+                    if (!(seen >> (4 * j + i) & 1)) {
+                        s[j][i] = -INFINITY;
+                        if constexpr (LEAN) lv[j][i] = vs[j][i] = 0.f;  // whatever the slot holds
+                    }
         }
         // ---- the reference
-        float top = s[0][0];
+        float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < T::NB; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, LEAN ? s[j][i] + lv[j][i] : s[j][i]);
         if (__ballot(top > m + (kSlack + kLift))) {  // m = -inf: any score
             top = max_groups(top);
             float mn = m;
@@ -355,22 +374,24 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         }
         // ---- weights
         const float ms = m == -INFINITY ? 0.f : m;
-        f16x8 ph[T::NB / 2], pl[T::NB / 2];
+        f16x8 ph[T::NB / 2], pl[TWO ? T::NB / 2 : 1];
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
-            f32x4 lv;
-            if constexpr (I8) lv = scale4(1, j);
+            f32x4 log_v;
+            if constexpr (I8 && !LEAN) log_v = scale4(1, j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = s[j][i] - ms, p = fast_exp2(x);
-                if constexpr (I8)
-                    sum += seen >> (4 * j + i) & 1 ? fast_exp2(x - lv[i]) : 0.f;
+                const float x = s[j][i] - ms;
+                float p = fast_exp2(x);
+                if constexpr (I8 && !LEAN)
+                    sum += seen >> (4 * j + i) & 1 ? fast_exp2(x - log_v[i]) : 0.f;
                 else
                     sum += p;
+                if constexpr (LEAN) p *= vs[j][i];
                 const int at = 4 * (j & 1) + i;
                 ph[j >> 1][at] = (f16)p;
-                pl[j >> 1][at] = (f16)(p - (float)(f16)p);
+                if constexpr (TWO) pl[j >> 1][at] = (f16)(p - (float)(f16)p);
             }
         }
         if constexpr (I8) wave_lds_order();  // the next tile's scales go where these were
@@ -401,12 +422,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 for (int e = 0; e < 2; ++e) {
                     const f16x8 vf = e ? i8x8_to_f16(t.v[d].z, t.v[d].w) : i8x8_to_f16(t.v[d].x, t.v[d].y);
                     o[d] = mfma16(vf, ph[e], o[d]);
-                    o[d] = mfma16(vf, pl[e], o[d]);
+                    if constexpr (TWO) o[d] = mfma16(vf, pl[e], o[d]);
                 }
             } else {
                 const f16x8 vf = __builtin_bit_cast(f16x8, t.v[d]);
                 o[d] = mfma16(vf, ph[0], o[d]);
-                o[d] = mfma16(vf, pl[0], o[d]);
+                if constexpr (TWO) o[d] = mfma16(vf, pl[0], o[d]);
             }
         }
         load_v<HD, I8>(a, next, it.h, t1, t);
@@ -850,21 +871,22 @@ static size_t most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
 //
 // Query rows a sequence may have per kv head for the rows kernel.  Eight sequences
 // of 2000-8000 positions, 16 heads on 4, us on the rows and on the chunk kernel:
-//   128 dims  f16            16 rows  31 and 31, 20 rows  49 and 32, 32 rows  50 and 31
-//             f16, f32 q.    16 rows  31 and 37, 20 rows  51 and 38
-//             8 bits         48 rows  38 and 40, 64 rows  42 and 40 (32 sequences of up to 64: 84 and 117)
-//             8 bits, f32 q. 64 rows  45 and 53, 96 rows  60 and 55
-//   64 dims   f16            16 rows  19 and 22, 20 rows  27 and 21;  f32 q.  19 and 27, 28 and 27
-//             8 bits         64 rows  29 and 31, 96 rows  36 and 31;  f32 q.  31 and 37, 38 and 38
-//   256 dims  f16            16 rows  64 and 59, 20 rows  96 and 63;  f32 q.  68 and 80, 98 and 82
-//             8 bits         96 rows 106 and 124, 128 rows 127 and 125
-//             8 bits, f32 q. 64 rows 104 and 101
-//   512 dims  f16             4 rows 211 and 114 (one sequence 56 and 71);  f32 q. 258 and 132 (67 and 89)
-//             8 bits          4 rows 150 and 104 (45 and 78);  f32 q. 16 rows 161 and 212, 20 rows 303 and 214
+//   128 dims  f16            16 rows  30 and 30, 20 rows  49 and 33 (f32 q. 31 and 37, 51 and 38)
+//             8 bits         64 rows  40 and 41, 80 rows  41 and 42, 96 rows  52 and 42
+//             8 bits, f32 q. 64 rows  46 and 53, 80 rows  44 and 55, 96 rows  55 and 55
+//             8 bits, 32 sequences of 4 to 64 rows and 16 to 8192 positions  79 and 117
+//   64 dims   f16            16 rows  18 and 22, 20 rows  27 and 21
+//             8 bits         64 rows  27 and 31, 80 rows  28 and 31, 96 rows  34 and 32 (f32 q. 32 and 38, 40 and 38)
+//   256 dims  f16            16 rows  64 and 59, 20 rows 102 and 64 (f32 q. 68 and 80, 98 and 82)
+//             8 bits         64 rows  77 and 121, 96 rows 95 and 124, 128 rows 108 and 126
+//             8 bits, f32 q. 64 rows  94 and 99, 96 rows 115 and 102
+//   512 dims  f16             4 rows  97 and 86, 16 rows 101 and 73; one sequence 54 and 71, 56 and 59
+//             8 bits          4 rows  74 and 80, 16 rows  79 and 68; one sequence 49 and 76, 52 and 64
+//             8 bits, f32 q. 16 rows 161 and 212
 constexpr int seen_most(int hd, bool i8, bool f32, int n_seq) {
-    if (hd == 512) return n_seq > 1 && !(i8 && f32) ? 0 : kBM;
+    if (hd == 512) return n_seq == 1 || (i8 && f32) ? kBM : i8 ? kBM / 2 : 0;
     if (!i8) return kBM;
-    return hd == 256 && !f32 ? 96 : 64;
+    return hd <= 128 ? 80 : f32 ? 64 : 128;
 }
 // 64-key units a split has at least where the work is short: one sequence of 6 rows
 // (16 heads on 8, f32) on 518, 2048, 8192 and 32768 keys, splits of 2 units 12.0,

@@ -209,7 +209,8 @@ __device__ __forceinline__ float second_part(float hi, float lo) { return fabsf(
 //
 // log2 of a V scale, of 2^-90 at least: finite, and values below 1e-24 are all
 // that notices.
-__device__ __forceinline__ float log_v_scale(float s) { return __builtin_amdgcn_logf(s < 0x1p-90f ? 0x1p-90f : s); }
+__device__ __forceinline__ float least_v_scale(float s) { return s < 0x1p-90f ? 0x1p-90f : s; }
+__device__ __forceinline__ float log_v_scale(float s) { return __builtin_amdgcn_logf(least_v_scale(s)); }
 // The weight of a partial output in a join, d below the highest reference.  Never
 // 0, which would make NaN of an infinity among V: 2^-126 of a finite output is
 // far below the last place of the weights beside it.

@@ -387,9 +387,8 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
     before its request's rows (with ``window`` > 0 those above its ``pos`` less the
     window) and the request's rows whose bits are set in its ``seen`` int64
     [n_tokens, words]; one that sees nothing gets zeros.  Types and workspaces are
-    ``paged_attention``'s, and its precision, but that with f16 ``q`` the weights have
-    11 bits where the batch's max_new * heads / kv heads is above 16 (f16 pages) or 64
-    (8 bits; 96 at 256 dims), and at 512 dims in every batch of several requests."""
+    ``paged_attention``'s, and its precision, but that with f16 ``q`` the softmax's
+    weights always have 11 bits."""
     hd = cache.head_dim
     head = q_head_stride or hd
     width = q.shape[-1] if q.dim() == 2 else -1
