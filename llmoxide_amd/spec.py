@@ -34,7 +34,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import NamedTuple, Optional, Sequence
+from typing import Optional, Sequence
 
 from . import F32, Workspace, _check, _need_cuda, _ptr, _stream, _torch, lib
 from . import paged as _paged
@@ -112,18 +112,13 @@ def _ints(what: str, t, size, at: int) -> None:
         raise ValueError(f"{what} has {size} elements, not {t.numel()}")
 
 
-class _At(NamedTuple):
-    """What _place looks at of a cache and a batch."""
-    device: object
-
-
-_at = functools.lru_cache(maxsize=64)(_At)
-
-
-def _here(device, *ts, stream=None, workspace=None) -> None:
-    """Tensors, stream and workspace of ``device``, which has to be the current one."""
-    at = _at(device)
-    _paged._place(at, at, *ts, stream=stream, workspace=workspace)
+def _fresh(like, shape, stream):
+    """A result allocated here, of ``like``'s type and device (1.1 us; by torch.empty,
+    which is told both, 1.6); one that another stream fills is marked as used there."""
+    out = like.new_empty(shape)
+    if stream is not None and stream != _torch().cuda.current_stream():
+        out.record_stream(stream)
+    return out
 
 
 class _Held:
@@ -240,7 +235,7 @@ def spec_plan(tables: PageTables, lens, new_rows, *, n_tokens: Optional[int] = N
     at = tables.at
     _ints("lens", lens, tables.n_seq, at)
     _ints("new_rows", new_rows, tables.n_seq, at)
-    _here(tables.device, out.cu, stream=stream)
+    _paged._place(tables, out, stream=stream)
     d = _plan_desc(tables.n_seq, n_tokens, tables.page_size, tables.entries, tables.n_pages, 1 if trim else 0)[1]
     _check("lmxs_plan", spec_lib().lmxs_plan(d, lens.data_ptr(), new_rows.data_ptr(), *tables.ptrs, *out.ptrs,
                                              _stream(stream)))
@@ -268,17 +263,16 @@ def spec_tree(parent, batch: PagedBatch, *, window: int = 0, out: Optional[SpecT
     row of the request that each continues (earlier than its own; -1: a root).  With
     ``window`` > 0 ancestors that far behind are not seen.  Rows of no request are
     left as they are."""
-    n_tokens = batch.n_tokens
+    n_tokens, at = batch.n_tokens, batch.device.index
+    _ints("parent", parent, n_tokens, at)
     if out is None:
-        torch = _torch()
         words = -(-batch.max_new // 64)
-        out = SpecTree._made(batch.device, batch.device.index, _new_out((n_tokens,), torch.int32, batch.device, stream),
-                             _new_out((n_tokens, words), torch.int64, batch.device, stream))
+        out = SpecTree._made(batch.device, at, _fresh(parent, n_tokens, stream),
+                             _new_out((n_tokens, words), _torch().int64, batch.device, stream))
         out.words = words
     elif out.pos.numel() != n_tokens:
         raise ValueError("out is of other rows")
-    _ints("parent", parent, n_tokens, out.at)
-    _here(batch.device, parent, stream=stream)
+    _paged._place(batch, out, stream=stream)
     pos, seen = out.ptrs
     _check("lmxs_tree", spec_lib().lmxs_tree(batch.ref, parent.data_ptr(), out.words, window, pos, seen, _stream(stream)))
     return out
@@ -365,7 +359,8 @@ def spec_prologue(q, k, v, cache: PagedCache, batch: PagedBatch, *, n_heads: int
     if pos is not None:
         _ints("pos", pos, batch.n_tokens, cache.at)
     if q_out is None:
-        q_out = _new_out((batch.n_tokens, n_heads * hd), q_dtype or torch.float32, cache.device, stream)
+        shape = batch.n_tokens, n_heads * hd
+        q_out = _fresh(q, shape, stream) if q_dtype is None else _new_out(shape, q_dtype, cache.device, stream)
     elif q_dtype is not None and q_out.dtype != q_dtype:
         raise TypeError("q_dtype differs from q_out's")
     if _rows(q_out, batch.n_tokens, n_heads * hd, "q_out"):
@@ -400,7 +395,7 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
     if pos is not None:
         _ints("pos", pos, batch.n_tokens, cache.at)
     if out is None:
-        out = _new_out((batch.n_tokens, n_heads * hd), q.dtype, cache.device, stream)
+        out = _fresh(q, (batch.n_tokens, n_heads * hd), stream)
     elif out.dtype != q.dtype or _rows(out, batch.n_tokens, n_heads * hd, "out"):
         raise ValueError("out is contiguous and of q's dtype")
     _paged._place(cache, batch, q, seen, out, stream=stream, workspace=workspace)
@@ -448,11 +443,13 @@ class Verified(_Held):
     @classmethod
     def empty(cls, n_seq: int, max_new: int, device, stream=None) -> "Verified":
         """Tensors for a verification to write."""
-        rows = n_seq * max_new
-        # (one allocation and its parts: 3.5 us, three of them 5.9)
-        path, accepted, token = _new_out((rows + 2 * n_seq,), _torch().int32, device, stream).split_with_sizes(
-            (rows, n_seq, n_seq))
-        return cls._made(path.device, path.get_device(), path.view(n_seq, max_new), accepted, token)
+        return cls._parts(_new_out((n_seq * (max_new + 2),), _torch().int32, device, stream), n_seq, max_new)
+
+    @classmethod
+    def _parts(cls, held, n_seq: int, max_new: int) -> "Verified":
+        """The three as parts of one allocation (which takes half the time of three)."""
+        path, accepted, token = held.split_with_sizes((n_seq * max_new, n_seq, n_seq))
+        return cls._made(held.device, held.get_device(), path.view(n_seq, max_new), accepted, token)
 
 
 @functools.lru_cache(maxsize=256)
@@ -495,10 +492,10 @@ def spec_verify(p, tokens, u, r, cu, *, max_new: int, parent=None, q=None, lens=
             if t is None or t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
                 raise ValueError(f"{what} is contiguous float32 [{n}]")
     if out is None:
-        out = Verified.empty(n_seq, max_new, p.device, stream)
+        out = Verified._parts(_fresh(cu, n_seq * (max_new + 2), stream), n_seq, max_new)
     elif out.path.shape != (n_seq, max_new):
         raise ValueError("out is of other requests or rows")
-    _here(p.device, u, r, q, out.path, stream=stream, workspace=workspace)
+    _paged._place(out, out, p, q, u, r, stream=stream, workspace=workspace)
     _, d, need = _verify_desc(n_seq, n_tokens, max_new, vocab, p_stride, q_stride, 1 if greedy else 0)
     ws_ptr, ws_bytes = _space(need, workspace, p.device, stream)
     _check("lmxs_verify", spec_lib().lmxs_verify(

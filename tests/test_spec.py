@@ -401,26 +401,6 @@ def test_calls_take_the_workspace_of_a_larger_batch(hd, seqs, small, store, dt, 
     assert attn(ws_bytes=has, **call) == S.E_ALIGN
 
 
-def test_streams_and_workspaces_of_another_device_are_refused(monkeypatch):
-    """Stand-ins for what two GPUs would give: the check reads nothing but devices."""
-    torch = pytest.importorskip("torch")
-
-    class On:
-        def __init__(self, index):
-            self.device = torch.device("cuda", index)
-            self.device_index = index
-
-        def get_device(self):
-            return self.device.index
-    monkeypatch.setattr(paged, "_current_device", lambda: 0)
-    here, there = On(0), On(1)
-    spec._here(here.device, here, None, stream=here, workspace=lmx.Workspace(device="cuda:0"))
-    for device, ts, kw in ((there.device, (there,), {}), (here.device, (there,), {}), (here.device, (here,), dict(stream=there)),
-                           (here.device, (here,), dict(workspace=lmx.Workspace(device="cuda:1")))):
-        with pytest.raises(ValueError):
-            spec._here(device, *ts, **kw)
-
-
 class Fake:
     """A tensor's looks, of device 0."""
 
@@ -443,6 +423,40 @@ class Fake:
 
     def data_ptr(self):
         return FAKE
+
+    def stride(self):
+        return tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
+
+def test_tensors_and_streams_of_another_device_are_refused(monkeypatch):
+    """Stand-ins for what two GPUs would give: nothing but devices is read before the call."""
+    pytest.importorskip("torch")
+
+    class Stream:
+        def __init__(self, at):
+            self.device_index, self.cuda_stream = at, None
+
+    def plan(at=0, lens=0, out=0, stream=None):
+        tables = spec.PageTables(*[Fake(*s, at=at) for s in ((3, 5), (3,), (9,), (2,))], page_size=16)
+        step = spec.StepPlan(Fake(4, at=out), Fake(3, at=out), None, Fake(7, at=out))
+        return spec.spec_plan(tables, Fake(3, at=lens), Fake(3, at=at), out=step, stream=stream)
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    for kw in (dict(lens=1), dict(out=1), dict(at=1, lens=1, out=1), dict(stream=Stream(1)), dict(lens=-1)):
+        with pytest.raises(ValueError):
+            plan(**kw)
+
+    def verify(cu=0, p=0, u=0, stream=None, workspace=None, out=None):
+        import torch
+        f32 = torch.float32
+        return spec.spec_verify(Fake(7, 30, dtype=f32, at=p), Fake(7, at=p), Fake(7, dtype=f32, at=u), Fake(3, dtype=f32, at=p),
+                                Fake(4, at=cu), max_new=4, out=out, stream=stream, workspace=workspace)
+
+    def held(at):
+        return spec.Verified(Fake(3, 4, at=at), Fake(3, at=at), Fake(3, at=at))
+    for kw in (dict(cu=1, out=held(0)), dict(u=1, out=held(0)), dict(out=held(1)), dict(p=1, cu=1, u=1, out=held(1)),
+               dict(stream=Stream(1), out=held(0)), dict(workspace=lmx.Workspace(device="cuda:1"), out=held(0))):
+        with pytest.raises(ValueError):
+            verify(**kw)
 
 
 def test_python_tables_and_plans_refuse_what_does_not_fit():
