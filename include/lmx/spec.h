@@ -50,7 +50,8 @@ extern "C" {
  *    left out: held[b] says how many entries there are, later positions are in
  *    no page, and the next call tries again.
  * A call that takes pages and one with the lengths before it that trims them
- * leave table and list as they were.
+ * leave table and list as they were.  A page goes back for every entry that names
+ * it: one that requests share has to be in no more than one of the tables by then.
  *   lens, new_rows  device int32 [n_seq]
  *   page_table      int32 [n_seq, table_stride]; what lies from held[b] on is not
  *                   read, and written where the request needs it
