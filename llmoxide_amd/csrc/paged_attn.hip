@@ -891,14 +891,37 @@ constexpr int seen_most(int hd, bool i8, bool f32, int n_seq) {
 // 64-key units a split has at least where the work is short: one sequence of 6 rows
 // (16 heads on 8, f32) on 518, 2048, 8192 and 32768 keys, splits of 2 units 12.0,
 // 13.1, 19.9 and 46.8 us, of 4 units 13.3, 14.6, 17.2 and 37.1, of 8 units 14.6,
-// 18.0, 18.7 and 38.5; so about half of target of them, up to 8 units.  No split of
-// up to 8 units in all: 300 keys of 64 dims 7.9 and 10.7 us, 32 8-bit sequences 9.9
-// and 14.9.  (Even splits: 32 8-bit sequences 92 -> 84 us.)
+// 18.0, 18.7 and 38.5; so about half of target of them, up to 8 units.  (Even
+// splits: 32 8-bit sequences 92 -> 84 us.)
 constexpr int seen_fine(int hd) { return rows_least(hd) / 4; }
-static Part seen_rows_part(const PagedGeom& g, int hd, int most) {
+// Units of the longest sequence up to which nothing is split, and nothing merged, by
+// the sequences times kv heads (`items`) that fill the CUs without.  Not split and
+// split, us, sequences of one length or up to it, 8 heads of 128 dims (4 of the others):
+//   items 256 and more, 128 dims  1000 keys 22 and 28 (8 bits 14 and 23), 2000 keys 44 and
+//                                 47 (21 and 29; one length 26 and 38), 4000 86 and 96 (46 and 58);
+//                                 8192 as uneven 151 and 128, so up to 2048
+//                       256 dims  1000 keys 46 and 55 (23 and 34), 2000 keys 82 and 83 (40 and 55)
+//                       64 dims   1000 keys 13 and 19 (10 and 19), 2000 keys 20 and 23 (14 and 21)
+//   items 128, 128 dims           500 keys 14 and 17 (11 and 14), 1000 keys 21 and 18 (13 and 15)
+//              256 dims           400 keys 21 and 25 (15 and 21), 1000 keys (21 and 33)
+//   items 64,  128 dims           500 keys 13 and 13 (9 and 12), 1000 keys 20 and 15 (13 and 13)
+//              256 dims           400 keys 21 and 20 (15 and 17), 1000 keys 37 and 20 (20 and 17)
+//   items 8    128 dims           300 keys 10.0 and 10.4, 400 keys 11.4 and 10.4 (700 keys 10.2 and
+//                                 10.4, 1000 keys 11.7 and 10.7)
+//              256 dims           200 keys 14.7 and 14.7, 300 keys 17.5 and 14.7 (13.5 and 12.7)
+//              64 dims            500 keys 8.1 and 9.7, 700 keys 9.4 and 9.1 (1000 keys 8.7 and 10.3)
+//   512 dims (8 bits, f32 queries) 1000 keys, items 128 116 and 112
+constexpr int kWholeLeast = 4;
+constexpr int seen_whole(int hd, bool i8, int64_t items) {
+    if (hd == 512) return kWholeLeast;
+    if (items >= 256) return i8 || hd <= 128 ? 32 : 16;
+    if (i8) return hd == 64 ? 16 : hd == 128 ? (items >= 64 ? 16 : 12) : items >= 128 ? 16 : items >= 64 ? 8 : kWholeLeast;
+    return hd == 64 || items >= 128 ? 8 : hd == 128 ? 5 : kWholeLeast;
+}
+static Part seen_rows_part(const PagedGeom& g, int hd, int most, int whole) {
     const int rows = (int)std::min<int64_t>((int64_t)g.max_new * g.G, most);
     const int64_t tiles = std::min<int64_t>(row_tiles_bound(g, kBM), (int64_t)g.n_seq * ((rows + kBM - 1) / kBM));
-    Part r = make_part(g, hd, kBM, tiles, rows, true, rows_target(hd), rows_least(hd));
+    Part r = make_part(g, hd, kBM, tiles, rows, true, rows_target(hd), whole);
     r.least = r.splits ? 1 : r.least;
     r.fine = r.splits ? seen_fine(hd) : 0;
     r.merge = r.splits ? tiles * g.Hkv * ((std::min(kBM, rows) + 3) / 4) : 0;
@@ -915,12 +938,13 @@ static Plan seen_plan(const PagedGeom& g, int hd, bool i8, bool f32) {
     Plan p{};
     const int most = seen_most(hd, i8, f32, g.n_seq);
     if ((int64_t)g.max_new * g.G > most) p.chunk = seen_chunk_part(g, hd, i8, f32);
-    else p.rows = seen_rows_part(g, hd, most);
+    else p.rows = seen_rows_part(g, hd, most, seen_whole(hd, i8, (int64_t)g.n_seq * g.Hkv));
     return p;
 }
-// The most of any smaller geometry, as most_workspace: of few rows, or of chunks.
+// The most of any smaller geometry, as most_workspace: of few rows (split, as fewer
+// sequences may be where these are not), or of chunks.
 static size_t seen_most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
-    size_t bytes = seen_rows_part(g, hd, seen_most(hd, i8, f32, 1)).bytes();
+    size_t bytes = seen_rows_part(g, hd, seen_most(hd, i8, f32, 1), kWholeLeast).bytes();
     if ((int64_t)g.max_new * g.G > seen_most(hd, i8, f32, g.n_seq)) {
         const int cm = chunk_rows(hd, i8, f32), slots = chunk_slots(hd, i8, f32);
         PagedGeom c = g;

@@ -1095,3 +1095,13 @@ def test_what_python_refuses():
         with pytest.raises((TypeError, ValueError, RuntimeError, lmx.LmxError)):
             call()
     assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
+
+
+@pytest.mark.parametrize("store,most", [("f16", 700), ("i8", 700), ("f16", 2048), ("f16", 2049)])
+def test_attention_of_sequences_that_fill_the_cus(store, most):
+    """Enough of them that the shorter are not split, and the first length at which they are."""
+    say("many sequences", store, most)
+    rng = np.random.default_rng(most)
+    ctx = [most] + [int(x) for x in rng.integers(3, most // 8, 63)]
+    c = po.PagedCase(80, new=[1 + i % 3 for i in range(64)], ctx=ctx, page=16, kv=4, hd=64, store=store)
+    check(c, 4, masks(c, 81, "tree"), q16=store == "f16")
