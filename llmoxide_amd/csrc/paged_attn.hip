@@ -899,7 +899,8 @@ constexpr int seen_fine(int hd) { return rows_least(hd) / 4; }
 // split, us, sequences of one length or up to it, 8 heads of 128 dims (4 of the others):
 //   items 256 and more, 128 dims  1000 keys 22 and 28 (8 bits 14 and 23), 2000 keys 44 and
 //                                 47 (21 and 29; one length 26 and 38), 4000 86 and 96 (46 and 58);
-//                                 8192 as uneven 151 and 128, so up to 2048
+//                                 8192 as uneven 151 and 128.  One sequence among empty ones:
+//                                 1000 keys 20 and 12, 2000 keys 34 and 13 (17 and 11), so f16 up to 1024
 //                       256 dims  1000 keys 46 and 55 (23 and 34), 2000 keys 82 and 83 (40 and 55)
 //                       64 dims   1000 keys 13 and 19 (10 and 19), 2000 keys 20 and 23 (14 and 21)
 //   items 128, 128 dims           500 keys 14 and 17 (11 and 14), 1000 keys 21 and 18 (13 and 15)
@@ -914,7 +915,7 @@ constexpr int seen_fine(int hd) { return rows_least(hd) / 4; }
 constexpr int kWholeLeast = 4;
 constexpr int seen_whole(int hd, bool i8, int64_t items) {
     if (hd == 512) return kWholeLeast;
-    if (items >= 256) return i8 || hd <= 128 ? 32 : 16;
+    if (items >= 256) return i8 ? 32 : 16;
     if (i8) return hd == 64 ? 16 : hd == 128 ? (items >= 64 ? 16 : 12) : items >= 128 ? 16 : items >= 64 ? 8 : kWholeLeast;
     return hd == 64 || items >= 128 ? 8 : hd == 128 ? 5 : kWholeLeast;
 }

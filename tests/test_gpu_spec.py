@@ -1097,7 +1097,7 @@ def test_what_python_refuses():
     assert torch.equal(cache.k, before[0]) and torch.equal(cache.v, before[1])
 
 
-@pytest.mark.parametrize("store,most", [("f16", 700), ("i8", 700), ("f16", 2048), ("f16", 2049)])
+@pytest.mark.parametrize("store,most", [("f16", 700), ("i8", 700), ("f16", 1024), ("f16", 1025), ("i8", 2048), ("i8", 2049)])
 def test_attention_of_sequences_that_fill_the_cus(store, most):
     """Enough of them that the shorter are not split, and the first length at which they are."""
     say("many sequences", store, most)
