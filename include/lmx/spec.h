@@ -125,8 +125,8 @@ lmx_status lmxs_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *   seen   uint64 [n_tokens, words], 8-byte aligned; words 1 to 16, 64 * words
  *          at least max_new
  *   pos    int32 [n_tokens]; may be NULL without a window
- * Types, layouts and precision are lmxp_attn's, but that f16 q and out always take
- * weights of 11 bits.  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
+ * Types, layouts and precision are lmxp_attn's, but that f16 q and out always have
+ * weights of 22 bits, as f32 q and out have.  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
  * what serves this batch and every one whose n_seq, n_tokens, max_new and max_ctx
  * are at most its own, for either dt and any window (0 for a description that is
  * refused). */

@@ -137,15 +137,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     constexpr int OP = HD + 4;  // floats a row of the exchange (16-byte rows, rows 4 banks apart)
     constexpr size_t kEx = 512 + 4 * 16 * OP * 4, kQ = QLDS ? (F32 ? 2 : 1) * KS * 64 * 16 : 0;
     __shared__ __align__(16) char smem[kEx > kQ ? kEx : kQ];
-    // By masks, f16 q and out have one part of the weights, as in the chunk kernel (a
-    // result's error against 64 bits is 2.2e-4 of itself with one, 2.1e-4 with two):
-    // a third of the products and 48 of a tile's 700 operations.
-    constexpr bool TWO = F32 || !SEEN;
     // By masks, 8 bits: one exponential a key, exp2(score - m), is the sum's, and times
-    // V's scale the weight.  Scales of 2^-90 to 2^100 keep both in range as above.  Both
-    // together: 32 sequences of 4 to 64 rows 79 -> 74 us a kernel; eight of 512 dims, whose
-    // registers then suffice, 150 -> 74 us a call, f16 pages 211 -> 97.
-    constexpr bool LEAN = I8 && SEEN;
+    // V's scale the weight.  Scales of 2^-90 to 2^100 keep both in range as above.  Eight
+    // sequences of 16 rows, us with one and with two exponentials: 128 dims 42.3 and 43.2,
+    // 256 dims 80.4 and 82.2; 512 dims, where it spills more registers, f32 queries 191 and
+    // 162 (f16 queries 160 and 158).
+    constexpr bool LEAN = I8 && SEEN && HD <= 256;
     __shared__ __align__(16) float scales[I8 ? 4 : 1][LEAN ? 3 : 2][64];  // a wave's: K's, log2 of V's, LEAN: V's
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -374,7 +371,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
         }
         // ---- weights
         const float ms = m == -INFINITY ? 0.f : m;
-        f16x8 ph[T::NB / 2], pl[TWO ? T::NB / 2 : 1];
+        f16x8 ph[T::NB / 2], pl[T::NB / 2];
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
@@ -391,7 +388,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 if constexpr (LEAN) p *= vs[j][i];
                 const int at = 4 * (j & 1) + i;
                 ph[j >> 1][at] = (f16)p;
-                if constexpr (TWO) pl[j >> 1][at] = (f16)(p - (float)(f16)p);
+                pl[j >> 1][at] = (f16)(p - (float)(f16)p);
             }
         }
         if constexpr (I8) wave_lds_order();  // the next tile's scales go where these were
@@ -422,12 +419,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 for (int e = 0; e < 2; ++e) {
                     const f16x8 vf = e ? i8x8_to_f16(t.v[d].z, t.v[d].w) : i8x8_to_f16(t.v[d].x, t.v[d].y);
                     o[d] = mfma16(vf, ph[e], o[d]);
-                    if constexpr (TWO) o[d] = mfma16(vf, pl[e], o[d]);
+                    o[d] = mfma16(vf, pl[e], o[d]);
                 }
             } else {
                 const f16x8 vf = __builtin_bit_cast(f16x8, t.v[d]);
                 o[d] = mfma16(vf, ph[0], o[d]);
-                if constexpr (TWO) o[d] = mfma16(vf, pl[0], o[d]);
+                o[d] = mfma16(vf, pl[0], o[d]);
             }
         }
         load_v<HD, I8>(a, next, it.h, t1, t);
@@ -871,20 +868,20 @@ static size_t most_workspace(const PagedGeom& g, int hd, bool i8, bool f32) {
 //
 // Query rows a sequence may have per kv head for the rows kernel.  Eight sequences
 // of 2000-8000 positions, 16 heads on 4, us on the rows and on the chunk kernel:
-//   128 dims  f16            16 rows  30 and 30, 20 rows  49 and 33 (f32 q. 31 and 37, 51 and 38)
-//             8 bits         64 rows  40 and 41, 80 rows  41 and 42, 96 rows  52 and 42
-//             8 bits, f32 q. 64 rows  46 and 53, 80 rows  44 and 55, 96 rows  55 and 55
-//             8 bits, 32 sequences of 4 to 64 rows and 16 to 8192 positions  79 and 117
-//   64 dims   f16            16 rows  18 and 22, 20 rows  27 and 21
-//             8 bits         64 rows  27 and 31, 80 rows  28 and 31, 96 rows  34 and 32 (f32 q. 32 and 38, 40 and 38)
-//   256 dims  f16            16 rows  64 and 59, 20 rows 102 and 64 (f32 q. 68 and 80, 98 and 82)
-//             8 bits         64 rows  77 and 121, 96 rows 95 and 124, 128 rows 108 and 126
-//             8 bits, f32 q. 64 rows  94 and 99, 96 rows 115 and 102
-//   512 dims  f16             4 rows  97 and 86, 16 rows 101 and 73; one sequence 54 and 71, 56 and 59
-//             8 bits          4 rows  74 and 80, 16 rows  79 and 68; one sequence 49 and 76, 52 and 64
-//             8 bits, f32 q. 16 rows 161 and 212
+//   128 dims  f16            16 rows  30 and 32, 20 rows  49 and 34 (f32 q. 32 and 37, 51 and 38)
+//             8 bits         64 rows  42 and 47, 80 rows  43 and 48, 96 rows  54 and 48
+//             8 bits, f32 q. 64 rows  45 and 53, 80 rows  46 and 55, 96 rows  56 and 55
+//             8 bits, 32 sequences of 4 to 64 rows and 16 to 8192 positions  124 and 163
+//   64 dims   f16            16 rows  18 and 22, 20 rows  27 and 23
+//             8 bits         64 rows  30 and 35, 80 rows  30 and 35, 96 rows  37 and 35 (f32 q. 32 and 38, 40 and 38)
+//   256 dims  f16            16 rows  64 and 67, 20 rows 101 and 71 (f32 q. 68 and 79, 103 and 81)
+//             8 bits         64 rows  80 and 135, 96 rows 99 and 138, 128 rows 114 and 140
+//             8 bits, f32 q. 64 rows  94 and 99, 96 rows 115 and 103
+//   512 dims  f16             4 rows 211 and 117, 16 rows 215 and 111; one sequence 58 and 77, 62 and 65
+//             8 bits          4 rows 151 and 107, 16 rows 157 and 103; one sequence 47 and 81, 50 and 69
+//             8 bits, f32 q.  4 rows 153 and 218, 16 rows 162 and 212
 constexpr int seen_most(int hd, bool i8, bool f32, int n_seq) {
-    if (hd == 512) return n_seq == 1 || (i8 && f32) ? kBM : i8 ? kBM / 2 : 0;
+    if (hd == 512) return n_seq == 1 || (i8 && f32) ? kBM : 0;
     if (!i8) return kBM;
     return hd <= 128 ? 80 : f32 ? 64 : 128;
 }
@@ -895,7 +892,8 @@ constexpr int seen_most(int hd, bool i8, bool f32, int n_seq) {
 // splits: 32 8-bit sequences 92 -> 84 us.)
 constexpr int seen_fine(int hd) { return rows_least(hd) / 4; }
 // Units of the longest sequence up to which nothing is split, and nothing merged, by
-// the sequences times kv heads (`items`) that fill the CUs without.  Not split and
+// the sequences times kv heads (`items`) that fill the CUs without.  (With weights of
+// one part, which take 1 to 4% less time on either side.)  Not split and
 // split, us, sequences of one length or up to it, 8 heads of 128 dims (4 of the others):
 //   items 256 and more, 128 dims  1000 keys 22 and 28 (8 bits 14 and 23), 2000 keys 44 and
 //                                 47 (21 and 29; one length 26 and 38), 4000 86 and 96 (46 and 58);

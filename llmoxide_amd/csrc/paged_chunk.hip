@@ -55,10 +55,11 @@ constexpr int kAhead = 6;
 // 793 us, 512 rows on 4k keys 57 -> 73, the 256-dim window 108 -> 148, 8-bit
 // chunks 361 -> 454.  The error of a result against 64 bits (root mean square, of
 // the result) is 2.7e-4, 2.9e-4, 2.8e-4 and 2.5e-4 with one part, 2.1e-4 with two,
-// as that of the exact result rounded to f16.
-template <bool F32>
+// as that of the exact result rounded to f16.  By masks f16 queries have two parts
+// all the same, as they have in the rows kernel: eight trees of 64 rows 72 -> 88 us.
+template <bool TWO>
 struct Lift {
-    static constexpr float lift = F32 ? 10.f : 6.f, most = 14.f;
+    static constexpr float lift = TWO ? 10.f : 6.f, most = 14.f;
 };
 
 // Place of row r's chunk c is c ^ swizzle(r): rows of 256 bytes and more start
@@ -103,7 +104,8 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     using T = ChunkTile<HD, BN, DS>;
     using QT = std::conditional_t<F32, float, f16>;
     constexpr int KS = T::KS, NB = T::NB, BM = T::BM, CH = T::CH, KB = T::KB, ST = T::ST, GR = T::GR, CV = T::CV;
-    constexpr float kLift = Lift<F32>::lift, kMost = Lift<F32>::most;
+    constexpr bool TWO = F32 || SEEN;  // parts of a weight
+    constexpr float kLift = Lift<TWO>::lift, kMost = Lift<TWO>::most;
     __shared__ __align__(1024) f16 tiles[2][T::STAGE];
     __shared__ __align__(16) float scales[I8 ? 2 : 1][2][BN];  // K's, log2 of V's
 
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
             }
         }
         // register i of block kb is key 32 kb + 16 (i / 8) + 8 hh + i % 8: granule 2 kb + i / 8
-        f16x8 ph[ST], pl[F32 ? ST : 1];
+        f16x8 ph[ST], pl[TWO ? ST : 1];
         float mb = m == -INFINITY ? 0.f : m;
         float top = -INFINITY;
 #pragma unroll
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 const f16x2 hi = __builtin_convertvector(f32x2{p0, p1}, f16x2);
                 ph[2 * kb + (i >> 3)][i & 7] = hi[0];
                 ph[2 * kb + (i >> 3)][(i & 7) + 1] = hi[1];
-                if constexpr (F32) {
+                if constexpr (TWO) {
                     const f16x2 lo = __builtin_convertvector(f32x2{p0 - (float)hi[0], p1 - (float)hi[1]}, f16x2);
                     pl[2 * kb + (i >> 3)][i & 7] = lo[0];
                     pl[2 * kb + (i >> 3)][(i & 7) + 1] = lo[1];
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     const float x0 = s[kb][i], x1 = s[kb][i + 1];
                     sum += WHOLE || x0 != -INFINITY ? fast_exp2(x0 - lv[0]) : 0.f;
                     sum += WHOLE || x1 != -INFINITY ? fast_exp2(x1 - lv[1]) : 0.f;
-                } else if constexpr (F32) {
+                } else if constexpr (TWO) {
                     sum += p0 + p1;
                 } else {
                     sum = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, sum, false);
@@ -421,14 +423,14 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                     vf = __builtin_bit_cast(f16x8, u);
                 }
                 o[nb] = mfma32(vf, ph[st], o[nb]);
-                if constexpr (F32) o[nb] = mfma32(vf, pl[st], o[nb]);
+                if constexpr (TWO) o[nb] = mfma32(vf, pl[st], o[nb]);
                 if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);  // few operands in flight: registers
             }
         if constexpr (WHOLE && !I8) {
             // the first operands are on their way during the first weights'
             // exponentials; the others' run beside the products
-            constexpr int N = ST * NB, PER = F32 ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
-            constexpr int FIRST = F32 ? 24 : 14, EACH = (F32 ? 24 : 13) * ST / N;
+            constexpr int N = ST * NB, PER = TWO ? 2 : 1, AHEAD = N < kAhead ? N : kAhead;
+            constexpr int FIRST = TWO ? 24 : 14, EACH = (TWO ? 24 : 13) * ST / N;
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
             __builtin_amdgcn_sched_group_barrier(0x2, FIRST, 0);
 #pragma unroll

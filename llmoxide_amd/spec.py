@@ -383,7 +383,7 @@ def spec_attention(q, cache: PagedCache, batch: PagedBatch, seen, *, n_heads: in
     window) and the request's rows whose bits are set in its ``seen`` int64
     [n_tokens, words]; one that sees nothing gets zeros.  Types and workspaces are
     ``paged_attention``'s, and its precision, but that with f16 ``q`` the softmax's
-    weights always have 11 bits."""
+    weights always have 22 bits, as with f32."""
     hd = cache.head_dim
     head = q_head_stride or hd
     width = q.shape[-1] if q.dim() == 2 else -1

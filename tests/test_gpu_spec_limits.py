@@ -1,0 +1,44 @@
+"""Steps with drafted tokens on the GPU at their limits: what a result's own rounding
+leaves, full tables, many requests, and streams beside the current one."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+
+from tests import paged_oracle as po
+from tests import spec_oracle as so
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import llmoxide_amd as lmx  # noqa: E402
+from tests.test_gpu_paged import gpu, on_gpu, rows, say  # noqa: E402
+from tests.test_gpu_spec import ints, masks  # noqa: E402
+
+
+# ------------------------------------------------------------------ precision --
+@pytest.mark.parametrize("new,ctx", [([1], [40]), ([4, 1, 3], [70, 5, 33]), ([20, 7], [60, 90]), ([70], [100])])
+@pytest.mark.parametrize("hd,kv,heads,store", [(64, 2, 8, "f16"), (64, 2, 8, "i8"), (128, 2, 8, "f16"), (128, 2, 8, "i8"),
+                                               (256, 1, 4, "i8"), (256, 1, 4, "f16"), (512, 1, 2, "f16"), (512, 1, 2, "i8")])
+def test_f16_results_by_masks_are_off_by_their_own_rounding(new, ctx, hd, kv, heads, store):
+    """With f16 q the weights have 22 bits, as with f32.  q has one element that is not 0
+    in each row head, so that a score is one product (exact: 22 bits) and attend_bound's
+    term of head_dim products is that of one.  What it then gives for f32 results, b, is
+    some 1e-5 of the result; f16(y) is off from y by 2^-11 |y|, or 2^-25 where f16's
+    steps are 2^-24: together (1 + 2^-11) b + 2^-11 |want| + 2^-25.  Weights of 11 bits
+    would add 2^-12 of each weighted value or so, half of the last place."""
+    say("f16 rounding", new, hd, store)
+    c = po.PagedCase(101, new=new, ctx=ctx, page=16, kv=kv, hd=hd, store=store)
+    cache, batch = on_gpu(c)
+    rng = np.random.default_rng(102)
+    q = np.zeros((c.tokens, heads, hd), np.float32)
+    at = rng.integers(0, hd, (c.tokens, heads, 1))
+    np.put_along_axis(q, at, (rng.standard_normal(at.shape) * 8).astype(np.float16).astype(np.float32), 2)
+    sees = masks(c, 103, "tree")
+    seen = gpu(np.concatenate([so.words_of(m, -(-max(new) // 64)) for m in sees]))
+    got = lmx.spec_attention(gpu(q.reshape(c.tokens, -1)).half(), cache, batch, seen, n_heads=heads)
+    want, mag, prod, top = so.attend(c, q, sees, heads=heads)
+    b = po.attend_bound(SimpleNamespace(hd=1, store=store), mag, prod, top, max(ctx), f32=True)
+    off = np.abs(got.double().cpu().numpy().reshape(want.shape) - want)
+    most = (1 + 2.0 ** -11) * b + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    assert np.all(off <= most), f"{(off > most).sum()} of {off.size} are off by up to {(off / most).max():.2f} times the bound"
