@@ -150,9 +150,8 @@ lmx_status lmxs_attn(const lmxp_pool *p, const lmxp_batch *b, const lmxp_attn_de
  *   q NULL    the children were chosen (the draft's best): c passes if
  *             u W < w(c), w = p; after one that does not, W -= w(c), w(c) = 0.
  * In the end the token is the least t with w(0) + .. + w(t) > r * sum of w, of
- * the last accepted row's w.  All of this is in 64 bits, but for the terms of a W
- * behind a refusal, which are rounded to 32 before they are added.  Where nothing
- * of w is left the token comes from p; where p has nothing either it is -1.
+ * the last accepted row's w.  All of this is in 64 bits.  Where nothing of w is left
+ * the token comes from p; where p has nothing either it is -1.
  *   greedy    a child passes if it is the largest p's index (the lowest of
  *             equals, NaN none of them); so the token.  p may be logits; q, u
  *             and r are not read.  -1 where every p is NaN.

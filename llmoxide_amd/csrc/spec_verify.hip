@@ -20,9 +20,9 @@
 //
 // Bound by latency: the last rows (4 or 8 bytes an entry) are 8 MB for 16 requests of
 // 131072 entries, chosen drafts: 8.8 us from a graph (weights 8.3, token 4.5 by
-// themselves), 15 from the host.  A pass takes a workgroup 8.5 us for 100003 entries of
-// p and q (94 GB/s of one CU): eight sampled trees of up to 24 rows 40 us, of which the
-// walk and its passes 36.
+// themselves), 15 from the host.  A pass takes a workgroup 9.7 us for 100003 entries of
+// p and q (82 GB/s of one CU; conversions to 64 bits are what it costs): eight sampled
+// trees of up to 24 rows 44 us.
 #include <type_traits>
 
 #include "spec.hpp"
@@ -428,11 +428,11 @@ __global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const SpecRows s = spec_rows(a.cu, b, a.n_tokens, a.max_new);
     load_rows<T, D, NT>(a, s, rows);
-    // Sum of (p - c q)+ over a row.  A term is made in 32 bits, by one rounding (c in
-    // two parts) and four terms added so; their sums are in 64 bits: the whole is
-    // off by some 1e-8 of itself.  (All in 64 bits a pass over 100003 entries takes
-    // 12 us, so 8.5: the conversions are what it costs.)  Entries that are no
-    // probabilities show in the largest of all bits, and ask for a careful pass.
+    // Sum of (p - c q)+ over a row, in 64 bits throughout: terms rounded to 32 leave a
+    // W of few entries off by 2^-24 of itself, which decides a test beside its border
+    // (and take 7.9 us a pass for 9.7).
+    // Entries that are no probabilities show in the largest of all bits, and ask for a
+    // careful pass.
     auto block = [&](double sum) {
         sum = wave_sum(sum);
         __syncthreads();
@@ -446,7 +446,6 @@ __global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
     auto mass = [&](int row, double c) {
         const T* pr = static_cast<const T*>(a.p) + (size_t)(s.row0 + row) * a.p_stride;
         const T* qr = static_cast<const T*>(a.q) + (size_t)(s.row0 + row) * a.q_stride;
-        const float c0 = (float)c, c1 = (float)(c - (double)c0);
         double sum = 0.0;
         uint32_t top = 0;
         auto bits = [](float x) { return __builtin_bit_cast(uint32_t, x); };
@@ -457,16 +456,13 @@ __global__ __launch_bounds__(1024) void spec_walk_kernel(VerifyArgs a) {
 #pragma unroll
             for (int k = 0; k < U; ++k) y[k] = four_of(qr, t0 + 4 * k * NT, a.vocab, 0.f);
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                float part = 0.f;
+            for (int k = 0; k < U; ++k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t u = bits(x[k][j]), v = bits(y[k][j]), w = u > v ? u : v;
                     top = top > w ? top : w;
-                    part += fmaxf(fmaf(-c1, y[k][j], fmaf(-c0, y[k][j], x[k][j])), 0.f);
+                    sum += fmax((double)x[k][j] - c * (double)y[k][j], 0.0);
                 }
-                sum += (double)part;
-            }
         }
         sum = block(top >= 0x7f800000u ? (double)__builtin_nanf("") : sum);
         if (sum != sum) {

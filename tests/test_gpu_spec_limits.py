@@ -42,3 +42,20 @@ def test_f16_results_by_masks_are_off_by_their_own_rounding(new, ctx, hd, kv, he
     off = np.abs(got.double().cpu().numpy().reshape(want.shape) - want)
     most = (1 + 2.0 ** -11) * b + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
     assert np.all(off <= most), f"{(off > most).sum()} of {off.size} are off by up to {(off / most).max():.2f} times the bound"
+
+
+# --------------------------------------------------------------- verification --
+@pytest.mark.parametrize("vocab", [3, 700, 32768, 40000])
+def test_a_test_beside_its_border_is_decided_in_64_bits(vocab):
+    """The root's second child: a is 1, W = (3/8 - 2^-27) + (5/8 - 1/2) = 1/2 - 2^-27, and
+    u W q = 1/2 W 1/2 = 1/8 - 2^-29 lies below w = 1/8.  With 3/8 - 2^-27 rounded to 24
+    bits W is 1/2, and the child, for which 1/8 < 1/8 fails, is refused."""
+    p, q = np.zeros((3, vocab), np.float32), np.zeros((3, vocab), np.float32)
+    p[0, :3], q[0, :3] = (0, 3 / 8, 5 / 8), (0.5, 2.0 ** -27, 0.5)
+    p[1:, 1] = q[1:, 1] = 1
+    tokens, u, r, parent = [0, 0, 2], [0, 0.5, 0.5], [0.5], [-1, 0, 0]
+    path, token = so.verify(p, tokens, u, r[0], parent, q)
+    assert path == [0, 2] and token == 1  # child 1, of p 0, is refused and makes a 1
+    got = lmx.spec_verify(gpu(p), ints(tokens), gpu(np.float32(u)), gpu(np.float32(r)), ints([0, 3]), max_new=3,
+                          parent=ints(parent), q=gpu(q))
+    assert got.path.tolist() == [[0, 2, -1]] and got.accepted.tolist() == [2] and got.token.tolist() == [1]
