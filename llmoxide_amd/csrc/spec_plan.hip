@@ -47,7 +47,9 @@ __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
 }
 
 // Inclusive scans over the workgroup of three counts that only its first `waves`
-// waves have; `sums` (48 words of LDS) may be used again afterwards.
+// waves have (the others get the totals, so that places behind the last request hold
+// no less than its: last_at needs rising numbers); `sums` (48 words of LDS) may be used
+// again afterwards.
 struct Three {
     int x[3];
 };
@@ -73,6 +75,7 @@ __device__ __forceinline__ Three block_scan(Three v, int waves, int* sums, Three
 #pragma unroll
         for (int i = 0; i < 3; ++i) total.x[i] = add_sat(total.x[i], sums[3 * k + i]);
     }
+    if (w >= waves) before = total;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 3; ++i) v.x[i] = add_sat(v.x[i], before.x[i]);

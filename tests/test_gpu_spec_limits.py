@@ -14,6 +14,7 @@ pytestmark = pytest.mark.gpu
 import llmoxide_amd as lmx  # noqa: E402
 from tests.test_gpu_paged import gpu, on_gpu, rows, say  # noqa: E402
 from tests.test_gpu_spec import ints, masks  # noqa: E402
+from tests.test_spec_plan import requests  # noqa: E402
 
 
 # ------------------------------------------------------------------ precision --
@@ -59,3 +60,24 @@ def test_a_test_beside_its_border_is_decided_in_64_bits(vocab):
     got = lmx.spec_verify(gpu(p), ints(tokens), gpu(np.float32(u)), gpu(np.float32(r)), ints([0, 3]), max_new=3,
                           parent=ints(parent), q=gpu(q))
     assert got.path.tolist() == [[0, 2, -1]] and got.accepted.tolist() == [2] and got.token.tolist() == [1]
+
+
+# ----------------------------------------------------------------------- plans --
+@pytest.mark.parametrize("n_seq", [129, 160, 192, 257, 300, 448, 513, 700, 832, 960, 1024 + 160])
+@pytest.mark.parametrize("trim", [False, True])
+@pytest.mark.parametrize("extra", [1, 9000])
+def test_plans_of_any_number_of_requests(n_seq, trim, extra):
+    """Numbers of requests between a power of two and the next, rows mapped by either
+    kernel; the tables lie among rows that have to stay as they are."""
+    say("plan", n_seq, trim, extra)
+    lens, new, table, held, free, n_free = requests(n_seq, n_seq, 16, 40)
+    n = int(new.sum()) + extra
+    wide = torch.full((3 * n_seq, table.shape[1]), 77, dtype=torch.int32, device="cuda")
+    wide[n_seq:2 * n_seq] = ints(table)
+    t = lmx.PageTables(wide[n_seq:2 * n_seq], ints(held), ints(free), ints(n_free), page_size=16)
+    got = lmx.spec_plan(t, ints(lens), ints(new), n_tokens=n, trim=trim)
+    want = so.plan(lens, new, table.astype(np.int32), held.astype(np.int32), free.astype(np.int32), n_free, page=16, n_tokens=n,
+                   n_pages=len(free), trim=trim)
+    for name, g, w in zip("table held free n_free cu ctx slots pos".split(), (t.page_table, t.held, t.free_pages, t.n_free, *got), want):
+        assert np.array_equal(g.cpu().numpy(), w), name
+    assert (wide[:n_seq] == 77).all() and (wide[2 * n_seq:] == 77).all()
