@@ -23,7 +23,10 @@
  *   cu          int32 [n_seq+1], rising from >= 0; rows outside [cu[0],
  *               cu[n_seq]) belong to no sequence: nothing is read or written
  *               for them.  Two equal entries: a sequence without new rows.
- *   ctx_lens    int32 [n_seq], each at most max_ctx and at least its new rows
+ *   ctx_lens    int32 [n_seq], each at most max_ctx and at least its new rows.
+ *               (The rows of a longer sequence keep their positions, of which
+ *               those behind the table are in no page and those behind max_ctx
+ *               are seen by no query; a shorter one's rows are in no page.)
  *   max_new     at least the largest number of new rows of a sequence
  *   max_ctx     at most table_stride * page_size
  * A call whose work would take 2^24 workgroups or more (some 10^8 row heads) is

@@ -59,13 +59,17 @@ extern "C" {
  *   free_pages      int32 [n_pages]; n_free[0] of them are free.  What lies
  *                   behind them is not read and stays.
  *   n_free          int32 [2], updated: pages that are free, entries lacking
- *   cu, ctx_lens    int32 [n_seq + 1] and [n_seq], written: lmxp_batch's
+ *   cu, ctx_lens    int32 [n_seq + 1] and [n_seq], written: lmxp_batch's.
+ *                   ctx_lens[b] is lens[b] + new_rows[b], also where the table ends
+ *                   before that: the rows behind its end are in no page, and what
+ *                   is cached stays as it is
  *   slots           int64 [n_tokens] or NULL, written: page * page_size + slot
  *                   of each row, -1 for a row in no page or of no request
  *   pos             int32 [n_tokens] or NULL, written: lens[b] + its place among
  *                   its request's rows; -1 for a row of no request
- * Negative lengths count as 0; a length ends at table_stride * page_size.  None
- * of these may overlap. */
+ * Negative lengths count as 0.  A request of more rows than its table has positions
+ * cannot be served: its ctx_lens is the table's positions, and the calls below put
+ * none of its rows in a page.  None of these may overlap. */
 typedef struct {
     uint32_t n_seq;
     uint32_t n_tokens;    /* rows of slots and pos: at least the new rows     */

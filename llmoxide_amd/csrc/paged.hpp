@@ -60,8 +60,8 @@ __device__ __forceinline__ RowPlace locate_row(const PagedArgs& a, int row, int 
     const PagedSeq s = paged_seq(a.g, cu0, cu1, a.ctx[seq]);
     if (row < s.row0 || row >= s.row0 + s.n) return p;
     p.seq = seq;
-    p.pos = s.ctx - s.n + (row - s.row0);
-    const int e = p.pos < s.ctx ? paged_entry(a.g, p.pos) : -1;
+    p.pos = s.first + (row - s.row0);
+    const int e = paged_entry(a.g, p.pos);
     if (e < 0) return p;
     p.page = paged_page(a.g, a.table[(size_t)seq * a.g.table_stride + e]);
     p.slot = p.pos & ((1 << a.g.ps_log2) - 1);
@@ -87,14 +87,14 @@ __device__ __forceinline__ bool find_block(const PagedArgs& a, int id, int& r0, 
     int base = 0;
     for (int c0 = 0; c0 < a.g.n_seq; c0 += 64) {
         const int b = c0 + lane;
-        PagedSeq s{0, 0, 0};
+        PagedSeq s{0, 0, 0, 0};
         if (b < a.g.n_seq) s = paged_seq(a.g, a.cu[b], a.cu[b + 1], a.ctx[b]);
         const int n = row_blocks(s, LOG2_R), upto = a.g.n_seq == 1 ? n : wave_scan(n);
         const uint64_t has = __ballot(base + upto > id);
         if (has) {
             const int l = __builtin_ctzll(has);
             auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-            const PagedSeq q{get(s.row0), get(s.n), get(s.ctx)};
+            const PagedSeq q{get(s.row0), get(s.n), get(s.ctx), get(s.first)};
             const RowBlock blk = row_block(q, id - base - (get(upto) - get(n)), LOG2_R);
             r0 = q.row0 + blk.first;
             n_rows = blk.count;
@@ -102,7 +102,7 @@ __device__ __forceinline__ bool find_block(const PagedArgs& a, int id, int& r0, 
             const int row = lane & ((1 << LOG2_R) - 1);
             if (row < n_rows) {
                 at.seq = c0 + l;
-                at.pos = q.ctx - q.n + blk.first + row;
+                at.pos = q.first + blk.first + row;
                 const int e = paged_entry(a.g, at.pos);
                 if (e >= 0) {
                     at.page = paged_page(a.g, a.table[(size_t)at.seq * a.g.table_stride + e]);

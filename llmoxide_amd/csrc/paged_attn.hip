@@ -165,18 +165,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
     const int row = it.tile * kBM + c;
     const bool have = row < it.s.n * pg.G;
     const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
-    const int pos = have ? it.s.ctx - it.s.n + tok : -1;
-    const int seen_lo = pg.window ? imax(pos - pg.window + 1, 0) : 0;
+    const int pos = have ? it.s.first + tok : -1;
+    const int seen_lo = pg.window ? imax(pos - pg.window + 1, 0) : 0, seen_hi = imin(pos, it.s.ctx - 1);
     Sight sight;
     if constexpr (SEEN) sight = sight_of(a, it.s, have, tok);
     // Keys that every row of the tile sees need no mask.
     const int r_last = imin(it.tile * kBM + kBM, it.s.n * pg.G) - 1;
-    const int p_first = it.s.ctx - it.s.n + (SEEN ? 0 : (it.tile * kBM) / pg.G);  // the first row's position, or the least
-    const int p_last = SEEN ? it.s.ctx - 1 : it.s.ctx - it.s.n + r_last / pg.G;   // the last row's, or the largest
-    const int all_hi = SEEN ? p_first - 1 : p_first;
+    const int p_first = it.s.first + (SEEN ? 0 : (it.tile * kBM) / pg.G);      // the first row's position, or the least
+    const int p_last = it.s.first + (SEEN ? it.s.n - 1 : r_last / pg.G);       // the last row's, or the largest
+    const int all_hi = imin(SEEN ? p_first - 1 : p_first, it.s.ctx - 1);
     const int all_lo = pg.window ? imax(p_last - pg.window + 1, 0) : 0;
     // Keys that some row sees: up to the last row's position, from the first row's window.
-    const int any_hi = p_last;
+    const int any_hi = imin(p_last, it.s.ctx - 1);
     const int any_lo = pg.window ? imax(p_first - pg.window + 1, 0) : 0;
 
     // Q: k-step s holds dims 32s + 8g (f16 tiles); an 8-bit tile's 16-byte load
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
             } else {
 #pragma unroll
                 for (int i = 0; i < QUART; ++i)
-                    seen |= (uint32_t)(page >= 0 && key + i <= pos && key + i >= seen_lo) << i;
+                    seen |= (uint32_t)(page >= 0 && key + i <= seen_hi && key + i >= seen_lo) << i;
             }
 #pragma unroll
             for (int j = 0; j < T::NB; ++j)
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_rows_kernel(Attn
                 if (key >= key_hi) break;
                 if (key >= pw.end(a.p)) pw.fill(a.p, key);
                 const int page = pw.at(a.p, key);
-                if (page < 0 || (SEEN ? !sight.sees(key) : key > pos || key < seen_lo)) continue;
+                if (page < 0 || (SEEN ? !sight.sees(key) : key > seen_hi || key < seen_lo)) continue;
                 const f16* e = reinterpret_cast<const f16*>(a.p.v) +
                                v_offset(a.p, page, it.h, key & ((1 << pg.ps_log2) - 1)) + ((4 * g) << pg.ps_log2);
 #pragma unroll

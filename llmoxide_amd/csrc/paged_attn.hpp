@@ -33,13 +33,14 @@ struct AttnPagedArgs {
 struct Sight {
     const uint64_t* bits;  // of the row; NULL: it sees nothing
     uint64_t word0;        // the first of them: of trees of up to 64 rows the only one
-    int words, lo, first, n;  // first: position of the sequence's row 0, n: its rows
+    int words, lo, first, n;  // first: position of the sequence's row 0, n: its rows within the length
+    int before;               // positions before its rows, within the length
     __device__ __forceinline__ uint64_t word(int i) const { return i == 0 ? word0 : i > 0 && i < words ? bits[i] : 0; }
     // Of the 64 positions from t0 on, those that it sees (pages apart).
     __device__ __forceinline__ uint64_t from(int t0) const {
         if (!bits) return 0;
         auto below = [](int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
-        uint64_t m = below(first - t0) & ~below(lo - t0);
+        uint64_t m = below(before - t0) & ~below(lo - t0);
         const int j = t0 - first;  // the sequence's row at t0: two words hold the 64 rows from there on
         if (j > -64 && j < n) {
             const int w = j >> 6, sh = j & 63;
@@ -56,11 +57,12 @@ __device__ __forceinline__ Sight sight_of(const AttnPagedArgs& a, const PagedSeq
     r.bits = have ? a.seen + (size_t)(s.row0 + row) * a.words : nullptr;
     r.word0 = have ? *r.bits : 0;
     r.words = a.words;
-    r.first = imax(s.ctx - s.n, 0);
-    r.n = imin(s.n, 64 * a.words);
+    r.first = s.first;
+    r.n = imin(imin(s.n, 64 * a.words), s.ctx - s.first);
+    r.before = imin(s.first, s.ctx);
     r.lo = 0;
     if (a.p.g.window && have)
-        r.lo = imax(imin(imax(a.at[s.row0 + row], r.first), s.ctx - 1) - a.p.g.window + 1, 0);
+        r.lo = imax(imin(imax(a.at[s.row0 + row], s.first), s.first + s.n - 1) - a.p.g.window + 1, 0);
     return r;
 }
 
@@ -88,7 +90,7 @@ struct Item {
 // Sequence b's rows and work; no work where it has none or another kernel's
 // share of them.
 __device__ __forceinline__ void load_work(const AttnPagedArgs& a, int b, int bm, PagedSeq& s, SeqWork& w) {
-    s = PagedSeq{0, 0, 0};
+    s = PagedSeq{0, 0, 0, 0};
     w = SeqWork{0, 0, 0};
     if (b < a.p.g.n_seq) {
         s = paged_seq(a.p.g, a.p.cu[b], a.p.cu[b + 1], a.p.ctx[b]);
@@ -123,7 +125,7 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
         // lanes behind the last sequence, of no work, stay where they are
         const int to = 4 * (lane < n ? rank : lane);
         auto put = [&](int& x) { x = __builtin_amdgcn_ds_permute(to, x); };
-        put(b), put(s.row0), put(s.n), put(s.ctx), put(w.rt), put(w.lo), put(w.units);
+        put(b), put(s.row0), put(s.n), put(s.ctx), put(s.first), put(w.rt), put(w.lo), put(w.units);
     };
     load(0);
     o.per = 1000000000;
@@ -152,7 +154,7 @@ __device__ __forceinline__ bool find_item(const AttnPagedArgs& a, int id, int bm
             const int l = __builtin_ctzll(has);
             auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
             o.b = get(b);
-            o.s = PagedSeq{get(s.row0), get(s.n), get(s.ctx)};
+            o.s = PagedSeq{get(s.row0), get(s.n), get(s.ctx), get(s.first)};
             o.w = SeqWork{get(w.rt), get(w.lo), get(w.units)};
             o.splits = seq_splits(o.w, o.per);
             if (a.even) o.per = (o.w.units + o.splits - 1) / o.splits;  // as many splits, of about one length

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
         a.rows[((size_t)it.b * pg.Hkv + it.h) * a.rt_max + it.tile] = make_int4(it.first, it.stride, it.splits, 0);
 
     // ---- rows, and the keys they see
-    const int n_rows = it.s.n * pg.G, first_pos = it.s.ctx - it.s.n;
+    const int n_rows = it.s.n * pg.G, first_pos = it.s.first;
     const int r0 = it.tile * BM, r1 = imin(r0 + BM, n_rows) - 1;
     auto pos_of = [&](int r) { return first_pos + r / pg.G; };
     auto low_of = [&](int pos) { return pg.window ? imax(pos - pg.window + 1, 0) : 0; };
@@ -127,22 +127,23 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
     const int split_hi = it.splits > 1 ? split_lo + it.per * kUnit : 0x7fffffff;
     // a tile's first and last position (by a mask: the least and the largest)
     auto least = [&](int r) { return SEEN ? first_pos : pos_of(r); };
-    auto most = [&](int r) { return SEEN ? it.s.ctx - 1 : pos_of(r); };
+    auto most = [&](int r) { return SEEN ? first_pos + it.s.n - 1 : pos_of(r); };
+    auto held = [&](int pos) { return imin(pos, it.s.ctx - 1); };  // the last key up to there
     const int k_lo = imax(low_of(least(r0)) & ~(BN - 1), split_lo);
-    const int k_hi = imin(most(r1) + 1, split_hi);  // one behind the last key
+    const int k_hi = imin(held(most(r1)) + 1, split_hi);  // one behind the last key
     const int n_t = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
     // the wave's: keys some row sees, keys all rows see
     const int w0 = r0 + w / DS * 32, w1 = imin(w0 + 32, n_rows) - 1;
     const int nb0 = w % DS * NB;  // the wave's first block of dims
     const bool live = w0 <= r1;
-    const int any_hi = live ? most(w1) : -1, all_hi = live ? least(w0) - SEEN : -1;
+    const int any_hi = live ? held(most(w1)) : -1, all_hi = live ? held(least(w0) - SEEN) : -1;
     const int any_lo = live ? low_of(least(w0)) : 0, all_lo = live ? low_of(most(w1)) : 0;
 
     f16x8 qh[KS], ql[F32 ? KS : 1];
     const int row = w0 + l32;
     const bool have = row < n_rows;
     const int tok = have ? row / pg.G : 0, head = it.h * pg.G + (have ? row % pg.G : 0);
-    const int pos = have ? first_pos + tok : -1, seen_lo = low_of(pos);
+    const int pos = have ? first_pos + tok : -1, seen_lo = low_of(pos), seen_hi = held(pos);
     Sight sight;
     if constexpr (SEEN) sight = sight_of(a, it.s, have, tok);
     float qs = a.c;  // what a score is multiplied by
@@ -359,7 +360,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int at = 32 * kb + 16 * (i >> 3) + (i & 7), key = t0 + 8 * hh + at;
-                    const bool on = p[2 * kb + (i >> 3)] >= 0 && (SEEN ? seen >> at & 1 : key <= pos && key >= seen_lo);
+                    const bool on = p[2 * kb + (i >> 3)] >= 0 && (SEEN ? seen >> at & 1 : key <= seen_hi && key >= seen_lo);
                     if (!on) s[kb][i] = -INFINITY;
                 }
         }
@@ -525,7 +526,7 @@ __global__ __launch_bounds__(256, OCC) void paged_chunk_kernel(AttnPagedArgs a) 
                 for (int key = k_lo; key < k_hi; ++key) {
                     if (key >= pw.end(a.p)) pw.fill(a.p, key);
                     const int page = pw.at(a.p, key);
-                    if (page < 0 || (SEEN ? !sight.sees(key) : key > pos || key < seen_lo)) continue;
+                    if (page < 0 || (SEEN ? !sight.sees(key) : key > seen_hi || key < seen_lo)) continue;
                     const f16* e = reinterpret_cast<const f16*>(a.p.v) + v_offset(a.p, page, it.h, key & psm) +
                                    ((32 * (nb0 + nb) + 4 * hh) << pg.ps_log2);
 #pragma unroll

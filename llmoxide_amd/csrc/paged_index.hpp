@@ -26,15 +26,21 @@ struct PagedGeom {
 LMX_FN int imin(int a, int b) { return a < b ? a : b; }
 LMX_FN int imax(int a, int b) { return a > b ? a : b; }
 
-// One sequence's rows [row0, row0 + n) and length, forced into range.
+// One sequence's rows [row0, row0 + n) and length, forced into range, and the position
+// of its first row.  That is the length's as it was given: of a sequence that is longer
+// than max_ctx the rows stay where they belong (those behind the table are then in no
+// page), and not on top of earlier positions.  A length below its rows gives them no
+// position at all (kNowhere and up, all below 0).
 struct PagedSeq {
-    int row0, n, ctx;
+    int row0, n, ctx, first;
 };
+constexpr int kNowhere = -(1 << 30);
 LMX_FN PagedSeq paged_seq(const PagedGeom& g, int cu0, int cu1, int ctx) {
     PagedSeq s;
     s.row0 = imin(imax(cu0, 0), g.n_tokens);
     s.n = imin(imax(cu1, s.row0), g.n_tokens) - s.row0;
     s.ctx = imin(imax(ctx, 0), g.max_ctx);
+    s.first = ctx >= s.n ? ctx - s.n : kNowhere;
     return s;
 }
 
@@ -53,8 +59,8 @@ LMX_FN int paged_page(const PagedGeom& g, int entry) {
 
 // ---- row blocks: a sequence's new rows, cut where its positions are multiples
 // of R (a power of two), so that a block's rows meet whole granules of a page
-// except at the sequence's own ends.  A first position below 0 (a length
-// shorter than its new rows) is cut the same way.
+// except at the sequence's own ends.  (A length out of range is cut as if it were
+// in range: its blocks then meet parts of granules.)
 LMX_FN int row_blocks(const PagedSeq& s, int log2_r) {
     return s.n ? ((s.ctx - 1) >> log2_r) - ((s.ctx - s.n) >> log2_r) + 1 : 0;
 }
@@ -92,8 +98,7 @@ struct SeqWork {
 LMX_FN SeqWork seq_work(const PagedGeom& g, const PagedSeq& s, int bm) {
     SeqWork w;
     w.rt = (int)(((int64_t)s.n * g.G + bm - 1) / bm);
-    const int first = s.ctx - s.n;  // position of the first row
-    int lo = g.window && first + 1 > g.window ? first + 1 - g.window : 0;
+    int lo = g.window ? imax(s.first - g.window + 1, 0) : 0;
     lo = imin(lo, s.ctx) & ~(kUnit - 1);
     w.lo = lo;
     w.units = (s.ctx - lo + kUnit - 1) / kUnit;

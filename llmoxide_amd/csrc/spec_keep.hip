@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void spec_keep_kernel(KeepArgs a) {
     const int cu0 = a.p.cu[b], cu1 = a.p.cu[b + 1], ctx = a.p.ctx[b], accepted = a.accepted[b];
     args_in_sgprs(cu0, cu1, ctx, accepted);  // one round of loads
     const PagedSeq s = paged_seq(g, cu0, cu1, ctx);
-    const int n = imin(imin(imax(accepted, 0), s.n), a.path_stride), first = s.ctx - s.n;
+    const int n = imin(imin(imax(accepted, 0), s.n), a.path_stride), first = s.first;
     const int ps = 1 << g.ps_log2, hd = a.p.hd;
     const int chunks = hd * ES / 16;  // 16-byte pieces of a K row
     const int kp = g.Hkv * chunks, vp = g.Hkv * hd;

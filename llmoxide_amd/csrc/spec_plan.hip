@@ -32,17 +32,20 @@ struct PlanArgs {
 constexpr int kPlan = 1024;  // threads, and requests at a time
 
 struct Request {
-    int len, rows, total, need, held;
+    int len, rows, need, held;
+    int ctx;  // length with its rows, from which their positions count back
 };
 __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
     Request r;
     r.len = imax(a.lens[b], 0);
     r.rows = imin(imax(a.fresh[b], 0), a.n_tokens);
     r.held = imin(imax(a.held[b], 0), a.stride);
-    const int64_t room = (int64_t)a.stride << a.ps_log2, total = (int64_t)r.len + r.rows;
-    r.total = (int)(total < room ? total : room < kMost ? room : kMost);
-    r.total = imin(r.total, kMost);
-    r.need = (int)(((int64_t)r.total + (1 << a.ps_log2) - 1) >> a.ps_log2);
+    const int64_t table = (int64_t)a.stride << a.ps_log2, total = (int64_t)r.len + r.rows;
+    const int room = (int)(table < kMost ? table : kMost), fits = (int)(total < room ? total : room);
+    r.need = (int)(((int64_t)fits + (1 << a.ps_log2) - 1) >> a.ps_log2);
+    // Not cut where the table ends: the rows' positions would move onto cached ones.  (More
+    // rows than the table has positions are a length below the rows, which have no positions.)
+    r.ctx = r.rows > room ? fits : (int)(total < 0x7fffffff ? total : 0x7fffffff);
     return r;
 }
 
@@ -92,7 +95,7 @@ __device__ __forceinline__ int last_at(const int* start, int n, int i) {
 __device__ __forceinline__ void map_row(const PlanArgs& a, int row, int b, int len, int j) {
     const int64_t p = (int64_t)len + j, e = p >> a.ps_log2;
     int page = -1;
-    if (e < a.stride) page = a.table[(size_t)b * a.stride + e];
+    if (e < a.stride && p < kMost) page = a.table[(size_t)b * a.stride + e];
     if (a.slots)
         a.slots[row] = (uint32_t)page < (uint32_t)a.n_pages ? ((int64_t)page << a.ps_log2) + (p & ((1 << a.ps_log2) - 1)) : -1;
     if (a.pos) a.pos[row] = (int32_t)(p < 0x7fffffff ? p : 0x7fffffff);
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(kPlan) void spec_plan_kernel(PlanArgs a) {
         const int b = c0 + tid, all_rows = c.all.x[kRows], all_want = c.all.x[kWant];
         if (b < a.n_seq) {
             a.cu[b + 1] = imin(add_sat(rows, c.upto.x[kRows]), a.n_tokens);
-            a.ctx[b] = c.r.total;
+            a.ctx[b] = c.r.ctx;
             a.held[b] = c.had + imin(imax(top - add_sat(taken, c.upto.x[kWant] - c.want), 0), c.want);
         }
         if (tid < size) {

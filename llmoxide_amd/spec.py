@@ -222,7 +222,9 @@ def spec_plan(tables: PageTables, lens, new_rows, *, n_tokens: Optional[int] = N
     and ``new_rows`` [n_seq] to come take from the free list the pages that they
     lack, in order; with ``trim`` those beyond what a request needs go back first
     (all of one with length 0 and no rows).  Pages that the list lacks are left out,
-    counted in ``tables.n_free[1]`` and asked for again by the next plan.
+    counted in ``tables.n_free[1]`` and asked for again by the next plan.  Where a
+    request's row of the table ends before its length does, ``ctx_lens`` says so, and
+    the rows behind are in no page.
     ``n_tokens`` is the rows of the batch (``out``'s maps have as many)."""
     if n_tokens is None:
         n_tokens = out and out.n_tokens

@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 import llmoxide_amd as lmx  # noqa: E402
 from tests.test_gpu_paged import gpu, on_gpu, rows, say  # noqa: E402
-from tests.test_gpu_spec import ints, masks  # noqa: E402
+from tests.test_gpu_spec import ints, masks, trees_of  # noqa: E402
 from tests.test_spec_plan import requests  # noqa: E402
 
 
@@ -81,3 +81,94 @@ def test_plans_of_any_number_of_requests(n_seq, trim, extra):
     for name, g, w in zip("table held free n_free cu ctx slots pos".split(), (t.page_table, t.held, t.free_pages, t.n_free, *got), want):
         assert np.array_equal(g.cpu().numpy(), w), name
     assert (wide[:n_seq] == 77).all() and (wide[2 * n_seq:] == 77).all()
+
+
+def beyond(c, entries):
+    """The cache of a PagedCase, and its batch with tables that end after ``entries``."""
+    c.table, c.stride = np.ascontiguousarray(c.table[:, :entries]), entries
+    cache, _ = on_gpu(c)
+    return cache, lmx.PagedBatch(gpu(c.cu), ints(c.ctx), gpu(c.table), n_tokens=c.tokens, max_new=max(c.new), max_ctx=entries * c.page)
+
+
+@pytest.mark.parametrize("new,ctx", [([1, 3, 2], [65, 66, 9]), ([4, 4, 4], [63, 70, 99]), ([40, 9, 3], [70, 80, 400]),
+                                     ([64, 7, 33], [127, 64, 65]), ([70, 2, 65], [64, 60, 80])])
+@pytest.mark.parametrize("store,hd", [("f16", 128), ("i8", 64), ("f16", 256)])
+def test_rows_behind_the_end_of_a_table(new, ctx, store, hd):
+    """Sequences that are longer than the 64 positions of their table: rows within it are
+    stored and attend as they should, the others are stored nowhere and see what is there;
+    what was cached keeps every bit.  Those with a length below their rows are in no page."""
+    say("table's end", new, ctx, store, hd)
+    heads, kv = 4, 2
+    c = po.PagedCase(110, new=new, ctx=ctx, page=16, kv=kv, hd=hd, store=store)
+    cache, batch = beyond(c, 4)
+    none = [b for b in range(3) if new[b] > ctx[b]]  # of these no row has a position
+    x = [rows(c, 111 + i, h) for i, h in enumerate((heads, kv, kv))]
+    q, k, v = (gpu(y.reshape(c.tokens, -1)) for y in x)
+    for b in none:
+        c.table[b] = -1  # the oracle's, whose rows would have positions below 0 and above
+    want = po.append(c, x[1], x[2])
+    lmx.paged_append(k, v, cache, batch)
+    for got, w in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), want):
+        if w is not None:
+            assert np.array_equal(got.cpu().numpy(), w)
+    k2, v2 = lmx.paged_read(cache, batch)
+    for row, _, _, at in c.row_places():
+        assert (k2[row].any() and v2[row].any()) == (at is not None)
+    # prologues: the same places
+    stored = np.zeros((c.n_pages, 16), bool)
+    for _, _, _, at in c.row_places():
+        if at is not None:
+            stored[at] = True
+    for call in (lmx.paged_prologue, lmx.spec_prologue):
+        twin, _ = on_gpu(c)
+        call(q, k, v, twin, batch, n_heads=heads)
+        assert np.array_equal((twin.k.cpu().numpy() != c.k).any((1, 3)), stored)
+        assert np.array_equal((twin.v.cpu().numpy() != c.v).any((1, 2)), stored)
+    c.k, c.v, c.k_scale, c.v_scale = want
+    # attention, causal and by masks
+    for window in (0, 20):
+        ref, mag, prod, top = po.attend(c, x[0], heads=heads, window=window)
+        got = lmx.paged_attention(q, cache, batch, n_heads=heads, window=window).cpu().numpy().reshape(ref.shape)
+        assert np.all(np.abs(got - ref) <= po.attend_bound(c, mag, prod, top, 64, f32=True))
+        trees = trees_of(c, 112)
+        sees = [so.tree(t, window)[1] for t in trees]
+        pos = np.concatenate([ctx[b] - new[b] + so.tree(t)[0] for b, t in enumerate(trees)])
+        seen = gpu(np.concatenate([so.words_of(m, 2) for m in sees]))
+        ref, mag, prod, top = so.attend(c, x[0], sees, heads=heads, window=window, pos=pos)
+        got = lmx.spec_attention(q, cache, batch, seen, n_heads=heads, window=window, pos=ints(pos)).cpu().numpy().reshape(ref.shape)
+        assert np.all(np.abs(got - ref) <= po.attend_bound(c, mag, prod, top, 64, f32=True))
+    # keeping: from places and to places that there are
+    path = np.full((3, max(new)), -1)
+    for b, n in enumerate(new):
+        path[b, :(n + 1) // 2] = np.arange(0, n, 2)
+    accepted = [(n + 1) // 2 for n in new]
+    want = so.keep(c, path, accepted, want)
+    lmx.spec_keep([cache], batch, ints(path), ints(accepted))
+    for got, w in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), want):
+        if w is not None:
+            assert np.array_equal(got.cpu().numpy(), w)
+
+
+def test_a_full_request_leaves_its_prefix_and_its_neighbours():
+    """Two requests share their first pages; one reaches the end of its row of the table in
+    this step, the other goes on.  The plan's lengths lead the prologue to the map's slots."""
+    page, kv, hd, heads, entries = 16, 1, 64, 2, 3
+    free = np.zeros(12, np.int32)
+    free[:6] = np.arange(6, 12)
+    t = lmx.PageTables(ints([[0, 1, -1], [0, 2, -1]]), ints([2, 2]), ints(free), ints([6, 0]), page_size=page)
+    cache = lmx.PagedCache.empty(12, page_size=page, n_kv_heads=kv, head_dim=hd)
+    cache.k.fill_(7), cache.v.fill_(9)
+    for new in ([18, 4], [40, 4], [5, 4]):
+        n, lens = sum(new), [32, 30]
+        step = lmx.spec_plan(t, ints(lens), ints(new), n_tokens=n, trim=True)
+        batch = lmx.PagedBatch(step.cu, step.ctx_lens, t.page_table, n_tokens=n, max_new=max(new), max_ctx=entries * page)
+        q, k, v = (torch.randn(n, h * hd, device="cuda") for h in (heads, kv, kv))
+        tree = lmx.spec_tree(ints(np.concatenate([np.arange(-1, m - 1) for m in new])), batch)
+        assert tree.pos.tolist() == step.pos.tolist() == [a + j for a, m in zip(lens, new) for j in range(m)]
+        cache.k.fill_(7), cache.v.fill_(9)
+        lmx.spec_prologue(q, k, v, cache, batch, n_heads=heads, n_rot=0, pos=tree.pos)
+        want_k, want_v = torch.full_like(cache.k, 7), torch.full_like(cache.v, 9)
+        for row, at in enumerate(step.slots.tolist()):
+            if at >= 0:
+                want_k[at // page, 0, at % page], want_v[at // page, 0, :, at % page] = k[row].half(), v[row].half()
+        assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v), new

@@ -115,3 +115,42 @@ def test_plans_of_any_number_of_requests(on_cpu, n_seq, trim):
         for name, g, w in zip("table held free n_free cu ctx slots pos".split(), got, want):
             assert np.array_equal(g, w), name
 
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_rows_stay_behind_the_cached_ones_where_a_table_ends(on_cpu, seed):
+    """Requests at the end of their rows of the table: a row's position, counted back from
+    ctx_lens, is that of the map, and not one that is cached.  (A request of more rows than
+    the table has positions gets a length below its rows: no positions.)"""
+    rng = np.random.default_rng(seed)
+    n_seq, entries, page = 40, int(rng.integers(1, 5)), int(rng.choice([16, 32]))
+    room = entries * page
+    lens = rng.integers(0, room + 20, n_seq)
+    lens[:3] = room, room - 1, (1 << 31) - 1
+    new = rng.integers(0, 2 * room, n_seq)
+    new[:3] = 1, 3, 5
+    n = int(new.sum())
+    _, held, _, n_free, cu, ctx, slots, pos = run(on_cpu, lens, new, np.full((n_seq, entries), -1), np.zeros(n_seq), np.arange(400),
+                                                  [400, 0], page=page, n_tokens=n, trim=bool(seed & 1))
+    assert cu.tolist() == [0, *np.cumsum(new)] and n_free[1] == 0
+    for b in range(n_seq):
+        assert held[b] == -(-min(lens[b] + new[b], room) // page)
+        if new[b] > room:
+            assert ctx[b] == room < new[b]
+            continue
+        assert int(ctx[b]) == min(lens[b] + new[b], (1 << 31) - 1)
+        for j in range(new[b]):
+            r, p = int(cu[b]) + j, int(ctx[b]) - int(new[b]) + j
+            assert (slots[r] >= 0) == (p < room) and (pos[r] == p if b != 2 else pos[r] >= p)
+
+
+def test_a_plan_reads_no_entry_behind_what_is_held(on_cpu):
+    """Lengths that pass the 2^30 positions that lengths are counted to: the table has more
+    entries, which hold anything, and no row is mapped by them."""
+    entries = (1 << 22) + 100  # of 256 positions: 2^30 and 25600
+    table = np.full((1, entries), 3, np.int32)
+    table[0, :10] = -1
+    lens = [(1 << 30) - 4]
+    _, _, _, _, _, ctx, slots, pos = run(on_cpu, lens, [9], table, [entries], np.arange(8), [0, 0], page=256, n_tokens=9, trim=False)
+    assert ctx[0] == lens[0] + 9 and pos.tolist() == [lens[0] + j for j in range(9)]
+    assert slots.tolist() == [3 * 256 + 252 + j for j in range(3)] + [-1] * 6
