@@ -201,8 +201,8 @@ lmx_status lmxs_verify(const lmxs_verify_desc *d, const int32_t *cu, const int32
  * not, and one that is no row of the request, is not moved, nor one from or to a
  * position in no page.
  *   pools     host array of n_pools (1 to 1024) pointers to pools (a layer each) of
- *             one geometry and store, whose pages the batch's table names; their K
- *             and V do not overlap
+ *             one geometry and store, whose pages the batch's table names; their K,
+ *             V and scales do not overlap
  *   b         the step's batch, its lengths with all of its rows
  *   path      int32 [n_seq, path_stride], path_stride at least max_new
  *   accepted  int32 [n_seq] */
