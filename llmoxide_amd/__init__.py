@@ -328,6 +328,24 @@ def _need_cuda(*ts) -> None:
             raise ValueError("tensors must be contiguous and on the GPU")
 
 
+def _allocated(make, stream):
+    """What ``make()`` allocates, for a call whose work goes to ``stream`` (None: the
+    current one).  torch hands out what was freed on a stream while kernels there may
+    still use it, as work behind them on that stream cannot overtake them; so memory
+    that another stream fills has to be of that stream's own, and is marked as used on
+    the current one, whose work the caller may give it to."""
+    if stream is None:
+        return make()
+    cuda = _torch().cuda
+    here = cuda.current_stream()
+    if stream == here:
+        return make()
+    with cuda.stream(stream):
+        out = make()
+    out.record_stream(here)
+    return out
+
+
 class Workspace:
     """A zero-initialized device scratch buffer shared by successive calls.
 
@@ -345,22 +363,17 @@ class Workspace:
 
     def ensure(self, nbytes: int, stream=None):
         """Grow to at least ``nbytes`` for work enqueued on ``stream`` (None:
-        torch's current stream).  torch's caching allocator orders frees and
-        reuse on the current stream only, so on another stream both the new
-        buffer and a replaced one are marked as used there
-        (``record_stream``): neither is handed out again while the stream
-        still has this workspace's kernels queued."""
+        torch's current stream).  The new buffer is of that stream's memory
+        (``_allocated``), and a replaced one is marked as used there: neither is
+        handed out again while the stream still has this workspace's kernels queued."""
         torch = _torch()
         if nbytes <= self.nbytes:
             return self
-        side = stream is not None and stream != torch.cuda.current_stream()
-        if side and self.buf is not None:
-            self.buf.record_stream(stream)
+        if self.buf is not None:
+            self.buf.record_stream(torch.cuda.current_stream() if stream is None else stream)
         nbytes = (nbytes + 255) // 256 * 256
-        self.buf = torch.empty(nbytes + 256, dtype=torch.uint8,
-                               device=self.device or torch.device("cuda"))
-        if side:
-            self.buf.record_stream(stream)
+        self.buf = _allocated(lambda: torch.empty(nbytes + 256, dtype=torch.uint8,
+                                                  device=self.device or torch.device("cuda")), stream)
         off = (-self.buf.data_ptr()) % 256
         self.base = self.buf.data_ptr() + off
         self.nbytes = nbytes
@@ -431,7 +444,8 @@ def attention(q, k_cache, v_cache, *, n_heads: int, n_kv_heads: int, head_dim: i
                     base_pos=base_pos, n_slots=k_cache.shape[0], window=window, bidi=bidi,
                     scale=scale, kv_dim=kv_dim)
     if out is None:
-        out = torch.empty((t, n_heads * head_dim), dtype=torch.float32, device=q.device)
+        out = _allocated(lambda: torch.empty((t, n_heads * head_dim), dtype=torch.float32,
+                                             device=q.device), stream)
     need = lib().lmx_attn_workspace_bytes(ctypes.byref(p))
     ws_ptr, ws_bytes = None, 0
     if need:
@@ -488,7 +502,8 @@ def attention_decode_batched(q, caches: BatchedCaches, ctx_lens, *, max_ctx: int
                     base_pos=0, n_slots=n_slots or caches.k_caches[0].shape[0], window=window,
                     scale=scale)
     if out is None:
-        out = torch.empty((B, n_heads * head_dim), dtype=torch.float32, device=q.device)
+        out = _allocated(lambda: torch.empty((B, n_heads * head_dim), dtype=torch.float32,
+                                             device=q.device), stream)
     need = lib().lmx_attn_decode_batched_workspace_bytes(ctypes.byref(p), B, max_ctx)
     ws_ptr, ws_bytes = None, 0
     if need:
@@ -516,7 +531,8 @@ def delta_recur(conv, alpha, beta, state, ssm_a, dt_bias, *, n_vh, n_kh, s_dim, 
     _need_cuda(conv, alpha, beta, state, ssm_a, dt_bias, out)
     op = dop(n_tok=conv.shape[0], n_vh=n_vh, n_kh=n_kh, s_dim=s_dim)
     if out is None:
-        out = torch.empty((conv.shape[0], op.d_inner), dtype=torch.float32, device=conv.device)
+        out = _allocated(lambda: torch.empty((conv.shape[0], op.d_inner), dtype=torch.float32,
+                                             device=conv.device), stream)
     rc = lib().lmx_deltanet_recur(ctypes.byref(op), _ptr(ssm_a), _ptr(dt_bias), _ptr(alpha),
                                   _ptr(beta), _ptr(conv), _ptr(state), _ptr(out), _stream(stream))
     _check("lmx_deltanet_recur", rc)
@@ -530,7 +546,8 @@ def delta_chunked(conv, alpha, beta, state, ssm_a, dt_bias, *, n_vh, n_kh, s_dim
     _need_cuda(conv, alpha, beta, state, ssm_a, dt_bias, out)
     op = dop(n_tok=conv.shape[0], n_vh=n_vh, n_kh=n_kh, s_dim=s_dim)
     if out is None:
-        out = torch.empty((conv.shape[0], op.d_inner), dtype=torch.float32, device=conv.device)
+        out = _allocated(lambda: torch.empty((conv.shape[0], op.d_inner), dtype=torch.float32,
+                                             device=conv.device), stream)
     need = lib().lmx_deltanet_chunked_workspace_bytes(ctypes.byref(op), chunk)
     ws_ptr, ws_bytes = None, 0
     if need:
@@ -553,7 +570,7 @@ def delta_front(x, taps, conv_state, conv_out=None, *, key_dim: int, s_dim: int,
     _need_cuda(x, taps, conv_state, conv_out)
     t, conv_dim = x.shape
     if conv_out is None:
-        conv_out = torch.empty_like(x)
+        conv_out = _allocated(lambda: torch.empty_like(x), stream)
     d = DeltaFrontDesc(t, conv_dim, key_dim, s_dim, taps.shape[-1], eps)
     rc = lib().lmx_deltanet_front(ctypes.byref(d), _ptr(x), _ptr(taps), _ptr(conv_state),
                                   _ptr(conv_out), _stream(stream))
@@ -579,7 +596,7 @@ def matvec(w, x, *, qtype, rows: int, in_dim: int, y=None, stream=None):
     ty = QTYPES[qtype] if isinstance(qtype, str) else int(qtype)
     n_tok = x.numel() // in_dim
     if y is None:
-        y = torch.empty((n_tok, rows), dtype=torch.float32, device=x.device)
+        y = _allocated(lambda: torch.empty((n_tok, rows), dtype=torch.float32, device=x.device), stream)
     d = QmvDesc(ty, rows, in_dim, n_tok)
     _check("lmx_matvec", lib().lmx_matvec(ctypes.byref(d), _ptr(w), _ptr(x), _ptr(y), _stream(stream)))
     return y

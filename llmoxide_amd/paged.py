@@ -25,7 +25,7 @@ import functools
 import math
 from typing import Optional
 
-from . import F16, F32, Workspace, _check, _need_cuda, _ptr, _stream, _torch, lib
+from . import F16, F32, Workspace, _allocated, _check, _need_cuda, _ptr, _stream, _torch, lib
 
 STORE_F16, STORE_I8 = 1, 2
 
@@ -246,12 +246,8 @@ def paged_append(k, v, cache: PagedCache, batch: PagedBatch, *, stream=None) -> 
 
 
 def _new_out(shape, dtype, device, stream):
-    """A result allocated here; one that another stream fills is marked as used there."""
-    torch = _torch()
-    out = torch.empty(shape, dtype=dtype, device=device)
-    if stream is not None and stream != torch.cuda.current_stream():
-        out.record_stream(stream)
-    return out
+    """A result allocated here, of the memory of the stream that fills it."""
+    return _allocated(lambda: _torch().empty(shape, dtype=dtype, device=device), stream)
 
 
 def paged_read(cache: PagedCache, batch: PagedBatch, *, dtype=None, k_out=None, v_out=None, stream=None):

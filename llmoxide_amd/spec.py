@@ -36,7 +36,7 @@ import functools
 import math
 from typing import Optional, Sequence
 
-from . import F32, Workspace, _check, _need_cuda, _ptr, _stream, _torch, lib
+from . import F32, Workspace, _allocated, _check, _need_cuda, _ptr, _stream, _torch, lib
 from . import paged as _paged
 from .paged import BatchDesc, PagedAttnDesc, PagedBatch, PagedCache, PagedPrologueDesc, PoolDesc, _new_out, _rows
 
@@ -113,12 +113,9 @@ def _ints(what: str, t, size, at: int) -> None:
 
 
 def _fresh(like, shape, stream):
-    """A result allocated here, of ``like``'s type and device (1.1 us; by torch.empty,
-    which is told both, 1.6); one that another stream fills is marked as used there."""
-    out = like.new_empty(shape)
-    if stream is not None and stream != _torch().cuda.current_stream():
-        out.record_stream(stream)
-    return out
+    """``_new_out`` of ``like``'s type and device (1.1 us; by torch.empty, which is told
+    both, 1.6)."""
+    return like.new_empty(shape) if stream is None else _allocated(lambda: like.new_empty(shape), stream)
 
 
 class _Held:
