@@ -33,20 +33,26 @@ constexpr int kPlan = 1024;  // threads, and requests at a time
 
 struct Request {
     int len, rows, need, held;
-    int ctx;  // length with its rows, from which their positions count back
 };
+__device__ __forceinline__ int room_of(const PlanArgs& a) {
+    const int64_t table = (int64_t)a.stride << a.ps_log2;
+    return (int)(table < kMost ? table : kMost);
+}
 __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
     Request r;
     r.len = imax(a.lens[b], 0);
     r.rows = imin(imax(a.fresh[b], 0), a.n_tokens);
     r.held = imin(imax(a.held[b], 0), a.stride);
-    const int64_t table = (int64_t)a.stride << a.ps_log2, total = (int64_t)r.len + r.rows;
-    const int room = (int)(table < kMost ? table : kMost), fits = (int)(total < room ? total : room);
-    r.need = (int)(((int64_t)fits + (1 << a.ps_log2) - 1) >> a.ps_log2);
-    // Not cut where the table ends: the rows' positions would move onto cached ones.  (More
-    // rows than the table has positions are a length below the rows, which have no positions.)
-    r.ctx = r.rows > room ? fits : (int)(total < 0x7fffffff ? total : 0x7fffffff);
+    const int64_t total = (int64_t)r.len + r.rows, room = room_of(a);
+    r.need = (int)(((total < room ? total : room) + (1 << a.ps_log2) - 1) >> a.ps_log2);
     return r;
+}
+// Length with n rows, from which their positions count back: not cut where the table
+// ends, which would move them onto cached ones.  (More rows than the table has positions
+// are a length below the rows, which have no positions.)
+__device__ __forceinline__ int length_with(const PlanArgs& a, int len, int n) {
+    const int64_t total = (int64_t)len + n;
+    return n > room_of(a) ? room_of(a) : (int)(total < 0x7fffffff ? total : 0x7fffffff);
 }
 
 // Inclusive scans over the workgroup of three counts that only its first `waves`
@@ -114,7 +120,7 @@ struct Chunk {
 };
 __device__ __forceinline__ Chunk load_chunk(const PlanArgs& a, int c0, int waves, int* sums) {
     Chunk c;
-    c.r = Request{0, 0, 0, 0, 0};
+    c.r = Request{0, 0, 0, 0};
     if (c0 + (int)threadIdx.x < a.n_seq) c.r = load_request(a, c0 + threadIdx.x);
     c.back = a.trim ? imax(c.r.held - c.r.need, 0) : 0;
     c.had = c.r.held - c.back;
@@ -169,8 +175,9 @@ __global__ __launch_bounds__(kPlan) void spec_plan_kernel(PlanArgs a) {
         if (c0) c = load_chunk(a, c0, waves, sums);  // (the first chunk is at hand)
         const int b = c0 + tid, all_rows = c.all.x[kRows], all_want = c.all.x[kWant];
         if (b < a.n_seq) {
-            a.cu[b + 1] = imin(add_sat(rows, c.upto.x[kRows]), a.n_tokens);
-            a.ctx[b] = c.r.ctx;
+            const int upto = imin(add_sat(rows, c.upto.x[kRows]), a.n_tokens);
+            a.cu[b + 1] = upto;
+            a.ctx[b] = length_with(a, c.r.len, upto - imin(add_sat(rows, c.upto.x[kRows] - c.r.rows), a.n_tokens));
             a.held[b] = c.had + imin(imax(top - add_sat(taken, c.upto.x[kWant] - c.want), 0), c.want);
         }
         if (tid < size) {

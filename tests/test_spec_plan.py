@@ -154,3 +154,19 @@ def test_a_plan_reads_no_entry_behind_what_is_held(on_cpu):
     _, _, _, _, _, ctx, slots, pos = run(on_cpu, lens, [9], table, [entries], np.arange(8), [0, 0], page=256, n_tokens=9, trim=False)
     assert ctx[0] == lens[0] + 9 and pos.tolist() == [lens[0] + j for j in range(9)]
     assert slots.tolist() == [3 * 256 + 252 + j for j in range(3)] + [-1] * 6
+
+
+@pytest.mark.parametrize("n_seq,n_tokens", [(1, 3), (5, 20), (70, 100), (300, 64)])
+def test_rows_that_the_maps_have_no_place_for_move_no_others(on_cpu, n_seq, n_tokens):
+    """More new rows than n_tokens, which a caller must not bring: the rows that are left
+    still stand behind the cached ones, by the lengths as by the map."""
+    rng = np.random.default_rng(n_seq)
+    lens, new = rng.integers(0, 40, n_seq), rng.integers(1, 9, n_seq)
+    new[-1] = 200  # more than the table has positions
+    _, _, _, _, cu, ctx, slots, pos = run(on_cpu, lens, new, np.full((n_seq, 4), -1), np.zeros(n_seq), np.arange(4 * n_seq),
+                                          [4 * n_seq, 0], page=16, n_tokens=n_tokens, trim=False)
+    assert cu.tolist() == [0, *np.minimum(np.cumsum(np.minimum(new, n_tokens)), n_tokens)]
+    for b in range(n_seq):
+        n = int(cu[b + 1] - cu[b])
+        assert ctx[b] == (64 if n > 64 else lens[b] + n)
+        assert pos[cu[b]:cu[b + 1]].tolist() == [lens[b] + j for j in range(n)]
