@@ -130,9 +130,9 @@ lmx_status lmxs_prologue(const lmxp_pool *p, const lmxp_batch *b, const lmxp_pro
  *          at least max_new
  *   pos    int32 [n_tokens]; may be NULL without a window
  * Types, layouts and precision are lmxp_attn's, but that f16 q and out always have
- * weights of 22 bits, as f32 q and out have.  The workspace is used as lmxp_attn's: lmxs_attn_workspace_bytes gives
- * what serves this batch and every one whose n_seq, n_tokens, max_new and max_ctx
- * are at most its own, for either dt and any window (0 for a description that is
+ * weights of 22 bits, as f32 q and out have.  The workspace is used as lmxp_attn's:
+ * lmxs_attn_workspace_bytes gives what serves this batch and every one whose n_seq,
+ * n_tokens, max_new and max_ctx are at most its own, for either dt and any window (0 for a description that is
  * refused). */
 size_t lmxs_attn_workspace_bytes(const lmxp_pool *p, const lmxp_batch *b,
                                  const lmxp_attn_desc *d);

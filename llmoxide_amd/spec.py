@@ -506,8 +506,8 @@ def spec_verify(p, tokens, u, r, cu, *, max_new: int, parent=None, q=None, lens=
 def spec_keep(caches: Sequence[PagedCache], batch: PagedBatch, path, accepted, *, stream=None) -> None:
     """Moves the accepted rows' K and V to the slots behind the cached positions, in
     all ``caches`` (layers of one geometry, whose pages and scales are each its own
-    memory) at once: row ``path[b][j]`` of request b to where its row j is.  ``batch`` is the step's, ``path`` and ``accepted`` are
-    ``spec_verify``'s."""
+    memory) at once: row ``path[b][j]`` of request b to where its row j is.  ``batch`` is
+    the step's, ``path`` and ``accepted`` are ``spec_verify``'s."""
     if not caches:
         raise ValueError("caches is empty")
     first = caches[0]

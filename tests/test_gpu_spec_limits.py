@@ -149,6 +149,51 @@ def test_rows_behind_the_end_of_a_table(new, ctx, store, hd):
             assert np.array_equal(got.cpu().numpy(), w)
 
 
+class Cut(po.PagedCase):
+    """What queries see of a case whose batch has ``max_ctx``."""
+    limit = 1 << 30
+
+    def place(self, b, pos):
+        return super().place(b, pos) if pos < self.limit else None
+
+
+@pytest.mark.parametrize("limit", [40, 48, 63])
+@pytest.mark.parametrize("new", [[3, 9, 1], [30, 5, 20], [60, 47, 64]])
+@pytest.mark.parametrize("store,hd,q16", [("f16", 128, False), ("f16", 64, True), ("i8", 128, True), ("i8", 256, False)])
+def test_rows_behind_a_batchs_longest_length(limit, new, store, hd, q16):
+    """Lengths that pass max_ctx, within the table: all rows are stored where they belong,
+    and none sees a position from max_ctx on."""
+    say("beyond max_ctx", limit, new, store, hd, q16)
+    heads, kv = 4, 2
+    c = Cut(115, new=new, ctx=[61, 64, 64], page=16, kv=kv, hd=hd, store=store)
+    cache, _ = on_gpu(c)
+    batch = lmx.PagedBatch(gpu(c.cu), ints(c.ctx), gpu(c.table), n_tokens=c.tokens, max_new=max(new), max_ctx=limit)
+    x = [rows(c, 116 + i, h) for i, h in enumerate((heads, kv, kv))]
+    q, k, v = (gpu(y.reshape(c.tokens, -1)) for y in x)
+    want = po.append(c, x[1], x[2])
+    lmx.paged_append(k, v, cache, batch)
+    for got, w in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), want):
+        if w is not None:
+            assert np.array_equal(got.cpu().numpy(), w)
+    c.k, c.v, c.k_scale, c.v_scale = want
+    c.limit = limit
+    if q16:
+        x[0] = x[0].astype(np.float16).astype(np.float32)
+        q = q.half()
+    for window in (0, 13):
+        trees = trees_of(c, 117)
+        sees = [so.tree(t, window)[1] for t in trees]
+        pos = np.concatenate([c.ctx[b] - new[b] + so.tree(t)[0] for b, t in enumerate(trees)])
+        seen = gpu(np.concatenate([so.words_of(m, 1) for m in sees]))
+        for ref, got in ((po.attend(c, x[0], heads=heads, window=window),
+                          lmx.paged_attention(q, cache, batch, n_heads=heads, window=window)),
+                         (so.attend(c, x[0], sees, heads=heads, window=window, pos=pos),
+                          lmx.spec_attention(q, cache, batch, seen, n_heads=heads, window=window, pos=ints(pos)))):
+            ref, mag, prod, top = ref
+            got = got.double().cpu().numpy().reshape(ref.shape)
+            assert np.all(np.abs(got - ref) <= po.attend_bound(c, mag, prod, top, 64, f32=not q16))
+
+
 def test_a_full_request_leaves_its_prefix_and_its_neighbours():
     """Two requests share their first pages; one reaches the end of its row of the table in
     this step, the other goes on.  The plan's lengths lead the prologue to the map's slots."""
